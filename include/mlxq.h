@@ -301,6 +301,156 @@ int mlxq_lokr_residual(const void* x, int x_dtype, int64_t M, int64_t K, const v
 int mlxq_cast(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n, void* stream);
 
 /*
+ * ---- Serving a decoder from a paged key/value cache ------------------------------------------
+ *
+ * The step between a decoder block's qkv projection and its output projection: rotate the new
+ * queries and keys by their positions, write keys and values into the pages of a cache, attend
+ * over the pages, and copy pages when sequences fork or the pool is compacted.  No counterpart in
+ * the reference, whose attention runs in MLX (mlx-gen-sensenova/src/qwen3.rs:463, forward_cached).
+ *
+ * Queries, keys, values, cache and result have one dtype (f32, bf16 or fp16).  Scores, softmax
+ * statistics and sums are f32; 16-bit types round the softmax weights to the type before the
+ * product with the values, and the result once.
+ *
+ * Cache: a pool of pages of page_size tokens, one pool for a layer's keys and one for its values.
+ * With C = 16 / sizeof(element) (8 for 16-bit types, 4 for f32), page p of the keys starts
+ * p * k_page_stride elements into k and holds [heads, page_size/16, head_dim/C, 16, C]: blocks of
+ * 16 tokens, each a run of 16-byte pieces with the token the faster index.  A page of the values
+ * holds [heads, page_size/C, head_dim, C]: C tokens of a feature side by side.  These are the
+ * operands of the matrix instructions as they lie, so the attention kernels read both without
+ * moving an element between lanes.  The pages of a pool need no order; head_dim is a multiple of 16
+ * up to 256, page_size a power of two from 16 to 1024.
+ *
+ * A page id that a call needs and that is outside [0, pages) is never followed: the token is not
+ * written (cache_append, copy_pages), the rows that see it become NaN (paged_attention).
+ */
+typedef struct {
+  void* data;             /* element (t, h, d) at data[t * token_stride + h * head_stride + d] */
+  int64_t heads;
+  int64_t token_stride;   /* elements; both strides a multiple of 16 bytes */
+  int64_t head_stride;
+} mlxq_heads;
+
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_page_stride;  /* elements from one page to the next, a multiple of 16 bytes */
+  int64_t v_page_stride;
+  int64_t pages, page_size, heads, head_dim;
+  int dtype;              /* mlxq_dtype of cache, queries, keys, values and result */
+} mlxq_paged_cache;
+
+/* The sequences of a step.  Sequence b owns the new tokens q_starts[b] .. q_starts[b+1] - 1 of the
+ * step's T (n of them, 0 allowed) and has kv_lens[b] tokens in the cache counting those: the i-th new
+ * one is its token kv_lens[b] - n + i.  Token j lies in page block_tables[b * table_stride +
+ * j / page_size].  All arrays are device int32; lengths past table_width pages are cut there.
+ * max_q and max_kv are what the launch is planned for (the longest n and kv length expected):
+ * results do not depend on them.  Steps' tokens outside every sequence are left alone. */
+typedef struct {
+  const int32_t* block_tables;
+  const int32_t* q_starts;  /* [sequences + 1], not decreasing */
+  const int32_t* kv_lens;   /* [sequences] */
+  int64_t sequences, table_width, table_stride;
+  int64_t max_q, max_kv;
+} mlxq_paged_batch;
+
+/* Long-context scalings of the rotation frequencies f_i = base^(-2i/rotary_dim). */
+typedef enum {
+  MLXQ_ROPE_NONE = 0,
+  MLXQ_ROPE_LINEAR = 1,  /* f_i / factor */
+  MLXQ_ROPE_NTK = 2,     /* base * factor^(r / (r - 2)), r = rotary_dim */
+  /* Blend by wavelength: with n_i = original_context * f_i / 2 pi turns over the trained context,
+   * f_i is kept where n_i >= high, divided by factor where n_i <= low, and between them mixed:
+   * YARN linearly in the pair index i between the (fractional) indexes of the two bounds, rounded
+   * outwards, LLAMA3 linearly in n_i.  YARN also scales cos and sin by 0.1 ln(factor) + 1. */
+  MLXQ_ROPE_YARN = 3,
+  MLXQ_ROPE_LLAMA3 = 4,
+} mlxq_rope_kind;
+
+typedef struct {
+  int kind;                 /* mlxq_rope_kind */
+  double factor;            /* >= 1; not read for NONE */
+  double original_context;  /* trained context, tokens (YARN, LLAMA3) */
+  double low, high;         /* turns, 0 < low < high (YARN: 1 and 32 are common, LLAMA3: 1 and 4) */
+} mlxq_rope_scaling;
+
+/* Host function: inv_freq[i], i < rotary_dim / 2, in radians a position, and the factor of cos and
+ * sin.  scaling NULL = none. */
+int mlxq_rotary_frequencies(int64_t rotary_dim, double base, const mlxq_rope_scaling* scaling,
+                            double* inv_freq, double* magnitude);
+
+/* table[p, i] = magnitude * (cos, sin)(p * inv_freq[i]) for positions p < positions, f32, each angle
+ * in 64 bits.  inv_freq is a host array of rotary_dim / 2 <= 128; table is
+ * [positions, rotary_dim/2, 2], 16-byte aligned. */
+int mlxq_rotary_table(const double* inv_freq, int64_t rotary_dim, double magnitude, int64_t positions,
+                      float* table, void* stream);
+
+/*
+ * Rotary positions: y[t, h] = x[t, h] with each pair (a, b) of its first rotary_dim features turned
+ * by the table's row positions[t]: (a c - b s, b c + a s).  Pair i is features (i, i + rotary_dim/2),
+ * or (2i, 2i + 1) when interleaved.  Features past rotary_dim are copied.  inverse != 0 turns by -s:
+ * the transpose, which takes the gradient of y to the gradient of x.  positions [T] int32; one outside
+ * [0, table_rows) gives NaN in the rotated features.  head_dim is a multiple of 16 bytes.  y may be x
+ * (same strides); otherwise they must not overlap.
+ */
+int mlxq_rotary(const mlxq_heads* x, int dtype, int64_t T, int64_t head_dim, const int32_t* positions,
+                const float* table, int64_t table_rows, int64_t rotary_dim, int interleaved,
+                int inverse, const mlxq_heads* y, void* stream);
+
+/*
+ * Writes a step's keys and values into the cache, in one launch with the rotation of its queries and
+ * keys.  k and v hold the T new tokens; the keys are rotated as mlxq_rotary does by the token's place
+ * in its sequence, or by positions[t] when positions is not NULL; table NULL (rotary_dim 0) writes
+ * them as they are.  q (NULL = none) is rotated alike into q_out, which may be q.  Tokens whose place
+ * is negative (more new tokens than kv_lens) are not written to the cache.
+ */
+int mlxq_cache_append(const mlxq_heads* k, const mlxq_heads* v, int64_t T, const mlxq_paged_cache* cache,
+                      const mlxq_paged_batch* batch, const int32_t* positions, const float* table,
+                      int64_t table_rows, int64_t rotary_dim, int interleaved, const mlxq_heads* q,
+                      const mlxq_heads* q_out, void* stream);
+
+/* Options of the attention.  Row h of the new token at place p of a sequence of L tokens sees the
+ * tokens j with  lo <= j < hi,  hi = causal ? min(L, max(p + 1, prefix)) : L,  lo = window ?
+ * max(0, p + 1 - window) : 0. */
+typedef struct {
+  float scale;                 /* > 0: z_j = scale * q.k_j */
+  int causal;
+  int64_t window;              /* 0 = none; counts the token itself */
+  float softcap;               /* 0 = none; z_j = softcap * tanh(z_j / softcap) */
+  const int32_t* prefix_lens;  /* [sequences] or NULL: tokens that every row of the sequence sees */
+  const float* alibi_slopes;   /* [q heads] or NULL: z_j -= slope * |p - j|, after the cap */
+  const float* sinks;          /* [q heads] or NULL: a score without a value, in the denominator only */
+} mlxq_attention;
+
+/*
+ * Attention of the step's new tokens over their sequences' cached tokens (a chunk of a prompt, drafted
+ * tokens or one token each, mixed at will):
+ *   out[t, h] = sum_j exp(z_j) v_j / (sum_j exp(z_j) + exp(sink_h))   over the visible j,
+ * zero for a row that sees nothing.  Query head h reads key head h / (q heads / cache heads).  What the
+ * masked and unwritten places of the cache hold (NaN and infinities included) does not reach the
+ * result.  out must not overlap q.  workspace: mlxq_paged_attention_workspace_size() bytes, whatever
+ * they hold (NULL when that is 0).  Launch shapes follow T, the batch's sizes and hints and the strides
+ * only, so a captured graph may be replayed with other lengths and tables.
+ */
+size_t mlxq_paged_attention_workspace_size(int64_t T, int64_t q_heads, const mlxq_paged_cache* cache,
+                                           const mlxq_paged_batch* batch, const mlxq_attention* options);
+int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache* cache,
+                         const mlxq_paged_batch* batch, const mlxq_attention* options,
+                         const mlxq_heads* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Copies pages src[i] to dst[i], i < count, in each of `planes` pools (the layers' keys and values):
+ * page p of plane l is the page_bytes bytes at cache + l * plane_stride_bytes + p * page_stride_bytes
+ * (strides and page_bytes multiples of 16).  tables (NULL = none): entries [rows, width], rows
+ * table_stride apart, that equal some src[i] become dst[i].  src and dst are device int32; no dst may
+ * be a src or appear twice, and a src that tables are to follow appears once.
+ */
+int mlxq_cache_copy_pages(void* cache, int64_t planes, int64_t plane_stride_bytes, int64_t pages,
+                          int64_t page_bytes, int64_t page_stride_bytes, const int32_t* src,
+                          const int32_t* dst, int64_t count, int32_t* tables, int64_t rows,
+                          int64_t width, int64_t table_stride, void* stream);
+
+/*
  * Host-side shape helper — replaces quant::packed_bits (src/quant.rs:38-41): from the packed
  * shapes infer bits = wq_cols*32 / (scales_cols*group_size).  Returns 4 or 8, or -1 (with
  * mlxq_last_error set) for a malformed triple instead of panicking.

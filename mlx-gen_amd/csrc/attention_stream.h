@@ -1,0 +1,389 @@
+// attention_stream.h — paged attention for few rows a key head (decode, drafted tokens) in any dtype,
+// and for f32 at every size.
+//
+// Rows are (token, query head) pairs of one sequence and key head, so the heads that share a key head
+// read it once.  A workgroup holds 16 * MT rows and a range of the sequence's keys; each of its waves
+// walks its own units of keys (32 for 16-bit types, 16 for f32) with its own running maximum and sum
+// (an online softmax), and the waves' results are joined in LDS at the end.  Long sequences are also
+// split over workgroups, whose sums a second kernel joins.
+//
+// Scores are computed transposed, S^T = K Q^T, and so is the result, O^T = V^T P^T: the cache's layout
+// is the A operand of both products, 16 bytes a lane straight from memory, and a lane of S^T holds
+// scores of one row.  With lane = 16 g + c, the D operand of the 16x16 products puts rows 4 g + i in lane
+// (g, c) where the B operand of the next product wants keys C g + e: the 16 keys of S^T tile t are
+// therefore those with key % C / 4 == t, so that element 4 t + i of lane group g is key C g + 4 t + i and
+// the exponentials are the next product's operand as they stand.
+//
+// Bound by the cache's bytes for one token: no LDS and no barrier in the loop, and the next unit's keys
+// are requested as soon as this one's are used.
+#pragma once
+
+#include "paged.h"
+
+namespace mlxq {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// acc += A (16 x one chunk a lane group) . B, one chunk = 8 16-bit or 4 f32 products deep a lane group.
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, f32x4 acc) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), acc, 0, 0, 0);
+    return acc;
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  }
+}
+
+// The four lane groups' values of a row: lanes c, 16 + c, 32 + c, 48 + c.
+__device__ __forceinline__ float group_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float group_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Whether any element of a chunk of a 16- or 32-bit float type is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(const u32x4& v) {
+  // All exponent bits set: adding one at the exponent's lowest bit carries into the sign bit.
+  constexpr uint32_t mask = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+  constexpr uint32_t top = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (v[i] & mask) + one;
+  return r & top;
+}
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// A score with its cap and bias, in units of log 2 (AttnArgs::scale is the caller's there).
+template <typename T>
+__device__ __forceinline__ float bent_score(const AttnArgs& a, float qk, float slope, int p, int j) {
+  float z = qk * a.scale;
+  if (a.softcap > 0.0f) z = a.softcap * (sizeof(T) == 4 ? tanhf(z / a.softcap) : tanh_hw(z / a.softcap));
+  return (z - slope * (float)abs(p - j)) * kLog2e;
+}
+
+// The rows that a lane's row index stands for, and what they see.
+struct RowRange {
+  int lo, hi;
+};
+__device__ __forceinline__ RowRange row_range(const AttnArgs& a, const Seq& s, int p, int prefix) {
+  const int hi = a.causal ? min(s.L, max(p + 1, prefix)) : s.L;
+  return {a.window ? max(0, p + 1 - a.window) : 0, hi};
+}
+
+// First to last key that any row of [row0, row1] sees, those that every one sees, and this split's.
+struct KeyRange {
+  int lo, hi;          // any row
+  int lo_all, hi_all;  // every row
+};
+__device__ __forceinline__ KeyRange key_range(const AttnArgs& a, const Seq& s, int row0, int row1, int prefix) {
+  const RowRange f = row_range(a, s, s.L - s.n + row0 / a.G, prefix), l = row_range(a, s, s.L - s.n + row1 / a.G, prefix);
+  return {f.lo, l.hi, l.lo, f.hi};
+}
+
+template <typename T, int DT, int MT, bool BENT>
+__global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
+  constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
+  constexpr int OD = 32, OROW = OD + 4;  // features of a step of the join, and its padded LDS row
+  __shared__ float lm[NW][TM], ll[NW][TM];
+  __shared__ __align__(16) float lo_[NW][TM][OROW];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c = lane & 15, unit = blockIdx.x / a.Hkv, h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
+  const Batch& bt = a.batch;
+  auto tiles_of = [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; };
+  int b = unit, first = 0;
+  if (!a.direct) find_unit(bt, unit, tiles_of, b, first);
+  if (b < 0) return;
+  const Seq s = load_seq(bt, b);
+  const int rows = s.n * a.G, prefix = a.prefix ? a.prefix[b] : 0;
+  const int last = a.direct ? tiles_of(s) : first + 1;
+  const int32_t* table = bt.tables + b * bt.table_stride;
+  const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1;  // blocks of a page
+  const int64_t head = ((int64_t)h << bt.page_log2) * a.D;
+  const T *kp = (const T*)a.k + head, *vp = (const T*)a.v + head;
+
+  for (int tile = first; tile < last; ++tile) {
+    const int row0 = tile * TM, row1 = min(rows, row0 + TM) - 1;
+    const KeyRange kr = key_range(a, s, row0, row1, prefix);
+    const int ub = kr.lo / KU, ue = kr.hi > kr.lo ? (kr.hi + KU - 1) / KU : ub, cu = a.chunk / KU;
+    const int ns = max(1, min(a.S, (ue - ub + cu - 1) / cu));
+    if (z >= ns) continue;
+    const int u0 = ub + z * cu, u1 = z == a.S - 1 ? ue : min(ue, u0 + cu);
+    const int blo = kr.lo >> 4, bhi = (kr.hi - 1) >> 4;  // blocks with keys that are seen
+
+    // This lane's rows.
+    int p[MT], lo[MT], hi[MT];
+    float slope[MT];
+    u32x4 qf[MT][NS];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = min(row0 + m * 16 + c, row1), i = r / a.G, qh = h * a.G + (r - i * a.G);
+      p[m] = s.L - s.n + i;
+      const RowRange rr = row_range(a, s, p[m], prefix);
+      lo[m] = rr.lo;
+      hi[m] = rr.hi;
+      slope[m] = BENT && a.slopes ? a.slopes[qh] : 0.0f;
+      const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        const int ch = 4 * k + g;
+        qf[m][k] = ch * C < a.D ? load_chunk(q + ch * C) : u32x4{0, 0, 0, 0};
+      }
+    }
+    f32x4 o[MT][ND];
+    float mx[MT], sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      mx[m] = -INFINITY;
+      sum[m] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[m][d] = f32x4{0, 0, 0, 0};
+    }
+
+    // A unit's block of 16 keys: its page, and the block's offset in it.  Blocks that no row sees are
+    // never looked up: their entries may name nothing.
+    auto page_of = [&](int blk) { return table[min(max(blk, blo), bhi) >> blog]; };
+    auto block_at = [&](int blk, int page, int64_t stride) {
+      const int in = min(max(blk, blo), bhi) & bmask;
+      return (int64_t)((unsigned)page < (unsigned)bt.pages ? page : 0) * stride + (int64_t)in * 16 * a.D;
+    };
+    u32x4 kf[NT][NS], vf[ND];
+    auto load_k = [&](int u, int pg0, int pg1) {
+      // Tile t, row c of the products is key C (c / 4) + 4 t + c % 4 of the unit.
+      const T* base = kp + block_at(u * (KU / 16), pg0, a.k_page);
+      if (KU == 32 && c >= 8) base = kp + block_at(u * 2 + 1, pg1, a.k_page);
+      const int key = (C * (c >> 2) + (c & 3)) & 15;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+          const int ch = 4 * k + g;
+          kf[t][k] = ch * C < a.D ? load_chunk(base + (ch * 16 + key + 4 * t) * C) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto load_v = [&](int u, int pg0, int pg1) {
+      const T* base = vp + block_at(u * (KU / 16), pg0, a.v_page);
+      if (KU == 32 && g >= 2) base = vp + block_at(u * 2 + 1, pg1, a.v_page);
+      const int grp = KU == 32 ? g & 1 : g;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        vf[d] = 16 * d < a.D ? load_chunk(base + (grp * a.D + 16 * d + c) * C) : u32x4{0, 0, 0, 0};
+    };
+
+    int u = u0 + w, pg0 = 0, pg1 = 0;
+    if (u < u1) {
+      pg0 = page_of(u * (KU / 16));
+      pg1 = KU == 32 ? page_of(u * 2 + 1) : pg0;
+      load_k(u, pg0, pg1);
+      load_v(u, pg0, pg1);
+    }
+    for (; u < u1; u += NW) {
+      const bool more = u + NW < u1;
+      int nx0 = 0, nx1 = 0;
+      if (more) {
+        nx0 = page_of((u + NW) * (KU / 16));
+        nx1 = KU == 32 ? page_of((u + NW) * 2 + 1) : nx0;
+      }
+      f32x4 st[MT][NT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          st[m][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < NS; ++k) st[m][t] = mma16<T>(kf[t][k], qf[m][k], st[m][t]);
+        }
+      if (more) load_k(u + NW, nx0, nx1);
+      const int key0 = u * KU + C * g;
+      const bool bad = (unsigned)pg0 >= (unsigned)bt.pages || (unsigned)pg1 >= (unsigned)bt.pages;
+      const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all || bad;
+      if (BENT || part) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = key0 + 4 * t + i;
+              float v = st[m][t][i];
+              if constexpr (BENT) v = bent_score<T>(a, v, slope[m], p[m], j);
+              if (part) {
+                if (bad && (unsigned)(j & 16 ? pg1 : pg0) >= (unsigned)bt.pages) v = __builtin_nanf("");
+                v = j >= lo[m] && j < hi[m] ? v : -INFINITY;
+              }
+              st[m][t][i] = v;
+            }
+      }
+      const float cs = BENT ? 1.0f : a.scale;
+      u32x4 pf[MT];
+      bool moved = false;
+      float alpha[MT], e[MT][C];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float v = st[m][0][0];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v = fmaxf(v, st[m][t][i]);
+        const float now = fmaxf(mx[m], group_max(v));
+        const float ref = now == -INFINITY ? 0.0f : now * cs;
+        alpha[m] = __builtin_amdgcn_exp2f(fmaf(mx[m], cs, -ref));
+        moved |= now != mx[m];
+        mx[m] = now;
+        float add = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[m][4 * t + i] = __builtin_amdgcn_exp2f(fmaf(st[m][t][i], cs, -ref));
+            add += e[m][4 * t + i];
+          }
+        sum[m] = fmaf(sum[m], alpha[m], add);
+        // 16-bit types: the softmax weights, at most 1, are rounded to the type for the product with the
+        // values (their f32 sum is not): 2^-9 of each weight in bf16, as the values themselves carry.
+        pf[m] = pack_chunk<T>(e[m]);
+      }
+      if (__any(moved)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[m][d] *= alpha[m];
+      }
+      bool rare = false;
+      if (part) {
+        // 0 * infinity: a hidden key's value must not meet its weight of zero in the matrix product.
+        uint32_t nf = 0;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) nf |= not_finite<T>(vf[d]);
+        rare = __any(nf != 0);
+      }
+      if (!rare) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(vf[d], pf[m], o[m][d]);
+      } else {
+        for (int k = 0; k < KU; ++k) {
+          const int blk = u * (KU / 16) + (k >> 4), el = k % C;
+          const T* v = vp + block_at(blk, k >= 16 ? pg1 : pg0, a.v_page) + (k % 16 / C) * a.D * C + el;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            float pk = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) pk = el == i ? e[m][i] : pk;
+            pk = __shfl(pk, k / C * 16 + c);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (16 * d < a.D && pk != 0.0f) o[m][d][i] += pk * Act<T>::ld(v, (16 * d + 4 * g + i) * C);
+          }
+        }
+      }
+      if (more) load_v(u + NW, nx0, nx1);
+      pg0 = nx0;
+      pg1 = nx1;
+    }
+
+    // Join the waves: maxima and sums first, then the results OD features at a time.
+    const float cs = BENT ? 1.0f : a.scale;
+    __syncthreads();  // the last tile's reads of LDS
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float t = group_sum(sum[m]);
+      if (g == 0) {
+        lm[w][m * 16 + c] = mx[m] * cs;
+        ll[w][m * 16 + c] = t;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) top = fmaxf(top, lm[i][m * 16 + c]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f(mx[m] * cs - ref);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[m][d] *= f;
+    }
+#pragma unroll
+    for (int d0 = 0; d0 < ND; d0 += OD / 16) {
+      if (16 * d0 >= a.D) break;
+      if (d0) __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int d = 0; d < OD / 16; ++d)
+          *reinterpret_cast<f32x4*>(&lo_[w][m * 16 + c][16 * d + 4 * g]) = o[m][d0 + d];
+      __syncthreads();
+      for (int i = tid; i < TM * (OD / 4); i += 64 * NW) {
+        const int rr = i / (OD / 4), d = (i - rr * (OD / 4)) * 4, r = row0 + rr;
+        if (r > row1 || 16 * d0 + d >= a.D) continue;
+        f32x4 v = {0, 0, 0, 0};
+        float top = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+          v += *reinterpret_cast<const f32x4*>(&lo_[k][rr][d]);
+          top = fmaxf(top, lm[k][rr]);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) l += ll[k][rr] * __builtin_amdgcn_exp2f(lm[k][rr] - ref);
+        const int tok = r / a.G, qh = h * a.G + (r - tok * a.G);
+        const int64_t orow = (int64_t)(s.q0 + tok) * a.Hkv * a.G + qh;
+        if (ns > 1) {
+          *reinterpret_cast<f32x4*>(a.part + (orow * a.S + z) * a.D + 16 * d0 + d) = v;
+          if (d0 == 0 && d == 0) {
+            *reinterpret_cast<f32x2*>(a.ml + (orow * a.S + z) * 2) = f32x2{top, l};
+            if (z == 0) a.splits[orow] = ns;
+          }
+        } else {
+          if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * kLog2e - ref);
+          if (a.S > 1 && d0 == 0 && d == 0) a.splits[orow] = 1;
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          T* y = (T*)a.out.p + (s.q0 + tok) * a.out.ts + qh * a.out.hs + 16 * d0 + d;
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(y) = v * inv;
+          else *reinterpret_cast<u32x2*>(y) = u32x2{Elem<T>::pack2(v[0] * inv, v[1] * inv), Elem<T>::pack2(v[2] * inv, v[3] * inv)};
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int DT, int MT>
+static int launch_stream(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
+  const dim3 grid((unsigned)(a.Hkv * plan.units), (unsigned)a.S);
+  if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, false>), grid, dim3(256), 0, st, a);
+  return check_launch("paged_attention");
+}
+
+template <typename T>
+static int stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
+  if (plan.rows == 16) {
+    if (a.D <= 64) return launch_stream<T, 64, 1>(a, plan, st);
+    if (a.D <= 128) return launch_stream<T, 128, 1>(a, plan, st);
+    return launch_stream<T, 256, 1>(a, plan, st);
+  }
+  if (a.D <= 64) return launch_stream<T, 64, 2>(a, plan, st);
+  return launch_stream<T, 128, 2>(a, plan, st);
+}
+
+}  // namespace mlxq

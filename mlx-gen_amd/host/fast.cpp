@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 
+#include <math.h>
 #include <string.h>
 
 #include <vector>
@@ -357,6 +358,272 @@ PyObject* quantize_batched(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- the paged cache (mlxq/paged.py) ---------------------------------------------------------------
+
+// A GPU tensor of one dtype and rank, whatever its strides.
+const at::Tensor* strided(PyObject* o, int64_t dim) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.is_nested() || t.is_conj() || t.is_neg() || t.dim() != dim) return nullptr;
+  return &t;
+}
+
+// [T, heads, D] with contiguous features and 16-byte heads.
+const at::Tensor* get_heads(PyObject* o, mlxq_heads& h) {
+  const at::Tensor* t = strided(o, 3);
+  if (!t || code_of(t->scalar_type()) < 0 || t->numel() == 0) return nullptr;
+  const int64_t C = 16 / t->element_size();
+  if (t->stride(2) != 1 || t->stride(0) % C != 0 || t->stride(1) % C != 0 ||
+      reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0)
+    return nullptr;
+  h = {t->data_ptr(), t->size(1), t->stride(0), t->stride(1)};
+  return t;
+}
+
+// A contiguous tensor of one dtype and shape on `like`'s device.
+const at::Tensor* get_exact(PyObject* o, at::ScalarType type, at::IntArrayRef shape, const at::Tensor& like) {
+  const at::Tensor* t = plain(o, 4);
+  if (!t || t->scalar_type() != type || t->sizes() != shape || t->device() != like.device()) return nullptr;
+  return t;
+}
+
+bool get_table(PyObject* o, const at::Tensor& like, const float*& p, int64_t& rows, int64_t& R, at::Tensor& keep) {
+  p = nullptr;
+  rows = R = 0;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o, 16);
+  if (!t || t->dim() != 3 || t->size(2) != 2 || t->numel() == 0 || t->scalar_type() != at::kFloat || t->device() != like.device())
+    return false;
+  p = t->data_ptr<float>();
+  rows = t->size(0);
+  R = 2 * t->size(1);
+  keep = *t;
+  return true;
+}
+
+// Tensors that a call points into are held for its time: the lock is released, and the caller's tuple may
+// change.
+struct Cache {
+  at::Tensor k, v;
+  mlxq_paged_cache c;
+};
+
+bool pages_apart(const at::Tensor& t, int64_t page, int64_t& stride) {
+  int64_t n = 1;
+  for (int64_t d = t.dim() - 1; d >= 1; --d) {
+    if (t.size(d) != 1 && t.stride(d) != n) return false;
+    n *= t.size(d);
+  }
+  stride = t.stride(0) < page ? page : t.stride(0);
+  return true;
+}
+
+bool get_cache(PyObject* ko, PyObject* vo, Cache& c) {
+  const at::Tensor *k = strided(ko, 6), *v = strided(vo, 5);
+  if (!k || !v) return false;
+  const int dt = code_of(k->scalar_type());
+  if (dt < 0 || v->scalar_type() != k->scalar_type() || v->device() != k->device() || k->numel() == 0) return false;
+  const int64_t C = 16 / k->element_size(), pages = k->size(0), heads = k->size(1), P = k->size(2) * 16, D = k->size(3) * C;
+  if (k->size(4) != 16 || k->size(5) != C || v->size(0) != pages || v->size(1) != heads || v->size(2) * C != P ||
+      v->size(3) != D || v->size(4) != C)
+    return false;
+  c.c = {k->data_ptr(), v->data_ptr(), 0, 0, pages, P, heads, D, dt};
+  if (!pages_apart(*k, heads * P * D, c.c.k_page_stride) || !pages_apart(*v, heads * P * D, c.c.v_page_stride)) return false;
+  c.k = *k;
+  c.v = *v;
+  return true;
+}
+
+struct Step {
+  at::Tensor tables, starts, lens;
+  mlxq_paged_batch b;
+};
+
+// (block_tables, q_starts, kv_lens, max_q, max_kv), a tuple or a subclass of one.
+bool get_batch(PyObject* o, const at::Tensor& like, Step& s) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) return false;
+  const at::Tensor* t = strided(PyTuple_GET_ITEM(o, 0), 2);
+  if (!t || t->scalar_type() != at::kInt || t->device() != like.device() || t->numel() == 0) return false;
+  const int64_t B = t->size(0);
+  if (t->stride(1) != 1 || (B > 1 && t->stride(0) < t->size(1))) return false;
+  const at::Tensor* q = get_exact(PyTuple_GET_ITEM(o, 1), at::kInt, {B + 1}, like);
+  const at::Tensor* l = get_exact(PyTuple_GET_ITEM(o, 2), at::kInt, {B}, like);
+  PyObject* n[2] = {PyTuple_GET_ITEM(o, 3), PyTuple_GET_ITEM(o, 4)};
+  long v[2];
+  if (!q || !l || !ints(n, 2, v)) return false;
+  s.tables = *t;
+  s.starts = *q;
+  s.lens = *l;
+  s.b = {t->data_ptr<int32_t>(), q->data_ptr<int32_t>(), l->data_ptr<int32_t>(), B, t->size(1), t->stride(0), v[0], v[1]};
+  return true;
+}
+
+bool truth(PyObject* o, int& v) {
+  if (!PyBool_Check(o)) return false;
+  v = o == Py_True;
+  return true;
+}
+
+at::Tensor like_heads(const at::Tensor& x, mlxq_heads& h) {
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  h = {y.data_ptr(), y.size(1), y.stride(0), y.stride(1)};
+  return y;
+}
+
+// rotary(x, positions, table, interleaved, inverse)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    mlxq_heads xh, yh;
+    int inter, inverse;
+    const float* table;
+    int64_t rows, R;
+    at::Tensor keep;
+    if (n != 5 || !truth(a[3], inter) || !truth(a[4], inverse)) return nullptr;
+    const at::Tensor* xp = get_heads(a[0], xh);
+    if (!xp) return nullptr;
+    const at::Tensor x = *xp;
+    const at::Tensor* pos = get_exact(a[1], at::kInt, {x.size(0)}, x);
+    if (!pos || !get_table(a[2], x, table, rows, R, keep) || !table) return nullptr;
+    const at::Tensor held = *pos;
+    bool ok;
+    void* st = stream_of(x, ok);
+    if (!ok) return nullptr;
+    at::Tensor y = like_heads(x, yh);
+    if (unlocked([&] {
+          return mlxq_rotary(&xh, code_of(x.scalar_type()), x.size(0), x.size(2), held.data_ptr<int32_t>(), table, rows, R,
+                             inter, inverse, &yh, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// cache_append(k, v, k_cache, v_cache, batch, q, table, positions, interleaved) -> the rotated q, True without q
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    mlxq_heads h[4];
+    Cache c;
+    Step s;
+    int inter;
+    const float* table;
+    int64_t rows, R;
+    at::Tensor t[3], keep, pos, out;
+    if (n != 9 || !truth(a[8], inter) || !get_cache(a[2], a[3], c) || !get_batch(a[4], c.k, s)) return nullptr;
+    const bool has_q = a[5] != Py_None;
+    PyObject* o[3] = {a[0], a[1], a[5]};
+    for (int i = 0; i < (has_q ? 3 : 2); ++i) {
+      const at::Tensor* p = get_heads(o[i], h[i]);
+      if (!p || p->scalar_type() != c.k.scalar_type() || p->device() != c.k.device() || p->size(2) != c.c.head_dim) return nullptr;
+      t[i] = *p;
+      if (t[i].size(0) != t[0].size(0) || (i < 2 && h[i].heads != c.c.heads)) return nullptr;
+    }
+    if (!get_table(a[6], c.k, table, rows, R, keep)) return nullptr;
+    if (a[7] != Py_None) {
+      const at::Tensor* p = get_exact(a[7], at::kInt, {t[0].size(0)}, c.k);
+      if (!p) return nullptr;
+      pos = *p;
+    }
+    bool ok;
+    void* st = stream_of(c.k, ok);
+    if (!ok) return nullptr;
+    if (has_q) out = like_heads(t[2], h[3]);
+    if (unlocked([&] {
+          return mlxq_cache_append(&h[0], &h[1], t[0].size(0), &c.c, &s.b, pos.defined() ? pos.data_ptr<int32_t>() : nullptr,
+                                   table, rows, R, inter, has_q ? &h[2] : nullptr, has_q ? &h[3] : nullptr, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    if (has_q) return THPVariable_Wrap(std::move(out));
+    Py_RETURN_TRUE;
+  });
+}
+
+// paged_attention(q, k_cache, v_cache, batch, scale, causal, window, softcap, prefix_lens, alibi_slopes, sinks)
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    mlxq_heads qh, oh;
+    Cache c;
+    Step s;
+    long window;
+    at::Tensor keep[3];
+    mlxq_attention opt = {};
+    if (n != 11 || !truth(a[5], opt.causal) || !ints(a + 6, 1, &window)) return nullptr;
+    const at::Tensor* qp = get_heads(a[0], qh);
+    if (!qp || !get_cache(a[1], a[2], c) || qp->scalar_type() != c.k.scalar_type() || qp->device() != c.k.device() ||
+        qp->size(2) != c.c.head_dim || qh.heads % c.c.heads != 0)
+      return nullptr;
+    const at::Tensor q = *qp;
+    if (!get_batch(a[3], q, s)) return nullptr;
+    opt.window = window;
+    opt.scale = a[4] == Py_None ? (float)(1.0 / sqrt((double)c.c.head_dim)) : (float)PyFloat_AsDouble(a[4]);
+    opt.softcap = (float)PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::ScalarType types[3] = {at::kInt, at::kFloat, at::kFloat};
+    const int64_t sizes[3] = {s.b.sequences, qh.heads, qh.heads};
+    for (int i = 0; i < 3; ++i) {
+      if (a[8 + i] == Py_None) continue;
+      const at::Tensor* t = get_exact(a[8 + i], types[i], {sizes[i]}, q);
+      if (!t) return nullptr;
+      keep[i] = *t;
+    }
+    opt.prefix_lens = keep[0].defined() ? keep[0].data_ptr<int32_t>() : nullptr;
+    opt.alibi_slopes = keep[1].defined() ? keep[1].data_ptr<float>() : nullptr;
+    opt.sinks = keep[2].defined() ? keep[2].data_ptr<float>() : nullptr;
+    bool ok;
+    void* st = stream_of(q, ok);
+    if (!ok) return nullptr;
+    const size_t need = mlxq_paged_attention_workspace_size(q.size(0), qh.heads, &c.c, &s.b, &opt);
+    at::Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+    at::Tensor out = like_heads(q, oh);
+    if (unlocked([&] {
+          return mlxq_paged_attention(&qh, q.size(0), &c.c, &s.b, &opt, &oh, need ? ws.data_ptr() : nullptr, need, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// copy_pages(cache, src, dst, block_tables, dim) -> True
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    long dim;
+    if (n != 5 || !ints(a + 4, 1, &dim)) return nullptr;
+    const at::Tensor* p = plain(a[0], 16);
+    if (!p || code_of(p->scalar_type()) < 0 || p->dim() < 5 || dim < 0 || dim >= p->dim() - 1 || p->numel() == 0) return nullptr;
+    const at::Tensor cache = *p;
+    const at::Tensor* sp = plain(a[1], 4);
+    if (!sp || sp->dim() != 1) return nullptr;
+    const int64_t count = sp->size(0);
+    sp = get_exact(a[1], at::kInt, {count}, cache);
+    const at::Tensor* dp = get_exact(a[2], at::kInt, {count}, cache);
+    if (!sp || !dp || count == 0) return nullptr;
+    const at::Tensor src = *sp, dst = *dp;
+    at::Tensor tables;
+    if (a[3] != Py_None) {
+      const at::Tensor* t = strided(a[3], 2);
+      if (!t || t->scalar_type() != at::kInt || t->device() != cache.device() || t->numel() == 0 || t->stride(1) != 1 ||
+          (t->size(0) > 1 && t->stride(0) < t->size(1)))
+        return nullptr;
+      tables = *t;
+    }
+    int64_t planes = 1, page = cache.element_size();
+    for (int64_t i = 0; i < dim; ++i) planes *= cache.size(i);
+    for (int64_t i = dim + 1; i < cache.dim(); ++i) page *= cache.size(i);
+    bool ok;
+    void* st = stream_of(cache, ok);
+    if (!ok) return nullptr;
+    if (unlocked([&] {
+          return mlxq_cache_copy_pages(cache.data_ptr(), planes, cache.size(dim) * page, cache.size(dim), page, page,
+                                       src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), count,
+                                       tables.defined() ? tables.data_ptr<int32_t>() : nullptr,
+                                       tables.defined() ? tables.size(0) : 0, tables.defined() ? tables.size(1) : 0,
+                                       tables.defined() ? tables.stride(0) : 0, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
 // set_error_type(MlxqError)
 PyObject* set_error_type(PyObject*, PyObject* type) {
   Py_INCREF(type);
@@ -372,6 +639,10 @@ PyMethodDef kMethods[] = {
     {"embedding", (PyCFunction)(void*)embedding, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void*)dequantize, METH_FASTCALL, nullptr},
     {"quantize_batched", (PyCFunction)(void*)quantize_batched, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
+    {"cache_append", (PyCFunction)(void*)cache_append, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},
+    {"copy_pages", (PyCFunction)(void*)copy_pages, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

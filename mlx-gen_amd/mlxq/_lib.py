@@ -26,6 +26,12 @@ MLXQ_ACT_GELU = 1
 MLXQ_ACT_GELU_TANH = 2
 MLXQ_ACT_GELU_EXACT = 3
 
+MLXQ_ROPE_NONE = 0
+MLXQ_ROPE_LINEAR = 1
+MLXQ_ROPE_NTK = 2
+MLXQ_ROPE_YARN = 3
+MLXQ_ROPE_LLAMA3 = 4
+
 # Size of the static per-device scratch array behind mlxq_linear_noalloc.
 MLXQ_NOALLOC_SCRATCH_BYTES = 8 << 20
 
@@ -53,6 +59,13 @@ EXPORTS = (
     "mlxq_cast",
     "mlxq_swiglu",
     "mlxq_qmm_experts",
+    "mlxq_rotary_frequencies",
+    "mlxq_rotary_table",
+    "mlxq_rotary",
+    "mlxq_cache_append",
+    "mlxq_paged_attention_workspace_size",
+    "mlxq_paged_attention",
+    "mlxq_cache_copy_pages",
 )
 
 
@@ -75,6 +88,34 @@ class Epilogue(ctypes.Structure):
         ("bias_dtype", ctypes.c_int),
         ("lora_dtype", ctypes.c_int),
     ]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("heads", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class PagedCacheView(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_page_stride", ctypes.c_int64),
+                ("v_page_stride", ctypes.c_int64), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("heads", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("dtype", ctypes.c_int)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("block_tables", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+                ("sequences", ctypes.c_int64), ("table_width", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+                ("max_q", ctypes.c_int64), ("max_kv", ctypes.c_int64)]
+
+
+class RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double), ("original_context", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_int64),
+                ("softcap", ctypes.c_float), ("prefix_lens", ctypes.c_void_p), ("alibi_slopes", ctypes.c_void_p),
+                ("sinks", ctypes.c_void_p)]
 
 
 _lib = None
@@ -129,6 +170,19 @@ def load():
                                 _int, _vp, _vp]
     lib.mlxq_embedding.argtypes = [_vp, _i64, _vp, _vp, _vp, _int, _i64, _i64, _int, _int, _vp, _int,
                                    _vp]
+    _heads, _cache, _batch, _attn = (ctypes.POINTER(t) for t in (Heads, PagedCacheView, PagedBatch, Attention))
+    _dbl, _pd = ctypes.c_double, ctypes.POINTER(ctypes.c_double)
+    lib.mlxq_rotary_frequencies.argtypes = [_i64, _dbl, ctypes.POINTER(RopeScaling), _pd, _pd]
+    lib.mlxq_rotary_table.argtypes = [_pd, _i64, _dbl, _i64, _vp, _vp]
+    lib.mlxq_rotary.argtypes = [_heads, _int, _i64, _i64, _vp, _vp, _i64, _i64, _int, _int, _heads, _vp]
+    lib.mlxq_cache_append.argtypes = [_heads, _heads, _i64, _cache, _batch, _vp, _vp, _i64, _i64, _int, _heads, _heads, _vp]
+    lib.mlxq_paged_attention_workspace_size.argtypes = [_i64, _i64, _cache, _batch, _attn]
+    lib.mlxq_paged_attention_workspace_size.restype = ctypes.c_size_t
+    lib.mlxq_paged_attention.argtypes = [_heads, _i64, _cache, _batch, _attn, _heads, _vp, ctypes.c_size_t, _vp]
+    lib.mlxq_cache_copy_pages.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp]
+    for name in ("mlxq_rotary_frequencies", "mlxq_rotary_table", "mlxq_rotary", "mlxq_cache_append",
+                 "mlxq_paged_attention", "mlxq_cache_copy_pages"):
+        getattr(lib, name).restype = _int
     for name in ("mlxq_quantize", "mlxq_quantize_batched", "mlxq_dequantize", "mlxq_quantized_matmul", "mlxq_qmm",
                  "mlxq_qmv", "mlxq_qmv_valu", "mlxq_linear", "mlxq_linear_noalloc", "mlxq_packed_bits", "mlxq_embedding",
                  "mlxq_lora_residual", "mlxq_lokr_residual", "mlxq_cast", "mlxq_swiglu",
