@@ -40,16 +40,18 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq, int6
 AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype, int64_t B, int64_t max_q,
                         int64_t max_kv, int64_t window) {
   AttnPlan p;
-  const int64_t G = Hq / Hkv, cus = device_cu_count();
-  // 32 rows of wide heads would not fit a wave's registers.
-  p.rows = max_q * G <= 16 || D > 128 ? 16 : 32;
-  p.direct = max_q * G <= p.rows;
+  const int64_t G = Hq / Hkv, cus = device_cu_count(), most = max_q * G;
+  // 32 rows of heads wider than 128 would not fit a wave's registers in the streaming kernel.
+  p.rows = most <= 16 || D > 128 ? 16 : 32;
+  p.tiled = dtype != MLXQ_FLOAT32 && most > p.rows;
+  if (p.tiled) p.rows = 128;
+  p.direct = !p.tiled && most <= p.rows;
   p.units = p.direct ? B : T * G / p.rows + B;
-  // Splits: enough workgroups of four waves for three on every CU, at least 256 tokens each.
+  // Splits: enough workgroups of four waves for two (tiled) or three on every CU, at least 256 tokens each.
   int64_t range = max_kv;
   if (window) range = std::min(range, window + max_q);
   const int64_t busy = std::min<int64_t>(p.units, T * G / p.rows + std::min(B, T)) * Hkv;
-  const int64_t want = std::max<int64_t>(1, 3 * cus / std::max<int64_t>(busy, 1));
+  const int64_t want = std::max<int64_t>(1, (p.tiled ? 2 : 3) * cus / std::max<int64_t>(busy, 1));
   int64_t chunk = std::max<int64_t>(256, (range + want - 1) / want);
   chunk = std::max<int64_t>((chunk + 127) / 128 * 128, ((range + 255) / 256 + 127) / 128 * 128);
   chunk = std::min<int64_t>(chunk, 0x40000000);
@@ -74,8 +76,9 @@ static int launch_join(const AttnArgs& a, hipStream_t st) {
 }
 
 int run_attention(const AttnArgs& a, int dtype, const AttnPlan& plan, hipStream_t st) {
-  const int rc = dtype == MLXQ_BFLOAT16 ? run_attn_stream_bf16(a, plan, st)
-                 : dtype == MLXQ_FLOAT16 ? run_attn_stream_f16(a, plan, st) : run_attn_stream_f32(a, plan, st);
+  const int rc = dtype == MLXQ_BFLOAT16 ? (plan.tiled ? run_attn_tile_bf16 : run_attn_stream_bf16)(a, plan, st)
+                 : dtype == MLXQ_FLOAT16 ? (plan.tiled ? run_attn_tile_f16 : run_attn_stream_f16)(a, plan, st)
+                                         : run_attn_stream_f32(a, plan, st);
   if (rc || a.S == 1) return rc;
   if (dtype == MLXQ_BFLOAT16) return launch_join<uint16_t>(a, st);
   if (dtype == MLXQ_FLOAT16) return launch_join<_Float16>(a, st);

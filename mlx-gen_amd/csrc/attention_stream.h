@@ -55,17 +55,72 @@ __device__ __forceinline__ float group_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Whether any element of a chunk of a 16- or 32-bit float type is infinite or NaN.
+// A value that is infinite or NaN must not meet the weight 0 of a row that does not see it.  Where a unit of
+// keys is hidden from some row, such values are taken out of the product (finite_mask) and, if there are any, added by a
+// second product of codes with indicators of the rows' non-zero weights: +inf counts 1, -inf 128, NaN both,
+// exact in all three types and, over at most 64 keys, in their sum.
 template <typename T>
-__device__ __forceinline__ uint32_t not_finite(const u32x4& v) {
+__device__ __forceinline__ uint32_t finite_mask(uint32_t v) {
   // All exponent bits set: adding one at the exponent's lowest bit carries into the sign bit.
-  constexpr uint32_t mask = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
-  constexpr uint32_t one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
-  constexpr uint32_t top = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
-  uint32_t r = 0;
+  if constexpr (sizeof(T) == 4) return (((v & 0x7f800000u) + 0x00800000u) >> 31) - 1u;
+  constexpr uint32_t mask = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+  return ~(((((v & mask) + one) & 0x80008000u) >> 15) * 0xffffu);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t value_code(uint32_t v) {
+  constexpr uint32_t pos = sizeof(T) == 4 ? 0x3f800000u : __is_same(T, _Float16) ? 0x3c00u : 0x3f80u;  // 1
+  constexpr uint32_t neg = sizeof(T) == 4 ? 0x43000000u : __is_same(T, _Float16) ? 0x5800u : 0x4300u;  // 128
+  constexpr uint32_t both = sizeof(T) == 4 ? 0x43010000u : __is_same(T, _Float16) ? 0x5808u : 0x4301u; // 129
+  const uint32_t bad = ~finite_mask<T>(v);
+  if constexpr (sizeof(T) == 4) return bad & ((v & 0x007fffffu) ? both : v >> 31 ? neg : pos);
+  constexpr uint32_t man = __is_same(T, _Float16) ? 0x03ffu : 0x007fu;
+  const uint32_t lo = (v & man) ? both : (v & 0x8000u) ? neg : pos;
+  const uint32_t hi = (v >> 16 & man) ? both : v >> 31 ? neg : pos;
+  return bad & (lo | hi << 16);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t weight_code(uint32_t v) {
+  if constexpr (sizeof(T) == 4) return v ? 0x3f800000u : 0u;
+  constexpr uint32_t one = __is_same(T, _Float16) ? 0x3c00u : 0x3f80u;
+  return (v & 0xffffu ? one : 0u) | (v >> 16 ? one << 16 : 0u);
+}
+__device__ __forceinline__ float decoded(float x) {
+  const float n = floorf(x * (1.0f / 128.0f));
+  return (x - 128.0f * n > 0.0f ? INFINITY : 0.0f) + (n > 0.0f ? -INFINITY : 0.0f);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 each(u32x4 v, uint32_t (*f)(uint32_t)) {
+  return u32x4{f(v[0]), f(v[1]), f(v[2]), f(v[3])};
+}
+
+// The running maximum a row's exponents are taken against moves only when a score passes it by this many
+// units of log 2: weights up to 2^8 are as exact as weights up to 1 (fp16's end at 2^16), and the sums
+// are rescaled rarely.
+constexpr float kSlack = 8.0f;
+
+// Whether any wave of the workgroup says so.  flags: LDS, one for each of the NW waves, used for nothing else.
+template <int NW>
+__device__ __forceinline__ bool any_wave(bool v, int* flags) {
+  if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int r = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r |= (v[i] & mask) + one;
-  return r & top;
+  for (int i = 0; i < NW; ++i) r |= flags[i];
+  return __builtin_amdgcn_readfirstlane(r) != 0;
+}
+
+// Rows (keys [lo, lo + span)) that see a key of [from, to) whose table entry names no page get a NaN sum.
+template <int N>
+__device__ __forceinline__ void poison(const Batch& bt, const int32_t* table, int from, int to, const int (&lo)[N],
+                                       const int (&span)[N], float (&sum)[N]) {
+  for (int i = from >> bt.page_log2; i <= (to - 1) >> bt.page_log2; ++i) {
+    if ((unsigned)table[i] < (unsigned)bt.pages) continue;
+    const int f = max(i << bt.page_log2, from), t = min((i + 1) << bt.page_log2, to);
+#pragma unroll
+    for (int m = 0; m < N; ++m)
+      if (max(f, lo[m]) < min(t, lo[m] + span[m])) sum[m] = __builtin_nanf("");
+  }
 }
 
 constexpr float kLog2e = 1.44269504088896341f;
@@ -97,15 +152,18 @@ __device__ __forceinline__ KeyRange key_range(const AttnArgs& a, const Seq& s, i
   return {f.lo, l.hi, l.lo, f.hi};
 }
 
-template <typename T, int DT, int MT, bool BENT>
-__global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
+// FULL: head_dim is DT, else below it and the rest of DT is zeros.
+template <typename T, int DT, int MT, bool BENT, bool FULL>
+__global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kernel(AttnArgs a) {
   constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
   constexpr int OD = 32, OROW = OD + 4;  // features of a step of the join, and its padded LDS row
   __shared__ float lm[NW][TM], ll[NW][TM];
+  __shared__ int flags[NW];
   __shared__ __align__(16) float lo_[NW][TM][OROW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15, unit = blockIdx.x / a.Hkv, h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
   const Batch& bt = a.batch;
+  const int D = FULL ? DT : a.D;
   auto tiles_of = [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; };
   int b = unit, first = 0;
   if (!a.direct) find_unit(bt, unit, tiles_of, b, first);
@@ -115,7 +173,7 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
   const int last = a.direct ? tiles_of(s) : first + 1;
   const int32_t* table = bt.tables + b * bt.table_stride;
   const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1;  // blocks of a page
-  const int64_t head = ((int64_t)h << bt.page_log2) * a.D;
+  const int64_t head = ((int64_t)h << bt.page_log2) * D;
   const T *kp = (const T*)a.k + head, *vp = (const T*)a.v + head;
 
   for (int tile = first; tile < last; ++tile) {
@@ -127,8 +185,50 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
     const int u0 = ub + z * cu, u1 = z == a.S - 1 ? ue : min(ue, u0 + cu);
     const int blo = kr.lo >> 4, bhi = (kr.hi - 1) >> 4;  // blocks with keys that are seen
 
+    // A unit's blocks of 16 keys: their pages, and the blocks' first elements.  Blocks that no row sees are
+    // never looked up: their entries may name nothing.
+    bool bad = false;
+    auto page_of = [&](int blk) { return table[min(max(blk, blo), bhi) >> blog]; };
+    auto block_at = [&](int blk, int page, int64_t stride) {
+      const bool in = (unsigned)page < (unsigned)bt.pages;
+      bad |= !in;
+      return (int64_t)(in ? page : 0) * stride + (int64_t)(min(max(blk, blo), bhi) & bmask) * 16 * D;
+    };
+    u32x4 kf[NT][NS], vf[ND];
+    auto load_k = [&](int u, int pg0, int pg1) {
+      // Tile t, row c of the products is key C (c / 4) + 4 t + c % 4 of the unit.
+      const T* base = kp + block_at(u * (KU / 16), pg0, a.k_page);
+      if constexpr (KU == 32) {
+        const T* other = kp + block_at(u * 2 + 1, pg1, a.k_page);
+        base = c >= 8 ? other : base;
+      }
+      const T* at = base + (g * 16 + ((C * (c >> 2) + (c & 3)) & 15)) * C;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+          kf[t][k] = FULL || (4 * k + g) * C < D ? load_chunk(at + (64 * k + 4 * t) * C) : u32x4{0, 0, 0, 0};
+    };
+    auto load_v = [&](int u, int pg0, int pg1) {
+      const T* base = vp + block_at(u * (KU / 16), pg0, a.v_page);
+      if constexpr (KU == 32) {
+        const T* other = vp + block_at(u * 2 + 1, pg1, a.v_page);
+        base = g >= 2 ? other : base;
+      }
+      const T* at = base + ((KU == 32 ? g & 1 : g) * D + c) * C;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) vf[d] = FULL || 16 * d < D ? load_chunk(at + 16 * d * C) : u32x4{0, 0, 0, 0};
+    };
+    int u = u0 + w, pg0 = 0, pg1 = 0;
+    if (u < u1) {
+      pg0 = page_of(u * (KU / 16));
+      pg1 = KU == 32 ? page_of(u * 2 + 1) : pg0;
+      load_k(u, pg0, pg1);
+      load_v(u, pg0, pg1);
+    }
+
     // This lane's rows.
-    int p[MT], lo[MT], hi[MT];
+    int p[MT], lo[MT], span[MT];
     float slope[MT];
     u32x4 qf[MT][NS];
 #pragma unroll
@@ -137,68 +237,28 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
       p[m] = s.L - s.n + i;
       const RowRange rr = row_range(a, s, p[m], prefix);
       lo[m] = rr.lo;
-      hi[m] = rr.hi;
+      span[m] = max(rr.hi - rr.lo, 0);
       slope[m] = BENT && a.slopes ? a.slopes[qh] : 0.0f;
       const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
 #pragma unroll
-      for (int k = 0; k < NS; ++k) {
-        const int ch = 4 * k + g;
-        qf[m][k] = ch * C < a.D ? load_chunk(q + ch * C) : u32x4{0, 0, 0, 0};
-      }
+      for (int k = 0; k < NS; ++k) qf[m][k] = FULL || (4 * k + g) * C < D ? load_chunk(q + (4 * k + g) * C) : u32x4{0, 0, 0, 0};
     }
     f32x4 o[MT][ND];
-    float mx[MT], sum[MT];
+    float ref[MT], sum[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      mx[m] = -INFINITY;
+      ref[m] = -INFINITY;
       sum[m] = 0.0f;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[m][d] = f32x4{0, 0, 0, 0};
     }
+    const float cs = BENT ? 1.0f : a.scale;
 
-    // A unit's block of 16 keys: its page, and the block's offset in it.  Blocks that no row sees are
-    // never looked up: their entries may name nothing.
-    auto page_of = [&](int blk) { return table[min(max(blk, blo), bhi) >> blog]; };
-    auto block_at = [&](int blk, int page, int64_t stride) {
-      const int in = min(max(blk, blo), bhi) & bmask;
-      return (int64_t)((unsigned)page < (unsigned)bt.pages ? page : 0) * stride + (int64_t)in * 16 * a.D;
-    };
-    u32x4 kf[NT][NS], vf[ND];
-    auto load_k = [&](int u, int pg0, int pg1) {
-      // Tile t, row c of the products is key C (c / 4) + 4 t + c % 4 of the unit.
-      const T* base = kp + block_at(u * (KU / 16), pg0, a.k_page);
-      if (KU == 32 && c >= 8) base = kp + block_at(u * 2 + 1, pg1, a.k_page);
-      const int key = (C * (c >> 2) + (c & 3)) & 15;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int k = 0; k < NS; ++k) {
-          const int ch = 4 * k + g;
-          kf[t][k] = ch * C < a.D ? load_chunk(base + (ch * 16 + key + 4 * t) * C) : u32x4{0, 0, 0, 0};
-        }
-    };
-    auto load_v = [&](int u, int pg0, int pg1) {
-      const T* base = vp + block_at(u * (KU / 16), pg0, a.v_page);
-      if (KU == 32 && g >= 2) base = vp + block_at(u * 2 + 1, pg1, a.v_page);
-      const int grp = KU == 32 ? g & 1 : g;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-        vf[d] = 16 * d < a.D ? load_chunk(base + (grp * a.D + 16 * d + c) * C) : u32x4{0, 0, 0, 0};
-    };
-
-    int u = u0 + w, pg0 = 0, pg1 = 0;
-    if (u < u1) {
-      pg0 = page_of(u * (KU / 16));
-      pg1 = KU == 32 ? page_of(u * 2 + 1) : pg0;
-      load_k(u, pg0, pg1);
-      load_v(u, pg0, pg1);
-    }
     for (; u < u1; u += NW) {
       const bool more = u + NW < u1;
-      int nx0 = 0, nx1 = 0;
       if (more) {
-        nx0 = page_of((u + NW) * (KU / 16));
-        nx1 = KU == 32 ? page_of((u + NW) * 2 + 1) : nx0;
+        pg0 = page_of((u + NW) * (KU / 16));
+        pg1 = KU == 32 ? page_of((u + NW) * 2 + 1) : pg0;
       }
       f32x4 st[MT][NT];
 #pragma unroll
@@ -209,10 +269,9 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
 #pragma unroll
           for (int k = 0; k < NS; ++k) st[m][t] = mma16<T>(kf[t][k], qf[m][k], st[m][t]);
         }
-      if (more) load_k(u + NW, nx0, nx1);
+      if (more) load_k(u + NW, pg0, pg1);
       const int key0 = u * KU + C * g;
-      const bool bad = (unsigned)pg0 >= (unsigned)bt.pages || (unsigned)pg1 >= (unsigned)bt.pages;
-      const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all || bad;
+      const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all;
       if (BENT || part) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -223,17 +282,11 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
               const int j = key0 + 4 * t + i;
               float v = st[m][t][i];
               if constexpr (BENT) v = bent_score<T>(a, v, slope[m], p[m], j);
-              if (part) {
-                if (bad && (unsigned)(j & 16 ? pg1 : pg0) >= (unsigned)bt.pages) v = __builtin_nanf("");
-                v = j >= lo[m] && j < hi[m] ? v : -INFINITY;
-              }
+              if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
               st[m][t][i] = v;
             }
       }
-      const float cs = BENT ? 1.0f : a.scale;
       u32x4 pf[MT];
-      bool moved = false;
-      float alpha[MT], e[MT][C];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float v = st[m][0][0];
@@ -241,74 +294,59 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) v = fmaxf(v, st[m][t][i]);
-        const float now = fmaxf(mx[m], group_max(v));
-        const float ref = now == -INFINITY ? 0.0f : now * cs;
-        alpha[m] = __builtin_amdgcn_exp2f(fmaf(mx[m], cs, -ref));
-        moved |= now != mx[m];
-        mx[m] = now;
-        float add = 0.0f;
+        v = group_max(v) * cs;
+        const bool up = v > ref[m] + kSlack;
+        if (__any(up)) {
+          const float now = up ? v : ref[m];
+          const float alpha = up ? __builtin_amdgcn_exp2f(ref[m] - now) : 1.0f;
+          ref[m] = now;
+          sum[m] *= alpha;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int d = 0; d < ND; ++d) o[m][d] *= alpha;
+        }
+        const float neg = ref[m] == -INFINITY ? 0.0f : -ref[m];  // nothing seen yet: all weights are exp2(-inf)
+        float e[C], add = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e[m][4 * t + i] = __builtin_amdgcn_exp2f(fmaf(st[m][t][i], cs, -ref));
-            add += e[m][4 * t + i];
-          }
-        sum[m] = fmaf(sum[m], alpha[m], add);
-        // 16-bit types: the softmax weights, at most 1, are rounded to the type for the product with the
-        // values (their f32 sum is not): 2^-9 of each weight in bf16, as the values themselves carry.
-        pf[m] = pack_chunk<T>(e[m]);
+        for (int i = 0; i < C; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(fmaf(st[m][i / 4][i % 4], cs, neg));
+          add += e[i];
+        }
+        sum[m] += add;
+        // 16-bit types: the softmax weights are rounded to the type for the product with the values (their
+        // f32 sum is not): half a unit in the last place of each weight, as the values themselves carry.
+        pf[m] = pack_chunk<T>(e);
       }
-      if (__any(moved)) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[m][d] *= alpha[m];
-      }
-      bool rare = false;
       if (part) {
-        // 0 * infinity: a hidden key's value must not meet its weight of zero in the matrix product.
         uint32_t nf = 0;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) nf |= not_finite<T>(vf[d]);
-        rare = __any(nf != 0);
-      }
-      if (!rare) {
+        for (int d = 0; d < ND; ++d) nf |= ~(finite_mask<T>(vf[d][0]) & finite_mask<T>(vf[d][1]) & finite_mask<T>(vf[d][2]) & finite_mask<T>(vf[d][3]));
+        if (__any(nf != 0)) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+          for (int d = 0; d < ND; ++d) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(vf[d], pf[m], o[m][d]);
-      } else {
-        for (int k = 0; k < KU; ++k) {
-          const int blk = u * (KU / 16) + (k >> 4), el = k % C;
-          const T* v = vp + block_at(blk, k >= 16 ? pg1 : pg0, a.v_page) + (k % 16 / C) * a.D * C + el;
+            for (int m = 0; m < MT; ++m) {
+              const f32x4 x = mma16<T>(each<T>(vf[d], value_code<T>), each<T>(pf[m], weight_code<T>), f32x4{0, 0, 0, 0});
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            float pk = 0.0f;
-#pragma unroll
-            for (int i = 0; i < C; ++i) pk = el == i ? e[m][i] : pk;
-            pk = __shfl(pk, k / C * 16 + c);
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (16 * d < a.D && pk != 0.0f) o[m][d][i] += pk * Act<T>::ld(v, (16 * d + 4 * g + i) * C);
+              for (int i = 0; i < 4; ++i) o[m][d][i] += decoded(x[i]);
+            }
+            vf[d] &= each<T>(vf[d], finite_mask<T>);
           }
         }
       }
-      if (more) load_v(u + NW, nx0, nx1);
-      pg0 = nx0;
-      pg1 = nx1;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(vf[d], pf[m], o[m][d]);
+      if (more) load_v(u + NW, pg0, pg1);
     }
 
     // Join the waves: maxima and sums first, then the results OD features at a time.
-    const float cs = BENT ? 1.0f : a.scale;
-    __syncthreads();  // the last tile's reads of LDS
+    if (any_wave<NW>(bad, flags)) poison(bt, table, max(u0 * KU, kr.lo), min(u1 * KU, kr.hi), lo, span, sum);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const float t = group_sum(sum[m]);
       if (g == 0) {
-        lm[w][m * 16 + c] = mx[m] * cs;
+        lm[w][m * 16 + c] = ref[m];
         ll[w][m * 16 + c] = t;
       }
     }
@@ -318,14 +356,13 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NW; ++i) top = fmaxf(top, lm[i][m * 16 + c]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      const float f = __builtin_amdgcn_exp2f(mx[m] * cs - ref);
+      const float f = __builtin_amdgcn_exp2f(ref[m] - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[m][d] *= f;
     }
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += OD / 16) {
-      if (16 * d0 >= a.D) break;
+      if (16 * d0 >= D) break;
       if (d0) __syncthreads();
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -335,7 +372,7 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
       __syncthreads();
       for (int i = tid; i < TM * (OD / 4); i += 64 * NW) {
         const int rr = i / (OD / 4), d = (i - rr * (OD / 4)) * 4, r = row0 + rr;
-        if (r > row1 || 16 * d0 + d >= a.D) continue;
+        if (r > row1 || 16 * d0 + d >= D) continue;
         f32x4 v = {0, 0, 0, 0};
         float top = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -343,19 +380,19 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
           v += *reinterpret_cast<const f32x4*>(&lo_[k][rr][d]);
           top = fmaxf(top, lm[k][rr]);
         }
-        const float ref = top == -INFINITY ? 0.0f : top;
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) l += ll[k][rr] * __builtin_amdgcn_exp2f(lm[k][rr] - ref);
+        for (int k = 0; k < NW; ++k) l += ll[k][rr] * __builtin_amdgcn_exp2f(lm[k][rr] - base);
         const int tok = r / a.G, qh = h * a.G + (r - tok * a.G);
         const int64_t orow = (int64_t)(s.q0 + tok) * a.Hkv * a.G + qh;
         if (ns > 1) {
-          *reinterpret_cast<f32x4*>(a.part + (orow * a.S + z) * a.D + 16 * d0 + d) = v;
+          *reinterpret_cast<f32x4*>(a.part + (orow * a.S + z) * D + 16 * d0 + d) = v;
           if (d0 == 0 && d == 0) {
             *reinterpret_cast<f32x2*>(a.ml + (orow * a.S + z) * 2) = f32x2{top, l};
             if (z == 0) a.splits[orow] = ns;
           }
         } else {
-          if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * kLog2e - ref);
+          if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * kLog2e - base);
           if (a.S > 1 && d0 == 0 && d == 0) a.splits[orow] = 1;
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           T* y = (T*)a.out.p + (s.q0 + tok) * a.out.ts + qh * a.out.hs + 16 * d0 + d;
@@ -364,15 +401,20 @@ __global__ __launch_bounds__(256) void attn_stream_kernel(AttnArgs a) {
         }
       }
     }
+    if (tile + 1 < last) __syncthreads();
   }
 }
 
+template <typename T, int DT, int MT, bool FULL>
+static int launch_stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
+  const dim3 grid((unsigned)(a.Hkv * plan.units), (unsigned)a.S);
+  if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, true, FULL>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, false, FULL>), grid, dim3(256), 0, st, a);
+  return check_launch("paged_attention");
+}
 template <typename T, int DT, int MT>
 static int launch_stream(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-  const dim3 grid((unsigned)(a.Hkv * plan.units), (unsigned)a.S);
-  if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, false>), grid, dim3(256), 0, st, a);
-  return check_launch("paged_attention");
+  return a.D == DT ? launch_stream_of<T, DT, MT, true>(a, plan, st) : launch_stream_of<T, DT, MT, false>(a, plan, st);
 }
 
 template <typename T>

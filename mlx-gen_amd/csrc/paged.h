@@ -159,8 +159,8 @@ int run_copy_pages(void* cache, int64_t planes, int64_t plane_stride, int64_t pa
 // How an attention call is cut up: rows of a workgroup's tile, splits of the tokens, and the units of
 // find_unit (or sequences, when direct) that the grid covers.
 struct AttnPlan {
-  int rows = 16, waves = 4, S = 1, chunk = 0;
-  bool direct = true;
+  int rows = 16, S = 1, chunk = 0;
+  bool tiled = false, direct = true;
   int64_t units = 0;
   size_t ml = 0, splits = 0, total = 0;  // workspace: byte offsets of ml and splits, and its size
 };
@@ -171,5 +171,8 @@ int run_attention(const AttnArgs& a, int dtype, const AttnPlan& plan, hipStream_
 int run_attn_stream_bf16(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
 int run_attn_stream_f16(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
 int run_attn_stream_f32(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
+// The instances of the tiled kernel.
+int run_attn_tile_bf16(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
+int run_attn_tile_f16(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
 
 }  // namespace mlxq
