@@ -296,16 +296,31 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
     }
   };
 
-  for (int t = t0; t < t1; ++t) {
+  // Tiles [ta, tb) are seen whole by every row; those before (a window's start) and after (the diagonal) are not.
+  // One loop each, run twice, so that the long one has no branch but the rescaling.
+  int ta = min(max((kr.lo_all + KT - 1) / KT, t0), t1);
+  const int tz = max(min(kr.hi_all / KT, t1), ta);
+  auto arrive = [&](int t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (t + 1 < t1) {
       dma(t + 1);
       pages(min(t + 2, t1 - 1));
     }
-    if (t * KT >= wk.hi || (t + 1) * KT <= wk.lo) continue;
-    if (t * KT < wk.lo_all || (t + 1) * KT > wk.hi_all) step(t, BoolConstant<true>{});
-    else step(t, BoolConstant<false>{});
+  };
+#pragma unroll 1
+  for (int t = t0; t < t1;) {
+#pragma unroll 1
+    for (; t < ta; ++t) {
+      arrive(t);
+      if (t * KT < wk.hi && (t + 1) * KT > wk.lo) step(t, BoolConstant<true>{});
+    }
+    ta = t1;
+#pragma unroll 1
+    for (; t < tz; ++t) {
+      arrive(t);
+      if (wr0 <= row1) step(t, BoolConstant<false>{});
+    }
   }
 
   __syncthreads();
