@@ -5,31 +5,46 @@
 
 namespace mlxq {
 
-// One row's splits, joined: thread (row, 4 features).  The splits' sums are relative to their own
-// maxima; each is weighted by exp2 of its maximum less the largest, in the order of the splits.
+// One row's splits, joined by a workgroup.  The splits' sums are relative to their own maxima; each is weighted by
+// exp2 of its maximum less the largest.  A thread takes 4 features of every (256 / (D / 4))-th split, so that a
+// long sequence's splits are in flight together; the threads' sums are added in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq, int64_t total) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= total) return;
-  const int per = a.D / 4;
-  const int64_t row = id / per, t = row / Hq;
-  const int d = (int)(id - row * per) * 4, qh = (int)(row - t * Hq);
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq) {
+  __shared__ float weight[kMaxSplits], top_of[4], sum_of[4];
+  __shared__ f32x4 add[256];
+  const int tid = threadIdx.x, t = blockIdx.x / Hq, qh = blockIdx.x - t * Hq;
   const int from = min(max(a.batch.q_starts[0], 0), a.batch.T), to = min(a.batch.q_starts[a.batch.B], a.batch.T);
   if (t < from || t >= to) return;
+  const int64_t row = blockIdx.x;
   const int ns = min(a.splits[row], a.S);
   if (ns <= 1) return;  // written by its one split
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml) + row * a.S;
-  float top = -INFINITY;
-  for (int k = 0; k < ns; ++k) top = fmaxf(top, ml[k][0]);
-  const float ref = top == -INFINITY ? 0.0f : top;
+  f32x2 e = {-INFINITY, 0.0f};
+  if (tid < ns) e = reinterpret_cast<const f32x2*>(a.ml)[row * a.S + tid];
+  float top = e[0];
+#pragma unroll
+  for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+  if ((tid & 63) == 0) top_of[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+  const float ref = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(e[0] - ref);
+  float l = e[1] * f;
+  weight[tid] = f;
+#pragma unroll
+  for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+  if ((tid & 63) == 0) sum_of[tid >> 6] = l;
+  __syncthreads();
+  const int per = a.D / 4, groups = 256 / per, gi = tid / per, d = (tid - gi * per) * 4;
   f32x4 v = {0, 0, 0, 0};
-  float l = 0.0f;
-  for (int k = 0; k < ns; ++k) {
-    const f32x2 e = ml[k];
-    const float f = __builtin_amdgcn_exp2f(e[0] - ref);
-    l += e[1] * f;
-    v += *reinterpret_cast<const f32x4*>(a.part + (row * a.S + k) * a.D + d) * f;
+  if (gi < groups) {
+    const float* p = a.part + row * a.S * a.D + d;
+#pragma unroll 4
+    for (int k = gi; k < ns; k += groups) v += *reinterpret_cast<const f32x4*>(p + (int64_t)k * a.D) * weight[k];
   }
+  add[tid] = v;
+  __syncthreads();
+  if (tid >= per) return;
+  for (int k = 1; k < groups; ++k) v += add[k * per + tid];
+  l = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
   if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * 1.44269504088896341f - ref);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T* y = (T*)a.out.p + t * a.out.ts + qh * a.out.hs + d;
@@ -45,18 +60,20 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   p.rows = most <= 16 || D > 128 ? 16 : 32;
   p.tiled = dtype != MLXQ_FLOAT32 && most > p.rows;
   if (p.tiled) p.rows = 128;
+  // Tiles of rows: at most one for every p.rows rows and a part one for every sequence.
+  const int64_t tiles = T * G / p.rows + std::min(B, T);
   p.direct = !p.tiled && most <= p.rows;
-  p.units = p.direct ? B : T * G / p.rows + B;
-  // Splits: enough workgroups of four waves for two (tiled) or three on every CU, at least 256 tokens each.
+  // Splits: enough workgroups of four waves for two (tiled) or three on every CU, of at least 128 tokens (a
+  // unit for each wave: one token over 777, 8 heads: 9.5 us; 256: 10.1, one split: 10.3) or 256 (tiled).  One row tile a
+  // sequence: of at most 1024, since the sequences of a step are of unequal length (48 of up to 6000: 25.9 us; 4096: 39.3).
   int64_t range = max_kv;
   if (window) range = std::min(range, window + max_q);
-  const int64_t busy = std::min<int64_t>(p.units, T * G / p.rows + std::min(B, T)) * Hkv;
-  const int64_t want = std::max<int64_t>(1, (p.tiled ? 2 : 3) * cus / std::max<int64_t>(busy, 1));
-  int64_t chunk = std::max<int64_t>(256, (range + want - 1) / want);
-  chunk = std::max<int64_t>((chunk + 127) / 128 * 128, ((range + 255) / 256 + 127) / 128 * 128);
-  chunk = std::min<int64_t>(chunk, 0x40000000);
-  p.chunk = (int)chunk;
-  p.S = (int)std::max<int64_t>(1, (range + chunk - 1) / chunk);
+  const int64_t want = std::max<int64_t>(1, (p.tiled ? 2 : 3) * cus / std::max<int64_t>(tiles * Hkv, 1));
+  p.chunk_log2 = p.tiled ? 8 : 7;
+  while ((want << p.chunk_log2) < range && !(p.direct && p.chunk_log2 == 10)) ++p.chunk_log2;
+  while (((int64_t)kMaxSplits << p.chunk_log2) < range) ++p.chunk_log2;
+  p.S = (int)std::max<int64_t>(1, (range + (1 << p.chunk_log2) - 1) >> p.chunk_log2);
+  p.blocks = (p.direct ? B * p.S : p.tiled ? tiles : tiles * p.S) * Hkv;
   if (p.S > 1) {
     auto align = [](size_t b) { return (b + 255) / 256 * 256; };
     const size_t rows = (size_t)(T * Hq);
@@ -69,9 +86,9 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
 
 template <typename T>
 static int launch_join(const AttnArgs& a, hipStream_t st) {
-  const int64_t total = (int64_t)a.batch.T * a.Hkv * a.G * (a.D / 4), blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "paged_attention: problem too large");
-  hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, st, a, a.Hkv * a.G, total);
+  const int64_t rows = (int64_t)a.batch.T * a.Hkv * a.G;
+  if (rows > 0x7fffffff) return set_error(MLXQ_EINVAL, "paged_attention: problem too large");
+  hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, a, a.Hkv * a.G);
   return check_launch("paged_attention");
 }
 

@@ -8,11 +8,11 @@
 // split over workgroups, whose sums a second kernel joins.
 //
 // Scores are computed transposed, S^T = K Q^T, and so is the result, O^T = V^T P^T: the cache's layout
-// is the A operand of both products, 16 bytes a lane straight from memory, and a lane of S^T holds
-// scores of one row.  With lane = 16 g + c, the D operand of the 16x16 products puts rows 4 g + i in lane
-// (g, c) where the B operand of the next product wants keys C g + e: the 16 keys of S^T tile t are
-// therefore those with key % C / 4 == t, so that element 4 t + i of lane group g is key C g + 4 t + i and
-// the exponentials are the next product's operand as they stand.
+// is the A operand of both products, 16 bytes a lane and 1 KB a wave straight from memory, and a lane of S^T
+// holds scores of one row.  With lane = 16 g + c, the D operand of the 16x16 products puts rows 4 g + i
+// in lane (g, c): element i of tile t is key 16 t + 4 g + i.  f32 values arrive in that order.  16-bit values arrive
+// as 8 keys a lane, group g = 2 b + a those from 8 a on of block b; two exchanges between lane groups
+// (even_keys) turn two blocks into keys 4 g .. 4 g + 3 of either, the order of the weights.
 //
 // Bound by the cache's bytes for one token: no LDS and no barrier in the loop, and the next unit's keys
 // are requested as soon as this one's are used.
@@ -59,13 +59,21 @@ __device__ __forceinline__ float group_sum(float v) {
 // keys is hidden from some row, such values are taken out of the product (finite_mask) and, if there are any, added by a
 // second product of codes with indicators of the rows' non-zero weights: +inf counts 1, -inf 128, NaN both,
 // exact in all three types and, over at most 64 keys, in their sum.
+//
+// carries(): the sign bits of the result are those of the values (two to a word in 16-bit types) whose exponent bits
+// are all set, where adding one at the exponent's lowest bit carries.
+template <typename T>
+constexpr uint32_t kCarry = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+template <typename T>
+__device__ __forceinline__ uint32_t carries(uint32_t v) {
+  constexpr uint32_t mask = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+  return (v & mask) + one;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t finite_mask(uint32_t v) {
-  // All exponent bits set: adding one at the exponent's lowest bit carries into the sign bit.
-  if constexpr (sizeof(T) == 4) return (((v & 0x7f800000u) + 0x00800000u) >> 31) - 1u;
-  constexpr uint32_t mask = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
-  constexpr uint32_t one = __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
-  return ~(((((v & mask) + one) & 0x80008000u) >> 15) * 0xffffu);
+  const uint32_t t = carries<T>(v) & kCarry<T>;
+  return sizeof(T) == 4 ? (t >> 31) - 1u : ~((t >> 15) * 0xffffu);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t value_code(uint32_t v) {
@@ -148,41 +156,58 @@ struct KeyRange {
   int lo_all, hi_all;  // every row
 };
 __device__ __forceinline__ KeyRange key_range(const AttnArgs& a, const Seq& s, int row0, int row1, int prefix) {
-  const RowRange f = row_range(a, s, s.L - s.n + row0 / a.G, prefix), l = row_range(a, s, s.L - s.n + row1 / a.G, prefix);
+  const RowRange f = row_range(a, s, s.L - s.n + a.by_g.div(row0), prefix), l = row_range(a, s, s.L - s.n + a.by_g.div(row1), prefix);
   return {f.lo, l.hi, l.lo, f.hi};
+}
+
+// v: a lane group's 8 keys of a block, see above, becomes 4 keys of block 0 and 4 of block 1.  With x and y the
+// halves of v by lane group, x = (x0, x1, x2, x3): rows 1 and 3 of x change places with rows 0 and 2 of y, then the upper
+// half of x with the lower half of y, which leaves x = (x0, y0, x1, y1) and y = (x2, y2, x3, y3).
+__device__ __forceinline__ u32x4 even_keys(u32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    auto a = __builtin_amdgcn_permlane16_swap(v[i], v[2 + i], false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(a[0], a[1], false, false);
+    v[i] = b[0];
+    v[2 + i] = b[1];
+  }
+  return v;
 }
 
 // FULL: head_dim is DT, else below it and the rest of DT is zeros.
 template <typename T, int DT, int MT, bool BENT, bool FULL>
-__global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) void attn_stream_kernel(AttnArgs a) {
   constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
-  constexpr int OD = 32, OROW = OD + 4;  // features of a step of the join, and its padded LDS row
+  constexpr int JD = DT * MT < 256 ? DT : DT / 2;  // features joined at a time: all that 64 KB hold
   __shared__ float lm[NW][TM], ll[NW][TM];
   __shared__ int flags[NW];
-  __shared__ __align__(16) float lo_[NW][TM][OROW];
+  __shared__ __align__(16) float lo_[NW][TM][JD + 4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, c = lane & 15, unit = blockIdx.x / a.Hkv, h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
+  const int g = lane >> 4, c = lane & 15;
+  // Workgroups go round the chip's eight dies in order of their number: the (tile, head) items of a split come
+  // together, each split's turned by one, so that a long sequence's splits fall on all dies.
+  const int z = a.by_items.div(blockIdx.x), turn = blockIdx.x - z * a.items + (z - a.by_items.div(z) * a.items);
+  const int item = turn < a.items ? turn : turn - a.items, unit = a.by_hkv.div(item), h = item - unit * a.Hkv;
   const Batch& bt = a.batch;
   const int D = FULL ? DT : a.D;
+  const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1, cu_log2 = a.chunk_log2 - (KU == 32 ? 5 : 4);  // blocks of a page, units of a split
   auto tiles_of = [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; };
   int b = unit, first = 0;
-  if (!a.direct) find_unit(bt, unit, tiles_of, b, first);
-  if (b < 0) return;
+  if (!a.direct && !Finder(bt, tiles_of).find(unit, b, first)) return;
   const Seq s = load_seq(bt, b);
   const int rows = s.n * a.G, prefix = a.prefix ? a.prefix[b] : 0;
   const int last = a.direct ? tiles_of(s) : first + 1;
   const int32_t* table = bt.tables + b * bt.table_stride;
-  const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1;  // blocks of a page
   const int64_t head = ((int64_t)h << bt.page_log2) * D;
   const T *kp = (const T*)a.k + head, *vp = (const T*)a.v + head;
 
   for (int tile = first; tile < last; ++tile) {
     const int row0 = tile * TM, row1 = min(rows, row0 + TM) - 1;
     const KeyRange kr = key_range(a, s, row0, row1, prefix);
-    const int ub = kr.lo / KU, ue = kr.hi > kr.lo ? (kr.hi + KU - 1) / KU : ub, cu = a.chunk / KU;
-    const int ns = max(1, min(a.S, (ue - ub + cu - 1) / cu));
+    const int ub = kr.lo / KU, ue = kr.hi > kr.lo ? (kr.hi + KU - 1) / KU : ub;
+    const int ns = max(1, min(a.S, (ue - ub + (1 << cu_log2) - 1) >> cu_log2));
     if (z >= ns) continue;
-    const int u0 = ub + z * cu, u1 = z == a.S - 1 ? ue : min(ue, u0 + cu);
+    const int u0 = ub + (z << cu_log2), u1 = z == a.S - 1 ? ue : min(ue, u0 + (1 << cu_log2));
     const int blo = kr.lo >> 4, bhi = (kr.hi - 1) >> 4;  // blocks with keys that are seen
 
     // A unit's blocks of 16 keys: their pages, and the blocks' first elements.  Blocks that no row sees are
@@ -196,18 +221,13 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
     };
     u32x4 kf[NT][NS], vf[ND];
     auto load_k = [&](int u, int pg0, int pg1) {
-      // Tile t, row c of the products is key C (c / 4) + 4 t + c % 4 of the unit.
-      const T* base = kp + block_at(u * (KU / 16), pg0, a.k_page);
-      if constexpr (KU == 32) {
-        const T* other = kp + block_at(u * 2 + 1, pg1, a.k_page);
-        base = c >= 8 ? other : base;
-      }
-      const T* at = base + (g * 16 + ((C * (c >> 2) + (c & 3)) & 15)) * C;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        const T* at = kp + block_at(u * NT + t, t ? pg1 : pg0, a.k_page) + lane * C;
 #pragma unroll
         for (int k = 0; k < NS; ++k)
-          kf[t][k] = FULL || (4 * k + g) * C < D ? load_chunk(at + (64 * k + 4 * t) * C) : u32x4{0, 0, 0, 0};
+          kf[t][k] = FULL || (4 * k + g) * C < D ? load_chunk(at + 64 * k * C) : u32x4{0, 0, 0, 0};
+      }
     };
     auto load_v = [&](int u, int pg0, int pg1) {
       const T* base = vp + block_at(u * (KU / 16), pg0, a.v_page);
@@ -233,7 +253,7 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
     u32x4 qf[MT][NS];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = min(row0 + m * 16 + c, row1), i = r / a.G, qh = h * a.G + (r - i * a.G);
+      const int r = min(row0 + m * 16 + c, row1), i = a.by_g.div(r), qh = h * a.G + (r - i * a.G);
       p[m] = s.L - s.n + i;
       const RowRange rr = row_range(a, s, p[m], prefix);
       lo[m] = rr.lo;
@@ -270,7 +290,7 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
           for (int k = 0; k < NS; ++k) st[m][t] = mma16<T>(kf[t][k], qf[m][k], st[m][t]);
         }
       if (more) load_k(u + NW, pg0, pg1);
-      const int key0 = u * KU + C * g;
+      const int key0 = u * KU + 4 * g;
       const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all;
       if (BENT || part) {
 #pragma unroll
@@ -279,7 +299,7 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int j = key0 + 4 * t + i;
+              const int j = key0 + 16 * t + i;
               float v = st[m][t][i];
               if constexpr (BENT) v = bent_score<T>(a, v, slope[m], p[m], j);
               if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
@@ -316,11 +336,15 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
         // f32 sum is not): half a unit in the last place of each weight, as the values themselves carry.
         pf[m] = pack_chunk<T>(e);
       }
+      if constexpr (KU == 32) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) vf[d] = even_keys(vf[d]);
+      }
       if (part) {
         uint32_t nf = 0;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) nf |= ~(finite_mask<T>(vf[d][0]) & finite_mask<T>(vf[d][1]) & finite_mask<T>(vf[d][2]) & finite_mask<T>(vf[d][3]));
-        if (__any(nf != 0)) {
+        for (int d = 0; d < ND; ++d) nf |= carries<T>(vf[d][0]) | carries<T>(vf[d][1]) | carries<T>(vf[d][2]) | carries<T>(vf[d][3]);
+        if (__builtin_expect(__any((nf & kCarry<T>) != 0), 0)) {
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
 #pragma unroll
@@ -340,7 +364,7 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
       if (more) load_v(u + NW, pg0, pg1);
     }
 
-    // Join the waves: maxima and sums first, then the results OD features at a time.
+    // Join the waves: maxima and sums first, then the results.
     if (any_wave<NW>(bad, flags)) poison(bt, table, max(u0 * KU, kr.lo), min(u1 * KU, kr.hi), lo, span, sum);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -361,41 +385,37 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
       for (int d = 0; d < ND; ++d) o[m][d] *= f;
     }
 #pragma unroll
-    for (int d0 = 0; d0 < ND; d0 += OD / 16) {
-      if (16 * d0 >= D) break;
-      if (d0) __syncthreads();
+    for (int j0 = 0; j0 < DT; j0 += JD) {
+      if (j0) __syncthreads();
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int d = 0; d < OD / 16; ++d)
-          *reinterpret_cast<f32x4*>(&lo_[w][m * 16 + c][16 * d + 4 * g]) = o[m][d0 + d];
+        for (int d = 0; d < JD / 16; ++d) *reinterpret_cast<f32x4*>(&lo_[w][m * 16 + c][16 * d + 4 * g]) = o[m][j0 / 16 + d];
       __syncthreads();
-      for (int i = tid; i < TM * (OD / 4); i += 64 * NW) {
-        const int rr = i / (OD / 4), d = (i - rr * (OD / 4)) * 4, r = row0 + rr;
-        if (r > row1 || 16 * d0 + d >= D) continue;
+#pragma unroll 1
+      for (int i = tid; i < TM * (JD / 4); i += 64 * NW) {
+        const int rr = i / (JD / 4), dj = (i - rr * (JD / 4)) * 4, d = j0 + dj, r = row0 + rr;
+        if (r > row1 || d >= D) continue;
         f32x4 v = {0, 0, 0, 0};
         float top = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-          v += *reinterpret_cast<const f32x4*>(&lo_[k][rr][d]);
+          v += *reinterpret_cast<const f32x4*>(&lo_[k][rr][dj]);
           top = fmaxf(top, lm[k][rr]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int k = 0; k < NW; ++k) l += ll[k][rr] * __builtin_amdgcn_exp2f(lm[k][rr] - base);
-        const int tok = r / a.G, qh = h * a.G + (r - tok * a.G);
+        const int tok = a.by_g.div(r), qh = h * a.G + (r - tok * a.G);
         const int64_t orow = (int64_t)(s.q0 + tok) * a.Hkv * a.G + qh;
+        if (a.S > 1 && z == 0 && d == 0) a.splits[orow] = ns;
         if (ns > 1) {
-          *reinterpret_cast<f32x4*>(a.part + (orow * a.S + z) * D + 16 * d0 + d) = v;
-          if (d0 == 0 && d == 0) {
-            *reinterpret_cast<f32x2*>(a.ml + (orow * a.S + z) * 2) = f32x2{top, l};
-            if (z == 0) a.splits[orow] = ns;
-          }
+          *reinterpret_cast<f32x4*>(a.part + (orow * a.S + z) * D + d) = v;
+          if (d == 0) *reinterpret_cast<f32x2*>(a.ml + (orow * a.S + z) * 2) = f32x2{top, l};
         } else {
           if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * kLog2e - base);
-          if (a.S > 1 && d0 == 0 && d == 0) a.splits[orow] = 1;
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          T* y = (T*)a.out.p + (s.q0 + tok) * a.out.ts + qh * a.out.hs + 16 * d0 + d;
+          T* y = (T*)a.out.p + (s.q0 + tok) * a.out.ts + qh * a.out.hs + d;
           if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(y) = v * inv;
           else *reinterpret_cast<u32x2*>(y) = u32x2{Elem<T>::pack2(v[0] * inv, v[1] * inv), Elem<T>::pack2(v[2] * inv, v[3] * inv)};
         }
@@ -407,7 +427,7 @@ __global__ __launch_bounds__(256, DT * MT <= 128 ? 2 : 1) void attn_stream_kerne
 
 template <typename T, int DT, int MT, bool FULL>
 static int launch_stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-  const dim3 grid((unsigned)(a.Hkv * plan.units), (unsigned)a.S);
+  const dim3 grid((unsigned)plan.blocks);
   if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, true, FULL>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, false, FULL>), grid, dim3(256), 0, st, a);
   return check_launch("paged_attention");

@@ -72,18 +72,17 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
   __shared__ __align__(1024) unsigned char lds[2 * BUF];  // the only LDS, from its start: M0 addresses 64 KB
   static_assert(sizeof(lds) <= 65536, "M0");
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int half = lane >> 5, c = lane & 31, unit = blockIdx.x / a.Hkv, h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
+  const int half = lane >> 5, c = lane & 31, unit = a.by_hkv.div(blockIdx.x), h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
   const Batch& bt = a.batch;
   int b, at;
-  find_unit(bt, unit, [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; }, b, at);
-  if (b < 0) return;
+  if (!Finder(bt, [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; }).find(unit, b, at)) return;
   const Seq s = load_seq(bt, b);
   const int rows = s.n * a.G, prefix = a.prefix ? a.prefix[b] : 0;
   const int row0 = ((rows + TM - 1) / TM - 1 - at) * TM;  // the longest first
   const int row1 = min(rows, row0 + TM) - 1;
   const KeyRange kr = key_range(a, s, row0, row1, prefix);
-  const int tb = kr.lo / KT, te = kr.hi > kr.lo ? (kr.hi + KT - 1) / KT : tb, ct = a.chunk / KT;
-  const int ns = max(1, min(a.S, (te - tb + ct - 1) / ct));
+  const int tb = kr.lo / KT, te = kr.hi > kr.lo ? (kr.hi + KT - 1) / KT : tb;
+  const int ct = (1 << a.chunk_log2) / KT, ns = max(1, min(a.S, (te - tb + ct - 1) >> (a.chunk_log2 - (KT == 64 ? 6 : 5))));
   if (z >= ns) return;
   const int t0 = tb + z * ct, t1 = z == a.S - 1 ? te : min(te, t0 + ct);
   const int blo = kr.lo >> 4, bhi = (kr.hi - 1) >> 4;  // blocks with keys that are seen
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
   u32x4 qf[RW][NS];
 #pragma unroll
   for (int m = 0; m < RW; ++m) {
-    const int r = min(wr0 + m * 32 + c, row1), i = r / a.G, qh = h * a.G + (r - i * a.G);
+    const int r = min(wr0 + m * 32 + c, row1), i = a.by_g.div(r), qh = h * a.G + (r - i * a.G);
     p[m] = s.L - s.n + i;
     const RowRange rr = row_range(a, s, p[m], prefix);
     lo[m] = rr.lo;
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
     const int r = wr0 + m * 32 + c;
     float l = half_sum(sum[m]);
     if (r > row1) continue;
-    const int tok = r / a.G, qh = h * a.G + (r - tok * a.G);
+    const int tok = a.by_g.div(r), qh = h * a.G + (r - tok * a.G);
     const int64_t orow = (int64_t)(s.q0 + tok) * a.Hkv * a.G + qh;
     if (ns > 1) {
       float* y = a.part + (orow * a.S + z) * D;
@@ -365,7 +364,7 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
 
 template <typename T, int DT, int RW>
 static int launch_tile(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-  const dim3 grid((unsigned)(a.Hkv * plan.units), (unsigned)a.S);
+  const dim3 grid((unsigned)plan.blocks, (unsigned)a.S);
   if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, false>), grid, dim3(256), 0, st, a);
   return check_launch("paged_attention");

@@ -55,6 +55,22 @@ __device__ __forceinline__ void store_chunk(T* p, const u32x4& v) {
   *reinterpret_cast<u32x4*>(p) = v;
 }
 
+// n / d for 0 <= n < 2^31 by a product: m = ceil(2^(31 + l) / d) with l = ceil(log2 d) is off from 2^(31 + l) / d by less
+// than 1, so n m 2^-(31 + l) by less than 2^-l <= 1 / d.  A division by a runtime value is some twenty instructions,
+// and a short launch's time is, for a good part, the fetching of its instructions.
+struct Divisor {
+  uint32_t d = 1, mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(int64_t div) : d((uint32_t)div) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    if (l == 0) return;
+    mul = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ int div(int n) const { return mul ? (int)(__umulhi((uint32_t)n, mul) >> shift) : n; }
+};
+
 // [token][head][feature] view; strides in elements.
 struct Heads {
   const void* p;
@@ -85,34 +101,45 @@ __device__ __forceinline__ Seq load_seq(const Batch& a, int b) {
   return {s, e - s, min(max(L, 0), a.capacity)};
 }
 
-// Sequences cut into units (blocks of tokens, tiles of rows): finds the sequence of unit u and u's
-// place in it, b = -1 when there are fewer units.  count(seq) gives a sequence's units.  Every wave
-// of the workgroup runs it by itself, 64 sequences at a time: a lane counts one sequence, an
-// inclusive scan adds them up.
+// Sequences cut into units (blocks of tokens, tiles of rows, ranges of keys): finds the sequence of a unit and the
+// unit's place in it.  Every wave runs it by itself, 64 sequences at a time: a lane counts the units of one, an
+// inclusive scan adds them up.  Units are asked for in ascending order, and the scan goes on from where it is.
 template <typename F>
-__device__ __forceinline__ void find_unit(const Batch& a, int u, F count, int& b, int& at) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < a.B; base += 64) {
-    const int i = base + lane;
-    const int n = i < a.B ? count(load_seq(a, i)) : 0;
-    int sum = n;
+struct Finder {
+  const Batch& a;
+  F count;  // Seq -> its units
+  int base = 0, before = 0, n = 0, sum = 0;
+
+  __device__ __forceinline__ Finder(const Batch& batch, F f) : a(batch), count(f) { scan(); }
+  __device__ __forceinline__ void scan() {
+    const int lane = threadIdx.x & 63, i = base + lane;
+    n = i < a.B ? count(load_seq(a, i)) : 0;
+    sum = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int t = __shfl_up(sum, d);
       if (lane >= d) sum += t;
     }
-    const unsigned long long past = __ballot(sum > u);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      b = __builtin_amdgcn_readfirstlane(base + l);
-      at = __builtin_amdgcn_readfirstlane(u - (__shfl(sum, l) - __shfl(n, l)));
-      return;
-    }
-    u -= __builtin_amdgcn_readlane(sum, 63);
   }
-  b = -1;
-  at = 0;
-}
+  // False when there is no unit u.
+  __device__ __forceinline__ bool find(int u, int& b, int& at) {
+    while (true) {
+      const unsigned long long past = __ballot(sum > u - before);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = base + l;
+        at = u - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
+        return true;
+      }
+      if (base + 64 >= a.B) return false;
+      before += __builtin_amdgcn_readlane(sum, 63);
+      base += 64;
+      scan();
+    }
+  }
+};
+template <typename F>
+Finder(const Batch&, F) -> Finder<F>;
 
 struct RotaryArgs {
   const float* table;        // [rows, R/2, 2]; null: no rotation
@@ -127,7 +154,7 @@ struct AppendArgs {
   Batch batch;
   RotaryArgs rot;
   int Hkv, Hq, D;
-  int direct;  // unit u is the u-th sequence (each loops over its blocks); 0: find_unit
+  int direct;  // unit u is the u-th sequence (each loops over its blocks); 0: by Finder
 };
 
 struct AttnArgs {
@@ -136,10 +163,12 @@ struct AttnArgs {
   int64_t k_page, v_page;
   Batch batch;
   int Hkv, G, D;
-  int S, chunk;       // splits of a sequence's tokens, tokens in each (the last takes the rest)
+  Divisor by_hkv, by_g, by_items;  // by_items: (tile, head) pairs of the streaming kernel's grid
+  int items;
+  int S, chunk_log2;  // splits of a sequence's tokens, tokens in each (the last takes the rest)
   float scale;        // multiplies q.k into units of log 2 (MOD: into the score itself)
   float softcap;      // 0: none
-  int causal, window, direct;
+  int causal, window, direct;  // direct: item u is the u-th sequence, else by Finder
   const int32_t* prefix;
   const float *slopes, *sinks;
   float* part;  // [T * Hq, S, D] sums of each split, then their (maximum, sum) pairs and the counts of
@@ -156,12 +185,13 @@ int run_copy_pages(void* cache, int64_t planes, int64_t plane_stride, int64_t pa
                    int64_t page_stride, const int32_t* src, const int32_t* dst, int64_t count, int32_t* tables,
                    int64_t rows, int64_t width, int64_t table_stride, hipStream_t st);
 
-// How an attention call is cut up: rows of a workgroup's tile, splits of the tokens, and the units of
-// find_unit (or sequences, when direct) that the grid covers.
+constexpr int kMaxSplits = 256;  // the join gives each a thread
+
+// How an attention call is cut up: rows of a workgroup's tile, splits of the tokens, and the grid.
 struct AttnPlan {
-  int rows = 16, S = 1, chunk = 0;
-  bool tiled = false, direct = true;
-  int64_t units = 0;
+  int rows = 16, S = 1, chunk_log2 = 0;
+  bool tiled = false, direct = false;
+  int64_t blocks = 0;  // workgroups (tiled: times S)
   size_t ml = 0, splits = 0, total = 0;  // workspace: byte offsets of ml and splits, and its size
 };
 AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype, int64_t B, int64_t max_q,

@@ -291,7 +291,7 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
       return set_error(MLXQ_EINVAL, "%s: workspace of %zu bytes is smaller than the %zu required", op, workspace_bytes, plan.total);
     if ((rc = check_ptr(op, "workspace", workspace, 16))) return rc;
   }
-  if (plan.units * cache->heads > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
+  if (plan.blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   AttnArgs a = {};
   a.q = view(q);
   a.out = view(out);
@@ -304,7 +304,11 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   a.G = (int)(q->heads / cache->heads);
   a.D = (int)D;
   a.S = plan.S;
-  a.chunk = plan.chunk;
+  a.chunk_log2 = plan.chunk_log2;
+  a.items = plan.tiled ? (int)plan.blocks : (int)(plan.blocks / plan.S);
+  a.by_hkv = Divisor(a.Hkv);
+  a.by_g = Divisor(a.G);
+  a.by_items = Divisor(a.items);
   a.softcap = o->softcap;
   const bool bent = o->softcap > 0.0f || o->alibi_slopes;
   a.scale = bent ? o->scale : o->scale * 1.44269504088896341f;

@@ -197,8 +197,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Batch& bt = a.batch;
   auto blocks_of = [](const Seq& s) { return s.n == 0 ? 0 : ((s.L - 1) >> 4) - ((s.L - s.n) >> 4) + 1; };
   int b = unit, first = 0;
-  if (!a.direct) find_unit(bt, unit, blocks_of, b, first);
-  if (b < 0) return;
+  if (!a.direct && !Finder(bt, blocks_of).find(unit, b, first)) return;
   const Seq s = load_seq(bt, b);
   const int G = a.q.p ? a.Hq / a.Hkv : 0;
   const int units = rot_units<C>(MODE, a.rot.R, D);
