@@ -133,12 +133,21 @@ __device__ __forceinline__ void poison(const Batch& bt, const int32_t* table, in
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-// A score with its cap and bias, in units of log 2 (AttnArgs::scale is the caller's there).
-template <typename T>
-__device__ __forceinline__ float bent_score(const AttnArgs& a, float qk, float slope, int p, int j) {
+// What happens to a score before the softmax: nothing, a cap, or a bias by distance (capped before it if
+// softcap is set).
+enum Bend : int { kPlain = 0, kCap = 1, kBias = 2 };
+// A capped or biased score, in units of log 2, from q.k and the distance of key and row.  cap tanh(z / cap) is cap - 2 cap /
+// (exp(2 z / cap) + 1): in 16-bit types with the hardware's exponential and reciprocal, off by a few 2^-24 cap.
+// AttnArgs::scale is 2 scale / (cap ln 2) with a cap, scale / ln 2 without; cap2 is softcap / ln 2.
+template <typename T, int BEND>
+__device__ __forceinline__ float bent_score(const AttnArgs& a, float qk, float slope2, float distance) {
   float z = qk * a.scale;
-  if (a.softcap > 0.0f) z = a.softcap * (sizeof(T) == 4 ? tanhf(z / a.softcap) : tanh_hw(z / a.softcap));
-  return (z - slope * (float)abs(p - j)) * kLog2e;
+  if (BEND == kCap || a.softcap > 0.0f) {
+    if constexpr (sizeof(T) == 4) z = a.cap2 * tanhf(z * 0.34657359027997265f);  // ln 2 / 2
+    else z = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.0f), a.cap2);
+  }
+  if constexpr (BEND == kBias) z = fmaf(-slope2, fabsf(distance), z);
+  return z;
 }
 
 // The rows that a lane's row index stands for, and what they see.
@@ -175,7 +184,7 @@ __device__ __forceinline__ u32x4 even_keys(u32x4 v) {
 }
 
 // FULL: head_dim is DT, else below it and the rest of DT is zeros.
-template <typename T, int DT, int MT, bool BENT, bool FULL>
+template <typename T, int DT, int MT, int BEND, bool FULL>
 __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) void attn_stream_kernel(AttnArgs a) {
   constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
   constexpr int JD = DT * MT < 256 ? DT : DT / 2;  // features joined at a time: all that 64 KB hold
@@ -248,17 +257,18 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
     }
 
     // This lane's rows.
-    int p[MT], lo[MT], span[MT];
+    int place[MT], lo[MT], span[MT];
     float slope[MT];
     u32x4 qf[MT][NS];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = min(row0 + m * 16 + c, row1), i = a.by_g.div(r), qh = h * a.G + (r - i * a.G);
-      p[m] = s.L - s.n + i;
-      const RowRange rr = row_range(a, s, p[m], prefix);
+      const int p = s.L - s.n + i;
+      const RowRange rr = row_range(a, s, p, prefix);
+      place[m] = p;
       lo[m] = rr.lo;
       span[m] = max(rr.hi - rr.lo, 0);
-      slope[m] = BENT && a.slopes ? a.slopes[qh] : 0.0f;
+      slope[m] = BEND == kBias ? a.slopes[qh] * kLog2e : 0.0f;
       const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
 #pragma unroll
       for (int k = 0; k < NS; ++k) qf[m][k] = FULL || (4 * k + g) * C < D ? load_chunk(q + (4 * k + g) * C) : u32x4{0, 0, 0, 0};
@@ -272,7 +282,7 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[m][d] = f32x4{0, 0, 0, 0};
     }
-    const float cs = BENT ? 1.0f : a.scale;
+    const float cs = BEND != kPlain ? 1.0f : a.scale;
 
     for (; u < u1; u += NW) {
       const bool more = u + NW < u1;
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
       if (more) load_k(u + NW, pg0, pg1);
       const int key0 = u * KU + 4 * g;
       const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all;
-      if (BENT || part) {
+      if (BEND != kPlain || part) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -301,7 +311,7 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
             for (int i = 0; i < 4; ++i) {
               const int j = key0 + 16 * t + i;
               float v = st[m][t][i];
-              if constexpr (BENT) v = bent_score<T>(a, v, slope[m], p[m], j);
+              if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope[m], (float)(j - place[m]));
               if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
               st[m][t][i] = v;
             }
@@ -428,8 +438,9 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
 template <typename T, int DT, int MT, bool FULL>
 static int launch_stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
   const dim3 grid((unsigned)plan.blocks);
-  if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, true, FULL>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, false, FULL>), grid, dim3(256), 0, st, a);
+  if (a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kBias, FULL>), grid, dim3(256), 0, st, a);
+  else if (a.softcap > 0.0f) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kCap, FULL>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kPlain, FULL>), grid, dim3(256), 0, st, a);
   return check_launch("paged_attention");
 }
 template <typename T, int DT, int MT>

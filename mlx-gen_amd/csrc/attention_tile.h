@@ -59,13 +59,30 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Tells the scheduler to keep READ_AHEAD LDS reads in flight before the matrix products that use them, one more read
+// for each read used.  By itself it reads into one register quad and waits for each where registers are short.
+#ifndef READ_AHEAD
+#define READ_AHEAD 4
+#endif
+template <int READS, int PER>
+__device__ __forceinline__ void reads_ahead() {
+  constexpr int kMfma = 0x008, kDsRead = 0x100, AHEAD = READ_AHEAD < READS ? READ_AHEAD : READS;
+  __builtin_amdgcn_sched_group_barrier(kDsRead, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < READS - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, PER, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD * PER, 0);
+}
+
 template <bool B>
 struct BoolConstant {
   static constexpr bool value = B;
 };
 
-template <typename T, int DT, int RW, bool BENT>
-__global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
+template <typename T, int DT, int RW, int BEND>
+__global__ __launch_bounds__(256, RW == 1 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
   constexpr int C = 8, KT = DT <= 128 ? 64 : 32, NB = KT / 16, NK = KT / 32, NS = DT / 16, ND = DT / 32, TM = 128 * RW;
   constexpr int BLOCK = 16 * DT * 2;   // bytes of a block's keys (or values) in LDS, at most
   constexpr int BUF = 2 * NB * BLOCK;  // a tile: the blocks' keys, then their values
@@ -133,21 +150,27 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
   // Rows of this wave, their queries, and what the wave's rows see.
   const int wr0 = row0 + w * 32 * RW, wr1 = min(row1, wr0 + 32 * RW - 1);
   const KeyRange wk = wr0 > row1 ? KeyRange{0, 0, 0, 0} : key_range(a, s, wr0, wr1, prefix);
-  int p[RW], lo[RW], span[RW];
+  int place[RW], lo[RW], span[RW];
   float slope[RW];
   u32x4 qf[RW][NS];
 #pragma unroll
   for (int m = 0; m < RW; ++m) {
     const int r = min(wr0 + m * 32 + c, row1), i = a.by_g.div(r), qh = h * a.G + (r - i * a.G);
-    p[m] = s.L - s.n + i;
-    const RowRange rr = row_range(a, s, p[m], prefix);
+    const int p = s.L - s.n + i;
+    const RowRange rr = row_range(a, s, p, prefix);
+    place[m] = p;
     lo[m] = rr.lo;
     span[m] = max(rr.hi - rr.lo, 0);
-    slope[m] = BENT && a.slopes ? a.slopes[qh] : 0.0f;
+    slope[m] = BEND == kBias ? a.slopes[qh] * kLog2e : 0.0f;
     const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
 #pragma unroll
     for (int k = 0; k < NS; ++k) qf[m][k] = 16 * k < D ? load_chunk(q + (2 * k + half) * C) : u32x4{0, 0, 0, 0};
   }
+  // The queries have to be there before the loop: a wait for them inside it would be one for the next tile's DMA too.
+#pragma unroll
+  for (int m = 0; m < RW; ++m)
+#pragma unroll
+    for (int k = 0; k < NS; ++k) asm volatile("" : "+v"(qf[m][k]));
   f32x16 o[RW][ND];
   float ref[RW], sum[RW];
 #pragma unroll
@@ -159,7 +182,7 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
   }
-  const float cs = BENT ? 1.0f : a.scale;
+  const float cs = BEND != kPlain ? 1.0f : a.scale;
 
   // One tile against this wave's rows.  PART: some row does not see some key of it.
   auto step = [&](int t, auto PARTIAL) {
@@ -178,28 +201,30 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
       const int key = (c & 3) | (c & 4) << 1 | (c & 8) >> 1;
       const unsigned char* base = kl + (c >> 4) * BLOCK + half * 256 + key * 16;
 #pragma unroll
-      for (int ss = 0; ss < NS; ++ss) {
+      for (int ss = 0; ss < NS; ++ss)
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
           const u32x4 kf = *reinterpret_cast<const u32x4*>(base + k * 2 * BLOCK + ss * 512);
 #pragma unroll
           for (int m = 0; m < RW; ++m) st[m][k] = mma32<T>(kf, qf[m][ss], st[m][k]);
         }
-      }
+      reads_ahead<NS * NK, RW>();
     }
-    if constexpr (BENT || PART) {
+    if constexpr (BEND != kPlain || PART) {
 #pragma unroll
-      for (int m = 0; m < RW; ++m)
+      for (int m = 0; m < RW; ++m) {
+        const float away = (float)(t * KT + 8 * half - place[m]);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int j = t * KT + 32 * k + 16 * (r >> 3) + 8 * half + (r & 7);
+            const int i = 32 * k + 16 * (r >> 3) + (r & 7), j = t * KT + 8 * half + i;
             float v = st[m][k][r];
-            if constexpr (BENT) v = bent_score<T>(a, v, slope[m], p[m], j);
+            if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope[m], away + (float)i);
             if constexpr (PART) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
             st[m][k][r] = v;
           }
+      }
     }
     u32x4 pf[RW][NB];
 #pragma unroll
@@ -244,6 +269,7 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
 #pragma unroll
           for (int m = 0; m < RW; ++m) o[m][d] = mma32<T>(vf, pf[m][j], o[m][d]);
         }
+      reads_ahead<NB * ND, RW>();
     } else {
       // Values of keys that no row of the workgroup sees are cleared; of the others, those that are not finite are
       // left to the second product.
@@ -365,8 +391,9 @@ __global__ __launch_bounds__(256, RW == 1 && DT <= 128 ? 2 : 1) void attn_tile_k
 template <typename T, int DT, int RW>
 static int launch_tile(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
   const dim3 grid((unsigned)plan.blocks, (unsigned)a.S);
-  if (a.softcap > 0.0f || a.slopes) hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, false>), grid, dim3(256), 0, st, a);
+  if (a.slopes) hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, kBias>), grid, dim3(256), 0, st, a);
+  else if (a.softcap > 0.0f) hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, kCap>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attn_tile_kernel<T, DT, RW, kPlain>), grid, dim3(256), 0, st, a);
   return check_launch("paged_attention");
 }
 

@@ -166,8 +166,8 @@ struct AttnArgs {
   Divisor by_hkv, by_g, by_items;  // by_items: (tile, head) pairs of the streaming kernel's grid
   int items;
   int S, chunk_log2;  // splits of a sequence's tokens, tokens in each (the last takes the rest)
-  float scale;        // multiplies q.k into units of log 2 (MOD: into the score itself)
-  float softcap;      // 0: none
+  float scale;          // multiplies q.k into units of log 2 (with a cap: see bent_score)
+  float softcap, cap2;  // 0: none; softcap in units of log 2
   int causal, window, direct;  // direct: item u is the u-th sequence, else by Finder
   const int32_t* prefix;
   const float *slopes, *sinks;

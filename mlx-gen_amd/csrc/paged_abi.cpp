@@ -310,8 +310,9 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   a.by_g = Divisor(a.G);
   a.by_items = Divisor(a.items);
   a.softcap = o->softcap;
-  const bool bent = o->softcap > 0.0f || o->alibi_slopes;
-  a.scale = bent ? o->scale : o->scale * 1.44269504088896341f;
+  const double log2e = 1.44269504088896341;
+  a.cap2 = (float)(o->softcap * log2e);
+  a.scale = (float)(o->softcap > 0.0f ? 2.0 * o->scale / o->softcap * log2e : o->scale * log2e);
   a.causal = o->causal != 0;
   a.window = (int)std::min<int64_t>(o->window, 0x3fffffff);
   a.direct = plan.direct;
