@@ -63,16 +63,19 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   // Tiles of rows: at most one for every p.rows rows and a part one for every sequence.
   const int64_t tiles = T * G / p.rows + std::min(B, T);
   p.direct = !p.tiled && most <= p.rows;
-  // Splits: enough workgroups of four waves for two (tiled) or three on every CU, of at least 128 tokens (a
-  // unit for each wave: one token over 777, 8 heads: 9.5 us; 256: 10.1, one split: 10.3) or 256 (tiled).  One row tile a
-  // sequence: of at most 1024, since the sequences of a step are of unequal length (48 of up to 6000: 25.9 us; 4096: 39.3).
+  // Splits: enough workgroups of four waves for those that the CUs hold (tiled: two each, one for heads past 128) or
+  // three on every CU, of at least 128 tokens (a unit for each wave: one token over 777, 8 heads: 9.5 us; 256: 10.1, one
+  // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 1024, since the sequences of a step are of unequal
+  // length (48 of up to 6000: 25.9 us; 4096: 39.3).
   int64_t range = max_kv;
   if (window) range = std::min(range, window + max_q);
-  const int64_t want = std::max<int64_t>(1, (p.tiled ? 2 : 3) * cus / std::max<int64_t>(tiles * Hkv, 1));
-  p.chunk_log2 = p.tiled ? 8 : 7;
-  while ((want << p.chunk_log2) < range && !(p.direct && p.chunk_log2 == 10)) ++p.chunk_log2;
-  while (((int64_t)kMaxSplits << p.chunk_log2) < range) ++p.chunk_log2;
-  p.S = (int)std::max<int64_t>(1, (range + (1 << p.chunk_log2) - 1) >> p.chunk_log2);
+  const int64_t slots = (!p.tiled ? 3 : D <= 128 ? 2 : 1) * cus, want = std::max<int64_t>(1, slots / std::max<int64_t>(tiles * Hkv, 1));
+  auto up128 = [](int64_t n) { return (n + 127) / 128 * 128; };
+  int64_t chunk = std::max<int64_t>(p.tiled ? 256 : 128, up128((range + want - 1) / want));
+  if (p.direct) chunk = std::min<int64_t>(chunk, 1024);
+  chunk = std::max(chunk, up128((range + kMaxSplits - 1) / kMaxSplits));
+  p.chunk = (int)std::min<int64_t>(chunk, 0x3fffff80);
+  p.S = (int)std::max<int64_t>(1, (range + p.chunk - 1) / p.chunk);
   p.blocks = (p.direct ? B * p.S : p.tiled ? tiles : tiles * p.S) * Hkv;
   if (p.S > 1) {
     auto align = [](size_t b) { return (b + 255) / 256 * 256; };

@@ -102,6 +102,16 @@ __device__ __forceinline__ u32x4 each(u32x4 v, uint32_t (*f)(uint32_t)) {
   return u32x4{f(v[0]), f(v[1]), f(v[2]), f(v[3])};
 }
 
+// The sum of a pair of 16-bit weights, added to acc.
+template <typename T>
+__device__ __forceinline__ float pair_sum(uint32_t v, float acc) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, _Float16))
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), f16x2{(_Float16)1.0f, (_Float16)1.0f}, acc, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, acc, false);
+}
+
 // The running maximum a row's exponents are taken against moves only when a score passes it by this many
 // units of log 2: weights up to 2^8 are as exact as weights up to 1 (fp16's end at 2^16), and the sums
 // are rescaled rarely.
@@ -199,7 +209,7 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
   const int item = turn < a.items ? turn : turn - a.items, unit = a.by_hkv.div(item), h = item - unit * a.Hkv;
   const Batch& bt = a.batch;
   const int D = FULL ? DT : a.D;
-  const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1, cu_log2 = a.chunk_log2 - (KU == 32 ? 5 : 4);  // blocks of a page, units of a split
+  const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1, cu = a.chunk / KU;  // blocks of a page, units of a split
   auto tiles_of = [&](const Seq& s) { return (s.n * a.G + TM - 1) / TM; };
   int b = unit, first = 0;
   if (!a.direct && !Finder(bt, tiles_of).find(unit, b, first)) return;
@@ -214,9 +224,9 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
     const int row0 = tile * TM, row1 = min(rows, row0 + TM) - 1;
     const KeyRange kr = key_range(a, s, row0, row1, prefix);
     const int ub = kr.lo / KU, ue = kr.hi > kr.lo ? (kr.hi + KU - 1) / KU : ub;
-    const int ns = max(1, min(a.S, (ue - ub + (1 << cu_log2) - 1) >> cu_log2));
+    const int ns = max(1, min(a.S, a.by_chunk.div((ue - ub) * KU + a.chunk - 1)));
     if (z >= ns) continue;
-    const int u0 = ub + (z << cu_log2), u1 = z == a.S - 1 ? ue : min(ue, u0 + (1 << cu_log2));
+    const int u0 = ub + z * cu, u1 = z == a.S - 1 ? ue : min(ue, u0 + cu);
     const int blo = kr.lo >> 4, bhi = (kr.hi - 1) >> 4;  // blocks with keys that are seen
 
     // A unit's blocks of 16 keys: their pages, and the blocks' first elements.  Blocks that no row sees are

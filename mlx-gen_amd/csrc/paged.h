@@ -165,7 +165,8 @@ struct AttnArgs {
   int Hkv, G, D;
   Divisor by_hkv, by_g, by_items;  // by_items: (tile, head) pairs of the streaming kernel's grid
   int items;
-  int S, chunk_log2;  // splits of a sequence's tokens, tokens in each (the last takes the rest)
+  int S, chunk;       // splits of a sequence's tokens, tokens in each (a multiple of 128; the last takes the rest)
+  Divisor by_chunk;
   float scale;          // multiplies q.k into units of log 2 (with a cap: see bent_score)
   float softcap, cap2;  // 0: none; softcap in units of log 2
   int causal, window, direct;  // direct: item u is the u-th sequence, else by Finder
@@ -189,7 +190,7 @@ constexpr int kMaxSplits = 256;  // the join gives each a thread
 
 // How an attention call is cut up: rows of a workgroup's tile, splits of the tokens, and the grid.
 struct AttnPlan {
-  int rows = 16, S = 1, chunk_log2 = 0;
+  int rows = 16, S = 1, chunk = 0;
   bool tiled = false, direct = false;
   int64_t blocks = 0;  // workgroups (tiled: times S)
   size_t ml = 0, splits = 0, total = 0;  // workspace: byte offsets of ml and splits, and its size

@@ -304,7 +304,8 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   a.G = (int)(q->heads / cache->heads);
   a.D = (int)D;
   a.S = plan.S;
-  a.chunk_log2 = plan.chunk_log2;
+  a.chunk = plan.chunk;
+  a.by_chunk = Divisor(a.chunk);
   a.items = plan.tiled ? (int)plan.blocks : (int)(plan.blocks / plan.S);
   a.by_hkv = Divisor(a.Hkv);
   a.by_g = Divisor(a.G);
