@@ -220,7 +220,8 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
   const int64_t head = ((int64_t)h << bt.page_log2) * D;
   const T *kp = (const T*)a.k + head, *vp = (const T*)a.v + head;
 
-  for (int tile = first; tile < last; ++tile) {
+  for (int at = first; at < last; ++at) {
+    const int tile = a.direct ? at : tiles_of(s) - 1 - at;  // the longest first
     const int row0 = tile * TM, row1 = min(rows, row0 + TM) - 1;
     const KeyRange kr = key_range(a, s, row0, row1, prefix);
     const int ub = kr.lo / KU, ue = kr.hi > kr.lo ? (kr.hi + KU - 1) / KU : ub;
@@ -307,7 +308,8 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
         for (int t = 0; t < NT; ++t) {
           st[m][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int k = 0; k < NS; ++k) st[m][t] = mma16<T>(kf[t][k], qf[m][k], st[m][t]);
+          for (int k = 0; k < NS; ++k)
+            if (FULL || 4 * k * C < D) st[m][t] = mma16<T>(kf[t][k], qf[m][k], st[m][t]);
         }
       if (more) load_k(u + NW, pg0, pg1);
       const int key0 = u * KU + 4 * g;
@@ -380,7 +382,8 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(vf[d], pf[m], o[m][d]);
+        for (int m = 0; m < MT; ++m)
+          if (FULL || 16 * d < D) o[m][d] = mma16<T>(vf[d], pf[m], o[m][d]);
       if (more) load_v(u + NW, pg0, pg1);
     }
 
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
         }
       }
     }
-    if (tile + 1 < last) __syncthreads();
+    if (at + 1 < last) __syncthreads();
   }
 }
 
