@@ -52,6 +52,46 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq) {
   else *reinterpret_cast<u32x2*>(y) = u32x2{Elem<T>::pack2(v[0] * inv, v[1] * inv), Elem<T>::pack2(v[2] * inv, v[3] * inv)};
 }
 
+// The same with a wave a row, for up to 64 splits: its lanes hold the splits' weights, 64 / (D / 4) groups of them the
+// features.  Most rows of a step have one split only, and a quarter of the workgroups find that out sooner.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a, Divisor by_hq, int rows) {
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int t = by_hq.div(row), qh = row - t * (int)by_hq.d;
+  const int from = min(max(a.batch.q_starts[0], 0), a.batch.T), to = min(a.batch.q_starts[a.batch.B], a.batch.T);
+  if (t < from || t >= to) return;
+  const int ns = min(a.splits[row], a.S);
+  if (ns <= 1) return;  // written by its one split
+  f32x2 e = {-INFINITY, 0.0f};
+  if (lane < ns) e = reinterpret_cast<const f32x2*>(a.ml)[(int64_t)row * a.S + lane];
+  const int per = a.D / 4, groups = 64 / per, gi = lane / per, d = (lane - gi * per) * 4;
+  float top = e[0];
+#pragma unroll
+  for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+  const float ref = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(e[0] - ref);
+  float l = e[1] * f;
+#pragma unroll
+  for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+  f32x4 v = {0, 0, 0, 0};
+  const float* p = a.part + (int64_t)row * a.S * a.D + d;
+  for (int k0 = 0; k0 < ns; k0 += groups) {
+    const int k = k0 + gi;
+    const float w = __shfl(f, k & 63);
+    if (gi < groups && k < ns) v += *reinterpret_cast<const f32x4*>(p + k * a.D) * w;
+  }
+  f32x4 all = v;
+  for (int k = 1; k < groups; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all[i] += __shfl(v[i], (lane + k * per) & 63);
+  if (gi) return;
+  if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[qh] * 1.44269504088896341f - ref);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* y = (T*)a.out.p + t * a.out.ts + qh * a.out.hs + d;
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(y) = all * inv;
+  else *reinterpret_cast<u32x2*>(y) = u32x2{Elem<T>::pack2(all[0] * inv, all[1] * inv), Elem<T>::pack2(all[2] * inv, all[3] * inv)};
+}
+
 AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype, int64_t B, int64_t max_q,
                         int64_t max_kv, int64_t window) {
   AttnPlan p;
@@ -66,14 +106,15 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   p.direct = !p.tiled && most <= p.rows;
   // Splits: enough workgroups of four waves for those that the CUs hold (tiled: two each, one for heads past 128) or
   // three on every CU, of at least 128 tokens (a unit for each wave: one token over 777, 8 heads: 9.5 us; 256: 10.1, one
-  // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 1024, since the sequences of a step are of unequal
-  // length (48 of up to 6000: 25.9 us; 4096: 39.3).
+  // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 768, since the sequences of a step are of unequal
+  // length and the workgroups of a long one fill the chip more evenly (48 of up to 6000 tokens: 24.1 us, with 1024 25.3, with
+  // 4096 39.3; one of 150001: 68.2, 71.7).
   int64_t range = max_kv;
   if (window) range = std::min(range, window + max_q);
   const int64_t slots = (!p.tiled ? 3 : D <= 128 ? 2 : 1) * cus, want = std::max<int64_t>(1, slots / std::max<int64_t>(tiles * Hkv, 1));
   auto up128 = [](int64_t n) { return (n + 127) / 128 * 128; };
   int64_t chunk = std::max<int64_t>(p.tiled ? 256 : 128, up128((range + want - 1) / want));
-  if (p.direct) chunk = std::min<int64_t>(chunk, 1024);
+  if (p.direct) chunk = std::min<int64_t>(chunk, 768);
   chunk = std::max(chunk, up128((range + kMaxSplits - 1) / kMaxSplits));
   p.chunk = (int)std::min<int64_t>(chunk, 0x3fffff80);
   p.S = (int)std::max<int64_t>(1, (range + p.chunk - 1) / p.chunk);
@@ -92,7 +133,11 @@ template <typename T>
 static int launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.batch.T * a.Hkv * a.G;
   if (rows > 0x7fffffff) return set_error(MLXQ_EINVAL, "paged_attention: problem too large");
-  hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, a, a.Hkv * a.G);
+  // A wave's 64 lanes hold the weights of 64 splits; it sums those in turn that a workgroup sums in parallel.
+  if (a.S <= 64)
+    hipLaunchKernelGGL((attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, Divisor(a.Hkv * a.G), (int)rows);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, a, a.Hkv * a.G);
   return check_launch("paged_attention");
 }
 
