@@ -220,6 +220,67 @@ struct StackedExperts {
   Array forward(const Array& x, bool per_expert = false, hipStream_t s = nullptr) const;
 };
 
+// ---- serving from a paged key/value cache (include/mlxq.h) -----------------------------------
+// The operators between a decoder block's qkv and output projections; the reference's attention runs in
+// MLX (mlx-gen-sensenova/src/qwen3.rs:463).  One dtype (f32, bf16 or fp16) for queries, keys, values, cache and result.
+// A layer's cache is two arrays, with C = 16 bytes of elements: keys [pages, heads, page_size/16, head_dim/C, 16, C],
+// values [pages, heads, page_size/C, head_dim, C].
+
+// Frequencies of the rotation, in radians a position, and the factor of cos and sin.
+struct RotaryFrequencies {
+  std::vector<double> inv_freq;  // rotary_dim / 2
+  double magnitude = 1.0;
+};
+// kind: an mlxq_rope_kind; the others as mlxq_rope_scaling.
+RotaryFrequencies rotary_frequencies(int64_t rotary_dim, double base = 10000.0, int kind = 0, double factor = 1.0,
+                                     double original_context = 0.0, double low = 0.0, double high = 0.0);
+// (cos, sin) of every position and pair: f32 [positions, rotary_dim/2, 2].
+Array rotary_table(int64_t positions, const RotaryFrequencies& f, hipStream_t s = nullptr);
+// x [T, heads, D] with its first rotary_dim features turned by positions [T] (int32); inverse turns back.
+Array rotary(const Array& x, const Array& positions, const Array& table, bool interleaved = false, bool inverse = false,
+             hipStream_t s = nullptr);
+
+std::pair<std::vector<int64_t>, std::vector<int64_t>> cache_shapes(int64_t pages, int64_t heads, int64_t page_size,
+                                                                   int64_t head_dim, Dtype dt);
+// The sequences of a step: block_tables [B, width], q_starts [B + 1] and kv_lens [B] (int32), and the longest
+// number of new and of cached tokens that launches are planned for (results do not depend on them).
+struct CacheBatch {
+  Array block_tables, q_starts, kv_lens;
+  int64_t max_q = 1, max_kv = 1;
+};
+// Writes k and v [T, heads, D] into the pages; with a table the keys, and q where given, are rotated in the same launch,
+// by each token's place or by positions [T].  Returns the rotated queries (an empty array without q).
+Array cache_append(const Array& k, const Array& v, const Array& k_cache, const Array& v_cache, const CacheBatch& batch,
+                   const Array* q = nullptr, const Array* table = nullptr, const Array* positions = nullptr,
+                   bool interleaved = false, hipStream_t s = nullptr);
+
+// Attention of a step's new tokens over their sequences' pages, with the options of mlxq_attention.  The workspace
+// is the object's own, kept between calls: calls on one object must be ordered on one stream.
+struct PagedAttention {
+  float scale = 0.0f;  // 0: 1 / sqrt(head_dim)
+  bool causal = true;
+  int64_t window = 0;
+  float softcap = 0.0f;
+  std::optional<Array> prefix_lens;   // [sequences] int32
+  std::optional<Array> alibi_slopes;  // [q heads] f32
+  std::optional<Array> sinks;         // [q heads] f32
+
+  // q [T, heads, D] -> [T, heads, D].
+  Array forward(const Array& q, const Array& k_cache, const Array& v_cache, const CacheBatch& batch,
+                hipStream_t s = nullptr) const;
+  // Into a caller's array of q's shape and dtype: after a first call with the same sizes nothing is allocated, so that it can
+  // be captured into a HIP graph.
+  void forward_into(const Array& q, const Array& k_cache, const Array& v_cache, const CacheBatch& batch, const Array& out,
+                    hipStream_t s = nullptr) const;
+
+  mutable std::shared_ptr<Array> workspace_;
+};
+
+// Pages src[i] of a pool to dst[i], in place: cache's dimension `dim` counts the pages, those before it the pools.
+// block_tables [B, width], where given, follow: entries equal to src[i] become dst[i].
+void copy_pages(const Array& cache, int dim, const Array& src, const Array& dst, const Array* block_tables = nullptr,
+                hipStream_t s = nullptr);
+
 // ---- quant.rs --------------------------------------------------------------------------------
 using Weights = std::map<std::string, Array>;
 const Array& require(const Weights& w, const std::string& key);  // throws on a missing key
