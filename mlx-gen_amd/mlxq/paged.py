@@ -435,17 +435,19 @@ class PagedCache:
             _bad("PagedCache.truncate", f"length {length} of a sequence of {old}")
         keep = -(-length // self.page_size)
         mine = pages[:keep]
-        if length % self.page_size and self._holders[mine[-1]] > 1:
-            if not self._free:
-                _bad("PagedCache.truncate", "1 page is needed and 0 are free")
+        last = pages[keep:]
+        shared = length % self.page_size and self._holders[mine[-1]] > 1
+        if shared and not self._free and all(self._holders[p] > 1 for p in last):
+            _bad("PagedCache.truncate", "1 page is needed and 0 are free")
+        for p in last:
+            self._holders[p] -= 1
+            if self._holders[p] == 0:
+                self._free.append(p)
+        if shared:
             copy = self._take(1)[0]
             self._copy([mine[-1]], [copy])
             self._holders[mine[-1]] -= 1
             mine[-1] = copy
-        for p in pages[keep:]:
-            self._holders[p] -= 1
-            if self._holders[p] == 0:
-                self._free.append(p)
         self._free.sort(reverse=True)
         self._seqs[seq] = (mine, length)
 

@@ -266,6 +266,20 @@ def test_paged_cache_refusals():
     assert c.free_pages == 4 and c.length(a) == 0
 
 
+def test_truncate_of_a_shared_page_in_a_full_pool():
+    c = _Host(4)
+    a = c.new()
+    c.batch([a], [48])
+    b, = c.fork([a])
+    c.batch([b], [16])
+    assert c.free_pages == 0
+    with pytest.raises(mlxq.MlxqError):
+        c.truncate(a, 40)  # its copy of the page would need a fifth
+    assert c.length(a) == 48 and c.pages_of(a) == c.pages_of(b)[:3]
+    c.truncate(b, 40)  # b's own fourth page holds the copy
+    assert c.pages_of(b) == [0, 1, 3] and c.pages_of(a) == [0, 1, 2] and c._holders == [2, 2, 1, 1] and c.free_pages == 0
+
+
 def test_layer_views():
     c = mlxq.PagedCache(3, 5, 2, 32, 32, torch.bfloat16, "cpu")
     for i in range(3):
