@@ -110,12 +110,12 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   // length and the workgroups of a long one fill the chip more evenly (48 of up to 6000 tokens: 24.1 us, with 1024 25.3, with
   // 4096 39.3; one of 150001: 68.2, 71.7).
   int64_t range = max_kv;
-  if (window) range = std::min(range, window + max_q);
+  if (window) range = std::min(range, window + std::min(max_q, p.rows / G + 1));
   const int64_t slots = (!p.tiled ? 3 : D <= 128 ? 2 : 1) * cus, want = std::max<int64_t>(1, slots / std::max<int64_t>(tiles * Hkv, 1));
-  auto up128 = [](int64_t n) { return (n + 127) / 128 * 128; };
-  int64_t chunk = std::max<int64_t>(p.tiled ? 256 : 128, up128((range + want - 1) / want));
+  auto whole = [&](int64_t n) { return p.tiled ? (n + 63) / 64 * 64 : (n + 127) / 128 * 128; };  // tiles; a unit a wave
+  int64_t chunk = std::max<int64_t>(p.tiled ? 256 : 128, whole((range + want - 1) / want));
   if (p.direct) chunk = std::min<int64_t>(chunk, 768);
-  chunk = std::max(chunk, up128((range + kMaxSplits - 1) / kMaxSplits));
+  chunk = std::max(chunk, whole((range + kMaxSplits - 1) / kMaxSplits));
   p.chunk = (int)std::min<int64_t>(chunk, 0x3fffff80);
   p.S = (int)std::max<int64_t>(1, (range + p.chunk - 1) / p.chunk);
   p.blocks = (p.direct ? B * p.S : p.tiled ? tiles : tiles * p.S) * Hkv;

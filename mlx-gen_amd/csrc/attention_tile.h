@@ -1,7 +1,7 @@
 // attention_tile.h — paged attention for many rows a key head (chunks of prompts) in 16-bit types.
 //
-// A workgroup holds 4 waves of 32 * RW rows, (token, query head) pairs of one sequence and key head, and
-// walks the sequence's keys in tiles of KT.  Keys and values go from the pages to LDS by DMA, one tile
+// A workgroup holds 4 waves of 32 rows, (token, query head) pairs of one sequence and key head, and
+// walks the sequence's keys in tiles of 64.  Keys and values go from the pages to LDS by DMA, one to three tiles
 // ahead: a block of 16 keys is contiguous in a page, so a copy is linear and a wave moves whole blocks.
 // As in the streaming kernel the products are S^T = K Q^T and O^T = V^T P^T, here with 32x32x16: a lane
 // holds one row's scores, the maximum needs one exchange between the halves of a wave, and the exponentials
@@ -89,13 +89,14 @@ struct BoolConstant {
 
 template <typename T, int DT, int BEND>
 __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
-  constexpr int C = 8, KT = DT <= 128 ? 64 : 32, NB = KT / 16, NK = KT / 32, NS = DT / 16, ND = DT / 32, TM = 128;
+  constexpr int C = 8, KT = 64, NB = KT / 16, NK = KT / 32, NS = DT / 16, ND = DT / 32, TM = 128;
   constexpr int BLOCK = 16 * DT * 2;   // bytes of a block's keys (or values) in LDS, at most
   constexpr int BUF = 2 * NB * BLOCK;  // a tile: the blocks' keys, then their values
-  // Tiles in LDS, one in use and the others on their way: as many as leave room for a second workgroup on the CU, or
-  // for heads past 128, whose accumulators take all registers of a SIMD, as fit beside nothing else.
-  constexpr int BUFS = DT == 64 || DT == 256 ? 4 : 2;
-  constexpr int PER = (NB == 4 ? 2 : 1) * ND;  // DMA loads of a wave a tile
+  // Tiles in LDS, one in use and the others on their way: as many as leave room for a second workgroup on the CU.  Heads
+  // past 128, whose accumulators leave a SIMD one wave, take its LDS too (500 tokens, 16 heads of 256, a window of
+  // 4096: 71 us; four tiles of 32 keys instead of two of 64: 75).
+  constexpr int BUFS = DT == 64 ? 4 : 2;
+  constexpr int PER = 2 * ND;  // DMA loads of a wave a tile
   __shared__ __align__(1024) unsigned char lds[BUFS * BUF];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, c = lane & 31, unit = a.by_hkv.div(blockIdx.x), h = blockIdx.x - unit * a.Hkv, z = blockIdx.y;
@@ -117,20 +118,18 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
   const auto* pages = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)table;
   const int blog = bt.page_log2 - 4, bmask = (1 << blog) - 1, D = a.D;
 
-  // DMA of a tile's keys and of its values: a wave moves one block of 16 of each, or of one of them where a tile has two
-  // blocks.  Blocks that no row sees are never looked up: their entries may name nothing.
-  const bool moves_k = NB == 4 || w < 2, moves_v = NB == 4 || w >= 2;
-  const int own = NB == 4 ? w : w & 1;
+  // DMA of a tile's keys and of its values: a wave moves one block of 16 of each.  Blocks that no row sees are never
+  // looked up: their entries may name nothing.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   const int64_t head = ((int64_t)h << bt.page_log2) * D;
   bool bad = false;
-  auto block_of = [&](int t) { return min(max(t * NB + own, blo), bhi); };
+  auto block_of = [&](int t) { return min(max(t * NB + w, blo), bhi); };
   auto page_of = [&](int t) { return pages[block_of(min(t, t1 - 1)) >> blog]; };
   auto dma = [&](int t, int page, const void* pool, int64_t stride, uint32_t to) {
     const bool in = (unsigned)page < (unsigned)bt.pages;
     bad |= !in;
     const T* src = (const T*)pool + head + (int64_t)(block_of(t) & bmask) * 16 * D + (int64_t)(in ? page : 0) * stride;
-    const uint32_t dst = lds0 + (t & (BUFS - 1)) * BUF + to + own * BLOCK;
+    const uint32_t dst = lds0 + (t & (BUFS - 1)) * BUF + to + w * BLOCK;
     constexpr int RUN = ND < 4 ? ND : 4;
     static_assert(ND % RUN == 0, "a block is whole runs");
     if (D == DT) {
@@ -143,8 +142,8 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
   };
   int page = 0;  // of the next tile's block
   auto load = [&](int t) {
-    if (moves_k) dma(t, page, a.k, a.k_page, 0);
-    if (moves_v) dma(t, page, a.v, a.v_page, NB * BLOCK);
+    dma(t, page, a.k, a.k_page, 0);
+    dma(t, page, a.v, a.v_page, NB * BLOCK);
     page = page_of(t + 1);
   };
   if (D < DT) {
@@ -173,8 +172,17 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
   for (int k = 0; k < NS; ++k) qf[k] = 16 * k < D ? load_chunk(q + (2 * k + half) * C) : u32x4{0, 0, 0, 0};
   // The queries have to be there before the loop: a wait for them inside it would be one for the next tile's DMA too.
 #pragma unroll
-  for (int k = 0; k < NS; ++k) asm volatile("" : "+v"(qf[k]));
+  for (int k = 0; k < NS; ++k) {
+    if constexpr (DT <= 128) asm volatile("" : "+v"(qf[k]));
+    else asm volatile("" : "+a"(qf[k]));
+  }
   f32x16 o[ND];
+  // Heads past 128: queries and results lie in the accumulation registers, which matrix products read and write directly.  Held
+  // there wherever anything else uses them; left to itself the compiler moves all results out and back every tile (83 us
+  // instead of 75 for the example above).
+  auto pin = [](f32x16& v) {
+    if constexpr (DT > 128) asm volatile("" : "+a"(v));
+  };
   float ref = -INFINITY, sum[1] = {0.0f};
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -195,8 +203,7 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
                                [&](int i, u32x4 v) { st[i % NK] = mma32<T>(v, qf[i / NK], st[i % NK]); });
   };
 
-  // Tile t with its scores st; the next tile's go to nx.  The two are independent and interleaved: a matrix product runs
-  // on while the exponentials are issued.  PART: some row does not see some key of the tile.
+  // Tile t.  PART: some row does not see some key of it.
   auto step = [&](int t, auto PARTIAL) {
     f32x16 st[NK];
     constexpr bool PART = decltype(PARTIAL)::value;
@@ -247,7 +254,11 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
       ref = now;
       sum[0] *= alpha;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= alpha;
+      for (int d = 0; d < ND; ++d) {
+        pin(o[d]);
+        o[d] *= alpha;
+        pin(o[d]);
+      }
       weights();
     }
     sum[0] += add;
@@ -295,7 +306,10 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
             for (int i = 0; i < 16; ++i) x[i] = 0.0f;
             x = mma32<T>(each<T>(value(j, d) & seen, value_code<T>), ch, x);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] += decoded(x[i]);
+            for (int i = 0; i < 16; ++i) x[i] = decoded(x[i]);
+            pin(o[d]);
+            o[d] += x;
+            pin(o[d]);
           }
         }
       }
@@ -332,6 +346,8 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     }
   }
 
+#pragma unroll
+  for (int d = 0; d < ND; ++d) pin(o[d]);
   __syncthreads();
   if (any_wave<4>(bad, reinterpret_cast<int*>(lds))) poison(bt, table, max(t0 * KT, kr.lo), min(t1 * KT, kr.hi), lo, span, sum);
   float l = half_sum(sum[0]);
