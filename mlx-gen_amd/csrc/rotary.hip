@@ -5,6 +5,8 @@
 // value once in 16-byte pieces and are bound by HBM; the table's rows (4 rotary_dim bytes a token, shared
 // by all heads of the token) come from L2.  A thread keeps the (c, s) of its pairs in registers over
 // several heads.  Products and sums are f32, rounded once to the dtype.
+//
+// Rotation of 8190 tokens, 40 f32 heads of 128: 71 us, 4.7 TB/s, the rate of a large copy.  4 tokens of 24 heads: 2.5 us.
 #include <algorithm>
 
 #include "paged.h"
@@ -161,6 +163,9 @@ struct Frequencies {
   double f[128];
 };
 
+// A thread a pair, in double precision: an angle of 2^20 radians is right to 2^-33, where f32 would be off by
+// 2^-4.  Bound by double arithmetic and the sincos of large arguments; made once for a model (131072 positions of 64 pairs,
+// 67 MB: 31 us).
 __global__ __launch_bounds__(256) void rotary_table_kernel(Frequencies fr, int half, double magnitude, int64_t total,
                                                            f32x2* __restrict__ table) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -188,6 +193,11 @@ int run_rotary_table(const double* inv_freq, int64_t half, double magnitude, int
 // and its query heads.  Keys: a token's chunks lie 16 chunks apart in the block, so the 16 tokens'
 // stores of a chunk make up 256 contiguous bytes (in L2).  Values: C tokens of a feature lie side by
 // side, which the workgroup turns around in LDS, storing whole chunks where all C tokens are new.
+//
+// One token of 24 sequences, 32 + 8 heads of 128: 5 us, a launch and three dependent reads (the sequence's bounds,
+// its page, the tokens).  Five prompts, 47 MB in fp16: 14 us, 3.4 TB/s: the same chain of reads in 1276 workgroups
+// that all fit the chip at once, so that nothing hides it.  More heads a thread at once, 14 -> 18 us, or two units
+// side by side, 15 us, lose workgroups a CU to registers.
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int C = Elem<T>::C;
