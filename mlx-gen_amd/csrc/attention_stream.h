@@ -198,10 +198,26 @@ __device__ __forceinline__ u32x4 even_keys(u32x4 v) {
   return v;
 }
 
+// Waves a SIMD for DT * MT = d: as many as the registers hold without spilling.
+template <typename T>
+constexpr int stream_waves(int d) {
+  if (sizeof(T) == 4) return d <= 80 ? 3 : d <= 128 ? 2 : 1;
+  return d <= 64 ? 4 : d <= 192 ? 2 : 1;
+}
+
+// Kernels of one wave a SIMD keep queries and results in the accumulation registers, which matrix products read and write
+// directly: held there wherever anything else uses them, since the compiler, left to itself, moves all results out and
+// back every unit or tile.
+template <bool ACC, typename V>
+__device__ __forceinline__ void pin(V& v) {
+  if constexpr (ACC) asm volatile("" : "+a"(v));
+}
+
 // FULL: head_dim is DT, else below it and the rest of DT is zeros.
 template <typename T, int DT, int MT, int BEND, bool FULL>
-__global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) void attn_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, stream_waves<T>(DT * MT)) void attn_stream_kernel(AttnArgs a) {
   constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
+  constexpr bool ACC = stream_waves<T>(DT * MT) == 1;
   constexpr int JD = DT * MT < 256 ? DT : DT / 2;  // features joined at a time: all that 64 KB hold
   __shared__ float lm[NW][TM], ll[NW][TM];
   __shared__ int flags[NW];
@@ -288,6 +304,8 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
       const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
 #pragma unroll
       for (int k = 0; k < NS; ++k) qf[m][k] = FULL || (4 * k + g) * C < D ? load_chunk(q + (4 * k + g) * C) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < NS; ++k) pin<ACC>(qf[m][k]);
     }
     f32x4 o[MT][ND];
     float ref[MT], sum[MT];
@@ -349,7 +367,11 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
           ref[m] = now;
           sum[m] *= alpha;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) o[m][d] *= alpha;
+          for (int d = 0; d < ND; ++d) {
+            pin<ACC>(o[m][d]);
+            o[m][d] *= alpha;
+            pin<ACC>(o[m][d]);
+          }
         }
         const float neg = ref[m] == -INFINITY ? 0.0f : -ref[m];  // nothing seen yet: all weights are exp2(-inf)
         float e[C], add = 0.0f;
@@ -377,8 +399,10 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
               const f32x4 x = mma16<T>(each<T>(vf[d], value_code<T>), each<T>(pf[m], weight_code<T>), f32x4{0, 0, 0, 0});
+              pin<ACC>(o[m][d]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[m][d][i] += decoded(x[i]);
+              pin<ACC>(o[m][d]);
             }
             vf[d] &= each<T>(vf[d], finite_mask<T>);
           }
@@ -410,7 +434,10 @@ __global__ __launch_bounds__(256, DT * MT <= 64 ? 4 : DT * MT <= 128 ? 2 : 1) vo
       for (int i = 0; i < NW; ++i) top = fmaxf(top, lm[i][m * 16 + c]);
       const float f = __builtin_amdgcn_exp2f(ref[m] - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[m][d] *= f;
+      for (int d = 0; d < ND; ++d) {
+        pin<ACC>(o[m][d]);
+        o[m][d] *= f;
+      }
     }
 #pragma unroll
     for (int j0 = 0; j0 < DT; j0 += JD) {
@@ -466,15 +493,25 @@ static int launch_stream(const AttnArgs& a, const AttnPlan& plan, hipStream_t st
   return a.D == DT ? launch_stream_of<T, DT, MT, true>(a, plan, st) : launch_stream_of<T, DT, MT, false>(a, plan, st);
 }
 
+// The narrowest width that holds the heads: what is past them costs registers, and with them waves a SIMD (f32, 400
+// tokens over 700, 4 heads: 80 wide 21.5 us as 80 and 28.9 as 128, 96 wide 24.9 and 32.1; bf16, 32 single tokens over up to
+// 4000, 8 heads of 96: 78 and 84).
 template <typename T>
 static int stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
   if (plan.rows == 16) {
     if (a.D <= 64) return launch_stream<T, 64, 1>(a, plan, st);
+    if constexpr (sizeof(T) == 4)
+      if (a.D <= 80) return launch_stream<T, 80, 1>(a, plan, st);
+    if (a.D <= 96) return launch_stream<T, 96, 1>(a, plan, st);
     if (a.D <= 128) return launch_stream<T, 128, 1>(a, plan, st);
     return launch_stream<T, 256, 1>(a, plan, st);
   }
-  if (a.D <= 64) return launch_stream<T, 64, 2>(a, plan, st);
-  return launch_stream<T, 128, 2>(a, plan, st);
+  if constexpr (sizeof(T) == 2) {
+    if (a.D <= 64) return launch_stream<T, 64, 2>(a, plan, st);
+    if (a.D <= 96) return launch_stream<T, 96, 2>(a, plan, st);
+    return launch_stream<T, 128, 2>(a, plan, st);
+  }
+  return set_error(MLXQ_EINVAL, "paged_attention: no kernel for %d rows", plan.rows);
 }
 
 }  // namespace mlxq
