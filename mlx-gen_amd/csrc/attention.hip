@@ -98,8 +98,8 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
                         int64_t max_kv, int64_t window) {
   AttnPlan p;
   const int64_t G = Hq / Hkv, cus = device_cu_count(), most = max_q * G;
-  // Two row tiles a wave where they fit its registers twice over a SIMD: not past 128 features, not in f32 (three
-  // prompts of up to 900, 80-wide heads: 77.7 us with 32 rows, 56.2 with 16).
+  // Two row tiles a wave where they leave a SIMD two waves: not past 128 features, not in f32 (three prompts of up to
+  // 900, 80-wide heads, in kernels of 128 features: 77.7 us with 32 rows, 56.2 with 16).
   p.rows = most <= 16 || D > 128 || dtype == MLXQ_FLOAT32 ? 16 : 32;
   p.tiled = dtype != MLXQ_FLOAT32 && most > p.rows;
   if (p.tiled) p.rows = 128;

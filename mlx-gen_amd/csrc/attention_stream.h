@@ -19,8 +19,9 @@
 // and 7 for the join, 307 MB at 5.0 TB/s (a plain read runs at 5.7-6.4).  48 of up to 6000, 64 + 8 heads of 64: 20 + 4 us;
 // the workgroups of splits that short sequences lack take 2.5 ns each.  One of 777: 5 + 5 us, all latency.
 // f32 prompts are bound by the f32 products, a sixteenth of bf16's rate: 3 prompts of up to 700 tokens over 900, 12
-// heads of 80: 54 us, 41 TFLOP/s where a large f32 product reaches 153; their tiles fill the chip 1.6 times, and half of
-// them meet the diagonal or the shared part's end.
+// heads of 80: 39 us, 57 TFLOP/s where a large f32 product reaches 153; their tiles fill the chip 1.5 times, half of
+// them meet the diagonal or the shared part's end, and bias, mask and softmax take the vector units as long as the
+// products take the matrix cores.
 #pragma once
 
 #include "paged.h"
@@ -198,11 +199,12 @@ __device__ __forceinline__ u32x4 even_keys(u32x4 v) {
   return v;
 }
 
-// Waves a SIMD for DT * MT = d: as many as the registers hold without spilling.
+// Waves a SIMD for DT * MT = d: as many as the registers hold without spilling; two row tiles of 128 features spill a dozen
+// and are faster so all the same (8 sequences of 4 tokens over up to 4000, 32 + 4 heads: 23.5 us, one wave 28.9).
 template <typename T>
-constexpr int stream_waves(int d) {
+constexpr int stream_waves(int d, int mt = 1) {
   if (sizeof(T) == 4) return d <= 80 ? 3 : d <= 128 ? 2 : 1;
-  return d <= 64 ? 4 : d <= 192 ? 2 : 1;
+  return d <= 64 ? 4 : d <= 128 || mt == 2 ? 2 : 1;
 }
 
 // Kernels of one wave a SIMD keep queries and results in the accumulation registers, which matrix products read and write
@@ -215,9 +217,9 @@ __device__ __forceinline__ void pin(V& v) {
 
 // FULL: head_dim is DT, else below it and the rest of DT is zeros.
 template <typename T, int DT, int MT, int BEND, bool FULL>
-__global__ __launch_bounds__(256, stream_waves<T>(DT * MT)) void attn_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream_kernel(AttnArgs a) {
   constexpr int C = Elem<T>::C, KU = 4 * C, NT = KU / 16, NS = DT / (4 * C), ND = DT / 16, TM = 16 * MT, NW = 4;
-  constexpr bool ACC = stream_waves<T>(DT * MT) == 1;
+  constexpr bool ACC = stream_waves<T>(DT * MT, MT) == 1;
   constexpr int JD = DT * MT < 256 ? DT : DT / 2;  // features joined at a time: all that 64 KB hold
   __shared__ float lm[NW][TM], ll[NW][TM];
   __shared__ int flags[NW];
