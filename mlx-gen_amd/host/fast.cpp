@@ -414,6 +414,7 @@ bool pages_apart(const at::Tensor& t, int64_t page, int64_t& stride) {
     if (t.size(d) != 1 && t.stride(d) != n) return false;
     n *= t.size(d);
   }
+  if (t.size(0) > 1 && t.stride(0) < page) return false;  // pages that share memory are refused
   stride = t.stride(0) < page ? page : t.stride(0);
   return true;
 }

@@ -115,8 +115,10 @@ def _cache(op, k, v):
             if size != 1 and stride != n:
                 _bad(op, f"the pages of {what} must be contiguous")
             n *= size
-    return PagedCacheView(k.data_ptr(), v.data_ptr(), max(k.stride(0), heads * P * D), max(v.stride(0), heads * P * D), pages,
-                          P, heads, D, _dt(k))
+        if pages > 1 and t.stride(0) < n:
+            _bad(op, f"the pages of {what} overlap")
+    n = heads * P * D  # a single page's stride means nothing
+    return PagedCacheView(k.data_ptr(), v.data_ptr(), max(k.stride(0), n), max(v.stride(0), n), pages, P, heads, D, _dt(k))
 
 
 def _batch(op, batch, device):
