@@ -3,6 +3,7 @@
 // memory, checks shapes the way the reference's callers rely on, and sequences ABI calls.
 #include "mlxq.hpp"
 
+#include <algorithm>
 #include <cstring>
 
 #include "../../include/mlxq.h"
@@ -143,6 +144,14 @@ Array Array::empty(std::vector<int64_t> shape, Dtype dt) {
     a.ptr_ = p;
   }
   return a;
+}
+
+const Array& Workspace::at_least(size_t bytes) {
+  static const Array none;
+  if (held_.empty() && bytes == 0) return none;
+  const size_t have = held_.empty() ? 0 : held_.back().nbytes();
+  if (have < bytes) held_.push_back(Array::empty({(int64_t)((std::max(bytes, 2 * have) + 3) / 4)}, Dtype::Uint32));
+  return held_.back();
 }
 
 std::pair<Array, Array> Array::empty_pair(std::vector<int64_t> shape, Dtype dt) {

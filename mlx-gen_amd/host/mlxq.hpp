@@ -80,6 +80,30 @@ class Array {
   Dtype dtype_ = Dtype::Float32;
 };
 
+// Device memory that an object keeps between its calls and grows on demand.  What it outgrew stays allocated as long
+// as the object does: a HIP graph captured from an earlier, smaller call still writes there.  Each growth at least
+// doubles it, so that all of it together is less than twice the last.  A copy starts without memory, and one
+// that is assigned to keeps its own: two objects never share any.
+class Workspace {
+ public:
+  Workspace() = default;
+  Workspace(const Workspace&) {}
+  Workspace& operator=(const Workspace&) { return *this; }
+  Workspace(Workspace&&) = default;
+  Workspace& operator=(Workspace&& o) {
+    if (this != &o) {
+      held_.insert(held_.begin(), o.held_.begin(), o.held_.end());
+      o.held_.clear();
+    }
+    return *this;
+  }
+  // At least that many bytes, or an empty array when none were ever needed.
+  const Array& at_least(size_t bytes);
+
+ private:
+  std::vector<Array> held_;  // the last is in use
+};
+
 // ---- ops (mlx_rs::ops) ----------------------------------------------------------------------
 struct Packed {
   Array wq, scales, biases;
@@ -255,7 +279,7 @@ Array cache_append(const Array& k, const Array& v, const Array& k_cache, const A
                    bool interleaved = false, hipStream_t s = nullptr);
 
 // Attention of a step's new tokens over their sequences' pages, with the options of mlxq_attention.  The workspace
-// is the object's own, kept between calls: calls on one object must be ordered on one stream.
+// is the object's own (a copy has another), kept between calls: calls on one object must be ordered on one stream.
 struct PagedAttention {
   float scale = 0.0f;  // 0: 1 / sqrt(head_dim)
   bool causal = true;
@@ -269,11 +293,11 @@ struct PagedAttention {
   Array forward(const Array& q, const Array& k_cache, const Array& v_cache, const CacheBatch& batch,
                 hipStream_t s = nullptr) const;
   // Into a caller's array of q's shape and dtype: after a first call with the same sizes nothing is allocated, so that it can
-  // be captured into a HIP graph.
+  // be captured into a HIP graph, which stays valid while the object lives, whatever is called later.
   void forward_into(const Array& q, const Array& k_cache, const Array& v_cache, const CacheBatch& batch, const Array& out,
                     hipStream_t s = nullptr) const;
 
-  mutable std::shared_ptr<Array> workspace_;
+  mutable Workspace workspace_;
 };
 
 // Pages src[i] of a pool to dst[i], in place: cache's dimension `dim` counts the pages, those before it the pools.

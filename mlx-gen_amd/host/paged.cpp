@@ -151,9 +151,8 @@ void PagedAttention::forward_into(const Array& q, const Array& k_cache, const Ar
   o.alibi_slopes = floats(alibi_slopes, q.dim(1), op, "alibi_slopes");
   o.sinks = floats(sinks, q.dim(1), op, "sinks");
   const size_t need = mlxq_paged_attention_workspace_size(q.dim(0), q.dim(1), &c, &b, &o);
-  if (!workspace_) workspace_ = std::make_shared<Array>();
-  if (workspace_->nbytes() < need) *workspace_ = Array::empty({(int64_t)((need + 3) / 4)}, Dtype::Uint32);
-  check(mlxq_paged_attention(&qh, q.dim(0), &c, &b, &o, &oh, workspace_->data(), workspace_->nbytes(), s));
+  const Array& ws = workspace_.at_least(need);
+  check(mlxq_paged_attention(&qh, q.dim(0), &c, &b, &o, &oh, ws.data(), ws.nbytes(), s));
 }
 
 Array PagedAttention::forward(const Array& q, const Array& k_cache, const Array& v_cache, const CacheBatch& batch,
