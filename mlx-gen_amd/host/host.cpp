@@ -76,14 +76,6 @@ int64_t check_pack(const char* op, const Array& wq, const Array& scales, const A
   return N;
 }
 
-// The layer's reusable workspace grown to `need` bytes (empty array when none is needed).  It
-// stays allocated with the layer, so forward calls after the first allocate nothing.
-Array& grow_workspace(std::shared_ptr<Array>& ws, size_t need) {
-  if (!ws) ws = std::make_shared<Array>();
-  if (ws->nbytes() < need) *ws = Array::empty({(int64_t)((need + 3) / 4)}, Dtype::Uint32);
-  return *ws;
-}
-
 }  // namespace
 
 size_t dtype_size(Dtype dt) {
@@ -446,7 +438,7 @@ Array QuantizedLinear::forward_fused(const Array& x, const Adapter* lora, int ac
   std::vector<int64_t> shape = x.shape();
   shape.back() = N;
   Array y = output_array(out, shape, from_abi(ydt), "linear");
-  Array& ws = grow_workspace(workspace_, mlxq_linear_workspace_size(xdt, sdt, M, N, &e));
+  const Array& ws = workspace_.at_least(mlxq_linear_workspace_size(xdt, sdt, M, N, &e));
   check(mlxq_linear(x.data(), xdt, M, K, (const uint32_t*)weight.data(), scales.data(), biases.data(),
                     sdt, N, group_size, bits, &e, y.data(), ws.nbytes() ? ws.data() : nullptr,
                     ws.nbytes(), s));
@@ -522,9 +514,8 @@ Array AdaptableLinear::forward_impl(const Array& x, const Array* out_arg, hipStr
     Dtype d1 = promote(promote(x.dtype(), q.scales.dtype()), q.bias ? q.bias->dtype() : x.dtype());
     if (fused) d1 = promote(d1, promote(x.dtype(), fused->a.dtype()));
     if (d1 != final_dt) {
-      if (!mid_ || mid_->shape() != out_arg->shape() || mid_->dtype() != d1)
-        mid_ = std::make_shared<Array>(Array::empty(out_arg->shape(), d1));
-      mid = *mid_;
+      const size_t bytes = (size_t)out_arg->size() * dtype_size(d1);
+      mid = Array::borrow(bytes ? mid_.at_least(bytes).data() : nullptr, out_arg->shape(), d1);
       first_out = &mid;
     }
   }
@@ -538,7 +529,7 @@ Array AdaptableLinear::forward_impl(const Array& x, const Array* out_arg, hipStr
         throw Error(MLXQ_EINVAL, "AdaptableLinear: a LoKr delta must be [out, in]");
       const Dtype odt = promote(y.dtype(), x.dtype());
       Array out = odt == y.dtype() ? y : (out_arg ? *out_arg : Array::empty(y.shape(), odt));
-      Array& ws = grow_workspace(workspace_, mlxq_lokr_residual_workspace_size(xdt, M, N));
+      const Array& ws = workspace_.at_least(mlxq_lokr_residual_workspace_size(xdt, M, N));
       check(mlxq_lokr_residual(x.data(), xdt, M, K, ad.delta.data(),
                                abi_dtype(ad.delta.dtype(), "AdaptableLinear::forward"), N, ad.scale,
                                y.data(), abi_dtype(y.dtype(), "AdaptableLinear::forward"), out.data(),
@@ -553,7 +544,7 @@ Array AdaptableLinear::forward_impl(const Array& x, const Array* out_arg, hipStr
     const int ldt = abi_dtype(ad.a.dtype(), "AdaptableLinear::forward");
     const Dtype odt = promote(y.dtype(), promote(x.dtype(), ad.a.dtype()));
     Array out = odt == y.dtype() ? y : (out_arg ? *out_arg : Array::empty(y.shape(), odt));
-    Array& ws = grow_workspace(workspace_, mlxq_lora_residual_workspace_size(xdt, ldt, M, N, rank));
+    const Array& ws = workspace_.at_least(mlxq_lora_residual_workspace_size(xdt, ldt, M, N, rank));
     check(mlxq_lora_residual(x.data(), xdt, M, K, ad.a.data(), ad.b.data(), ldt, N, rank, ad.scale,
                              y.data(), abi_dtype(y.dtype(), "AdaptableLinear::forward"), out.data(),
                              ws.data(), ws.nbytes(), s));

@@ -164,7 +164,7 @@ struct QuantizedLinear {
   // Device workspace of mlxq_linear, kept with the layer and grown on demand, so that forward
   // calls after the first allocate none (last member: aggregate initialisation leaves it empty).
   // Calls on one layer must be ordered on one stream.
-  mutable std::shared_ptr<Array> workspace_;
+  mutable Workspace workspace_;
 };
 
 class AdaptableLinear {
@@ -187,7 +187,7 @@ class AdaptableLinear {
   Array forward(const Array& x, hipStream_t s = nullptr) const;
   // forward into a caller's array of shape [..., out] and dtype out_dtype(x.dtype()): after a
   // first call with the same shapes this allocates nothing and never waits for the device, so it
-  // can be captured into a HIP graph.
+  // can be captured into a HIP graph, which stays valid while the layer lives, whatever is called later.
   void forward_into(const Array& x, const Array& out, hipStream_t s = nullptr) const;
   Dtype out_dtype(Dtype x_dtype) const;
 
@@ -196,8 +196,8 @@ class AdaptableLinear {
   std::optional<Array> dense_weight_, dense_bias_;
   std::optional<QuantizedLinear> quantized_;
   std::vector<Adapter> adapters_;
-  mutable std::shared_ptr<Array> workspace_;  // mlxq_{lora,lokr}_residual staging, grown on demand
-  mutable std::shared_ptr<Array> mid_;        // a bf16 partial sum before an f32 adapter
+  mutable Workspace workspace_;  // mlxq_{lora,lokr}_residual staging, grown on demand
+  mutable Workspace mid_;        // a bf16 partial sum before an f32 adapter
 };
 
 class TokenEmbedding {

@@ -114,6 +114,64 @@ static void attention_cpu() {
   EXPECT(g_frees == g_allocs);
 }
 
+// A refused call: its output or its workspace starts 8 bytes off.
+template <typename F>
+static void refused(F&& f) {
+  bool yes = false;
+  try {
+    f();
+  } catch (const Error& e) {
+    yes = e.status == MLXQ_EINVAL && strstr(e.what(), "must be 16-byte aligned");
+  }
+  EXPECT(yes);
+}
+
+static void linear_cpu() {
+  constexpr int64_t K = 256, N = 512, R = 16;
+  const Dtype B = Dtype::Bfloat16;
+  g_allocs = g_frees = 0;
+  {
+    banner("QuantizedLinear: more rows keep the memory of fewer, a copy has its own");
+    const QuantizedLinear q{fake({N, K / 8}, Dtype::Uint32), fake({N, K / 64}, B), fake({N, K / 64}, B), std::nullopt, 64, 4};
+    const Adapter lora = Adapter::lora(fake({K, R}, B), fake({R, N}, B), 1.0f);
+    auto call = [&](const QuantizedLinear& l, int64_t M) {
+      const Array out = fake({M, N}, B);
+      refused([&] { l.forward_fused(fake({M, K}, B), &lora, MLXQ_ACT_NONE, nullptr, &out); });
+    };
+    call(q, 1);
+    call(q, 1);
+    EXPECT(g_allocs == 1);
+    call(q, 4000);
+    EXPECT(g_allocs == 2 && g_frees == 0);
+    const QuantizedLinear r = q;
+    call(r, 4000);
+    EXPECT(g_allocs == 3 && g_frees == 0);
+    call(q, 4000);
+    EXPECT(g_allocs == 3);
+  }
+  EXPECT(g_frees == 3);
+  g_allocs = g_frees = 0;
+  {
+    banner("AdaptableLinear: so does a partial sum that an f32 adapter follows");
+    AdaptableLinear l = AdaptableLinear::from_quantized_parts(fake({N, K / 8}, Dtype::Uint32), fake({N, K / 64}, B), fake({N, K / 64}, B),
+                                                              std::nullopt, 64, 4);
+    l.push(Adapter::lora(fake({K, R}, B), fake({R, N}, B), 1.0f));
+    l.push(Adapter::lora(fake({K, R}, Dtype::Float32), fake({R, N}, Dtype::Float32), 1.0f));
+    auto call = [&](const AdaptableLinear& l, int64_t M) { refused([&] { l.forward_into(fake({M, K}, B), fake({M, N}, Dtype::Float32)); }); };
+    call(l, 2);
+    EXPECT(g_allocs == 2);  // the sum, and the base layer's workspace
+    call(l, 4000);
+    EXPECT(g_allocs == 4 && g_frees == 0);
+    call(l, 2);
+    call(l, 300);
+    EXPECT(g_allocs == 4 && g_frees == 0);
+    const AdaptableLinear c = l;
+    call(c, 2);
+    EXPECT(g_allocs == 6 && g_frees == 0);
+  }
+  EXPECT(g_frees == 6);
+}
+
 static Array upload(const std::vector<float>& v, std::vector<int64_t> shape) { return Array::from_host(v.data(), std::move(shape), Dtype::Float32); }
 static Array upload(const std::vector<int32_t>& v, std::vector<int64_t> shape) { return Array::from_host(v.data(), std::move(shape), Dtype::Int32); }
 
@@ -174,12 +232,65 @@ static void attention_gpu() {
   (void)hipStreamDestroy(s);
 }
 
+static void linear_gpu() {
+  banner("a captured layer with two adapters, more rows, the layer replayed");
+  constexpr int64_t K = 256, N = 512, R = 16, M = 4, MANY = 700;
+  std::mt19937 g(5);
+  std::normal_distribution<float> nd;
+  auto randn = [&](std::vector<int64_t> shape, float std) {
+    std::vector<float> v(shape[0] * shape[1]);
+    for (auto& x : v) x = nd(g) * std;
+    return upload(v, shape);
+  };
+  auto bf16 = [&](std::vector<int64_t> shape, float std) { return as_dtype(randn(shape, std), Dtype::Bfloat16); };
+  const Packed p = quantize(bf16({N, K}, 0.05f), 64, 4);
+  AdaptableLinear l = AdaptableLinear::from_quantized_parts(p.wq, p.scales, p.biases, std::nullopt, 64, 4);
+  l.push(Adapter::lora(bf16({K, R}, 0.1f), bf16({R, N}, 0.1f), 0.5f));
+  l.push(Adapter::lora(randn({K, R}, 0.1f), randn({R, N}, 0.1f), 1.25f));
+  const Array x = bf16({M, K}, 1.0f), many = bf16({MANY, K}, 1.0f);
+  const Array out = Array::empty({M, N}, Dtype::Float32);
+  l.forward_into(x, out);
+  const std::vector<float> want = host(out);
+  hipStream_t s;
+  hipGraph_t gr;
+  hipGraphExec_t ex;
+  EXPECT(hipStreamCreate(&s) == hipSuccess);
+  EXPECT(hipDeviceSynchronize() == hipSuccess);
+  EXPECT(hipStreamBeginCapture(s, hipStreamCaptureModeGlobal) == hipSuccess);
+  l.forward_into(x, out, s);
+  EXPECT(hipStreamEndCapture(s, &gr) == hipSuccess);
+  EXPECT(hipGraphInstantiate(&ex, gr, nullptr, nullptr, 0) == hipSuccess);
+  const Array wide = Array::empty({MANY, N}, Dtype::Float32);
+  l.forward_into(many, wide);
+  const std::vector<float> other = host(wide);
+  std::vector<Array> rest;
+  for (int i = 0; i < 40; ++i) rest.push_back(upload(std::vector<float>(256 << (i % 10), 1.0f + i), {256 << (i % 10)}));
+  for (int i = 0; i < 4; ++i) {
+    EXPECT(hipMemset(out.data(), 0xff, out.nbytes()) == hipSuccess);
+    EXPECT(hipDeviceSynchronize() == hipSuccess);
+    EXPECT(hipGraphLaunch(ex, s) == hipSuccess);
+    EXPECT(hipStreamSynchronize(s) == hipSuccess);
+    EXPECT(host(out) == want);
+    l.forward_into(many, wide);
+    EXPECT(host(wide) == other);
+  }
+  for (int i = 0; i < 40; ++i) EXPECT(host(rest[i]) == std::vector<float>(256 << (i % 10), 1.0f + i));
+  (void)hipGraphExecDestroy(ex);
+  (void)hipGraphDestroy(gr);
+  (void)hipStreamDestroy(s);
+}
+
 int main(int argc, char** argv) {
   const std::string what = argc > 1 ? argv[1] : "cpu";
   try {
     g_count = what != "gpu";
-    if (g_count) attention_cpu();
-    else attention_gpu();
+    if (g_count) {
+      attention_cpu();
+      linear_cpu();
+    } else {
+      attention_gpu();
+      linear_gpu();
+    }
   } catch (const std::exception& e) {
     fprintf(stderr, "FAIL: %s\n", e.what());
     ++g_failures;
