@@ -134,7 +134,6 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
 template <typename T>
 static int launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.batch.T * a.Hkv * a.G;
-  if (rows > 0x7fffffff) return set_error(MLXQ_EINVAL, "paged_attention: problem too large");
   // A wave's 64 lanes hold the weights of 64 splits; it sums those in turn that a workgroup sums in parallel.
   if (a.S <= 64)
     hipLaunchKernelGGL((attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, Divisor(a.Hkv * a.G), (int)rows);

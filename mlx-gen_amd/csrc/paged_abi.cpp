@@ -110,6 +110,10 @@ int check_attention(const char* op, int64_t T, int64_t q_heads, const mlxq_paged
   if ((rc = check_batch(op, batch, T)) || (rc = check_cache(op, cache, T))) return rc;
   if (q_heads < 1 || q_heads > 65535 || q_heads % cache->heads != 0)
     return set_error(MLXQ_EINVAL, "%s: %lld query heads over %lld key heads", op, (long long)q_heads, (long long)cache->heads);
+  // A sequence's rows, (token, query head) pairs of a key head, and a tile of 128 past them are counted in 31 bits.
+  if (T * (q_heads / cache->heads) > 0x7fffffff - 128)
+    return set_error(MLXQ_EINVAL, "%s: %lld tokens of %lld query heads a key head are too many rows", op, (long long)T,
+                     (long long)(q_heads / cache->heads));
   if (!o) return set_error(MLXQ_EINVAL, "%s: options are null", op);
   if (!(o->scale > 0.0f) || !isfinite(o->scale)) return set_error(MLXQ_EINVAL, "%s: scale must be positive and finite", op);
   if (!(o->softcap >= 0.0f) || !isfinite(o->softcap))
@@ -124,10 +128,15 @@ int check_attention(const char* op, int64_t T, int64_t q_heads, const mlxq_paged
   return MLXQ_OK;
 }
 
-AttnPlan plan_of(int64_t T, int64_t q_heads, const mlxq_paged_cache* c, const mlxq_paged_batch* b, const mlxq_attention* o) {
+// The plan of a checked call, unless its launches count past 31 bits: workgroups, or the rows of split results.
+int plan_of(const char* op, int64_t T, int64_t q_heads, const mlxq_paged_cache* c, const mlxq_paged_batch* b,
+            const mlxq_attention* o, AttnPlan& plan) {
   const int64_t capacity = b->table_width * c->page_size;
-  return plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, std::max<int64_t>(b->max_q, 1),
+  plan = plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, std::max<int64_t>(b->max_q, 1),
                         std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), o->window);
+  if (plan.blocks > 0x7fffffff || (plan.S > 1 && T * q_heads > 0x7fffffff))
+    return set_error(MLXQ_EINVAL, "%s: problem too large", op);
+  return MLXQ_OK;
 }
 
 }  // namespace
@@ -268,8 +277,12 @@ int mlxq_cache_append(const mlxq_heads* k, const mlxq_heads* v, int64_t T, const
 
 size_t mlxq_paged_attention_workspace_size(int64_t T, int64_t q_heads, const mlxq_paged_cache* cache,
                                            const mlxq_paged_batch* batch, const mlxq_attention* options) {
-  if (check_attention("paged_attention", T, q_heads, cache, batch, options) || T == 0 || batch->sequences == 0) return 0;
-  return plan_of(T, q_heads, cache, batch, options).total;
+  const char* op = "paged_attention";
+  AttnPlan plan;
+  if (check_attention(op, T, q_heads, cache, batch, options) || T == 0 || batch->sequences == 0 ||
+      plan_of(op, T, q_heads, cache, batch, options, plan))
+    return 0;
+  return plan.total;
 }
 
 int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache* cache, const mlxq_paged_batch* batch,
@@ -285,13 +298,13 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   if ((rc = check_heads(op, "q", q, cache->dtype, D)) || (rc = check_heads(op, "out", out, cache->dtype, D, T)))
     return rc;
   if (out->heads != q->heads) return set_error(MLXQ_EINVAL, "%s: q and out have different heads", op);
-  const AttnPlan plan = plan_of(T, q->heads, cache, batch, o);
+  AttnPlan plan;
+  if ((rc = plan_of(op, T, q->heads, cache, batch, o, plan))) return rc;
   if (plan.total > 0) {
     if (workspace == nullptr || workspace_bytes < plan.total)
       return set_error(MLXQ_EINVAL, "%s: workspace of %zu bytes is smaller than the %zu required", op, workspace_bytes, plan.total);
     if ((rc = check_ptr(op, "workspace", workspace, 16))) return rc;
   }
-  if (plan.blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   AttnArgs a = {};
   a.q = view(q);
   a.out = view(out);

@@ -1,0 +1,49 @@
+"""Sizes past what the paged-cache kernels count in 31 bits are refused before anything is launched, and what the launches are
+planned for is bounded.  On the CPU: the checks and the plan need no device."""
+import ctypes
+
+import pytest
+
+from mlxq import _lib
+
+P = 4096  # any aligned address: nothing below gets as far as reading it
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def _attention(lib, T, Hq, Hkv, D=64, dtype=1, B=3, max_q=1, max_kv=64, width=4, size=False, **opts):
+    """(status, message) of a call whose workspace is too small, or its workspace size."""
+    cache = _lib.PagedCacheView(P, P, Hkv * 16 * D, Hkv * 16 * D, 2 ** 30, 16, Hkv, D, dtype)
+    batch = _lib.PagedBatch(P, P, P, B, width, width, max_q, max_kv)
+    o = _lib.Attention(**{**dict(scale=0.125, causal=1, window=0, softcap=0.0, prefix_lens=None, alibi_slopes=None, sinks=None), **opts})
+    q = _lib.Heads(P, Hq, Hq * D, D)
+    r = ctypes.byref
+    if size:
+        return lib.mlxq_paged_attention_workspace_size(T, Hq, r(cache), r(batch), r(o))
+    rc = lib.mlxq_paged_attention(r(q), T, r(cache), r(batch), r(o), r(q), None, 0, None)
+    return rc, lib.mlxq_last_error().decode()
+
+
+LONG = dict(B=1, max_kv=10 ** 6, width=10 ** 5)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(2 ** 26, 64, 2), (2 ** 30 - 1, 2, 1), (2 ** 30 - 1, 65535, 1), (2 ** 16, 32768, 1)])
+def test_rows_past_31_bits_are_refused(lib, T, Hq, Hkv):
+    """A key head's rows, (token, query head) pairs, and a tile after them are counted in 31 bits."""
+    for D, dtype, max_q in ((64, 1, 1), (64, 1, T), (256, _lib.MLXQ_FLOAT16, 500), (64, 0, T)):
+        kw = dict(D=D, dtype=dtype, max_q=max_q, **LONG)
+        rc, msg = _attention(lib, T, Hq, Hkv, **kw)
+        assert rc == _lib.MLXQ_EINVAL and "rows" in msg, msg
+        assert _attention(lib, T, Hq, Hkv, size=True, **kw) == 0
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(2 ** 25, 64, 64), (2 ** 30 - 1, 32, 32)])
+def test_split_results_past_31_bits_are_refused(lib, T, Hq, Hkv):
+    """Where sequences are split, a row of results of every query head has a place in the workspace, counted in 31 bits: refused
+    before the first kernel, not between it and the join."""
+    rc, msg = _attention(lib, T, Hq, Hkv, **LONG)
+    assert rc == _lib.MLXQ_EINVAL and "too large" in msg, msg
+    assert _attention(lib, T, Hq, Hkv, size=True, **LONG) == 0
