@@ -87,6 +87,9 @@ int check_batch(const char* op, const mlxq_paged_batch* b, int64_t T) {
   return check_ptr(op, "kv_lens", b->kv_lens, 4);
 }
 
+// A window as the kernels and their plan count it: past every place it hides nothing.
+int64_t window_of(const mlxq_attention* o) { return std::min<int64_t>(o->window, 0x3fffffff); }
+
 Heads view(const mlxq_heads* x) { return {x->data, x->token_stride, x->head_stride}; }
 
 Batch view(const mlxq_paged_batch* b, const mlxq_paged_cache* c, int64_t T) {
@@ -133,7 +136,7 @@ int plan_of(const char* op, int64_t T, int64_t q_heads, const mlxq_paged_cache* 
             const mlxq_attention* o, AttnPlan& plan) {
   const int64_t capacity = b->table_width * c->page_size;
   plan = plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, std::max<int64_t>(b->max_q, 1),
-                        std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), o->window);
+                        std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), window_of(o));
   if (plan.blocks > 0x7fffffff || (plan.S > 1 && T * q_heads > 0x7fffffff))
     return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   return MLXQ_OK;
@@ -328,7 +331,7 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   a.cap2 = (float)(o->softcap * log2e);
   a.scale = (float)(o->softcap > 0.0f ? 2.0 * o->scale / o->softcap * log2e : o->scale * log2e);
   a.causal = o->causal != 0;
-  a.window = (int)std::min<int64_t>(o->window, 0x3fffffff);
+  a.window = (int)window_of(o);
   a.direct = plan.direct;
   a.prefix = o->prefix_lens;
   a.slopes = o->alibi_slopes;

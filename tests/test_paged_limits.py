@@ -47,3 +47,11 @@ def test_split_results_past_31_bits_are_refused(lib, T, Hq, Hkv):
     rc, msg = _attention(lib, T, Hq, Hkv, **LONG)
     assert rc == _lib.MLXQ_EINVAL and "too large" in msg, msg
     assert _attention(lib, T, Hq, Hkv, size=True, **LONG) == 0
+
+
+@pytest.mark.parametrize("window", [10 ** 6, 2 ** 40, 2 ** 62, 2 ** 63 - 1])
+def test_a_window_past_every_context_plans_as_none(lib, window):
+    """"No limit" is often written as the largest integer."""
+    for kw in (dict(T=2, Hq=8, Hkv=2, B=2, max_kv=150001, width=10 ** 4), dict(T=300, Hq=8, Hkv=2, B=1, max_q=300, max_kv=9000, width=10 ** 3)):
+        want = _attention(lib, size=True, **kw)
+        assert want > 0 and _attention(lib, size=True, window=window, **kw) == want
