@@ -196,7 +196,7 @@ struct AttnPlan {
   size_t ml = 0, splits = 0, total = 0;  // workspace: byte offsets of ml and splits, and its size
 };
 AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype, int64_t B, int64_t max_q,
-                        int64_t max_kv, int64_t window);
+                        int64_t max_kv, int64_t window, bool causal);
 int run_attention(const AttnArgs& a, int dtype, const AttnPlan& plan, hipStream_t st);
 // The instances of the streaming kernel, by dtype.
 int run_attn_stream_bf16(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);

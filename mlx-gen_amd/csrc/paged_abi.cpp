@@ -136,7 +136,7 @@ int plan_of(const char* op, int64_t T, int64_t q_heads, const mlxq_paged_cache* 
             const mlxq_attention* o, AttnPlan& plan) {
   const int64_t capacity = b->table_width * c->page_size;
   plan = plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, std::max<int64_t>(b->max_q, 1),
-                        std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), window_of(o));
+                        std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), window_of(o), o->causal != 0);
   if (plan.blocks > 0x7fffffff || (plan.S > 1 && T * q_heads > 0x7fffffff))
     return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   return MLXQ_OK;

@@ -55,3 +55,23 @@ def test_a_window_past_every_context_plans_as_none(lib, window):
     for kw in (dict(T=2, Hq=8, Hkv=2, B=2, max_kv=150001, width=10 ** 4), dict(T=300, Hq=8, Hkv=2, B=1, max_q=300, max_kv=9000, width=10 ** 3)):
         want = _attention(lib, size=True, **kw)
         assert want > 0 and _attention(lib, size=True, window=window, **kw) == want
+
+
+def _splits(lib, Hq=4, Hkv=2, D=64, **kw):
+    """Splits of a plan, from its workspace: rows of S x D sums, of S (maximum, sum) pairs and of counts, each rounded up."""
+    T = kw["T"]
+    need = _attention(lib, Hq=Hq, Hkv=Hkv, D=D, size=True, **kw)
+    up = lambda b: -(-b // 256) * 256  # noqa: E731
+    return next((S for S in range(2, 300) if up(T * Hq * S * D * 4) + up(T * Hq * S * 8) + up(T * Hq * 4) == need), 1 if need == 0 else None)
+
+
+@pytest.mark.parametrize("T,max_kv", [(500, 16384), (16384, 16384), (40, 9000)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_rows_that_see_past_their_window_are_planned_for(lib, T, max_kv, dtype):
+    """With a window, a causal row sees no more tokens than that; one that sees all later tokens, up to as many more as the step
+    has, and no split may be left with most of them.  Prefixes, which are on the device, change no plan."""
+    kw = dict(T=T, B=1, max_q=T, max_kv=max_kv, width=10 ** 4, dtype=dtype, window=128)
+    reach = min(max_kv, 128 + T)
+    plain = _splits(lib, **{**kw, "max_kv": reach, "window": 0})  # the same rows over as many tokens, all of them seen
+    assert _splits(lib, causal=0, **kw) == plain
+    assert _splits(lib, prefix_lens=P, **kw) == _splits(lib, **kw) <= max(plain, 2)
