@@ -75,3 +75,14 @@ def test_rows_that_see_past_their_window_are_planned_for(lib, T, max_kv, dtype):
     plain = _splits(lib, **{**kw, "max_kv": reach, "window": 0})  # the same rows over as many tokens, all of them seen
     assert _splits(lib, causal=0, **kw) == plain
     assert _splits(lib, prefix_lens=P, **kw) == _splits(lib, **kw) <= max(plain, 2)
+
+
+@pytest.mark.parametrize("hint", [2 ** 31, 2 ** 47, 2 ** 62, 2 ** 63 - 1])
+def test_hints_past_every_step_plan_alike(lib, hint):
+    """max_q and max_kv are hints of any size: neither is multiplied past 63 bits."""
+    kw = dict(T=300, Hq=8, Hkv=2, B=2, width=10 ** 3, dtype=0)
+    want = _attention(lib, size=True, **kw, max_q=2 ** 30, max_kv=2 ** 30)
+    assert want > 0 and _attention(lib, size=True, **kw, max_q=hint, max_kv=2 ** 30) == want
+    assert _attention(lib, size=True, **kw, max_q=hint, max_kv=hint) == want
+    assert _attention(lib, size=True, **{**kw, "dtype": 1}, max_q=hint, max_kv=hint) == \
+        _attention(lib, size=True, **{**kw, "dtype": 1}, max_q=2 ** 30, max_kv=2 ** 30)
