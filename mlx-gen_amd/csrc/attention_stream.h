@@ -149,21 +149,46 @@ __device__ __forceinline__ void poison(const Batch& bt, const int32_t* table, in
 
 constexpr float kLog2e = 1.44269504088896341f;
 
+constexpr float kNearCap = 256.0f;
+
 // What happens to a score before the softmax: nothing, a cap, or a bias by distance (capped before it if
 // softcap is set).
 enum Bend : int { kPlain = 0, kCap = 1, kBias = 2 };
-// A capped or biased score, in units of log 2, from q.k and the distance of key and row.  cap tanh(z / cap) is cap - 2 cap /
-// (exp(2 z / cap) + 1): in 16-bit types with the hardware's exponential and reciprocal, off by a few 2^-24 cap.
-// AttnArgs::scale is 2 scale / (cap ln 2) with a cap, scale / ln 2 without; cap2 is softcap / ln 2.
-template <typename T, int BEND>
+// A capped or biased score, in units of log 2, from q.k and the distance of key and row.  With x = score / cap, cap tanh(x) is
+// cap - 2 cap / (exp(2 x) + 1), in 16-bit types with the hardware's exponential and reciprocal, off by up to 5 2^-24 cap: up to
+// kNearCap less than a third of what rounding a weight to fp16 is.  FAR: caps above, where |x| < 1/4 by the first four terms of
+// tanh's series times the cap, score (1 - x^2/3 + 2 x^4/15 - 17 x^6/315), off by 6 2^-24 of the score, whatever the
+// cap (7001 tokens at once, 32 + 8 heads of 128: 590 us, near caps 475, no cap 410).
+// y = AttnArgs::cap_scale q.k is 2 x in units of log 2; cap2 is the cap in those units.
+template <typename T, int BEND, bool FAR>
 __device__ __forceinline__ float bent_score(const AttnArgs& a, float qk, float slope2, float distance) {
   float z = qk * a.scale;
   if (BEND == kCap || a.softcap > 0.0f) {
-    if constexpr (sizeof(T) == 4) z = a.cap2 * tanhf(z * 0.34657359027997265f);  // ln 2 / 2
-    else z = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.0f), a.cap2);
+    constexpr float kHalf = 0.34657359027997265f;  // ln 2 / 2: x = kHalf y
+    const float y = qk * a.cap_scale;
+    if constexpr (sizeof(T) == 4) {
+      z = a.cap2 * tanhf(y * kHalf);
+    } else {
+      const float bent = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.0f), a.cap2);
+      constexpr float c1 = -kHalf * kHalf / 3.0f, c2 = 2.0f * kHalf * kHalf * kHalf * kHalf / 15.0f,
+                      c3 = -17.0f * kHalf * kHalf * kHalf * kHalf * kHalf * kHalf / 315.0f;
+      const float t = y * y, series = fmaf(z * t, fmaf(t, fmaf(t, c3, c2), c1), z);
+      z = FAR && fabsf(y) < 0.25f / kHalf ? series : bent;
+    }
   }
   if constexpr (BEND == kBias) z = fmaf(-slope2, fabsf(distance), z);
   return z;
+}
+
+template <bool B>
+struct BoolConstant {
+  static constexpr bool value = B;
+};
+// f(FAR), by the call's cap.
+template <typename T, int BEND, typename F>
+__device__ __forceinline__ void by_cap(const AttnArgs& a, F f) {
+  if (sizeof(T) == 2 && BEND != kPlain && a.softcap > kNearCap) f(BoolConstant<true>{});
+  else f(BoolConstant<false>{});
 }
 
 // The rows that a lane's row index stands for, and what they see.
@@ -340,18 +365,20 @@ __global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream
       const int key0 = u * KU + 4 * g;
       const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all;
       if (BEND != kPlain || part) {
+        by_cap<T, BEND>(a, [&](auto FAR) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = key0 + 16 * t + i;
-              float v = st[m][t][i];
-              if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope[m], (float)(j - place[m]));
-              if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
-              st[m][t][i] = v;
-            }
+              for (int i = 0; i < 4; ++i) {
+                const int j = key0 + 16 * t + i;
+                float v = st[m][t][i];
+                if constexpr (BEND != kPlain) v = bent_score<T, BEND, decltype(FAR)::value>(a, v, slope[m], (float)(j - place[m]));
+                if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
+                st[m][t][i] = v;
+              }
+        });
       }
       u32x4 pf[MT];
 #pragma unroll

@@ -85,11 +85,6 @@ __device__ __forceinline__ void read_and_multiply(R read, U use) {
 // The largest sum of weights that a lane takes from a tile: fp16's weights end at 2^16.
 constexpr float kMost = 32768.0f;
 
-template <bool B>
-struct BoolConstant {
-  static constexpr bool value = B;
-};
-
 template <typename T, int DT, int BEND>
 __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
   constexpr bool ACC = DT > 128;  // 500 tokens, 16 heads of 256, a window of 4096: 75 us instead of 83
@@ -210,16 +205,18 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     products(t, st);
     if constexpr (BEND != kPlain || PART) {
       const float away = (float)(t * KT + 8 * half - place);
+      by_cap<T, BEND>(a, [&](auto FAR) {
 #pragma unroll
-      for (int k = 0; k < NK; ++k)
+        for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = 32 * k + 16 * (r >> 3) + (r & 7), j = t * KT + 8 * half + i;
-          float v = st[k][r];
-          if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope, away + (float)i);
-          if constexpr (PART) v = (unsigned)(j - lo[0]) < (unsigned)span[0] ? v : -INFINITY;
-          st[k][r] = v;
-        }
+          for (int r = 0; r < 16; ++r) {
+            const int i = 32 * k + 16 * (r >> 3) + (r & 7), j = t * KT + 8 * half + i;
+            float v = st[k][r];
+            if constexpr (BEND != kPlain) v = bent_score<T, BEND, decltype(FAR)::value>(a, v, slope, away + (float)i);
+            if constexpr (PART) v = (unsigned)(j - lo[0]) < (unsigned)span[0] ? v : -INFINITY;
+            st[k][r] = v;
+          }
+      });
     }
     // Weights against the reference that the row has.  The maximum is looked for only where that gives a sum of
     // weights past kMost (or no key was seen before): far from overflow in the types, and as exact.
