@@ -111,7 +111,7 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 768, since the sequences of a step are of unequal
   // length and the workgroups of a long one fill the chip more evenly (48 of up to 6000 tokens: 24.1 us, with 1024 25.3, with
   // 4096 39.3; one of 150001: 68.2, 71.7).
-  int64_t range = max_kv;
+  int64_t range = std::min<int64_t>(max_kv, 0x3fffffff);  // as far as places go
   // With a window a tile's rows see as many tokens as it holds and one for each of theirs, or, where they see all later
   // tokens, one for each of the step's, since the first row's window starts that far before the sequence's end (2000 tokens
   // over 16384, 8 heads of 128, window 128: 37.6 us, planned as causal 45.8; 300: 17.6 and 16.6).  How far a prefix
@@ -120,7 +120,15 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   const int64_t slots = (!p.tiled ? 3 : D <= 128 ? 2 : 1) * cus, want = std::max<int64_t>(1, slots / std::max<int64_t>(tiles * Hkv, 1));
   auto whole = [&](int64_t n) { return p.tiled ? (n + 63) / 64 * 64 : (n + 127) / 128 * 128; };  // tiles; a unit a wave
   int64_t chunk = std::max<int64_t>(p.tiled ? 256 : 128, whole((range + want - 1) / want));
-  if (p.direct) chunk = std::min<int64_t>(chunk, 768);
+  // With many sequences and a long hint that is many workgroups and partial results: at most 16 for each that the chip
+  // holds, and 256 MiB (which only more tokens than max_q promises reach).  256 sequences of up to 2000 tokens, 64 + 8
+  // heads of 128, planned for 131072: 228 us and 55 MB, without the bound 835 and 1.46 GB, with 4 for each 224; one of them
+  // of 131072 tokens: 600, 958 and 1215.
+  if (p.direct) {
+    const int64_t items = std::min(std::min(B, T) * Hkv, 16 * slots), most_splits = std::max<int64_t>(1, (256 << 20) / (T * Hq * D * 4));
+    chunk = std::min<int64_t>(chunk, 768);
+    chunk = std::max({chunk, whole((range * items + 16 * slots - 1) / (16 * slots)), whole((range + most_splits - 1) / most_splits)});
+  }
   chunk = std::max(chunk, whole((range + kMaxSplits - 1) / kMaxSplits));
   p.chunk = (int)std::min<int64_t>(chunk, 0x3fffff80);
   p.S = (int)std::max<int64_t>(1, (range + p.chunk - 1) / p.chunk);
@@ -137,7 +145,7 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
 
 template <typename T>
 static int launch_join(const AttnArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.batch.T * a.Hkv * a.G;
+  const int64_t rows = (int64_t)a.batch.T * a.Hkv * a.G;  // with splits, of 31 bits: see plan_attention's bounds
   // A wave's 64 lanes hold the weights of 64 splits; it sums those in turn that a workgroup sums in parallel.
   if (a.S <= 64)
     hipLaunchKernelGGL((attn_join_rows_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, Divisor(a.Hkv * a.G), (int)rows);

@@ -131,15 +131,14 @@ int check_attention(const char* op, int64_t T, int64_t q_heads, const mlxq_paged
   return MLXQ_OK;
 }
 
-// The plan of a checked call, unless its launches count past 31 bits: workgroups, or the rows of split results.
+// The plan of a checked call, unless its workgroups pass 31 bits.
 int plan_of(const char* op, int64_t T, int64_t q_heads, const mlxq_paged_cache* c, const mlxq_paged_batch* b,
             const mlxq_attention* o, AttnPlan& plan) {
   const int64_t capacity = b->table_width * c->page_size;
   const int64_t max_q = std::min<int64_t>(std::max<int64_t>(b->max_q, 1), 0x3fffffff);
   plan = plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, max_q,
                         std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), window_of(o), o->causal != 0);
-  if (plan.blocks > 0x7fffffff || (plan.S > 1 && T * q_heads > 0x7fffffff))
-    return set_error(MLXQ_EINVAL, "%s: problem too large", op);
+  if (plan.blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   return MLXQ_OK;
 }
 

@@ -41,11 +41,8 @@ def test_rows_past_31_bits_are_refused(lib, T, Hq, Hkv):
 
 
 @pytest.mark.parametrize("T,Hq,Hkv", [(2 ** 25, 64, 64), (2 ** 30 - 1, 32, 32)])
-def test_split_results_past_31_bits_are_refused(lib, T, Hq, Hkv):
-    """Where sequences are split, a row of results of every query head has a place in the workspace, counted in 31 bits: refused
-    before the first kernel, not between it and the join."""
-    rc, msg = _attention(lib, T, Hq, Hkv, **LONG)
-    assert rc == _lib.MLXQ_EINVAL and "too large" in msg, msg
+def test_results_past_31_bits_are_not_split(lib, T, Hq, Hkv):
+    """Where sequences are split, a row of results of every query head has a place in the workspace, counted in 31 bits."""
     assert _attention(lib, T, Hq, Hkv, size=True, **LONG) == 0
 
 
@@ -86,3 +83,32 @@ def test_hints_past_every_step_plan_alike(lib, hint):
     assert _attention(lib, size=True, **kw, max_q=hint, max_kv=hint) == want
     assert _attention(lib, size=True, **{**kw, "dtype": 1}, max_q=hint, max_kv=hint) == \
         _attention(lib, size=True, **{**kw, "dtype": 1}, max_q=2 ** 30, max_kv=2 ** 30)
+
+
+@pytest.mark.parametrize("B,new,Hq,Hkv,D,max_kv", [(256, 1, 64, 8, 128, 131072), (256, 2, 64, 8, 128, 131072), (2048, 1, 8, 1, 64, 32768),
+                                                   (100, 2, 32, 8, 256, 10 ** 6), (4096, 4, 32, 8, 128, 10 ** 6), (300, 1, 32, 1, 64, 2 ** 24)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_many_sequences_under_a_long_hint(lib, B, new, Hq, Hkv, D, max_kv, dtype):
+    """A replayed step is planned for the longest context; how many sequences it has bounds the splits, and with them the workspace
+    and the workgroups that find nothing to do."""
+    kw = dict(T=B * new, B=B, max_q=new, max_kv=max_kv, width=max_kv // 16, dtype=dtype)
+    S = _splits(lib, Hq=Hq, Hkv=Hkv, D=D, **kw)
+    assert S is not None and S * B * Hkv <= 16 * 3 * 256 + B * Hkv
+    assert _attention(lib, Hq=Hq, Hkv=Hkv, D=D, size=True, **kw) <= 2 ** 28 + 2 ** 24
+
+
+def test_the_longest_tables_and_the_most_sequences(lib):
+    kw = dict(T=2 ** 24 - 1, Hq=64, Hkv=64, B=2 ** 24 - 1, width=2 ** 31 - 1)
+    assert _attention(lib, size=True, max_kv=2 ** 63 - 1, **kw) == _attention(lib, size=True, max_kv=2 ** 30 - 1, **kw) == 0
+
+
+def test_more_tokens_than_hinted(lib):
+    """max_q is a hint: the workspace stays bounded for a step that has many more tokens."""
+    assert _attention(lib, T=100000, Hq=32, Hkv=8, D=128, B=1, max_q=1, max_kv=131072, width=8192, size=True) <= 2 ** 28 + 2 ** 24
+
+
+def test_few_sequences_are_still_split(lib):
+    """768 tokens a split where the chip has room for the workgroups."""
+    assert _splits(lib, Hq=64, Hkv=8, T=48, B=48, max_kv=6000, width=375) == 8
+    assert _splits(lib, Hq=28, Hkv=4, D=128, T=2, B=2, max_kv=150001, width=9376) == 196
+    assert _splits(lib, Hq=32, Hkv=8, D=128, T=8, B=1, max_q=8, max_kv=131072, width=8192) > 40
