@@ -111,7 +111,7 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 768, since the sequences of a step are of unequal
   // length and the workgroups of a long one fill the chip more evenly (48 of up to 6000 tokens: 24.1 us, with 1024 25.3, with
   // 4096 39.3; one of 150001: 68.2, 71.7).
-  int64_t range = std::min<int64_t>(max_kv, 0x3fffffff);  // as far as places go
+  int64_t range = std::min<int64_t>(max_kv, 0x3fffff80);  // places end at 2^30
   // With a window a tile's rows see as many tokens as it holds and one for each of theirs, or, where they see all later
   // tokens, one for each of the step's, since the first row's window starts that far before the sequence's end (2000 tokens
   // over 16384, 8 heads of 128, window 128: 37.6 us, planned as causal 45.8; 300: 17.6 and 16.6).  How far a prefix
@@ -130,7 +130,7 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
     chunk = std::max({chunk, whole((range * items + 16 * slots - 1) / (16 * slots)), whole((range + most_splits - 1) / most_splits)});
   }
   chunk = std::max(chunk, whole((range + kMaxSplits - 1) / kMaxSplits));
-  p.chunk = (int)std::min<int64_t>(chunk, 0x3fffff80);
+  p.chunk = (int)chunk;
   p.S = (int)std::max<int64_t>(1, (range + p.chunk - 1) / p.chunk);
   p.blocks = (p.direct ? B * p.S : p.tiled ? tiles : tiles * p.S) * Hkv;
   if (p.S > 1) {
