@@ -269,10 +269,12 @@ def paged_attention(q, k_cache, v_cache, batch, scale: float | None = None, caus
 def copy_pages(cache, src, dst, block_tables=None, dim: int | None = None):
     """cache[..., dst, :] = cache[..., src, :] in place, over the pages of one pool or of several at once ([planes...,
     pages, heads, ...]: every layer's keys and values, say).  dim is the dimension of the pages: by default the
-    sixth from last, or the first of a value pool's five.  src and dst: int32, no page of dst also in src.
-    block_tables [B, width] (int32, on the GPU): entries that name a page of src then name its copy."""
+    sixth from last of key pools, which have 16 tokens next to last, and the fifth from last of value pools (of a
+    stack of value pools whose head_dim is 16, which looks alike, dim has to be given).  src and dst: int32, no
+    page of dst also in src.  block_tables [B, width] (int32, on the GPU): entries that name a page of src then
+    name its copy."""
     if dim is None:
-        dim = max(cache.dim() - 6, 0)
+        dim = max(cache.dim() - (6 if cache.dim() > 5 and cache.shape[-2] == 16 else 5), 0)
     if _lib.fast().copy_pages(cache, src, dst, block_tables, dim):
         return
     op = "copy_pages"

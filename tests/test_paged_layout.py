@@ -45,3 +45,37 @@ def test_one_page_of_any_stride():
     one = [t.as_strided(t.shape, (0, *t.stride()[1:])) for t in (k, v)]
     mlxq.cache_append(x, x, *one, batch)
     assert torch.equal(mlxq.paged_attention(x, *one, batch), x)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("head_dim,page", [(32, 16), (64, 64), (128, 16), (256, 128)])
+def test_the_pages_dimension(monkeypatch, dtype, head_dim, page):
+    """By default the pages are the dimension before a pool's own, for stacks of key pools and of value pools alike."""
+    seen = []
+
+    class Fast:
+        @staticmethod
+        def copy_pages(cache, src, dst, tables, dim):
+            seen.append(dim)
+            return True
+
+    monkeypatch.setattr(mlxq._lib, "_fast", Fast)
+    for shape in mlxq.cache_shapes(3, 2, page, head_dim, dtype):
+        for lead in ((), (4,), (4, 2)):
+            mlxq.copy_pages(torch.empty(*lead, *shape, dtype=dtype), None, None)
+            assert seen.pop() == len(lead), (lead, shape)
+            mlxq.copy_pages(torch.empty(*lead, *shape, dtype=dtype), None, None, dim=7)
+            assert seen.pop() == 7
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(), (3,)])
+def test_copies_in_a_stack_of_value_pools(lead):
+    v = torch.arange(24, device="cuda", dtype=torch.float32).view(*lead, -1, 1, 1, 1, 1) if lead else torch.arange(24., device="cuda").view(-1, 1, 1, 1, 1)
+    v = v.expand(*v.shape[:len(lead) + 1], 2, 4, 64, 4).contiguous()
+    want = v.clone()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    mlxq.copy_pages(v, i32(0, 5), i32(2, 1))
+    at = (slice(None),) * len(lead)
+    want[(*at, 2)], want[(*at, 1)] = want[(*at, 0)].clone(), want[(*at, 5)].clone()
+    assert torch.equal(v, want)
