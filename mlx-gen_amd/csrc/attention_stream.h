@@ -149,46 +149,41 @@ __device__ __forceinline__ void poison(const Batch& bt, const int32_t* table, in
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-constexpr float kNearCap = 256.0f;
-
 // What happens to a score before the softmax: nothing, a cap, or a bias by distance (capped before it if
-// softcap is set).
-enum Bend : int { kPlain = 0, kCap = 1, kBias = 2 };
+// softcap is set).  kFar: a cap past kNearCap, in 16-bit types, and then the bias if there is one.
+enum Bend : int { kPlain = 0, kCap = 1, kBias = 2, kFar = 3 };
+constexpr float kNearCap = 256.0f;
 // A capped or biased score, in units of log 2, from q.k and the distance of key and row.  With x = score / cap, cap tanh(x) is
 // cap - 2 cap / (exp(2 x) + 1), in 16-bit types with the hardware's exponential and reciprocal, off by up to 5 2^-24 cap: up to
-// kNearCap less than a third of what rounding a weight to fp16 is.  FAR: caps above, where |x| < 1/4 by the first four terms of
+// kNearCap less than a third of what rounding a weight to fp16 is.  Past it, where |x| < 1/4, it is the first four terms of
 // tanh's series times the cap, score (1 - x^2/3 + 2 x^4/15 - 17 x^6/315), off by 6 2^-24 of the score, whatever the
-// cap (7001 tokens at once, 32 + 8 heads of 128: 590 us, near caps 475, no cap 410).
-// y = AttnArgs::cap_scale q.k is 2 x in units of log 2; cap2 is the cap in those units.
-template <typename T, int BEND, bool FAR>
+// cap.  As kernels of its own, since both in one take registers from the nearer caps.
+// AttnArgs::scale is 2 scale / (cap ln 2) with a cap, so that z is 2 x in units of log 2, and scale / ln 2 without, as
+// score_scale always is; cap2 is softcap / ln 2.
+template <typename T, int BEND>
 __device__ __forceinline__ float bent_score(const AttnArgs& a, float qk, float slope2, float distance) {
+  constexpr float kHalf = 0.34657359027997265f;  // ln 2 / 2: x = kHalf z
   float z = qk * a.scale;
-  if (BEND == kCap || a.softcap > 0.0f) {
-    constexpr float kHalf = 0.34657359027997265f;  // ln 2 / 2: x = kHalf y
-    const float y = qk * a.cap_scale;
+  if (BEND == kCap || BEND == kFar || a.softcap > 0.0f) {
     if constexpr (sizeof(T) == 4) {
-      z = a.cap2 * tanhf(y * kHalf);
+      z = a.cap2 * tanhf(z * kHalf);
     } else {
-      const float bent = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.0f), a.cap2);
-      constexpr float c1 = -kHalf * kHalf / 3.0f, c2 = 2.0f * kHalf * kHalf * kHalf * kHalf / 15.0f,
-                      c3 = -17.0f * kHalf * kHalf * kHalf * kHalf * kHalf * kHalf / 315.0f;
-      const float t = y * y, series = fmaf(z * t, fmaf(t, fmaf(t, c3, c2), c1), z);
-      z = FAR && fabsf(y) < 0.25f / kHalf ? series : bent;
+      const float bent = fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.0f), a.cap2);
+      if constexpr (BEND == kFar) {
+        constexpr float h2 = kHalf * kHalf, c1 = -h2 / 3.0f, c2 = 2.0f * h2 * h2 / 15.0f, c3 = -17.0f * h2 * h2 * h2 / 315.0f;
+        const float score = qk * a.score_scale, t = z * z, series = fmaf(score * t, fmaf(t, fmaf(t, c3, c2), c1), score);
+        z = fabsf(z) < 0.25f / kHalf ? series : bent;
+      } else {
+        z = bent;
+      }
     }
   }
-  if constexpr (BEND == kBias) z = fmaf(-slope2, fabsf(distance), z);
+  if constexpr (BEND == kBias || BEND == kFar) z = fmaf(-slope2, fabsf(distance), z);
   return z;
 }
-
-template <bool B>
-struct BoolConstant {
-  static constexpr bool value = B;
-};
-// f(FAR), by the call's cap.
-template <typename T, int BEND, typename F>
-__device__ __forceinline__ void by_cap(const AttnArgs& a, F f) {
-  if (sizeof(T) == 2 && BEND != kPlain && a.softcap > kNearCap) f(BoolConstant<true>{});
-  else f(BoolConstant<false>{});
+template <int BEND>
+__device__ __forceinline__ float slope_of(const AttnArgs& a, int qh) {
+  return BEND == kBias || (BEND == kFar && a.slopes) ? a.slopes[qh] * kLog2e : 0.0f;
 }
 
 // The rows that a lane's row index stands for, and what they see.
@@ -327,7 +322,7 @@ __global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream
       place[m] = p;
       lo[m] = rr.lo;
       span[m] = max(rr.hi - rr.lo, 0);
-      slope[m] = BEND == kBias ? a.slopes[qh] * kLog2e : 0.0f;
+      slope[m] = slope_of<BEND>(a, qh);
       const T* q = (const T*)a.q.p + (s.q0 + i) * a.q.ts + qh * a.q.hs;
 #pragma unroll
       for (int k = 0; k < NS; ++k) qf[m][k] = FULL || (4 * k + g) * C < D ? load_chunk(q + (4 * k + g) * C) : u32x4{0, 0, 0, 0};
@@ -365,20 +360,18 @@ __global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream
       const int key0 = u * KU + 4 * g;
       const bool part = u * KU < kr.lo_all || (u + 1) * KU > kr.hi_all;
       if (BEND != kPlain || part) {
-        by_cap<T, BEND>(a, [&](auto FAR) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int j = key0 + 16 * t + i;
-                float v = st[m][t][i];
-                if constexpr (BEND != kPlain) v = bent_score<T, BEND, decltype(FAR)::value>(a, v, slope[m], (float)(j - place[m]));
-                if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
-                st[m][t][i] = v;
-              }
-        });
+            for (int i = 0; i < 4; ++i) {
+              const int j = key0 + 16 * t + i;
+              float v = st[m][t][i];
+              if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope[m], (float)(j - place[m]));
+              if (part) v = (unsigned)(j - lo[m]) < (unsigned)span[m] ? v : -INFINITY;
+              st[m][t][i] = v;
+            }
       }
       u32x4 pf[MT];
 #pragma unroll
@@ -512,6 +505,12 @@ __global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream
 template <typename T, int DT, int MT, bool FULL>
 static int launch_stream_of(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
   const dim3 grid((unsigned)plan.blocks);
+  if constexpr (sizeof(T) == 2) {
+    if (a.softcap > kNearCap) {
+      hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kFar, FULL>), grid, dim3(256), 0, st, a);
+      return check_launch("paged_attention");
+    }
+  }
   if (a.slopes) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kBias, FULL>), grid, dim3(256), 0, st, a);
   else if (a.softcap > 0.0f) hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kCap, FULL>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attn_stream_kernel<T, DT, MT, kPlain, FULL>), grid, dim3(256), 0, st, a);

@@ -85,6 +85,11 @@ __device__ __forceinline__ void read_and_multiply(R read, U use) {
 // The largest sum of weights that a lane takes from a tile: fp16's weights end at 2^16.
 constexpr float kMost = 32768.0f;
 
+template <bool B>
+struct BoolConstant {
+  static constexpr bool value = B;
+};
+
 template <typename T, int DT, int BEND>
 __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
   constexpr bool ACC = DT > 128;  // 500 tokens, 16 heads of 256, a window of 4096: 75 us instead of 83
@@ -164,7 +169,7 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
   const int r = min(wr0 + c, row1), tok = a.by_g.div(r), qh = h * a.G + (r - tok * a.G), place = s.L - s.n + tok;
   const RowRange rr = row_range(a, s, place, prefix);
   const int lo[1] = {rr.lo}, span[1] = {max(rr.hi - rr.lo, 0)};
-  const float slope = BEND == kBias ? a.slopes[qh] * kLog2e : 0.0f;
+  const float slope = slope_of<BEND>(a, qh);
   u32x4 qf[NS];
   const T* q = (const T*)a.q.p + (s.q0 + tok) * a.q.ts + qh * a.q.hs;
 #pragma unroll
@@ -205,18 +210,16 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     products(t, st);
     if constexpr (BEND != kPlain || PART) {
       const float away = (float)(t * KT + 8 * half - place);
-      by_cap<T, BEND>(a, [&](auto FAR) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+      for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = 32 * k + 16 * (r >> 3) + (r & 7), j = t * KT + 8 * half + i;
-            float v = st[k][r];
-            if constexpr (BEND != kPlain) v = bent_score<T, BEND, decltype(FAR)::value>(a, v, slope, away + (float)i);
-            if constexpr (PART) v = (unsigned)(j - lo[0]) < (unsigned)span[0] ? v : -INFINITY;
-            st[k][r] = v;
-          }
-      });
+        for (int r = 0; r < 16; ++r) {
+          const int i = 32 * k + 16 * (r >> 3) + (r & 7), j = t * KT + 8 * half + i;
+          float v = st[k][r];
+          if constexpr (BEND != kPlain) v = bent_score<T, BEND>(a, v, slope, away + (float)i);
+          if constexpr (PART) v = (unsigned)(j - lo[0]) < (unsigned)span[0] ? v : -INFINITY;
+          st[k][r] = v;
+        }
     }
     // Weights against the reference that the row has.  The maximum is looked for only where that gives a sum of
     // weights past kMost (or no key was seen before): far from overflow in the types, and as exact.
@@ -381,7 +384,8 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
 template <typename T, int DT>
 static int launch_tile(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
   const dim3 grid((unsigned)plan.blocks, (unsigned)a.S);
-  if (a.slopes) hipLaunchKernelGGL((attn_tile_kernel<T, DT, kBias>), grid, dim3(256), 0, st, a);
+  if (a.softcap > kNearCap) hipLaunchKernelGGL((attn_tile_kernel<T, DT, kFar>), grid, dim3(256), 0, st, a);
+  else if (a.slopes) hipLaunchKernelGGL((attn_tile_kernel<T, DT, kBias>), grid, dim3(256), 0, st, a);
   else if (a.softcap > 0.0f) hipLaunchKernelGGL((attn_tile_kernel<T, DT, kCap>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attn_tile_kernel<T, DT, kPlain>), grid, dim3(256), 0, st, a);
   return check_launch("paged_attention");

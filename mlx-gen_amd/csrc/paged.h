@@ -167,8 +167,8 @@ struct AttnArgs {
   int items;
   int S, chunk;       // splits of a sequence's tokens, tokens in each (a multiple of 128; the last takes the rest)
   Divisor by_chunk;
-  float scale;          // multiplies q.k into units of log 2
-  float softcap, cap2, cap_scale;  // 0: none; see bent_score
+  float scale;          // multiplies q.k into units of log 2 (with a cap: see bent_score)
+  float softcap, cap2, score_scale;  // softcap 0: none; see bent_score
   int causal, window, direct;  // direct: item u is the u-th sequence, else by Finder
   const int32_t* prefix;
   const float *slopes, *sinks;

@@ -327,13 +327,13 @@ int mlxq_paged_attention(const mlxq_heads* q, int64_t T, const mlxq_paged_cache*
   a.by_g = Divisor(a.G);
   a.by_items = Divisor(a.items);
   const double log2e = 1.44269504088896341;
-  a.scale = (float)(o->scale * log2e);
+  a.scale = a.score_scale = (float)(o->scale * log2e);
   if (o->softcap > 0.0f) {
-    // Caps past 1e30 are as far out of every score's reach; cap2 and, for small caps, cap_scale stay finite.
+    // Caps past 1e30 are as far out of every score's reach; cap2 and, for small caps, the scale stay finite.
     const double cap = std::min((double)o->softcap, 1e30);
     a.softcap = (float)cap;
     a.cap2 = (float)(cap * log2e);
-    a.cap_scale = (float)std::min(2.0 * o->scale / cap * log2e, 3.4e38);
+    a.scale = (float)std::min(2.0 * o->scale / cap * log2e, 3.4e38);
   }
   a.causal = o->causal != 0;
   a.window = (int)window_of(o);
