@@ -343,7 +343,8 @@ typedef struct {
 /* The sequences of a step.  Sequence b owns the new tokens q_starts[b] .. q_starts[b+1] - 1 of the
  * step's T (n of them, 0 allowed) and has kv_lens[b] tokens in the cache counting those: the i-th new
  * one is its token kv_lens[b] - n + i.  Token j lies in page block_tables[b * table_stride +
- * j / page_size].  All arrays are device int32; lengths past table_width pages are cut there.
+ * j / page_size].  All arrays are device int32.  A token past table_width pages (or past 2^30 - 16) has no
+ * page: it is not written, and rows that see it become NaN.
  * max_q and max_kv are what the launch is planned for (the longest n and kv length expected):
  * results do not depend on them.  Steps' tokens outside every sequence are left alone. */
 typedef struct {

@@ -186,13 +186,18 @@ __device__ __forceinline__ float slope_of(const AttnArgs& a, int qh) {
   return BEND == kBias || (BEND == kFar && a.slopes) ? a.slopes[qh] * kLog2e : 0.0f;
 }
 
-// The rows that a lane's row index stands for, and what they see.
+// What a row sees of the tokens that have a page.
 struct RowRange {
   int lo, hi;
 };
 __device__ __forceinline__ RowRange row_range(const AttnArgs& a, const Seq& s, int p, int prefix) {
-  const int hi = a.causal ? min(s.L, max(p + 1, prefix)) : s.L;
+  const int hi = a.causal ? min(s.paged, max(p + 1, prefix)) : s.paged;
   return {a.window ? max(0, p + 1 - a.window) : 0, hi};
+}
+// Where the sum of weights of the row at place p starts: at NaN, which stays, if the row sees a token past the table.
+__device__ __forceinline__ float first_sum(const AttnArgs& a, const Seq& s, int p, int prefix) {
+  if (s.L == s.paged) return 0.0f;
+  return !a.causal || max(p + 1, prefix) > s.paged ? __builtin_nanf("") : 0.0f;
 }
 
 // First to last key that any row of [row0, row1] sees, those that every one sees, and this split's.
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(256, stream_waves<T>(DT * MT, MT)) void attn_stream
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       ref[m] = -INFINITY;
-      sum[m] = 0.0f;
+      sum[m] = first_sum(a, s, place[m], prefix);
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[m][d] = f32x4{0, 0, 0, 0};
     }

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256, DT <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     else asm volatile("" : "+v"(qf[k]));
   }
   f32x16 o[ND];
-  float ref = -INFINITY, sum[1] = {0.0f};
+  float ref = -INFINITY, sum[1] = {first_sum(a, s, place, prefix)};
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll

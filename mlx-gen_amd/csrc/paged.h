@@ -84,21 +84,23 @@ struct Batch {
   const int32_t* kv_lens;
   int64_t table_stride;
   int B, T;
-  int capacity;   // tokens that the table's width names
+  int capacity;   // tokens that the table's width names, a multiple of 16 below 2^30; those past it have no page
   int page_log2;  // log2(page_size)
   int pages;
 };
 
-// One sequence: its new tokens are [q0, q0 + n) of the step and places [L - n, L) of the sequence.
+// One sequence: its new tokens are [q0, q0 + n) of the step and places [L - n, L) of the sequence, of which those below
+// `paged` have a page.
 struct Seq {
-  int q0, n, L;
+  int q0, n, L, paged;
 };
 
 __device__ __forceinline__ Seq load_seq(const Batch& a, int b) {
   int s = a.q_starts[b], e = a.q_starts[b + 1], L = a.kv_lens[b];
   s = min(max(s, 0), a.T);
   e = min(max(e, s), a.T);
-  return {s, e - s, min(max(L, 0), a.capacity)};
+  L = min(max(L, 0), 0x7fffffe0);  // a place and the end of its block fit 31 bits
+  return {s, e - s, L, min(L, a.capacity)};
 }
 
 // Sequences cut into units (blocks of tokens, tiles of rows, ranges of keys): finds the sequence of a unit and the

@@ -101,8 +101,8 @@ Batch view(const mlxq_paged_batch* b, const mlxq_paged_cache* c, int64_t T) {
   r.B = (int)b->sequences;
   r.T = (int)T;
   while ((1 << r.page_log2) < c->page_size) ++r.page_log2;
-  // Places are kept below 2^30, so that a place plus a tile never passes 31 bits.
-  r.capacity = (int)std::min<int64_t>(b->table_width * c->page_size, 0x3fffffff);
+  // Places with a page are kept below 2^30, so that a place plus a tile never passes 31 bits.
+  r.capacity = (int)std::min<int64_t>(b->table_width * c->page_size, 0x3ffffff0);
   r.pages = (int)c->pages;
   return r;
 }

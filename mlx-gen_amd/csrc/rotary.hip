@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int p0 = max(blk * 16, s.L - s.n), p1 = min(blk * 16 + 16, s.L), nt = p1 - p0;
     const int64_t t0 = s.q0 + (p0 - (s.L - s.n));
     int page = -1;
-    if (blk >= 0) page = bt.tables[b * bt.table_stride + (blk >> (bt.page_log2 - 4))];
+    if (blk >= 0 && blk < bt.capacity >> 4) page = bt.tables[b * bt.table_stride + (blk >> (bt.page_log2 - 4))];
     const bool write = (unsigned)page < (unsigned)bt.pages;
     const int64_t in_page = ((int64_t)h << bt.page_log2) * D + (int64_t)(blk & ((1 << (bt.page_log2 - 4)) - 1)) * 16 * D;
     T* kb = (T*)a.k_cache + page * a.k_page + in_page;
