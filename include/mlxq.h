@@ -309,8 +309,11 @@ int mlxq_cast(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t 
  * the reference, whose attention runs in MLX (mlx-gen-sensenova/src/qwen3.rs:463, forward_cached).
  *
  * Queries, keys, values, cache and result have one dtype (f32, bf16 or fp16).  Scores, softmax
- * statistics and sums are f32; 16-bit types round the softmax weights to the type before the
- * product with the values, and the result once.
+ * statistics and sums are f32, and the result is rounded once.  f32 rounds nothing between.  16-bit
+ * types round the softmax weights to the type before the product with the values: weights are taken
+ * against a running maximum, so that fp16's below 2^-25 of it are 0.  Chunks (more than 32 rows, pairs
+ * of a token and a query head, a key head; 16 for heads past 128) sum the rounded weights, shorter calls
+ * the f32 ones: the same row may differ between the two by what that rounding is.
  *
  * Cache: a pool of pages of page_size tokens, one pool for a layer's keys and one for its values.
  * With C = 16 / sizeof(element) (8 for 16-bit types, 4 for f32), page p of the keys starts
@@ -345,8 +348,9 @@ typedef struct {
  * one is its token kv_lens[b] - n + i.  Token j lies in page block_tables[b * table_stride +
  * j / page_size].  All arrays are device int32.  A token past table_width pages (or past 2^30 - 16) has no
  * page: it is not written, and rows that see it become NaN.
- * max_q and max_kv are what the launch is planned for (the longest n and kv length expected):
- * results do not depend on them.  Steps' tokens outside every sequence are left alone. */
+ * max_q and max_kv are what the launch is planned for (the longest n and kv length expected): any values
+ * give right results, which differ in their last bits where the plan sums in another order.  Steps' tokens
+ * outside every sequence are left alone. */
 typedef struct {
   const int32_t* block_tables;
   const int32_t* q_starts;  /* [sequences + 1], not decreasing */
@@ -417,7 +421,8 @@ typedef struct {
   float scale;                 /* > 0: z_j = scale * q.k_j */
   int causal;
   int64_t window;              /* 0 = none; counts the token itself */
-  float softcap;               /* 0 = none; z_j = softcap * tanh(z_j / softcap) */
+  float softcap;               /* 0 = none; z_j = softcap * tanh(z_j / softcap), any finite one; 16-bit types
+                                * are off by up to 5 2^-24 softcap of a score for caps up to 256 */
   const int32_t* prefix_lens;  /* [sequences] or NULL: tokens that every row of the sequence sees */
   const float* alibi_slopes;   /* [q heads] or NULL: z_j -= slope * |p - j|, after the cap */
   const float* sinks;          /* [q heads] or NULL: a score without a value, in the denominator only */
@@ -430,7 +435,8 @@ typedef struct {
  * zero for a row that sees nothing.  Query head h reads key head h / (q heads / cache heads).  What the
  * masked and unwritten places of the cache hold (NaN and infinities included) does not reach the
  * result.  out must not overlap q.  workspace: mlxq_paged_attention_workspace_size() bytes, whatever
- * they hold (NULL when that is 0).  Launch shapes follow T, the batch's sizes and hints and the strides
+ * they hold (NULL when that is 0), at most some 300 MB.  T * (q heads / cache heads) must be below 2^31 - 128.
+ * Launch shapes follow T, the batch's sizes and hints and the strides
  * only, so a captured graph may be replayed with other lengths and tables.
  */
 size_t mlxq_paged_attention_workspace_size(int64_t T, int64_t q_heads, const mlxq_paged_cache* cache,

@@ -224,8 +224,12 @@ __device__ __forceinline__ u32x4 even_keys(u32x4 v) {
   return v;
 }
 
-// Waves a SIMD for DT * MT = d: as many as the registers hold without spilling; two row tiles of 128 features spill a dozen
-// and are faster so all the same (8 sequences of 4 tokens over up to 4000, 32 + 4 heads: 23.5 us, one wave 28.9).
+// Waves a SIMD for DT * MT = d: as many as the registers hold without spilling, and one step more in two places that are
+// faster with spills (16-bit types; narrower heads, caps and biases spill more than full heads).  Two row tiles of 128
+// features, 12 to 66 registers: 8 sequences of 4 tokens over 4000, 32 + 4 heads, bf16 23.4 us, fp16 24.1, one wave a SIMD
+// 28.6 and 28.9, and 19 to 37 % more with a cap, a bias or heads of 112.  One of 64 features at four waves, 0 to 28
+// registers: 49 sequences of 300 to 6000 tokens, 64 + 8 heads, bf16 34.8 us, fp16 35.7, three waves 37.8 and 38.5; 8 of
+// 5000 and 32 of 777 tokens within 6 % either way.
 template <typename T>
 constexpr int stream_waves(int d, int mt = 1) {
   if (sizeof(T) == 4) return d <= 80 ? 3 : d <= 128 ? 2 : 1;

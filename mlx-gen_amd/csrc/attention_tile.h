@@ -12,7 +12,7 @@
 // Bound by the matrix cores and, nearly as much, by the exponentials (a quarter-rate instruction each) and the LDS
 // reads, one for every product.  7001 tokens, 32 + 8 bf16 heads of 128: 385-395 us, 1020-1045 TFLOP/s, 90 % of what a
 // large bf16 product reaches.  Heads past 128 have one wave a SIMD and wait for their own chain of products and
-// exponentials: 500 tokens, 16 + 8 heads of 256 over a window of 4096, capped, in four splits: 63 us and 8 for the join.
+// exponentials: 500 tokens, 16 + 8 heads of 256 over a window of 4096, capped, in four splits: 64-73 us, 8 of them the join.
 #pragma once
 
 #include "attention_stream.h"

@@ -167,7 +167,7 @@ struct AttnArgs {
   int Hkv, G, D;
   Divisor by_hkv, by_g, by_items;  // by_items: (tile, head) pairs of the streaming kernel's grid
   int items;
-  int S, chunk;       // splits of a sequence's tokens, tokens in each (a multiple of 128; the last takes the rest)
+  int S, chunk;       // splits of a sequence's tokens, tokens in each (a multiple of 128, tiled of 64; the last takes the rest)
   Divisor by_chunk;
   float scale;          // multiplies q.k into units of log 2 (with a cap: see bent_score)
   float softcap, cap2, score_scale;  // softcap 0: none; see bent_score

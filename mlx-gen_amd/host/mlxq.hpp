@@ -267,7 +267,7 @@ Array rotary(const Array& x, const Array& positions, const Array& table, bool in
 std::pair<std::vector<int64_t>, std::vector<int64_t>> cache_shapes(int64_t pages, int64_t heads, int64_t page_size,
                                                                    int64_t head_dim, Dtype dt);
 // The sequences of a step: block_tables [B, width], q_starts [B + 1] and kv_lens [B] (int32), and the longest
-// number of new and of cached tokens that launches are planned for (results do not depend on them).
+// number of new and of cached tokens that launches are planned for (any values give right results, up to the last bits).
 struct CacheBatch {
   Array block_tables, q_starts, kv_lens;
   int64_t max_q = 1, max_kv = 1;

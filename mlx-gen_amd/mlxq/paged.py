@@ -31,7 +31,7 @@ _BOUNDS = {"yarn": (1.0, 32.0), "llama3": (1.0, 4.0)}
 class CacheBatch(NamedTuple):
     """The sequences of a step: block_tables [B, width], q_starts [B + 1] and kv_lens [B] (int32, on the
     GPU), and the longest number of new tokens and of cached tokens that the launches are planned for
-    (results do not depend on those two)."""
+    (any values give right results; where a plan sums in another order they differ in the last bits)."""
     block_tables: torch.Tensor
     q_starts: torch.Tensor
     kv_lens: torch.Tensor
@@ -168,7 +168,8 @@ def rotary_table(positions: int, inv_freq: torch.Tensor, magnitude: float = 1.0,
 
 def rotary(x, positions, table, interleaved: bool = False, inverse: bool = False, out=None):
     """x [T, heads, D] with its first 2 * table.shape[1] features turned by positions [T] (int32): pairs
-    (i, i + half), or neighbours when interleaved.  inverse turns back: the gradient of x from y's.  out may be x."""
+    (i, i + half), or neighbours when interleaved.  inverse turns back: the gradient of x from y's (as with the other
+    operators, autograd records nothing by itself).  out may be x."""
     if out is None:
         y = _lib.fast().rotary(x, positions, table, interleaved, inverse)
         if y is not None:
