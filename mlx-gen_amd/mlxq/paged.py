@@ -316,7 +316,8 @@ class PagedCache:
     holders.  A step: `batch` makes room for its new tokens and returns the CacheBatch for cache_append and
     paged_attention of every layer.  fork() shares a sequence's full pages and copies its last, partly filled
     one; a page that several sequences hold is never written.  free() gives pages back; compact() moves the
-    held pages to the front of the pool.  Calls on one cache are ordered on the current stream."""
+    held pages to the front of the pool.  A call that fails changes nothing.  Calls on one cache are ordered on the
+    current stream."""
 
     def __init__(self, layers: int, pages: int, heads: int, head_dim: int, page_size: int = 16, dtype=torch.bfloat16,
                  device="cuda"):
@@ -367,9 +368,15 @@ class PagedCache:
             self._holders[p] = 1
         return got
 
+    def _drop(self, pages):
+        for p in pages:
+            self._holders[p] -= 1
+            if self._holders[p] == 0:
+                self._free.append(p)
+        self._free.sort(reverse=True)
+
     def batch(self, seqs, new) -> CacheBatch:
-        """Room for new[i] tokens of seqs[i], and the step's CacheBatch.  Nothing changes when the pool has too
-        few free pages."""
+        """Room for new[i] tokens of seqs[i], and the step's CacheBatch."""
         seqs, new = list(seqs), [int(n) for n in new]
         if not seqs or len(seqs) != len(new) or min(new) < 0 or len(set(seqs)) != len(seqs):
             _bad("PagedCache.batch", "one number of new tokens is needed for each of some different sequences")
@@ -379,13 +386,17 @@ class PagedCache:
             need.append(-(-(length + n) // self.page_size) - len(pages))
         if sum(need) > len(self._free):
             _bad("PagedCache.batch", f"{sum(need)} pages are needed and {len(self._free)} are free")
-        for s, n, more in zip(seqs, new, need):
-            pages, length = self._seqs[s]
-            self._seqs[s] = (pages + self._take(more), length + n)
-        return self._describe(seqs, new)
+        got = [self._take(more) for more in need]
+        held = [(self._seqs[s][0] + pages, self._seqs[s][1] + n) for s, n, pages in zip(seqs, new, got)]
+        try:
+            step = self._describe(held, new)
+        except BaseException:
+            self._drop([p for pages in got for p in pages])
+            raise
+        self._seqs.update(zip(seqs, held))
+        return step
 
-    def _describe(self, seqs, new):
-        held = [self._seqs[s] for s in seqs]
+    def _describe(self, held, new):
         width = max(max(len(p) for p, _ in held), 1)
         rows = [p + [-1] * (width - len(p)) for p, _ in held]
         starts = [0]
@@ -393,7 +404,7 @@ class PagedCache:
             starts.append(starts[-1] + n)
         lens = [n for _, n in held]
         flat = torch.tensor([*starts, *lens, *(p for r in rows for p in r)], dtype=torch.int32).to(self.pool.device)
-        B = len(seqs)
+        B = len(held)
         return CacheBatch(flat[2 * B + 1:].view(B, width), flat[:B + 1], flat[B + 1:2 * B + 1], max(new), max(lens))
 
     def fork(self, seqs):
@@ -403,19 +414,21 @@ class PagedCache:
         part = [n % self.page_size != 0 for _, n in held]
         if sum(part) > len(self._free):
             _bad("PagedCache.fork", f"{sum(part)} pages are needed and {len(self._free)} are free")
-        ids, src, dst = [], [], []
+        src = [pages[-1] for (pages, _), copied in zip(held, part) if copied]
+        dst = self._take(len(src))
+        try:
+            if src:
+                self._copy(src, dst)
+        except BaseException:
+            self._drop(dst)
+            raise
+        ids, copies = [], iter(dst)
         for (pages, length), copied in zip(held, part):
-            mine = list(pages)
-            if copied:
-                src.append(mine[-1])
-                mine[-1] = self._take(1)[0]
-                dst.append(mine[-1])
-            for p in mine[:-1] if copied else mine:
+            shared = pages[:-1] if copied else list(pages)
+            for p in shared:
                 self._holders[p] += 1
             ids.append(self.new())
-            self._seqs[ids[-1]] = (mine, length)
-        if src:
-            self._copy(src, dst)
+            self._seqs[ids[-1]] = (shared + [next(copies)] if copied else shared, length)
         return ids
 
     def _copy(self, src, dst, tables=None):
@@ -426,11 +439,7 @@ class PagedCache:
         """Forgets a sequence; pages that no other holds are free again."""
         pages, _ = self._of("PagedCache.free", seq)
         del self._seqs[seq]
-        for p in pages:
-            self._holders[p] -= 1
-            if self._holders[p] == 0:
-                self._free.append(p)
-        self._free.sort(reverse=True)
+        self._drop(pages)
 
     def truncate(self, seq: int, length: int) -> None:
         """Drops a sequence's tokens from `length` on (rejected drafts).  A page cut short that other sequences
@@ -441,19 +450,20 @@ class PagedCache:
         keep = -(-length // self.page_size)
         mine = pages[:keep]
         last = pages[keep:]
-        shared = length % self.page_size and self._holders[mine[-1]] > 1
-        if shared and not self._free and all(self._holders[p] > 1 for p in last):
-            _bad("PagedCache.truncate", "1 page is needed and 0 are free")
-        for p in last:
-            self._holders[p] -= 1
-            if self._holders[p] == 0:
-                self._free.append(p)
-        if shared:
-            copy = self._take(1)[0]
-            self._copy([mine[-1]], [copy])
-            self._holders[mine[-1]] -= 1
-            mine[-1] = copy
-        self._free.sort(reverse=True)
+        if length % self.page_size and self._holders[mine[-1]] > 1:
+            # The copy goes to a page that the sequence gives back, if there is one.
+            copy = next((p for p in reversed(last) if self._holders[p] == 1), None)
+            if copy is None and not self._free:
+                _bad("PagedCache.truncate", "1 page is needed and 0 are free")
+            to = self._free[-1] if copy is None else copy
+            self._copy([mine[-1]], [to])
+            if copy is None:
+                self._take(1)
+            else:
+                last.remove(copy)
+            last.append(mine[-1])
+            mine[-1] = to
+        self._drop(last)
         self._seqs[seq] = (mine, length)
 
     def compact(self, block_tables=None) -> int:
