@@ -110,7 +110,7 @@ AttnPlan plan_attention(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype
   // three on every CU, of at least 128 tokens (a unit for each wave: one token over 777, 8 heads: 9.5 us; 256: 10.1, one
   // split: 10.3) or 256 (tiled).  One row tile a sequence: of at most 768, since the sequences of a step are of unequal
   // length and the workgroups of a long one fill the chip more evenly (48 of up to 6000 tokens: 24.1 us, with 1024 25.3, with
-  // 4096 39.3; one of 150001: 68.2, 71.7; 16 of up to 20000, most of them short: 44.9, with 8192 64.6).  Nine other shapes
+  // 4096 39.3; one of 150001: 68.2, 71.7; 16 of up to 20000, most of them short: 44.9, with 8192 64.6).  Eight other shapes
   // in bf16 and fp16 are within 6 % of the best of 384 to 8192; f32 likes longer ones (12 of up to 9000: 50.9, with 2048 43.6).
   int64_t range = std::min<int64_t>(max_kv, 0x3fffff80);  // places end at 2^30
   // With a window a tile's rows see as many tokens as it holds and one for each of theirs, or, where they see all later
