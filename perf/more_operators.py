@@ -1,0 +1,585 @@
+"""Operators of a packed decoder block in microscaled types, and the work they are measured by.
+
+Five operators: quantisation to microscaled 4- and 8-bit floating point (and back); the product of two
+such tensors; root-mean-square norms with the residual's addition, their 8-bit results and their
+gradient; the routing of tokens to experts and its gradient; and the products of the experts that each
+token was routed to.  Every case is a dict of plain values; prepare() makes what a program holds before
+the call, run() makes one call, either in plain torch operations (own False) or through the framework
+(own True), exact() gives the result in 64 bits.
+
+A microscaled tensor is (codes, scales): blocks of 32 values along the last dimension share a scale, a
+byte b that stands for 2^(b - 127) (255: NaN).  Codes are e2m1, two to a uint8, low half first, or
+float8_e4m3fn.  A block's scale is the smallest power of two, from 2^-127 on, by which its largest magnitude
+divided is at most the code's largest value (6 or 448); values are rounded to nearest, ties to even; a
+block with an infinity or a NaN has scale 255.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32, "f16": torch.float16}
+#: bits of a value with its share of the scale, over eight
+_BYTES = {"e2m1": 17 / 32, "e4m3": 33 / 32}
+
+
+def _framework():
+    pkg = os.path.join(os.getcwd(), "mlx-gen_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import mlxq
+    return mlxq
+
+
+def _quantize(name, rows, K, format, dtype="bf16"):
+    return {"name": name, "kind": "quantize", "rows": rows, "K": K, "format": format, "dtype": dtype}
+
+
+def _product(name, M, K, N, format="e4m3", dtype="bf16", bias=False):
+    return {"name": name, "kind": "product", "M": M, "K": K, "N": N, "format": format, "dtype": dtype, "bias": bias}
+
+
+def _norm(name, T, H, D, dtype="bf16", residual=False, mx=False, weight=True):
+    return {"name": name, "kind": "norm", "T": T, "H": H, "D": D, "dtype": dtype, "residual": residual, "mx": mx,
+            "weight": weight}
+
+
+def _norm_grad(name, T, H, D, dtype="bf16", residual=False, weight=True):
+    return {"name": name, "kind": "norm_grad", "T": T, "H": H, "D": D, "dtype": dtype, "residual": residual,
+            "weight": weight}
+
+
+def _route(name, T, E, k, scoring="softmax", dtype="bf16", bias=False, groups=1, kept=1, best=1, normalize=True,
+           scale=1.0, active=False, grad=False):
+    return {"name": name, "kind": "route_grad" if grad else "route", "T": T, "E": E, "k": k, "scoring": scoring,
+            "dtype": dtype, "bias": bias, "groups": groups, "kept": kept, "best": best, "normalize": normalize,
+            "scale": scale, "active": active}
+
+
+def _experts(name, T, E, k, K, N, format="e4m3", dtype="bf16", bias=False, combine=False, routed=False):
+    return {"name": name, "kind": "experts", "T": T, "E": E, "k": k, "K": K, "N": N, "format": format, "dtype": dtype,
+            "bias": bias, "combine": combine, "routed": routed}
+
+
+def listed():
+    return [
+        # A prompt's activations to 8 bits before a product, and back.
+        _quantize("quantize_prompt", 4099, 5120, "e4m3"),
+        # A weight of a checkpoint in f32 packed to 4 bits, and back.
+        _quantize("quantize_weight", 5119, 13824, "e2m1", dtype="f32"),
+        # One token through a packed projection: latency and the weight's bytes.
+        _product("product_one", 1, 4096, 6144),
+        # A prompt of a text encoder, 4-bit activations, rows that fill no tile and a last block of K that fills no
+        # step, with a bias, to f32.
+        _product("product_ragged", 173, 2912, 5152, format="e2m1", dtype="f32", bias=True),
+        # A long prompt through an MLP's projection.  The most arithmetic.
+        _product("product_prompt", 8190, 4096, 14336),
+        # A decode step of five sequences: the block's residual is added, the norm goes to 8 bits.  The smallest call.
+        _norm("norm_step", 5, 1, 4096, residual=True, mx=True),
+        # Norms of the query heads of a prompt, slices of one projection's output, fp16.
+        _norm("norm_heads", 4096, 32, 128, dtype="f16"),
+        # The gradient of a training batch's norm, with the gradient that arrives on the residual.
+        _norm_grad("norm_grad", 8190, 1, 5120, residual=True),
+        # A decode step of 17 tokens over 128 experts in groups, sigmoid scores with a bias for balance.
+        _route("route_step", 17, 128, 8, scoring="sigmoid", bias=True, groups=8, kept=4, best=2, scale=2.5, dtype="f32"),
+        # The gradient of a training batch's routing weights.
+        _route("route_grad", 16381, 256, 8, grad=True),
+        # A decode step of three tokens through the experts that they were routed to.
+        _experts("experts_step", 3, 32, 4, 2880, 5760, bias=True),
+        # A padded batch of prompts routed and through the experts' second projection, summed with the routing weights.
+        _experts("experts_prompt", 4090, 32, 4, 2880, 2880, bias=True, combine=True, routed=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["quantize", "product", "product", "norm", "norm", "norm_grad", "route", "route_grad", "experts",
+                       "experts"])
+    dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
+    format = rng.choice(["e4m3", "e4m3", "e2m1"])
+    wide = 32 * _log(rng, 4, 256)
+    if kind == "quantize":
+        c = _quantize(None, _log(rng, 1, 5000), 32 * _log(rng, 1, 420), format, dtype)
+    elif kind == "product":
+        c = _product(None, _log(rng, 1, 6000), wide, _log(rng, 16, 12000), format, dtype, rng.random() < 0.4)
+    elif kind in ("norm", "norm_grad"):
+        if rng.random() < 0.3:
+            H, D, T = rng.randint(1, 40), rng.choice([64, 80, 96, 128, 256]), _log(rng, 1, 6000)
+        else:
+            H, D, T = 1, rng.choice([32 * _log(rng, 2, 400), _log(rng, 33, 9000)]), _log(rng, 1, 9000)
+        T = min(T, 40000000 // (H * D))
+        residual, weight = rng.random() < 0.5, rng.random() < 0.85
+        if kind == "norm":
+            c = _norm(None, T, H, D, dtype, residual, H == 1 and D % 32 == 0 and rng.random() < 0.5, weight)
+        else:
+            c = _norm_grad(None, T, H, D, dtype, residual, weight)
+    elif kind in ("route", "route_grad"):
+        E = rng.choice([8, 16, 32, 60, 64, 128, 160, 256, 384])
+        groups = rng.choice([1, 1, 4])
+        kept = rng.randint(1, groups)
+        k = rng.randint(1, min(10, E // groups * kept))
+        c = _route(None, _log(rng, 1, 16000), E, k, rng.choice(["softmax", "sigmoid"]), dtype, rng.random() < 0.5, groups,
+                   kept, rng.choice([1, 2]) if groups > 1 else 1, rng.random() < 0.7, rng.choice([1.0, 2.5]),
+                   rng.random() < 0.3, kind == "route_grad")
+    else:
+        E = rng.choice([4, 8, 16, 32, 60])
+        c = _experts(None, _log(rng, 1, 3000), E, rng.randint(1, min(8, E)), 32 * _log(rng, 8, 96), _log(rng, 64, 3000),
+                     format, rng.choice(["bf16", "bf16", "f16"]), rng.random() < 0.5, rng.random() < 0.5, rng.random() < 0.4)
+    del c["name"]
+    # no drawn case is larger than the largest listed ones
+    while work(c)["flops"] > 4e11:
+        rows = "M" if kind == "product" else "T"
+        c[rows] = c[rows] * 2 // 3
+    return c
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(int(seed))
+
+
+def _randn(g, shape, std, dtype=torch.float32):
+    return (torch.randn(shape, generator=g, device="cuda", dtype=torch.float32) * std).to(dtype)
+
+
+def _wide(g, shape, dtype):
+    """Activations as blocks see them: some features and some rows much larger than others."""
+    x = _randn(g, shape, 1.0)
+    x *= torch.exp(_randn(g, (shape[-1],), 0.7)) * torch.exp(_randn(g, (*shape[:-1], 1), 0.5))
+    return x.to(dtype)
+
+
+# ---- the plain forms ---------------------------------------------------------------------------
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _mx(x, format):
+    """(codes, scales) of x: in 64 bits, since values next to the border of two codes go by their last bits."""
+    x = x.double().unflatten(-1, (-1, 32))
+    top = x.abs().amax(-1)
+    m, e = torch.frexp(top)  # top = m 2^e, m from 1/2 up to 1
+    e = e - 3 + (m > 0.75).int() if format == "e2m1" else e - 9 + (m > 0.875).int()  # 6 = 0.75 2^3, 448 = 0.875 2^9
+    bad = ~torch.isfinite(top)
+    e = torch.where((top == 0) | bad, -127, e.clamp(min=-127))
+    y = torch.where(bad[..., None], 0.0, x * torch.exp2(-e.double())[..., None]).flatten(-2)
+    scales = torch.where(bad, 255, e + 127).to(torch.uint8)
+    if format == "e4m3":
+        step = torch.exp2(torch.frexp(y).exponent.clamp(min=-5).double() - 4)  # of the four bits that a value keeps
+        return (torch.round(y / step) * step).float().to(torch.float8_e4m3fn), scales
+    m = y.abs()
+    code = (m > 0.25).int() + (m >= 0.75) + (m > 1.25) + (m >= 1.75) + (m > 2.5) + (m >= 3.5) + (m > 5.0)
+    code = (code + 8 * torch.signbit(y)).to(torch.uint8).unflatten(-1, (-1, 2))
+    return code[..., 0] | code[..., 1] << 4, scales
+
+
+def _values(codes, scales, dtype=torch.float32):
+    """What codes and scales stand for."""
+    if codes.dtype == torch.uint8:
+        table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), dtype=dtype, device=codes.device)
+        v = table[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).int()]
+    else:
+        v = codes.to(dtype)
+    s = torch.ldexp(torch.ones((), dtype=dtype, device=codes.device), scales.int() - 127)
+    s = torch.where(scales == 255, math.nan, s)
+    return (v.unflatten(-1, (-1, 32)) * s[..., None]).flatten(-2)
+
+
+def _plain_norm(s):
+    c = s["case"]
+    wide = torch.float64 if c["mx"] else torch.float32
+    x, h = s["x"].to(wide), None
+    if c["residual"]:
+        h = (s["x"].float() + s["residual"].float()).to(s["x"].dtype)
+        x = h.to(wide)
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+    if s["weight"] is not None:
+        y = y * s["weight"].to(wide)
+    y = _values(*_mx(y, "e4m3")).to(torch.bfloat16) if c["mx"] else y.to(s["x"].dtype)
+    return y if h is None else (y, h)
+
+
+def _plain_norm_grad(s):
+    x, dy, w = s["x"].float(), s["dy"].float(), s["weight"]
+    D = x.shape[-1]
+    r = torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+    n = x * r
+    g = dy if w is None else dy * w.float()
+    dx = r * (g - n * ((g * n).sum(-1, keepdim=True) / D))
+    if s["dsum"] is not None:
+        dx = dx + s["dsum"].float()
+    dx = dx.to(s["x"].dtype)
+    return dx if w is None else (dx, (dy * n).double().reshape(-1, D).sum(0).to(w.dtype))
+
+
+def _scores(z, scoring):
+    z = z.double()
+    if scoring == "sigmoid":
+        return 1.0 / (1.0 + torch.exp(-z))
+    e = torch.exp(z - z.amax(-1, keepdim=True))
+    return e / e.sum(-1, keepdim=True)
+
+
+def _first(x, k):
+    """The places of the k largest, the lowest place first among equal ones."""
+    return torch.sort(x, dim=-1, descending=True, stable=True).indices[..., :k]
+
+
+def _plan(ids, E):
+    """(starts, rows): the entries of ids in the order of their experts, those without one last."""
+    flat = ids.reshape(-1).long()
+    flat = torch.where((flat >= 0) & (flat < E), flat, E)
+    rows = torch.sort(flat, stable=True).indices
+    counts = (flat[:, None] == torch.arange(E, device=ids.device)).sum(0)
+    starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    return starts.int(), rows.int()
+
+
+def _plain_route(logits, c, bias, active):
+    z, E, G = logits.double(), c["E"], c["groups"]
+    s = _scores(logits, c["scoring"])
+    by = z if bias is None else s + bias.double()
+    if c["kept"] < G:
+        # groups by the sum of their best scores; by the logits where that is one score without a bias
+        of = (s if bias is None and c["best"] > 1 else by).unflatten(-1, (G, E // G))
+        best = torch.sort(of, dim=-1, descending=True).values[..., :c["best"]].sum(-1)
+        keep = torch.zeros(best.shape, dtype=torch.bool, device=z.device).scatter_(-1, _first(best, c["kept"]), True)
+        by = torch.where(keep.repeat_interleave(E // G, -1), by, -math.inf)
+    ids = _first(by, c["k"])
+    w = s.gather(-1, ids)
+    if c["normalize"]:
+        w = w / w.sum(-1, keepdim=True)
+    ids, w = ids.int(), (w * c["scale"]).float()
+    if active is not None:
+        ids, w = torch.where(active[:, None], ids, -1), torch.where(active[:, None], w, 0.0)
+    return (ids, w, *_plan(ids, E))
+
+
+def _route_gradient(logits, c, ids, dw, dtype):
+    """The gradient of the logits from that of the chosen experts' weights."""
+    s = _scores(logits, c["scoring"]).to(dtype)
+    at = ids.clamp(min=0).long()
+    live = ids >= 0
+    p = s.gather(-1, at)
+    dp = torch.where(live, dw.to(dtype) * c["scale"], 0.0)
+    if c["normalize"]:
+        total = p.sum(-1, keepdim=True)
+        dp = torch.where(live, (dp - (dp * p).sum(-1, keepdim=True) / total) / total, 0.0)
+    ds = torch.zeros_like(s).scatter_add_(-1, at, dp)
+    if c["scoring"] == "sigmoid":
+        return ds * s * (1.0 - s)
+    return s * (ds - (ds * s).sum(-1, keepdim=True))
+
+
+def _plain_experts(s):
+    c = s["case"]
+    E, k = c["E"], c["k"]
+    route = _plain_route(s["logits"], s["router"], None, s["active"]) if c["routed"] else s["routing"]
+    ids, weights, starts, rows = route
+    x, w = _values(*s["x"]), _values(*s["w"])
+    T, A = ids.shape[0], ids.numel()
+    x = x.reshape(A, -1) if x.dim() == 3 else x.repeat_interleave(k, 0)
+    # each expert's rows, padded to the most that any has
+    most = max(1, int((starts[1:] - starts[:-1]).max()))
+    e = ids.reshape(-1).long()
+    live = e >= 0
+    e = e.clamp(min=0)
+    place = torch.empty(A, dtype=torch.long, device=x.device)
+    place[rows.long()] = torch.arange(A, device=x.device)
+    place = torch.where(live, place - starts.long()[e], most)
+    held = x.new_zeros(E, most + 1, x.shape[1])
+    held[e, place] = x
+    y = torch.bmm(held, w.transpose(1, 2).contiguous())
+    if s["bias"] is not None:
+        y += s["bias"].float()[:, None]
+    y = torch.where(live[:, None], y[e, place], 0.0).view(T, k, -1)
+    if c["combine"]:
+        y = (y * weights[..., None]).sum(1)
+    y = y.to(_DTYPES[c["dtype"]])
+    return (y, *route) if c["routed"] else y
+
+
+def _plain(s):
+    c = s["case"]
+    k = c["kind"]
+    if k == "quantize":
+        codes, scales = _mx(s["x"], c["format"])
+        return _values(codes, scales).to(torch.bfloat16), scales
+    if k == "product":
+        y = torch.mm(_values(*s["x"]), _values(*s["w"]).t().contiguous())
+        if s["bias"] is not None:
+            y += s["bias"].float()
+        return y.to(_DTYPES[c["dtype"]])
+    if k == "route":
+        return _plain_route(s["logits"], c, s["bias"], s["active"])
+    if k == "route_grad":
+        return _route_gradient(s["logits"], c, s["ids"], s["dweights"], torch.float32).to(s["logits"].dtype)
+    return {"norm": _plain_norm, "norm_grad": _plain_norm_grad, "experts": _plain_experts}[k](s)
+
+
+# ---- inputs --------------------------------------------------------------------------------------
+
+
+def _logits(g, T, E, dtype):
+    """A router's scores: a token's own spread, and experts that are liked more than others."""
+    return (_randn(g, (T, E), 1.5) + _randn(g, (E,), 0.5)).to(dtype)
+
+
+def _active(g, T):
+    """A padded batch: about one token in eight is none."""
+    return torch.rand(T, generator=g, device="cuda") > 0.125
+
+
+def prepare(case, seed):
+    g, k = _gen(seed), case["kind"]
+    dt = _DTYPES[case["dtype"]]
+    s = {"case": case}
+    if k == "quantize":
+        s["x"] = _wide(g, (case["rows"], case["K"]), dt)
+    elif k == "product":
+        s["x"] = _mx(_wide(g, (case["M"], case["K"]), torch.float32), case["format"])
+        s["w"] = _mx(_randn(g, (case["N"], case["K"]), case["K"] ** -0.5), "e2m1")
+        s["bias"] = _randn(g, (case["N"],), 0.2, dt) if case["bias"] else None
+    elif k in ("norm", "norm_grad"):
+        T, H, D = case["T"], case["H"], case["D"]
+        # heads are slices of one projection's output
+        shape = (T, H + 8, D) if H > 1 else (T, D)
+        cut = (lambda t: t[:, :H]) if H > 1 else (lambda t: t)
+        s["x"] = cut(_wide(g, shape, dt))
+        s["weight"] = (1.0 + _randn(g, (D,), 0.2)).to(dt) if case["weight"] else None
+        if k == "norm":
+            s["residual"] = cut(_wide(g, shape, dt)) if case["residual"] else None
+        else:
+            s["dy"] = cut(_randn(g, shape, 1.0, dt))
+            s["dsum"] = cut(_randn(g, shape, 1.0, dt)) if case["residual"] else None
+    elif k in ("route", "route_grad"):
+        s["logits"] = _logits(g, case["T"], case["E"], dt)
+        s["bias"] = _randn(g, (case["E"],), 0.1) if case["bias"] else None
+        s["active"] = _active(g, case["T"]) if case["active"] else None
+        if k == "route_grad":
+            s["ids"] = _plain_route(s["logits"], case, s["bias"], s["active"])[0]
+            s["dweights"] = _randn(g, (case["T"], case["k"]), 1.0)
+    else:
+        T, E, n, K, N = (case[t] for t in ("T", "E", "k", "K", "N"))
+        # a second projection has a row for each of a token's experts
+        shape = (T, n, K) if case["combine"] else (T, K)
+        s["x"] = _mx(_wide(g, shape, torch.float32), case["format"])
+        s["w"] = _mx(_randn(g, (E, N, K), K ** -0.5), "e2m1")
+        s["bias"] = _randn(g, (E, N), 0.2, dt) if case["bias"] else None
+        s["logits"] = _logits(g, T, E, torch.bfloat16)
+        s["router"] = _route(None, T, E, n)
+        s["active"] = _active(g, T) if case["routed"] else None
+        if not case["routed"]:
+            s["routing"] = _plain_route(s["logits"], s["router"], None, None)
+    return s
+
+
+def _own(s):
+    mlxq, c = _framework(), s["case"]
+    k = c["kind"]
+    if k == "quantize":
+        q = mlxq.mx_quantize(s["x"], c["format"])
+        return mlxq.mx_dequantize(q, torch.bfloat16), q.scales
+    if k == "product":
+        return mlxq.mx_matmul(s["x"], s["w"], bias=s["bias"], out_dtype=_DTYPES[c["dtype"]])
+    if k == "norm":
+        r = mlxq.rms_norm(s["x"], s["weight"], residual=s["residual"], eps=1e-6, mx=c["mx"])
+        if not c["mx"]:
+            return r
+        y = mlxq.mx_dequantize(r[0] if c["residual"] else r, torch.bfloat16)
+        return (y, r[1]) if c["residual"] else y
+    if k == "norm_grad":
+        dx, dw = mlxq.rms_norm_backward(s["dy"], s["x"], s["weight"], dsum=s["dsum"], eps=1e-6)
+        return dx if dw is None else (dx, dw)
+    if k == "route":
+        return tuple(mlxq.route_experts(s["logits"], c["k"], c["scoring"], bias=s["bias"], groups=c["groups"],
+                                        kept_groups=c["kept"], group_best=c["best"], normalize=c["normalize"],
+                                        scale=c["scale"], active=s["active"]))
+    if k == "route_grad":
+        return mlxq.route_experts_backward(s["dweights"], s["logits"], s["ids"], c["scoring"], normalize=c["normalize"],
+                                           scale=c["scale"])
+    routing = mlxq.route_experts(s["logits"], c["k"], active=s["active"]) if c["routed"] else mlxq.Routing(*s["routing"])
+    y = mlxq.mx_experts(s["x"], s["w"], routing, bias=s["bias"], combine=c["combine"], out_dtype=_DTYPES[c["dtype"]])
+    return (y, *routing) if c["routed"] else y
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+# ---- what the work cannot do without -------------------------------------------------------------
+
+
+def work(case):
+    k = case["kind"]
+    esz = _DTYPES[case["dtype"]].itemsize
+    if k == "quantize":
+        n = case["rows"] * case["K"]
+        return {"bytes": n * (esz + 2) + n // 32, "flops": 0}
+    if k == "product":
+        M, K, N = case["M"], case["K"], case["N"]
+        return {"bytes": M * K * _BYTES[case["format"]] + N * K * _BYTES["e2m1"] + M * N * esz, "flops": 2 * M * N * K}
+    if k in ("norm", "norm_grad"):
+        n = case["T"] * case["H"] * case["D"]
+        streams = 2 + 2 * case["residual"] if k == "norm" else 3 + case["residual"]
+        return {"bytes": n * streams * esz + case["D"] * esz * (case["weight"] + (k == "norm_grad")),
+                "flops": n * (4 if k == "norm" else 10)}
+    if k in ("route", "route_grad"):
+        T, E, n = case["T"], case["E"], case["k"]
+        if k == "route":
+            return {"bytes": T * E * esz + T * n * 12 + 4 * E, "flops": 4 * T * E}
+        return {"bytes": 2 * T * E * esz + T * n * 8, "flops": 8 * T * E}
+    T, E, n, K, N = (case[t] for t in ("T", "E", "k", "K", "N"))
+    A = T * n
+    used = E * (1.0 - (1.0 - n / E) ** T)  # experts that any token is expected at
+    rows_in, rows_out = (A, T) if case["combine"] else (T, A)
+    return {"bytes": rows_in * K * _BYTES[case["format"]] + used * N * K * _BYTES["e2m1"] + rows_out * N * esz,
+            "flops": 2 * A * N * K}
+
+
+# ---- the same in 64 bits ---------------------------------------------------------------------------
+
+
+def _mx64(codes, scales):
+    """The values of a microscaled tensor, from the fields of its codes."""
+    if codes.dtype == torch.uint8:
+        c = torch.stack([codes % 16, codes // 16], -1).flatten(-2).long()
+        e, m, sign, bias, wide = (c >> 1) & 3, c & 1, c >> 3, 1, 2.0
+    else:
+        c = codes.view(torch.uint8).long()
+        e, m, sign, bias, wide = (c >> 3) & 15, c & 7, c >> 7, 7, 8.0
+    v = torch.where(e == 0, m / wide * 2.0 ** (1 - bias), (1 + m / wide) * torch.exp2((e - bias).double()))
+    v = torch.where(sign == 1, -v, v)
+    s = scales.long().repeat_interleave(32, -1)
+    return v * torch.exp2((s - 127).double())
+
+
+def _rounded64(x, format):
+    """(values, scales) of x: each magnitude over its block's scale to the nearest of all the code's values."""
+    if format == "e2m1":
+        table = torch.tensor(_E2M1, dtype=torch.float64, device=x.device)
+    else:
+        table = torch.arange(127, device=x.device, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    top = x.unflatten(-1, (-1, 32)).abs().amax(-1)
+    e = torch.ceil(torch.log2(top / table[-1])).clamp(min=-127)
+    scale = torch.exp2(e).repeat_interleave(32, -1)
+    m = x.abs() / scale
+    middle = (table[1:] + table[:-1]) / 2
+    at = torch.searchsorted(middle, m)
+    # a value in the middle goes to the even code
+    at += ((m == middle[at.clamp(max=len(middle) - 1)]) & (at % 2 == 1)).long()
+    return torch.copysign(table[at] * scale, x), (e + 127).to(torch.uint8)
+
+
+def _exact_norm(s):
+    c, x = s["case"], s["x"].double()
+    h = None
+    if c["residual"]:
+        h = x + s["residual"].double()
+        x = h.to(s["x"].dtype).double()  # the norm is that of the sum as it is written
+    y = x / (x.pow(2).sum(-1, keepdim=True) / x.shape[-1] + 1e-6).sqrt()
+    y = y if s["weight"] is None else y * s["weight"].double()
+    y = _rounded64(y, "e4m3")[0] if c["mx"] else y
+    return y if h is None else (y, h)
+
+
+def _exact_norm_grad(s):
+    x, dy, w = s["x"].double(), s["dy"].double(), s["weight"]
+    inv = (x.pow(2).mean(-1, keepdim=True) + 1e-6).pow(-0.5)
+    g = dy if w is None else dy * w.double()
+    dx = inv * g - inv.pow(3) * x * (g * x).mean(-1, keepdim=True)
+    dx = dx if s["dsum"] is None else dx + s["dsum"].double()
+    return dx if w is None else (dx, (dy * x * inv).flatten(0, -2).sum(0))
+
+
+def _exact_route(logits, c, bias, active):
+    z = logits.double()
+    s = torch.sigmoid(z) if c["scoring"] == "sigmoid" else torch.softmax(z, -1)
+    choice = z.clone() if bias is None else s + bias.double()
+    T, E = z.shape
+    size = E // c["groups"]
+    index = torch.arange(E, device=z.device)
+    if c["kept"] < c["groups"]:
+        of = choice if bias is not None or c["best"] == 1 else s
+        of = of.view(T, c["groups"], size).clone()
+        score = torch.zeros(T, c["groups"], dtype=torch.float64, device=z.device)
+        for _ in range(min(c["best"], size)):
+            top = of.max(-1)
+            score += top.values
+            at = (of == top.values[..., None]).int().argmax(-1, keepdim=True)
+            of.scatter_(-1, at, -math.inf)
+        # a group's rank: those that score more, and the lower ones that score as much
+        lower = torch.ones(c["groups"], c["groups"], dtype=torch.bool, device=z.device).tril(-1)
+        rank = (score[:, None] > score[..., None]).sum(-1) + ((score[:, None] == score[..., None]) & lower).sum(-1)
+        choice = torch.where((rank < c["kept"])[:, index // size], choice, -math.inf)
+    ids = []
+    for _ in range(c["k"]):
+        best = (choice == choice.amax(-1, keepdim=True)).int().argmax(-1)
+        ids.append(best)
+        choice.scatter_(-1, best[:, None], -math.inf)
+    ids = torch.stack(ids, -1)
+    w = s.gather(-1, ids)
+    w = c["scale"] * (w / w.sum(-1, keepdim=True) if c["normalize"] else w)
+    if active is not None:
+        ids[~active], w[~active] = -1, 0.0
+    flat = ids.flatten()
+    order = torch.argsort(torch.where(flat < 0, E, flat) * flat.numel() + torch.arange(flat.numel(), device=z.device))
+    starts = torch.searchsorted(torch.where(flat < 0, E, flat)[order].contiguous(), torch.arange(E + 1, device=z.device))
+    return ids.int(), w, starts.int(), order.int()
+
+
+def _exact_route_grad(s):
+    """The gradient by the chain rule over the whole Jacobian's action, a row at a time in one batch."""
+    c, z, ids = s["case"], s["logits"].double(), s["ids"].long()
+    chosen = torch.zeros(z.shape, dtype=torch.float64, device=z.device)
+    up = torch.zeros_like(chosen)
+    live = ids >= 0
+    t = torch.arange(z.shape[0], device=z.device)[:, None].expand_as(ids)[live]
+    chosen[t, ids[live]] = 1.0
+    up[t, ids[live]] = s["dweights"].double()[live] * c["scale"]
+    p = torch.sigmoid(z) if c["scoring"] == "sigmoid" else torch.softmax(z, -1)
+    if c["normalize"]:
+        total = (p * chosen).sum(-1, keepdim=True)
+        total = torch.where(total > 0, total, 1.0)
+        up = chosen * (up / total - (up * p).sum(-1, keepdim=True) / total ** 2)
+    if c["scoring"] == "sigmoid":
+        return up * p * torch.sigmoid(-z)
+    return p * up - p * (p * up).sum(-1, keepdim=True)
+
+
+def _exact_experts(s):
+    c = s["case"]
+    route = _exact_route(s["logits"], s["router"], None, s["active"]) if c["routed"] else s["routing"]
+    ids, weights = route[0].long(), route[1].double()
+    x = _mx64(*s["x"])
+    y = torch.zeros(*ids.shape, c["N"], dtype=torch.float64, device=x.device)
+    for e in range(c["E"]):
+        t, j = (ids == e).nonzero(as_tuple=True)
+        rows = x[t, j] if x.dim() == 3 else x[t]
+        y[t, j] = rows @ _mx64(s["w"][0][e], s["w"][1][e]).t() + (0.0 if s["bias"] is None else s["bias"][e].double())
+    if c["combine"]:
+        y = (weights[..., None] * y).sum(1)
+    return (y, *route) if c["routed"] else y
+
+
+def exact(case, seed):
+    s, k = prepare(case, seed), case["kind"]
+    if k == "quantize":
+        return _rounded64(s["x"].double(), case["format"])
+    if k == "product":
+        y = _mx64(*s["x"]) @ _mx64(*s["w"]).t()
+        return y if s["bias"] is None else y + s["bias"].double()
+    if k == "norm":
+        return _exact_norm(s)
+    if k == "norm_grad":
+        return _exact_norm_grad(s)
+    if k == "route":
+        return _exact_route(s["logits"], case, s["bias"], s["active"])
+    if k == "route_grad":
+        return _exact_route_grad(s)
+    return _exact_experts(s)
