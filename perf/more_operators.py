@@ -325,6 +325,15 @@ def _plain(s):
 # ---- inputs --------------------------------------------------------------------------------------
 
 
+def _held(x, format):
+    """x quantised, the scales of each row from a multiple of 4 bytes on, as a program keeps them."""
+    codes, scales = _mx(x, format)
+    n = scales.shape[-1]
+    room = torch.zeros((*scales.shape[:-1], -(-n // 4) * 4), dtype=torch.uint8, device=scales.device)
+    room[..., :n] = scales
+    return codes, room[..., :n]
+
+
 def _logits(g, T, E, dtype):
     """A router's scores: a token's own spread, and experts that are liked more than others."""
     return (_randn(g, (T, E), 1.5) + _randn(g, (E,), 0.5)).to(dtype)
@@ -342,8 +351,8 @@ def prepare(case, seed):
     if k == "quantize":
         s["x"] = _wide(g, (case["rows"], case["K"]), dt)
     elif k == "product":
-        s["x"] = _mx(_wide(g, (case["M"], case["K"]), torch.float32), case["format"])
-        s["w"] = _mx(_randn(g, (case["N"], case["K"]), case["K"] ** -0.5), "e2m1")
+        s["x"] = _held(_wide(g, (case["M"], case["K"]), torch.float32), case["format"])
+        s["w"] = _held(_randn(g, (case["N"], case["K"]), case["K"] ** -0.5), "e2m1")
         s["bias"] = _randn(g, (case["N"],), 0.2, dt) if case["bias"] else None
     elif k in ("norm", "norm_grad"):
         T, H, D = case["T"], case["H"], case["D"]
@@ -368,8 +377,8 @@ def prepare(case, seed):
         T, E, n, K, N = (case[t] for t in ("T", "E", "k", "K", "N"))
         # a second projection has a row for each of a token's experts
         shape = (T, n, K) if case["combine"] else (T, K)
-        s["x"] = _mx(_wide(g, shape, torch.float32), case["format"])
-        s["w"] = _mx(_randn(g, (E, N, K), K ** -0.5), "e2m1")
+        s["x"] = _held(_wide(g, shape, torch.float32), case["format"])
+        s["w"] = _held(_randn(g, (E, N, K), K ** -0.5), "e2m1")
         s["bias"] = _randn(g, (E, N), 0.2, dt) if case["bias"] else None
         s["logits"] = _logits(g, T, E, torch.bfloat16)
         s["router"] = _route(None, T, E, n)
