@@ -458,6 +458,150 @@ int mlxq_cache_copy_pages(void* cache, int64_t planes, int64_t plane_stride_byte
                           int64_t width, int64_t table_stride, void* stream);
 
 /*
+ * ---- A decoder block in microscaled types: quantisation, products, norms, routing to experts ------
+ *
+ * No counterpart in the reference, whose norms, routers and microscaled products run in MLX
+ * (mlx-gen-sensenova/src/qwen3.rs:178-181; mlx-gen-lens/src/text_encoder/gpt_oss.rs:396-440 turns its
+ * microscaled experts into affine packs).
+ *
+ * A microscaled matrix [rows, K], K a multiple of 32: blocks of 32 values of a row share a scale, a byte
+ * b that stands for 2^(b - 127) (255: NaN, and so the whole block).  Codes are e2m1 (0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives, two to a byte, the first in the low half) or e4m3 (a byte each, largest
+ * 448, 0x7f and 0xff NaN), the Open Compute Project's types.  Codes are contiguous, rows * K / 2 or
+ * rows * K bytes, 16-byte aligned; the scales of a row, K / 32 bytes, start scale_stride bytes after the
+ * row before's, a multiple of 4 and at least K / 32, and 4-byte aligned.  Bytes between them are not
+ * read for a result and may hold anything; up to the next multiple of 4 quantisation writes them as 0.
+ */
+typedef enum { MLXQ_MX_E2M1 = 0, MLXQ_MX_E4M3 = 1 } mlxq_mx_format;
+
+typedef struct {
+  void* codes;
+  void* scales;
+  int64_t scale_stride; /* bytes */
+  int format;           /* mlxq_mx_format */
+} mlxq_mx;
+
+/*
+ * x [rows, K] (f32, bf16, fp16; row_stride elements from one row to the next, rows 16-byte aligned) to
+ * microscaled codes.  A block's scale is the smallest power of two from 2^-127 on by which its largest
+ * magnitude divided is at most 6 (e2m1) or 448 (e4m3), so that nothing saturates; values are rounded to
+ * nearest, ties to even.  A block with an infinity or a NaN has scale 255 and codes 0.  Every step
+ * but the rounding is exact.
+ */
+int mlxq_mx_quantize(const void* x, int dtype, int64_t rows, int64_t K, int64_t row_stride,
+                     const mlxq_mx* out, void* stream);
+
+/* out [rows, K] in out_dtype: code times scale, rounded once (bf16 and f32 hold all of them but bf16 those
+ * below 2^-133; fp16 overflows past 65504). */
+int mlxq_mx_dequantize(const mlxq_mx* x, int64_t rows, int64_t K, void* out, int out_dtype, void* stream);
+
+/*
+ * y [M, N] = x . w^T + bias: x [M, K] in either format, w [N, K] e2m1, bias [N] in bias_dtype or NULL; y
+ * in y_dtype (f32, bf16, fp16).  Products of codes and scales are exact, sums f32, one rounding at the
+ * end.  workspace: mlxq_mx_matmul_workspace_size() bytes, 16-byte aligned, whatever they hold (NULL when
+ * that is 0).  Sums are taken in an order that follows M, N, K and the format only.
+ */
+size_t mlxq_mx_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int x_format);
+int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int64_t N, const void* bias,
+                   int bias_dtype, void* y, int y_dtype, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/*
+ * Root-mean-square norm over the last dimension of [T, heads, D]:
+ *   h = x + residual (rounded to dtype and written to sum; without residual h = x and sum is NULL)
+ *   y = h * (mean(h^2) + eps)^(-1/2) * weight            (weight [D] in weight_dtype, NULL: ones)
+ * x, residual, sum and y have one dtype and any strides that are whole elements.  Sums are f32, and y is
+ * rounded once.  Exactly one of y and y_mx is given: y_mx (e4m3, rows T * heads of D, D a multiple of 32)
+ * is what mlxq_mx_quantize would make of the exact norm, which is taken in 64 bits there, so that
+ * no code depends on the order of a sum.  sum may be x or residual (same strides), y may be x; otherwise
+ * nothing may overlap.  D up to 32768.
+ */
+int mlxq_rms_norm(const mlxq_heads* x, int dtype, int64_t T, int64_t D, const mlxq_heads* residual,
+                  const mlxq_heads* sum, const void* weight, int weight_dtype, float eps,
+                  const mlxq_heads* y, const mlxq_mx* y_mx, void* stream);
+
+/*
+ * Its gradient.  With r = (mean(x^2) + eps)^(-1/2), n = x r and g = dy * weight:
+ *   dx = r (g - n mean(g n)) + dsum,     dweight = sum over tokens and heads of dy n
+ * x is what was normed (the sum, if there was a residual: dx is then the gradient of both), dsum (NULL =
+ * none) the gradient that arrives at the sum from elsewhere.  dweight [D] in weight_dtype, NULL when
+ * weight is.  f32 sums in a fixed order, each result rounded once.  dx may be dy or dsum (same strides).
+ * workspace: mlxq_rms_norm_backward_workspace_size() bytes, 16-byte aligned, whatever they hold.
+ */
+size_t mlxq_rms_norm_backward_workspace_size(int64_t T, int64_t heads, int64_t D, int dtype);
+int mlxq_rms_norm_backward(const mlxq_heads* dy, const mlxq_heads* x, int dtype, int64_t T, int64_t D,
+                           const void* weight, int weight_dtype, const mlxq_heads* dsum, float eps,
+                           const mlxq_heads* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* How a router chooses. */
+typedef enum { MLXQ_ROUTE_SOFTMAX = 0, MLXQ_ROUTE_SIGMOID = 1 } mlxq_route_scoring;
+
+typedef struct {
+  int scoring;          /* mlxq_route_scoring: s = softmax(z) over all experts, or sigmoid(z) */
+  int64_t top_k;        /* experts a token goes to, 1 to 64 */
+  const float* bias;    /* [experts] or NULL: added to s for the choice only */
+  int64_t groups;       /* equal runs of experts, 1 to 64; only those of the kept_groups best groups are chosen */
+  int64_t kept_groups;  /* from */
+  int64_t group_best;   /* a group counts as the sum of its 1 or 2 best experts */
+  int normalize;        /* weights are divided by their sum */
+  float scale;          /* and multiplied by this */
+} mlxq_router;
+
+/* Where tokens go: ids [tokens, top_k] and weights [tokens, top_k], and the plan of the experts' products:
+ * rows lists the choices t * top_k + j in the order of their experts (those of one expert ascending), expert
+ * e's from starts[e] up to starts[e + 1]; choices without an expert (an id outside [0, experts)) come last.
+ * All device arrays, int32 but for the f32 weights. */
+typedef struct {
+  int32_t* ids;
+  float* weights;
+  int32_t* starts; /* [experts + 1] */
+  int32_t* rows;   /* [tokens * top_k] */
+  int64_t tokens, top_k, experts;
+} mlxq_routing;
+
+/*
+ * Routes tokens by their logits [T, experts] (dtype, row_stride elements from row to row).  The top_k
+ * experts with the largest s + bias (without a bias: the largest logits) among the kept groups, best first,
+ * the lowest expert first among equal ones; weights are s of the chosen, normalized and scaled.  The choice
+ * is made in 64 bits.  active (NULL = all): tokens whose byte is 0 get ids -1 and weights 0.
+ * NaN logits come after all others of the kept groups; a row with a NaN or +infinity has NaN weights under
+ * softmax, and where the chosen scores sum to 0 (all -infinity) the weights are 0.  top_k is at most
+ * kept_groups * (experts / groups).  experts up to 1024, tokens * top_k below 2^31 - 2^20.
+ * workspace: mlxq_route_workspace_size() bytes, 16-byte aligned, whatever they hold.
+ */
+size_t mlxq_route_workspace_size(int64_t choices, int64_t experts);
+int mlxq_route_experts(const void* logits, int dtype, int64_t row_stride, const mlxq_router* router,
+                       const uint8_t* active, const mlxq_routing* out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* starts and rows for given ids (of out; its weights are not read). */
+int mlxq_route_plan(const mlxq_routing* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The gradient of the logits from that of the weights, dweights [tokens, top_k] f32, for the choice that
+ * ids holds (ids outside [0, experts) pass nothing on; no expert twice in a row): dlogits [tokens, experts]
+ * contiguous, in dtype.  f32 arithmetic.  Of router, scoring, normalize and scale are read.
+ */
+int mlxq_route_experts_backward(const float* dweights, const void* logits, int dtype, int64_t row_stride,
+                                const mlxq_router* router, const mlxq_routing* routing, void* dlogits,
+                                void* stream);
+
+/*
+ * The products of the experts that tokens were routed to: y[t, j] = x[t] . w[ids[t, j]]^T + bias[ids[t, j]]
+ * with w [experts, N, K] e2m1 (one stack of experts * N rows), bias [experts, N] in bias_dtype or NULL, x
+ * [tokens, K], or with x_per_choice [tokens, top_k, K].  y is [tokens, top_k, N] in y_dtype, zero for choices
+ * without an expert; with combine it is [tokens, N], sum_j weights[t, j] y[t, j]: each product is rounded to
+ * y_dtype, as separate products would be, and the sum is f32.  starts and rows must be ids' plan; entries
+ * outside their ranges are skipped.  workspace as above.
+ */
+size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t experts, int64_t K, int64_t N,
+                                      int x_format, int combine, int y_dtype);
+int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx* w, int64_t N,
+                    const void* bias, int bias_dtype, const mlxq_routing* routing, int combine, void* y,
+                    int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Host-side shape helper — replaces quant::packed_bits (src/quant.rs:38-41): from the packed
  * shapes infer bits = wq_cols*32 / (scales_cols*group_size).  Returns 4 or 8, or -1 (with
  * mlxq_last_error set) for a malformed triple instead of panicking.

@@ -1,0 +1,434 @@
+// mx_matmul.h — products of microscaled operands: y[m, n] = sum_k x[m, k] w[n, k], dense or of routed experts.
+//
+// The matrix cores multiply 16 weight rows by 16 rows of x over 128 values of K and apply the blocks' scales
+// themselves, so codes go from memory to the operands as they lie: nothing is converted.  The weights are the A operand
+// and x the B operand, so that a lane's results are four neighbouring features of one row.  With lane = 16 g + c, a
+// lane holds of row c: e2m1 the values 32 g .. 32 g + 31 of the 128; e4m3 16 g .. 16 g + 15 and those 64 further on;
+// and the scale of values 32 g .. 32 g + 31 in either.
+//
+// The 8-bit instruction adds its products with fewer bits than f32 has: sums are off by up to 2^-12 of the largest product
+// they hold, 2e-5 of a result in all, which a 16-bit result does not show.  f32 results of e4m3 take bf16 instructions
+// instead (EXACT): codes times scales are bf16 numbers, and their sums are as f32's.  Lane group g then holds the values
+// 32 g .. 32 g + 31 of either operand, eight to each of four instructions.  e2m1 by e2m1 is exact as it is.
+//
+// Routed products go by a plan: runs of choices of one expert, cut into tiles.  Every workgroup finds its tile by a
+// scan over the runs' lengths; the last run, of choices without an expert, is written as zeros.
+#pragma once
+
+#include "mx.h"
+
+namespace mlxq {
+
+// Zeros that lanes past the end of K read.
+static __device__ const u32x4 mx_zeros = {0, 0, 0, 0};
+
+// A tile of rows: positions [first, first + count) of y's rows (dense) or of the plan; expert e (E: none).
+struct MxTile {
+  int first, count, e;
+  bool found;
+};
+
+// Tile `at` of `tiles`, cut TM rows at a time; `total` gives all tiles of all runs.
+struct MxTiles {
+  const MxProduct& p;
+  int TM;
+  __device__ __forceinline__ int bound(int i) const {  // the start of run i; the last ends with the choices
+    const int M = (int)p.M;
+    return i > p.E ? M : min(max(p.starts[i], 0), M);
+  }
+  __device__ __forceinline__ int tiles_of(int i) const { return (max(bound(i + 1) - bound(i), 0) + TM - 1) / TM; }
+  __device__ __forceinline__ int scan(int i, int& own) const {
+    const int lane = threadIdx.x & 63;
+    own = i <= p.E ? tiles_of(i) : 0;
+    int s = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(s, d);
+      if (lane >= d) s += o;
+    }
+    return s;
+  }
+  __device__ __forceinline__ int total() const {
+    if (p.E == 0) return ((int)p.M + TM - 1) / TM;
+    int n = 0, own;
+    for (int i0 = 0; i0 <= p.E; i0 += 64) n += __builtin_amdgcn_readlane(scan(i0 + (threadIdx.x & 63), own), 63);
+    return n;
+  }
+  __device__ __forceinline__ MxTile find(int at) const {
+    const int M = (int)p.M;
+    if (p.E == 0) return {at * TM, min(TM, M - at * TM), 0, at * TM < M};
+    for (int i0 = 0; i0 <= p.E; i0 += 64) {
+      int own;
+      const int s = scan(i0 + (threadIdx.x & 63), own), all = __builtin_amdgcn_readlane(s, 63);
+      if (at < all) {
+        const int l = __builtin_ctzll(__ballot(s > at)), i = i0 + l;
+        const int k = at - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(own, l));
+        const int first = bound(i) + k * TM;
+        return {first, min(TM, bound(i + 1) - first), i, true};
+      }
+      at -= all;
+    }
+    return {0, 0, 0, false};
+  }
+  // The row of y at a position; -1 where the plan names none.
+  __device__ __forceinline__ int row(int position) const {
+    if (p.E == 0) return position;
+    const int r = p.rows[position];
+    return (unsigned)r < (unsigned)p.M ? r : -1;
+  }
+  __device__ __forceinline__ int64_t x_row(int row) const {
+    if (p.E == 0) return row;
+    return p.by_choices.div(max(row, 0));
+  }
+};
+
+// Four neighbouring features of a row, rounded to y's type (f32 partial sums where K is split).
+__device__ __forceinline__ float mx_bias(const MxProduct& p, int64_t at) {
+  return p.bias_dtype == MLXQ_BFLOAT16 ? Act<uint16_t>::ld((const uint16_t*)p.bias, at)
+         : p.bias_dtype == MLXQ_FLOAT16 ? Act<_Float16>::ld((const _Float16*)p.bias, at) : ((const float*)p.bias)[at];
+}
+__device__ __forceinline__ void mx_store(const MxProduct& p, int e, int row, int n, f32x4 v) {
+  const int N = (int)p.N;
+  if (n >= N) return;
+  const int64_t at = (int64_t)row * N + n;
+  const bool four = n + 4 <= N;
+  if (p.bias && e < max(p.E, 1)) {
+    const int64_t b = (int64_t)e * N + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < N) v[i] += mx_bias(p, b + i);
+  }
+  // Rows of any N start at any element.
+  if (p.y_dtype == MLXQ_FLOAT32) {
+    float* y = (float*)p.y + at;
+    if (four) {
+      __builtin_memcpy(y, &v, 16);
+    } else {
+      for (int i = 0; i < 4; ++i)
+        if (n + i < N) y[i] = v[i];
+    }
+    return;
+  }
+  const u32x2 h = p.y_dtype == MLXQ_BFLOAT16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
+                                             : u32x2{Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
+  uint16_t* y = (uint16_t*)p.y + at;
+  if (four) {
+    __builtin_memcpy(y, &h, 8);
+  } else {
+    for (int i = 0; i < 4; ++i)
+      if (n + i < N) y[i] = (uint16_t)(h[i / 2] >> 16 * (i % 2));
+  }
+}
+
+// What a lane holds of 16 rows over 128 values of K, ready for the matrix cores.
+template <int XF, bool EXACT>
+struct MxFrag {
+  static constexpr int N = XF == kE4M3 ? 2 : 1;  // 16-byte pieces
+  i32x8 v;
+  int scale;
+  __device__ __forceinline__ void set(const u32x4 (&p)[N], int s) {
+    scale = s;
+    v = i32x8{(int)p[0][0], (int)p[0][1], (int)p[0][2], (int)p[0][3], 0, 0, 0, 0};
+    if constexpr (N == 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 + i] = (int)p[1][i];
+  }
+};
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+template <int XF>
+struct MxFrag<XF, true> {
+  static constexpr int N = XF == kE4M3 ? 2 : 1;
+  bf16x8 v[4];
+  __device__ __forceinline__ void set(const u32x4 (&p)[N], int s) {
+    const float f = mx_scale((uint32_t)s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bf16x2v h[4];
+      if constexpr (XF == kE4M3) {
+        const uint32_t lo = p[i / 2][2 * (i % 2)], hi = p[i / 2][2 * (i % 2) + 1];
+        h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, f, false);
+        h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, f, true);
+        h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, f, false);
+        h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, f, true);
+      } else {
+        const uint32_t w = p[0][i];
+        h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0);
+        h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1);
+        h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2);
+        h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
+      }
+      __builtin_memcpy(&v[i], h, 16);
+    }
+  }
+};
+template <int XF, bool EXACT>
+__device__ __forceinline__ f32x4 mx_mma(const MxFrag<kE2M1, EXACT>& w, const MxFrag<XF, EXACT>& x, f32x4 c) {
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], c, 0, 0, 0);
+    return c;
+  } else {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, c, 4, XF == kE4M3 ? 0 : 4, 0, w.scale, 0, x.scale);
+  }
+}
+
+// ---- many rows -----------------------------------------------------------------------------------
+
+// 16 or 4 bytes a lane from memory to LDS, lane i's to lds + 16 i (4 i).  As inline asm without a result, so that the
+// compiler adds no wait of its own before later LDS reads; callers wait for vmcnt themselves.  M0 holds the LDS address
+// and is restored.
+#define MLXQ_DMA(LOAD, FROM, LDS)                                                                                       \
+  {                                                                                                                    \
+    uint32_t saved;                                                                                                    \
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t" LOAD " %2, off\n\ts_mov_b32 m0, %0\n\ts_nop 0" \
+                 : "=&s"(saved)                                                                                        \
+                 : "s"(LDS), "v"(FROM)                                                                                 \
+                 : "memory");                                                                                          \
+  }
+__device__ __forceinline__ void mx_dma16(const unsigned char* from, uint32_t lds) MLXQ_DMA("global_load_lds_dwordx4", from, lds)
+__device__ __forceinline__ void mx_dma4(const unsigned char* from, uint32_t lds) MLXQ_DMA("global_load_lds_dword", from, lds)
+#undef MLXQ_DMA
+
+// A workgroup of WM x WN waves takes TM rows by TN features; steps of 128 values of K go through a ring of STAGES
+// buffers in LDS by DMA, one barrier a step.
+template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int n_tiles) {
+  constexpr int NW = WM * WN, XB = XF == kE4M3 ? 128 : 64, XN = XF == kE4M3 ? 2 : 1;
+  constexpr int FM = TM / WM / 16, FN = TN / WN / 16;
+  constexpr int XI = TM * XB / 1024 / NW, WI = TN * 64 / 1024 / NW, PER = XI + WI + 1;  // DMA loads of a wave a step
+  constexpr int W0 = TM * XB, S0 = W0 + TN * 64, STAGE = S0 + (TM + TN) * 4;
+  static_assert(XI >= 1 && WI >= 1 && STAGE * STAGES <= 163840 && (TM + TN) / 64 <= NW, "a step is whole loads of each wave");
+  __shared__ __align__(1024) unsigned char lds[STAGE * STAGES];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+
+  // Neighbouring workgroups go to different dies: each die takes a run of tiles of its own, in blocks of 8 tiles of
+  // rows by all of the features, so that what its workgroups read at a time shares its cache.
+  MxTiles tiles{p, TM};
+  const int m_tiles = tiles.total(), all = m_tiles * n_tiles, chunk = (all + 7) / 8;
+  const int l = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= chunk || l >= all) return;
+  const int band = l / (8 * n_tiles), in = l - band * 8 * n_tiles, high = min(8, m_tiles - 8 * band);
+  const int nt = in / high, mt = 8 * band + in - nt * high;
+  const MxTile tile = tiles.find(mt);
+  if (!tile.found) return;
+  const int n0 = nt * TN, N = (int)p.N, K = (int)p.K;
+  const int steps = (K + 127) / 128, s0 = 0, s1 = steps;
+
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  if (tile.e < max(p.E, 1)) {
+    const unsigned char *xp[XI], *wp[WI], *sp;
+    int xk[XI], wk;  // the first value of K of a lane's piece
+    const int64_t x_pitch = XF == kE4M3 ? K : K / 2, w_pitch = K / 2;
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      const int j = w * XI + i, r = XF == kE4M3 ? 8 * j + (lane >> 3) : 16 * j + (lane >> 2);
+      const int piece = XF == kE4M3 ? (lane & 7) ^ (r & 7) : (lane & 3) ^ (r >> 1 & 3);
+      const int64_t row = tiles.x_row(tiles.row(tile.first + min(r, tile.count - 1)));
+      xk[i] = piece * (XF == kE4M3 ? 16 : 32);
+      xp[i] = p.x.codes + row * x_pitch + piece * 16;
+    }
+    const int64_t w_row0 = (int64_t)tile.e * N;
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+      const int r = 16 * (w * WI + i) + (lane >> 2), piece = (lane & 3) ^ (r >> 1 & 3);
+      wk = piece * 32;
+      wp[i] = p.w.codes + (w_row0 + min(n0 + r, N - 1)) * w_pitch + piece * 16;
+    }
+    const int si = min(w, (TM + TN) / 64 - 1), sr = 64 * si + lane;
+    sp = sr < TM ? p.x.scales + tiles.x_row(tiles.row(tile.first + min(sr, tile.count - 1))) * p.x.scale_stride
+                 : p.w.scales + (w_row0 + min(n0 + sr - TM, N - 1)) * p.w.scale_stride;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+    const unsigned char* zeros = reinterpret_cast<const unsigned char*>(&mx_zeros);
+    const bool ragged = K % 128 != 0;
+
+    auto load = [&](int s) {
+      const uint32_t to = base + (uint32_t)(s % STAGES) * STAGE;
+      const int left = ragged && s == steps - 1 ? K - s * 128 : 128;
+#pragma unroll
+      for (int i = 0; i < XI; ++i)
+        mx_dma16(xk[i] < left ? xp[i] + (int64_t)s * XB : zeros, to + (w * XI + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < WI; ++i) mx_dma16(wk < left ? wp[i] + (int64_t)s * 64 : zeros, to + W0 + (w * WI + i) * 1024);
+      mx_dma4(sp + s * 4, to + S0 + si * 256);
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (s0 + i < s1) load(s0 + i);
+
+    const int wm = w % WM, wn = w / WM;
+    const int xr = wm * (TM / WM) + c, wr = wn * (TN / WN) + c;  // this lane's rows of the first fragments
+    // Of an e4m3 row a lane reads pieces g and g + 4 (EXACT: 2 g and 2 g + 1); piece i of row r lies at i ^ (r % 8).
+    constexpr int SECOND = EXACT ? 16 : 64;
+    const int x_at = XF == kE4M3 ? xr * 128 + (((EXACT ? 2 * g : g) ^ (c & 7)) * 16) : xr * 64 + ((g ^ (c >> 1 & 3)) * 16);
+    const int w_at = W0 + wr * 64 + ((g ^ (c >> 1 & 3)) * 16);
+    const int xs_at = S0 + xr * 4 + g, ws_at = S0 + (TM + wr) * 4 + g;
+
+    for (int s = s0; s < s1; ++s) {
+      if (s + STAGES - 2 < s1) mlxq_vmcnt<(STAGES - 2) * PER>();
+      else mlxq_vmcnt<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + STAGES - 1 < s1) load(s + STAGES - 1);
+      const unsigned char* b = lds + (s % STAGES) * STAGE;
+      const bool past = ragged && s == steps - 1 && g * 32 >= K - s * 128;  // this lane's block is past K
+      MxFrag<XF, EXACT> x[FM];
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        u32x4 v[XN];
+        v[0] = *reinterpret_cast<const u32x4*>(b + x_at + j * 16 * XB);
+        if constexpr (XN == 2) v[1] = *reinterpret_cast<const u32x4*>(b + (x_at ^ SECOND) + j * 16 * XB);
+        x[j].set(v, past ? 0 : b[xs_at + j * 64]);
+      }
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        MxFrag<kE2M1, EXACT> a;
+        const u32x4 v[1] = {*reinterpret_cast<const u32x4*>(b + w_at + i * 1024)};
+        a.set(v, past ? 0 : b[ws_at + i * 64]);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = mx_mma<XF, EXACT>(a, x[j], acc[i][j]);
+      }
+    }
+  }
+  const int wm = w % WM, wn = w / WM;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int r = wm * (TM / WM) + j * 16 + c;
+    if (r >= tile.count) continue;
+    const int row = tiles.row(tile.first + r);
+    if (row < 0) continue;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) mx_store(p, tile.e, row, n0 + wn * (TN / WN) + i * 16 + 4 * g, acc[i][j]);
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------
+
+// 16 FM rows by 16 features a workgroup; its NW waves take a run of K each, weights and x straight from memory to the
+// operands, and join their sums in LDS.
+template <int XF, bool EXACT, int FM, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_stream_kernel(MxProduct p, int n_tiles) {
+  constexpr int XN = XF == kE4M3 ? 2 : 1, AHEAD = FM > 1 ? 2 : 4;
+  __shared__ f32x4 part[NW][FM][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  MxTiles tiles{p, 16 * FM};
+  const int mt = blockIdx.x / n_tiles, n0 = (blockIdx.x - mt * n_tiles) * 16;
+  const MxTile tile = tiles.find(mt);
+  if (!tile.found) return;
+  const int N = (int)p.N, K = (int)p.K, steps = (K + 127) / 128;
+  f32x4 acc[FM];
+#pragma unroll
+  for (int j = 0; j < FM; ++j) acc[j] = f32x4{0, 0, 0, 0};
+  if (tile.e < max(p.E, 1)) {
+    const int64_t wrow = (int64_t)tile.e * N + min(n0 + c, N - 1);
+    const unsigned char *wp = p.w.codes + wrow * (K / 2) + g * 16, *ws = p.w.scales + wrow * p.w.scale_stride + g;
+    const unsigned char *xp[FM], *xs[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int64_t row = tiles.x_row(tiles.row(tile.first + min(j * 16 + c, tile.count - 1)));
+      xp[j] = p.x.codes + row * (XF == kE4M3 ? K : K / 2) + g * (EXACT && XF == kE4M3 ? 32 : 16);
+      xs[j] = p.x.scales + row * p.x.scale_stride + g;
+    }
+    const int per = (steps + NW - 1) / NW, s0 = min(steps, w * per), s1 = min(steps, s0 + per);
+    const int blocks = K / 32;
+    for (int s = s0; s < s1; s += AHEAD) {
+      u32x4 a[AHEAD], x[AHEAD][FM][XN];
+      int as[AHEAD], bs[AHEAD][FM];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        // Past the end of K (or of the wave's run) codes and scales are 0.
+        const int t = s + k, block = 4 * t + g;
+        const bool in = t < s1 && block < blocks;
+        a[k] = u32x4{0, 0, 0, 0};
+        as[k] = 0;
+        if (in) {
+          a[k] = *reinterpret_cast<const u32x4*>(wp + (int64_t)t * 64);
+          as[k] = ws[4 * t];
+        }
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          bs[k][j] = in ? xs[j][4 * t] : 0;
+          if constexpr (XF == kE4M3) {
+            x[k][j][0] = x[k][j][1] = u32x4{0, 0, 0, 0};
+            constexpr int SECOND = EXACT ? 16 : 64;
+            const int first = 128 * t + (EXACT ? 32 : 16) * g;
+            if (t < s1 && first < K) x[k][j][0] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 128);
+            if (t < s1 && first + SECOND < K) x[k][j][1] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 128 + SECOND);
+          } else {
+            x[k][j][0] = u32x4{0, 0, 0, 0};
+            if (in) x[k][j][0] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 64);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        MxFrag<kE2M1, EXACT> fa;
+        const u32x4 v[1] = {a[k]};
+        fa.set(v, as[k]);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          MxFrag<XF, EXACT> fx;
+          fx.set(x[k][j], bs[k][j]);
+          acc[j] = mx_mma<XF, EXACT>(fa, fx, acc[j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < FM; ++j) part[w][j][lane] = acc[j];
+  __syncthreads();
+  for (int j = w; j < FM; j += NW) {
+    f32x4 v = part[0][j][lane];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) v += part[k][j][lane];
+    const int r = j * 16 + c;
+    if (r >= tile.count) continue;
+    const int row = tiles.row(tile.first + r);
+    if (row >= 0) mx_store(p, tile.e, row, n0 + 4 * g, v);
+  }
+}
+
+namespace {
+
+// Tiles of TM rows that a launch is made for: as many as there can be, by sizes alone.
+inline int64_t mx_most_tiles(const MxProduct& p, int64_t TM) {
+  if (p.E == 0) return (p.M + TM - 1) / TM;
+  return p.M / TM + (p.M < p.E + 1 ? p.M : p.E + 1);
+}
+
+template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES>
+int mx_launch_tile(const MxProduct& p, hipStream_t st) {
+  const int64_t n_tiles = (p.N + TN - 1) / TN, grid = (mx_most_tiles(p, TM) * n_tiles + 7) / 8 * 8;
+  if (grid > 0x7fffffff) return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles", (long long)grid);
+  mx_tile_kernel<XF, EXACT, TM, TN, WM, WN, STAGES><<<(unsigned)grid, 64 * WM * WN, 0, st>>>(p, (int)n_tiles);
+  return check_launch("mx product");
+}
+
+template <int XF, bool EXACT, int FM, int NW>
+int mx_launch_stream(const MxProduct& p, hipStream_t st) {
+  const int64_t n_tiles = (p.N + 15) / 16, grid = mx_most_tiles(p, 16 * FM) * n_tiles;
+  if (grid > 0x7fffffff) return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles", (long long)grid);
+  mx_stream_kernel<XF, EXACT, FM, NW><<<(unsigned)grid, 64 * NW, 0, st>>>(p, (int)n_tiles);
+  return check_launch("mx product");
+}
+
+template <int XF, bool EXACT>
+int mx_product(const MxProduct& p, hipStream_t st) {
+  const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;  // of an expert, about
+  if (rows <= 16) return mx_launch_stream<XF, EXACT, 1, 8>(p, st);
+  if (rows <= 64) return mx_launch_stream<XF, EXACT, 4, 8>(p, st);
+  const int64_t big = mx_most_tiles(p, 256) * ((p.N + 255) / 256), mid = mx_most_tiles(p, 128) * ((p.N + 127) / 128);
+  if (big >= 512) return mx_launch_tile<XF, EXACT, 256, 256, 4, 2, 3>(p, st);
+  if (mid >= 256) return mx_launch_tile<XF, EXACT, 128, 128, 2, 2, 3>(p, st);
+  return mx_launch_tile<XF, EXACT, 64, 64, 2, 2, 4>(p, st);
+}
+
+}  // namespace
+
+}  // namespace mlxq

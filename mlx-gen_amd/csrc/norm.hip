@@ -1,0 +1,416 @@
+// norm.hip — root-mean-square norms with the residual's addition, their 8-bit results, and their gradient.
+//
+//   y = h (mean(h^2) + eps)^(-1/2) w,  h = x + residual
+//   dx = r g - r^3 x mean(g x) + dsum,  g = dy w;   dw = sum of dy x r over the rows
+//
+// A row is held in registers by 8 to 64 lanes of a wave (short rows: several to a wave), by a workgroup of 256 or by
+// one of 1024, in 16-byte pieces, and is read once; the sums take exchanges within a wave and one step through LDS
+// between waves.  Both directions are bound by HBM.  Pieces are loaded at the element's alignment, so that rows of odd
+// length or stride take the same path; only a row's last, partial piece goes element by element.
+//
+// The gradient of the weight is a sum over all rows: each workgroup walks many rows, the next one's loads in
+// flight while it reduces this one's, and holds its features' sums in registers; they go to the workspace once
+// and a second launch adds them up in a fixed order.
+#include <algorithm>
+
+#include "mx.h"
+
+namespace mlxq {
+
+namespace {
+
+template <typename T>
+constexpr int kC = Elem<T>::C;
+
+// 16 bytes at any element of a row; the part past its end is zero.
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* row, int e, int D) {
+  u32x4 v = {0, 0, 0, 0};
+  if (e + kC<T> <= D) {
+    __builtin_memcpy(&v, row + e, 16);
+  } else if (e < D) {
+#pragma unroll
+    for (int i = 0; i < kC<T>; ++i)
+      if (e + i < D) {
+        if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(row[e + i]);
+        else v[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[e + i]) << 16 * (i % 2);
+      }
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* row, int e, int D, const u32x4& v) {
+  if (e + kC<T> <= D) {
+    __builtin_memcpy(row + e, &v, 16);
+  } else if (e < D) {
+#pragma unroll
+    for (int i = 0; i < kC<T>; ++i)
+      if (e + i < D) {
+        if constexpr (sizeof(T) == 4) row[e + i] = __uint_as_float(v[i]);
+        else row[e + i] = __builtin_bit_cast(T, (uint16_t)(v[i / 2] >> 16 * (i % 2)));
+      }
+  }
+}
+
+template <typename W, int C>
+__device__ __forceinline__ void load_weights_of(const W* w, int e, int D, float (&f)[C]) {
+#pragma unroll
+  for (int k = 0; k < C; k += kC<W>) {
+    const u32x4 v = load_piece(w, e + k, D);
+#pragma unroll
+    for (int i = 0; i < kC<W> && i < C; ++i) f[k + i] = Elem<W>::get(v, i);
+  }
+}
+// C weights from feature e on; ones without a weight.
+template <int C>
+__device__ __forceinline__ void load_weights(const void* w, int dtype, int e, int D, float (&f)[C]) {
+  if (dtype < 0) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) f[i] = 1.0f;
+  } else if (dtype == MLXQ_BFLOAT16) {
+    load_weights_of((const uint16_t*)w, e, D, f);
+  } else if (dtype == MLXQ_FLOAT16) {
+    load_weights_of((const _Float16*)w, e, D, f);
+  } else {
+    load_weights_of((const float*)w, e, D, f);
+  }
+}
+
+// The sums of v over a row's LANES lanes, in every lane.  Rows of several waves go through `slot`, which nothing
+// may still be reading: callers take turns between two.
+template <int LANES, int N, typename V>
+__device__ __forceinline__ void row_sum(V (&v)[N], V* slot) {
+#pragma unroll
+  for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d);
+  if constexpr (LANES > 64) {
+    constexpr int W = LANES / 64;
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[w * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = slot[i];
+#pragma unroll
+    for (int k = 1; k < W; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += slot[k * N + i];
+  }
+}
+
+// The f32 that has y's leading bits and, where any were lost, an odd last one: rounding it to fewer bits is
+// rounding y.
+__device__ __forceinline__ float round_to_odd(double y) {
+  const float f = (float)y;
+  const double back = (double)f;
+  uint32_t b = __float_as_uint(f);
+  b -= fabs(back) > fabs(y);
+  return __uint_as_float(back != y ? b | 1u : b);
+}
+
+__device__ __forceinline__ double ldexp_f64(double v, int e) { return __builtin_amdgcn_ldexp(v, e); }
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const RowsView& v, int t, int h) {
+  return reinterpret_cast<T*>(v.p) + t * v.ts + h * v.hs;
+}
+
+template <typename T, int LANES, int CH, bool MX>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(NormArgs a) {
+  constexpr int C = kC<T>, R = LANES > 256 ? 1 : 256 / LANES, TW = LANES / 64 > 0 ? LANES / 64 : 1;
+  using Sum = typename std::conditional<MX, double, float>::type;
+  __shared__ Sum slot[TW];
+  const int lane = threadIdx.x % LANES, D = a.D;
+  const int64_t at = (int64_t)blockIdx.x * R + threadIdx.x / LANES;
+  const bool live = at < a.rows;
+  const int row = (int)(live ? at : a.rows - 1);
+  const int t = a.by_heads.div(row), h = row - t * a.heads;
+  const T* x = row_of<const T>(a.x, t, h);
+  u32x4 v[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) v[i] = load_piece(x, (i * LANES + lane) * C, D);
+  if (a.res.p) {
+    const T* res = row_of<const T>(a.res, t, h);
+    u32x4 r[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) r[i] = load_piece(res, (i * LANES + lane) * C, D);
+    T* sum = row_of<T>(a.sum, t, h);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      float f[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) f[e] = Elem<T>::get(v[i], e) + Elem<T>::get(r[i], e);
+      v[i] = pack_chunk<T>(f);
+      if (live) store_piece(sum, (i * LANES + lane) * C, D, v[i]);
+    }
+  }
+  // The weights of short rows are under way while the sum is taken.
+  constexpr bool EARLY = CH <= 2;
+  float w[EARLY ? CH : 1][C];
+  if constexpr (EARLY)
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[i]);
+  Sum s[1] = {0};
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+      const Sum f = Elem<T>::get(v[i], e);
+      s[0] += f * f;
+    }
+  row_sum<LANES>(s, slot);
+  if constexpr (!MX) {
+    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps);
+    if (!live) return;
+    T* y = row_of<T>(a.y, t, h);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e0 = (i * LANES + lane) * C;
+      if constexpr (!EARLY) load_weights(a.w, a.w_dtype, e0, D, w[0]);
+      float f[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) f[e] = Elem<T>::get(v[i], e) * r * w[EARLY ? i : 0][e];
+      store_piece(y, e0, D, pack_chunk<T>(f));
+    }
+  } else {
+    // In 64 bits up to the rounding to 8: which code a value next to a border gets, and a block its scale, is then
+    // not a matter of the order of the sum.
+    const double r = 1.0 / sqrt(s[0] / (double)D + (double)a.eps);
+    if (!live) return;
+    unsigned char* codes = a.mx.codes + (int64_t)row * D;
+    unsigned char* scales = a.mx.scales + row * a.mx.scale_stride;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e0 = (i * LANES + lane) * C;
+      if (e0 >= D) break;  // D is a multiple of 32: whole blocks of lanes
+      if constexpr (!EARLY) load_weights(a.w, a.w_dtype, e0, D, w[0]);
+      double y[C];
+      unsigned long long top = 0;
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        y[e] = (double)Elem<T>::get(v[i], e) * r * (double)w[EARLY ? i : 0][e];
+        top = max(top, (unsigned long long)__double_as_longlong(y[e]) & 0x7fffffffffffffffull);
+      }
+#pragma unroll
+      for (int d = 1; d < 32 / C; d <<= 1) top = max(top, (unsigned long long)__shfl_xor((long long)top, d));
+      // 448 = 1.75 * 2^8; magnitudes past f32 are as infinite as f32's infinity
+      int ex = max((int)(top >> 52) - 1023 - 8 + ((top & 0xfffffffffffffull) > 0xc000000000000ull), -127);
+      const bool bad = top >= 0x47f0000000000000ull;
+      float f[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) f[e] = bad ? 0.0f : round_to_odd(ldexp_f64(y[e], -ex));
+      if constexpr (C == 8)
+        *reinterpret_cast<u32x2*>(codes + e0) = u32x2{mx_pack_e4m3(f[0], f[1], f[2], f[3]), mx_pack_e4m3(f[4], f[5], f[6], f[7])};
+      else
+        *reinterpret_cast<uint32_t*>(codes + e0) = mx_pack_e4m3(f[0], f[1], f[2], f[3]);
+      if (e0 % 32 == 0) {
+        scales[e0 / 32] = bad ? 255 : (unsigned char)(ex + 127);
+        if (e0 + 32 == D)
+          for (int b = D / 32; b < (D / 32 + 3 & ~3); ++b) scales[b] = 0;
+      }
+    }
+  }
+}
+
+template <typename T, int LANES, int CH>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kernel(NormGradArgs a) {
+  constexpr int C = kC<T>, R = LANES > 256 ? 1 : 256 / LANES, TW = LANES / 64 > 0 ? LANES / 64 : 1;
+  __shared__ float slot[2][2 * TW];
+  const int lane = threadIdx.x % LANES, D = a.D;
+  const bool has_w = a.w_dtype >= 0;
+  // A workgroup of 1024 has 128 registers a lane: weights and dsum are then loaded where they are used, and no row ahead.
+  constexpr bool LEAN = LANES > 256;
+  float w[LEAN ? 1 : CH][C], dw[CH][C];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if constexpr (!LEAN) load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[i]);
+#pragma unroll
+    for (int e = 0; e < C; ++e) dw[i][e] = 0.0f;
+  }
+  u32x4 x[CH], dy[CH], ds[LEAN ? 1 : CH];
+  auto load = [&](int64_t at) {
+    const int row = (int)min(at, a.rows - 1), t = a.by_heads.div(row), h = row - t * a.heads;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e = (i * LANES + lane) * C;
+      x[i] = load_piece(row_of<const T>(a.x, t, h), e, D);
+      dy[i] = load_piece(row_of<const T>(a.dy, t, h), e, D);
+    }
+    if constexpr (!LEAN)
+      if (a.dsum.p)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) ds[i] = load_piece(row_of<const T>(a.dsum, t, h), (i * LANES + lane) * C, D);
+  };
+  const int64_t step = (int64_t)gridDim.x * R;
+  int64_t first = (int64_t)blockIdx.x * R;
+  int turn = 0;
+  load(first + threadIdx.x / LANES);
+  for (; first < a.rows; first += step, turn ^= 1) {  // the same count for every lane
+    const int64_t at = first + threadIdx.x / LANES;
+    const bool live = at < a.rows;
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      if constexpr (LEAN) load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[0]);
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const float xv = Elem<T>::get(x[i], e);
+        s[0] = fmaf(xv, xv, s[0]);
+        s[1] = fmaf(Elem<T>::get(dy[i], e) * w[LEAN ? 0 : i][e], xv, s[1]);
+      }
+    }
+    u32x4 x0[CH], dy0[CH], ds0[LEAN ? 1 : CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      x0[i] = x[i];
+      dy0[i] = dy[i];
+      if constexpr (!LEAN) ds0[i] = ds[i];
+    }
+    if (!LEAN && first + step < a.rows) load(at + step);
+    row_sum<LANES>(s, slot[turn]);
+    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
+    if (!live) continue;
+    const int row = (int)at, t = a.by_heads.div(row), h = row - t * a.heads;
+    T* dx = row_of<T>(a.dx, t, h);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e0 = (i * LANES + lane) * C;
+      if constexpr (LEAN) {
+        load_weights(a.w, a.w_dtype, e0, D, w[0]);
+        if (a.dsum.p) ds0[0] = load_piece(row_of<const T>(a.dsum, t, h), e0, D);
+      }
+      float f[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const float xv = Elem<T>::get(x0[i], e), g = Elem<T>::get(dy0[i], e);
+        f[e] = r * (g * w[LEAN ? 0 : i][e]) - c * xv;
+        dw[i][e] = fmaf(g, xv * r, dw[i][e]);
+      }
+      if (a.dsum.p)
+#pragma unroll
+        for (int e = 0; e < C; ++e) f[e] += Elem<T>::get(ds0[LEAN ? 0 : i], e);
+      store_piece(dx, e0, D, pack_chunk<T>(f));
+    }
+    if (LEAN && first + step < a.rows) load(at + step);
+  }
+  if (!has_w) return;
+  // The workgroup's rows are added up, then its sums are one row of the workspace.
+  float* part = a.part + (int64_t)blockIdx.x * D;
+  if constexpr (R > 1) {
+    __shared__ float all[R][LANES * CH * C];
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < C; ++e) all[threadIdx.x / LANES][(i * LANES + lane) * C + e] = dw[i][e];
+    __syncthreads();
+    for (int e = threadIdx.x; e < D; e += 256) {
+      float s = 0.0f;
+      for (int k = 0; k < R; ++k) s += all[k][e];
+      part[e] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const int at = (i * LANES + lane) * C + e;
+        if (at < D) part[at] = dw[i][e];
+      }
+  }
+}
+
+// 64 features a workgroup, its sixteen waves a sixteenth of the parts each.
+template <typename W>
+__global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* __restrict__ part, W* __restrict__ dw, int D, int parts) {
+  __shared__ float s[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+  float sum = 0.0f;
+  if (e < D) {
+#pragma unroll 8
+    for (int k = w; k < parts; k += 16) sum += part[(int64_t)k * D + e];
+  }
+  s[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && e < D) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) sum += s[k][lane];
+    Act<W>::st(dw, e, sum);
+  }
+}
+
+// Lanes of a row and pieces of a lane, by the pieces of a row.
+template <typename F>
+int by_pieces(int64_t pieces, F&& f) {
+#define MLXQ_ROW(MOST, LANES, CH) \
+  if (pieces <= MOST) return f(std::integral_constant<int, LANES>{}, std::integral_constant<int, CH>{})
+  MLXQ_ROW(8, 8, 1);
+  MLXQ_ROW(16, 16, 1);
+  MLXQ_ROW(32, 32, 1);
+  MLXQ_ROW(64, 64, 1);
+  MLXQ_ROW(128, 64, 2);
+  MLXQ_ROW(256, 256, 1);
+  MLXQ_ROW(512, 256, 2);
+  MLXQ_ROW(1024, 256, 4);
+  MLXQ_ROW(2048, 256, 8);
+  MLXQ_ROW(4096, 1024, 4);
+  return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
+#undef MLXQ_ROW
+}
+
+template <typename T>
+int norm(const NormArgs& a, hipStream_t st) {
+  return by_pieces((a.D + kC<T> - 1) / kC<T>, [&](auto lanes, auto ch) {
+    constexpr int LANES = decltype(lanes)::value, CH = decltype(ch)::value, R = LANES > 256 ? 1 : 256 / LANES;
+    if constexpr (LANES * CH * kC<T> <= 32768) {
+      const unsigned grid = (unsigned)((a.rows + R - 1) / R), threads = LANES > 256 ? LANES : 256;
+      if (a.mx.codes) rms_norm_kernel<T, LANES, CH, true><<<grid, threads, 0, st>>>(a);
+      else rms_norm_kernel<T, LANES, CH, false><<<grid, threads, 0, st>>>(a);
+    }
+    return check_launch("rms_norm");
+  });
+}
+
+template <typename T>
+int norm_grad(const NormGradArgs& a, hipStream_t st) {
+  return by_pieces((a.D + kC<T> - 1) / kC<T>, [&](auto lanes, auto ch) {
+    constexpr int LANES = decltype(lanes)::value, CH = decltype(ch)::value;
+    if constexpr (LANES * CH * kC<T> <= 32768)
+      rms_norm_grad_kernel<T, LANES, CH><<<(unsigned)a.parts, LANES > 256 ? LANES : 256, 0, st>>>(a);
+    return check_launch("rms_norm_backward");
+  });
+}
+
+}  // namespace
+
+int run_rms_norm(const NormArgs& a, int dtype, hipStream_t st) {
+  if (dtype == MLXQ_BFLOAT16) return norm<uint16_t>(a, st);
+  if (dtype == MLXQ_FLOAT16) return norm<_Float16>(a, st);
+  return norm<float>(a, st);
+}
+
+// Workgroups of the gradient: two to a CU of the MI355X's 256 (four of short rows), fewer where there are no rows for
+// them.  By sizes alone, so that sums are the same everywhere.
+int64_t norm_grad_parts(int64_t rows, int64_t D, int dtype) {
+  const int64_t C = dtype == MLXQ_FLOAT32 ? 4 : 8, pieces = (D + C - 1) / C;
+  const int64_t lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : pieces <= 128 ? 64 : 256;
+  const int64_t groups = (rows + 256 / lanes - 1) / (256 / lanes);
+  return std::min<int64_t>(groups, pieces <= 128 ? 1024 : 512);
+}
+
+int run_rms_norm_backward(const NormGradArgs& a, int dtype, hipStream_t st) {
+  int rc = MLXQ_OK;
+  if (a.parts == 0) {}  // no rows: the weight's gradient is 0
+  else if (dtype == MLXQ_BFLOAT16) rc = norm_grad<uint16_t>(a, st);
+  else if (dtype == MLXQ_FLOAT16) rc = norm_grad<_Float16>(a, st);
+  else rc = norm_grad<float>(a, st);
+  if (rc != MLXQ_OK || a.w_dtype < 0) return rc;
+  const unsigned grid = (unsigned)((a.D + 63) / 64);
+  if (a.w_dtype == MLXQ_BFLOAT16) rms_norm_weight_kernel<<<grid, 1024, 0, st>>>(a.part, (uint16_t*)a.dw, a.D, a.parts);
+  else if (a.w_dtype == MLXQ_FLOAT16) rms_norm_weight_kernel<<<grid, 1024, 0, st>>>(a.part, (_Float16*)a.dw, a.D, a.parts);
+  else rms_norm_weight_kernel<<<grid, 1024, 0, st>>>(a.part, (float*)a.dw, a.D, a.parts);
+  return check_launch("rms_norm_backward");
+}
+
+}  // namespace mlxq

@@ -1,0 +1,477 @@
+// route.hip — routing of tokens to experts, the plan of the experts' products, and the gradient of the weights.
+//
+// A wave a token; expert e lies in lane e % 64, place e / 64.  Scores are compared as integers whose order is that of
+// the numbers: the logits' own bits where there is no bias (f32: exact, and as the scores' order), else s + bias in 64
+// bits.  top_k rounds of a maximum over the wave; ballots then find the lowest expert that has it.  A few loads and a few
+// hundred instructions a token: a short call is a launch's latency, a long one bound by the vector units.
+//
+// The plan is a stable counting sort of the choices by expert: segments count their experts, and each choice's place is
+// its expert's start, plus that expert's choices in earlier segments, plus its rank in its own; the rank among 64 is
+// found by ballots, so that no result depends on the order of an atomic.
+#include <algorithm>
+
+#include "mx.h"
+
+namespace mlxq {
+
+namespace {
+
+// Integers in the order of the numbers, above those for NaN (1) and for what is not to be chosen (0).
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (v != v) return 1;
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 as 0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long key_of(double v) {
+  if (v != v) return 1;
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+  return v;
+}
+__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = max(v, (unsigned long long)__shfl_xor((long long)v, d));
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// WIDE: the choice is by s + bias, or a group's score is a sum: scores in 64 bits.
+template <typename T, int NE, bool WIDE>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  using Key = typename std::conditional<WIDE, unsigned long long, uint32_t>::type;
+  using Val = typename std::conditional<WIDE, double, float>::type;
+  __shared__ Val of_group[WIDE || NE > 0 ? 4 : 1][NE * 64];  // a wave's scores, for its groups
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = a.E;
+  const int t = blockIdx.x * 4 + wave;
+  if (t >= a.T) return;  // whole waves; no barrier below
+  float z[NE];
+  const T* row = (const T*)a.logits + t * a.row_stride;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) z[i] = i * 64 + lane < E ? Act<T>::ld(row, i * 64 + lane) : -INFINITY;
+  if (a.active && !a.active[t]) {
+    if (lane < a.k) {
+      a.ids[(int64_t)t * a.k + lane] = -1;
+      a.weights[(int64_t)t * a.k + lane] = 0.0f;
+    }
+    return;
+  }
+  const bool soft = a.scoring == MLXQ_ROUTE_SOFTMAX;
+  float top = -INFINITY;
+  bool undefined = false;  // softmax of a row with NaN or +infinity
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    top = fmaxf(top, z[i]);
+    undefined |= z[i] != z[i] || z[i] == INFINITY;
+  }
+  double total = 0.0, top64 = 0.0;
+  if (soft) {
+    top = wave_max(top);
+    undefined = __any(undefined);
+    top64 = top == -INFINITY ? 0.0 : (double)top;  // no expert is wanted: all scores 0
+    if (WIDE || !a.normalize) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) sum += i * 64 + lane < E ? exp((double)z[i] - top64) : 0.0;
+      total = wave_sum(sum);
+    }
+  }
+  auto score = [&](float v) {  // in 64 bits; softmax without its denominator where that cancels
+    if (!soft) return 1.0 / (1.0 + exp(-(double)v));
+    const double e = exp((double)v - top64);
+    return WIDE || !a.normalize ? (total > 0.0 ? e / total : 0.0) : e;
+  };
+  Val val[NE];
+  Key key[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int e = i * 64 + lane;
+    if constexpr (WIDE) {
+      // A group's score without a bias is of scores; the choice then goes by the logits, whose order is theirs.
+      val[i] = e < E ? score(z[i]) : 0.0;
+      if (a.bias) val[i] += e < E ? (double)a.bias[e] : 0.0;
+      key[i] = e < E ? a.bias ? key_of(val[i]) : (Key)key_of(z[i]) : 0;
+    } else {
+      val[i] = z[i];
+      key[i] = e < E ? key_of(z[i]) : 0;
+    }
+  }
+  if (a.kept < a.groups) {
+    // Lane g scores group g: its best, or the sum of its two best.  NaN counts as -infinity here.
+    const int size = E / a.groups;
+    Val* mine = of_group[wave];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = val[i];
+    __builtin_amdgcn_wave_barrier();
+    Val best = -INFINITY, next = -INFINITY;
+    if (lane < a.groups)
+      for (int e = 0; e < size; ++e) {
+        const Val v = mine[lane * size + e];
+        if (v > best) {
+          next = best;
+          best = v;
+        } else if (v > next) {
+          next = v;
+        }
+      }
+    Key gk = lane < a.groups ? key_of(a.best > 1 && size > 1 ? best + next : best) : 0;
+    unsigned long long kept = 0;
+    for (int j = 0; j < a.kept; ++j) {
+      const Key m = wave_max(gk);
+      const int g = __builtin_ctzll(__ballot(gk == m));
+      kept |= 1ull << g;
+      if (lane == g) gk = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = i * 64 + lane;
+      if (e < E && !(kept >> (e / size) & 1)) key[i] = 0;
+    }
+  }
+  int id = 0;  // lane j < k: the j-th choice
+  float zj = 0.0f;
+  for (int j = 0; j < a.k; ++j) {
+    Key m = key[0];
+#pragma unroll
+    for (int i = 1; i < NE; ++i) m = max(m, key[i]);
+    m = wave_max(m);
+    int e = 0;
+    float v = 0.0f;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const unsigned long long has = __ballot(key[i] == m);
+      if (!found && has) {
+        const int l = __builtin_ctzll(has);
+        found = true;
+        e = i * 64 + l;
+        v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(z[i]), l));
+        if (lane == l) key[i] = 0;
+      }
+    }
+    if (lane == j) {
+      id = e;
+      zj = v;
+    }
+  }
+  double w = lane < a.k ? score(zj) : 0.0;
+  if (a.normalize) {
+    const double sum = wave_sum(w);
+    w = sum == 0.0 ? 0.0 : w / sum;
+  }
+  if (soft && undefined) w = __longlong_as_double(0x7ff8000000000000ll);
+  if (lane < a.k) {
+    a.ids[(int64_t)t * a.k + lane] = id;
+    a.weights[(int64_t)t * a.k + lane] = (float)(w * (double)a.scale);
+  }
+}
+
+// dz from dw.  p: the scores; up: what arrives at a chosen one's.
+template <typename T, int NE>
+__global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const float* __restrict__ dweights, T* __restrict__ dz) {
+  const int lane = threadIdx.x & 63, E = a.E;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= a.T) return;
+  float p[NE], up[NE];
+  const T* row = (const T*)a.logits + t * a.row_stride;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    p[i] = i * 64 + lane < E ? Act<T>::ld(row, i * 64 + lane) : -INFINITY;
+    up[i] = 0.0f;
+  }
+  int id = -1;
+  float dw = 0.0f;
+  if (lane < a.k) {
+    id = a.ids[(int64_t)t * a.k + lane];
+    dw = dweights[(int64_t)t * a.k + lane] * a.scale;
+  }
+  const bool soft = a.scoring == MLXQ_ROUTE_SOFTMAX;
+  float q[NE];  // sigmoid: 1 - p
+  if (soft) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) top = fmaxf(top, p[i]);
+    top = wave_max(top);
+    if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      p[i] = expf(p[i] - top);
+      sum += p[i];
+    }
+    sum = wave_sum(sum);
+    const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) p[i] *= inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const float e = expf(-fabsf(p[i])), big = 1.0f / (1.0f + e), small = e * big;
+      q[i] = p[i] >= 0.0f ? small : big;
+      p[i] = p[i] >= 0.0f ? big : p[i] != p[i] ? p[i] : small;
+    }
+  }
+  // The choices go to their experts' lanes; what they share is summed on the way.
+  float sum = 0.0f, dot = 0.0f;
+  bool chosen[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) chosen[i] = false;
+  for (int j = 0; j < a.k; ++j) {
+    const int e = __builtin_amdgcn_readlane(id, j);
+    if ((unsigned)e >= (unsigned)E) continue;
+    const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dw), j));
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (i * 64 + lane == e) {
+        up[i] = g;
+        chosen[i] = true;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+    if (chosen[i]) {
+      sum += p[i];
+      dot += up[i] * p[i];
+    }
+  sum = wave_sum(sum);
+  dot = wave_sum(dot);
+  if (a.normalize) {
+    // w = p / sum: what arrives at p is (dw - dot / sum) / sum, and its mean under p is 0
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const float mean = dot * inv;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) up[i] = chosen[i] ? (up[i] - mean) * inv : 0.0f;
+    dot = 0.0f;
+  }
+  T* out = dz + (int64_t)t * E;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int e = i * 64 + lane;
+    if (e < E) Act<T>::st(out, e, soft ? p[i] * (up[i] - dot) : up[i] * p[i] * q[i]);
+  }
+}
+
+// ---- the plan ------------------------------------------------------------------------------------
+
+// Lanes of the wave whose expert is this lane's, as a mask: one ballot a bit.
+__device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
+  unsigned long long m = ~0ull;
+  for (int b = 0; b < bits; ++b) {
+    const unsigned long long set = __ballot(e >> b & 1);
+    m &= e >> b & 1 ? set : ~set;
+  }
+  return m;
+}
+
+// A segment of choices, by one wave, in steps of 64: f(choice, expert (E: none), lanes with the same one).
+template <typename F>
+__device__ __forceinline__ void walk(const int32_t* ids, int first, int last, int E, int bits, F&& f) {
+  const int lane = threadIdx.x & 63;
+  for (int c0 = first; c0 < last; c0 += 64) {
+    const int c = c0 + lane;
+    int e = c < last ? ids[c] : -1;
+    e = (unsigned)e < (unsigned)E ? e : E;
+    const unsigned long long in = __ballot(c < last);
+    f(c, c < last, e, same_expert(e, bits) & in);
+  }
+}
+
+// Counts of each segment's experts, [segments][E + 1].
+__global__ __launch_bounds__(64) void route_count_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
+                                                         int32_t* __restrict__ counts) {
+  __shared__ int count[1025];
+  const int lane = threadIdx.x, first = blockIdx.x * segment;
+  for (int e = lane; e <= E; e += 64) count[e] = 0;
+  __syncthreads();
+  walk(ids, first, min(n, first + segment), E, bits, [&](int, bool live, int e, unsigned long long same) {
+    if (live && lane == __builtin_ctzll(same)) count[e] += __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  });
+  __syncthreads();
+  for (int e = lane; e <= E; e += 64) counts[(int64_t)blockIdx.x * (E + 1) + e] = count[e];
+}
+
+// A segment a workgroup of W waves... with one segment there are no counts yet.
+__global__ __launch_bounds__(1024) void route_small_plan_kernel(const int32_t* __restrict__ ids, int n, int E, int bits,
+                                                                int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
+  __shared__ int next[16][1025];  // a wave's counts, then where its next choice of an expert goes
+  __shared__ int sums[1025 + 63];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, W = blockDim.x >> 6;
+  const int per = ((n + W - 1) / W + 63) & ~63, first = min(n, w * per), last = min(n, first + per);
+  for (int e = lane; e <= E; e += 64) next[w][e] = 0;
+  __builtin_amdgcn_wave_barrier();
+  walk(ids, first, last, E, bits, [&](int, bool live, int e, unsigned long long same) {
+    if (live && lane == __builtin_ctzll(same)) next[w][e] += __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  });
+  __syncthreads();
+  for (int e = tid; e <= E; e += blockDim.x) {
+    int s = 0;
+    for (int k = 0; k < W; ++k) s += next[k][e];
+    sums[e] = s;
+  }
+  __syncthreads();
+  if (w == 0) {
+    int before = 0;
+    for (int e0 = 0; e0 <= E; e0 += 64) {
+      const int e = e0 + lane, own = e <= E ? sums[e] : 0;
+      int s = own;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+      }
+      if (e <= E) {
+        sums[e] = before + s - own;
+        starts[e] = before + s - own;
+      }
+      before += __builtin_amdgcn_readlane(s, 63);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e <= E; e += blockDim.x) {
+    int s = sums[e];
+    for (int k = 0; k < W; ++k) {
+      const int c = next[k][e];
+      next[k][e] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+  walk(ids, first, last, E, bits, [&](int c, bool live, int e, unsigned long long same) {
+    const int at = live ? next[w][e] : 0, rank = __popcll(same & ((1ull << lane) - 1));
+    __builtin_amdgcn_wave_barrier();
+    if (live) {
+      rows[at + rank] = c;
+      if (rank == 0) next[w][e] = at + __popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
+  });
+}
+
+// Segment blockIdx.x's choices to their places: the totals of all segments, then those of the earlier ones.
+__global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
+                                                          const int32_t* __restrict__ counts, int segments,
+                                                          int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
+  __shared__ int sums[1025], next[1025];
+  const int tid = threadIdx.x, lane = tid & 63, mine = blockIdx.x;
+  for (int e = tid; e <= E; e += 256) {
+    int all = 0, before = 0;
+    for (int s = 0; s < segments; ++s) {
+      const int c = counts[(int64_t)s * (E + 1) + e];
+      all += c;
+      before += s < mine ? c : 0;
+    }
+    sums[e] = all;
+    next[e] = before;
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  int before = 0;
+  for (int e0 = 0; e0 <= E; e0 += 64) {
+    const int e = e0 + lane, own = e <= E ? sums[e] : 0;
+    int s = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(s, d);
+      if (lane >= d) s += o;
+    }
+    if (e <= E) {
+      next[e] += before + s - own;
+      if (mine == 0) starts[e] = before + s - own;
+    }
+    before += __builtin_amdgcn_readlane(s, 63);
+  }
+  __builtin_amdgcn_wave_barrier();
+  const int first = mine * segment;
+  walk(ids, first, min(n, first + segment), E, bits, [&](int c, bool live, int e, unsigned long long same) {
+    const int at = live ? next[e] : 0, rank = __popcll(same & ((1ull << lane) - 1));
+    __builtin_amdgcn_wave_barrier();
+    if (live) {
+      rows[at + rank] = c;
+      if (rank == 0) next[e] = at + __popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
+  });
+}
+
+constexpr int kOneGroup = 16384;  // choices that one workgroup sorts by itself
+int64_t segment_of(int64_t n) { return std::max<int64_t>(1024, ((n + 255) / 256 + 63) / 64 * 64); }
+
+template <typename F>
+int by_experts(int E, F&& f) {
+  if (E <= 64) return f(std::integral_constant<int, 1>{});
+  if (E <= 128) return f(std::integral_constant<int, 2>{});
+  if (E <= 256) return f(std::integral_constant<int, 4>{});
+  if (E <= 512) return f(std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 16>{});
+}
+
+template <typename T>
+int route(const RouteArgs& a, hipStream_t st) {
+  return by_experts(a.E, [&](auto n) {
+    constexpr int NE = decltype(n)::value;
+    const unsigned grid = (unsigned)((a.T + 3) / 4);
+    if (a.bias || (a.kept < a.groups && a.best > 1)) route_kernel<T, NE, true><<<grid, 256, 0, st>>>(a);
+    else route_kernel<T, NE, false><<<grid, 256, 0, st>>>(a);
+    return check_launch("route_experts");
+  });
+}
+
+template <typename T>
+int route_backward(const RouteArgs& a, const float* dweights, void* dz, hipStream_t st) {
+  return by_experts(a.E, [&](auto n) {
+    route_grad_kernel<T, decltype(n)::value><<<(unsigned)((a.T + 3) / 4), 256, 0, st>>>(a, dweights, (T*)dz);
+    return check_launch("route_experts_backward");
+  });
+}
+
+}  // namespace
+
+int run_route(const RouteArgs& a, int dtype, hipStream_t st) {
+  if (dtype == MLXQ_BFLOAT16) return route<uint16_t>(a, st);
+  if (dtype == MLXQ_FLOAT16) return route<_Float16>(a, st);
+  return route<float>(a, st);
+}
+
+int run_route_backward(const RouteArgs& a, int dtype, const float* dweights, void* dz, hipStream_t st) {
+  if (dtype == MLXQ_BFLOAT16) return route_backward<uint16_t>(a, dweights, dz, st);
+  if (dtype == MLXQ_FLOAT16) return route_backward<_Float16>(a, dweights, dz, st);
+  return route_backward<float>(a, dweights, dz, st);
+}
+
+size_t route_plan_workspace(int64_t choices, int64_t E) {
+  if (choices <= kOneGroup) return 0;
+  const int64_t seg = segment_of(choices);
+  return (size_t)((choices + seg - 1) / seg * (E + 1) * 4);
+}
+
+int run_route_plan(const int32_t* ids, int64_t choices, int64_t E, int32_t* starts, int32_t* rows, void* ws, hipStream_t st) {
+  int bits = 0;
+  while ((1 << bits) < E + 1) ++bits;
+  if (choices <= kOneGroup) {
+    const int waves = (int)std::min<int64_t>(16, std::max<int64_t>(1, (choices + 63) / 64));
+    route_small_plan_kernel<<<1, 64 * waves, 0, st>>>(ids, (int)choices, (int)E, bits, starts, rows);
+    return check_launch("route_plan");
+  }
+  const int64_t seg = segment_of(choices), n = (choices + seg - 1) / seg;
+  route_count_kernel<<<(unsigned)n, 64, 0, st>>>(ids, (int)choices, (int)E, bits, (int)seg, (int32_t*)ws);
+  if (int rc = check_launch("route_plan")) return rc;
+  route_place_kernel<<<(unsigned)n, 256, 0, st>>>(ids, (int)choices, (int)E, bits, (int)seg, (const int32_t*)ws, (int)n, starts, rows);
+  return check_launch("route_plan");
+}
+
+}  // namespace mlxq

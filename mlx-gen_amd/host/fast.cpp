@@ -625,6 +625,414 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- a decoder block in microscaled types (mlxq/mx.py) ---------------------------------------------
+
+// The one stride between the rows (last dimension) of t; false where there is none.
+bool row_stride(const at::Tensor& t, int64_t& stride) {
+  const int64_t d = t.dim();
+  if (d < 1 || (t.size(d - 1) > 1 && t.stride(d - 1) != 1)) return false;
+  int64_t rows = 0;
+  stride = t.size(d - 1);
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (rows == 0) {
+      stride = t.stride(i);
+      rows = t.size(i);
+    } else if (t.stride(i) != stride * rows) {
+      return false;
+    } else {
+      rows *= t.size(i);
+    }
+  }
+  return true;
+}
+
+const at::Tensor* any_gpu(PyObject* o) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.is_nested() || t.is_conj() || t.is_neg() || t.dim() < 1 || t.numel() == 0)
+    return nullptr;
+  return &t;
+}
+
+struct MxOperand {
+  at::Tensor codes, scales;
+  int64_t rows, K;
+  mlxq_mx m;
+};
+
+int64_t scale_pitch(int64_t K) { return (K / 32 + 3) / 4 * 4; }
+
+// (codes, scales), a tuple or a subclass of one, as the library reads them.
+bool get_mx(PyObject* o, MxOperand& x) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+  const at::Tensor *c = plain(PyTuple_GET_ITEM(o, 0), 16), *s = any_gpu(PyTuple_GET_ITEM(o, 1));
+  if (!c || !s || c->dim() < 1 || c->numel() == 0 || s->scalar_type() != at::kByte || s->dim() != c->dim() || s->device() != c->device())
+    return false;
+  const bool four = c->scalar_type() == at::kByte;
+  if (!four && c->scalar_type() != at::kFloat8_e4m3fn) return false;
+  x.K = c->size(-1) * (four ? 2 : 1);
+  if (x.K % 32 != 0 || s->size(-1) * 32 != x.K) return false;
+  for (int64_t i = 0; i + 1 < c->dim(); ++i)
+    if (c->size(i) != s->size(i)) return false;
+  x.rows = c->numel() / c->size(-1);
+  int64_t stride;
+  if (!row_stride(*s, stride) || reinterpret_cast<uintptr_t>(s->data_ptr()) % 4 != 0) return false;
+  if (x.rows == 1) stride = scale_pitch(x.K);
+  if (stride % 4 != 0 || stride < x.K / 32) return false;
+  x.codes = *c;
+  x.scales = *s;
+  x.m = {c->data_ptr(), s->data_ptr(), stride, four ? MLXQ_MX_E2M1 : MLXQ_MX_E4M3};
+  return true;
+}
+
+// New codes and scales for rows of K; `lead` are the dimensions before it.
+void new_mx(const at::Tensor& like, at::IntArrayRef shape, int format, MxOperand& x) {
+  at::DimVector d(shape.begin(), shape.end());
+  x.K = d.back();
+  d.back() = format == MLXQ_MX_E2M1 ? x.K / 2 : x.K;
+  x.codes = at::empty(d, like.options().dtype(format == MLXQ_MX_E2M1 ? at::kByte : at::kFloat8_e4m3fn));
+  const int64_t n = x.K / 32, pitch = scale_pitch(x.K);
+  d.back() = pitch;
+  x.scales = at::empty(d, like.options().dtype(at::kByte));
+  x.m = {x.codes.data_ptr(), x.scales.data_ptr(), pitch, format};
+  if (n != pitch) x.scales = x.scales.narrow(-1, 0, n);
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    PyObject* v = out ? THPVariable_Wrap(t) : nullptr;
+    if (!v) {
+      Py_XDECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, v);
+  }
+  return out;
+}
+
+at::ScalarType float_type(int dt) { return dt == MLXQ_BFLOAT16 ? at::kBFloat16 : dt == MLXQ_FLOAT16 ? at::kHalf : at::kFloat; }
+
+// A float scalar of any Python number.
+bool number(PyObject* o, float& v) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  v = (float)PyFloat_AsDouble(o);
+  return !PyErr_Occurred();
+}
+
+// None, or a contiguous float tensor of this shape.
+bool get_float(PyObject* o, at::IntArrayRef shape, const at::Tensor& like, at::Tensor& keep, int& dt) {
+  dt = 0;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o, 1);
+  if (!t || code_of(t->scalar_type()) < 0 || t->sizes() != shape || t->device() != like.device()) return false;
+  keep = *t;
+  dt = code_of(t->scalar_type());
+  return true;
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+at::Tensor workspace(const at::Tensor& like, size_t need) {
+  return need ? at::empty({(int64_t)need}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// mx_quantize(x, e4m3) -> (codes, scales)
+PyObject* mx_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int e4m3;
+    if (n != 2 || !truth(a[1], e4m3)) return nullptr;
+    const at::Tensor* p = any_gpu(a[0]);
+    if (!p || code_of(p->scalar_type()) < 0) return nullptr;
+    const at::Tensor x = *p;
+    int64_t stride;
+    const int64_t K = x.size(-1), C = 16 / x.element_size();
+    if (K % 32 != 0 || !row_stride(x, stride) || stride % C != 0 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return nullptr;
+    bool ok;
+    void* st = stream_of(x, ok);
+    if (!ok) return nullptr;
+    MxOperand out;
+    new_mx(x, x.sizes(), e4m3 ? MLXQ_MX_E4M3 : MLXQ_MX_E2M1, out);
+    if (unlocked([&] { return mlxq_mx_quantize(x.data_ptr(), code_of(x.scalar_type()), x.numel() / K, K, stride, &out.m, st); }) != MLXQ_OK)
+      return nullptr;
+    return tuple_of({out.codes, out.scales});
+  });
+}
+
+// mx_dequantize(x, dtype code)
+PyObject* mx_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    MxOperand x;
+    long dt;
+    if (n != 2 || !get_mx(a[0], x) || !ints(a + 1, 1, &dt)) return nullptr;
+    bool ok;
+    void* st = stream_of(x.codes, ok);
+    if (!ok) return nullptr;
+    at::DimVector d(x.codes.sizes().begin(), x.codes.sizes().end());
+    d.back() = x.K;
+    at::Tensor out = at::empty(d, x.codes.options().dtype(float_type((int)dt)));
+    if (unlocked([&] { return mlxq_mx_dequantize(&x.m, x.rows, x.K, out.data_ptr(), (int)dt, st); }) != MLXQ_OK) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// mx_matmul(x, w, bias, dtype code)
+PyObject* mx_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    MxOperand x, w;
+    long dt;
+    if (n != 4 || !get_mx(a[0], x) || !get_mx(a[1], w) || !ints(a + 3, 1, &dt)) return nullptr;
+    if (w.codes.dim() != 2 || w.K != x.K || w.codes.device() != x.codes.device()) return nullptr;
+    const int64_t N = w.rows;
+    at::Tensor bias;
+    int bias_dt;
+    if (!get_float(a[2], {N}, x.codes, bias, bias_dt)) return nullptr;
+    bool ok;
+    void* st = stream_of(x.codes, ok);
+    if (!ok) return nullptr;
+    at::DimVector d(x.codes.sizes().begin(), x.codes.sizes().end());
+    d.back() = N;
+    at::Tensor out = at::empty(d, x.codes.options().dtype(float_type((int)dt)));
+    const size_t need = mlxq_mx_matmul_workspace_size(x.rows, x.K, N, x.m.format);
+    at::Tensor ws = workspace(x.codes, need);
+    if (unlocked([&] {
+          return mlxq_mx_matmul(&x.m, x.rows, x.K, &w.m, N, ptr(bias), bias_dt, out.data_ptr(), (int)dt, ptr(ws), need, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// [..., D] as [tokens, heads, D] with two strides.
+bool get_rows(PyObject* o, at::Tensor& keep, mlxq_heads& h, int64_t& T) {
+  const at::Tensor* p = any_gpu(o);
+  if (!p || code_of(p->scalar_type()) < 0) return false;
+  const at::Tensor& t = *p;
+  const int64_t d = t.dim(), D = t.size(d - 1);
+  if (D > 1 && t.stride(d - 1) != 1) return false;
+  if (d == 1) {
+    h = {t.data_ptr(), 1, D, 0};
+    T = 1;
+  } else if (d == 2) {
+    h = {t.data_ptr(), 1, t.stride(0), 0};
+    T = t.size(0);
+  } else if (d == 3) {
+    h = {t.data_ptr(), t.size(1), t.stride(0), t.stride(1)};
+    T = t.size(0);
+  } else {
+    if (!t.is_contiguous()) return false;
+    h = {t.data_ptr(), t.size(d - 2), t.size(d - 2) * D, D};
+    T = t.numel() / (D * t.size(d - 2));
+  }
+  keep = t;
+  return true;
+}
+
+bool get_rows_like(PyObject* o, const at::Tensor& like, at::Tensor& keep, mlxq_heads& h) {
+  int64_t T;
+  if (o == Py_None) return true;
+  return get_rows(o, keep, h, T) && keep.sizes() == like.sizes() && keep.scalar_type() == like.scalar_type() && keep.device() == like.device();
+}
+
+at::Tensor new_rows(const at::Tensor& x, const mlxq_heads& like, mlxq_heads& h) {
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  const int64_t D = x.size(-1);
+  h = {y.data_ptr(), like.heads, like.heads * D, D};
+  return y;
+}
+
+// rms_norm(x, weight, residual, eps, mx) -> y, (y, sum), (codes, scales) or (codes, scales, sum)
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    at::Tensor x, res, w, y, sum;
+    mlxq_heads xh, rh, yh, sh;
+    int64_t T;
+    float eps;
+    int mx, w_dt;
+    if (n != 5 || !number(a[3], eps) || !truth(a[4], mx) || !get_rows(a[0], x, xh, T) || !get_rows_like(a[2], x, res, rh)) return nullptr;
+    const int64_t D = x.size(-1);
+    if ((mx && D % 32 != 0) || !get_float(a[1], {D}, x, w, w_dt)) return nullptr;
+    bool ok;
+    void* st = stream_of(x, ok);
+    if (!ok) return nullptr;
+    MxOperand q;
+    if (mx) new_mx(x, x.sizes(), MLXQ_MX_E4M3, q);
+    else y = new_rows(x, xh, yh);
+    if (res.defined()) sum = new_rows(x, xh, sh);
+    if (unlocked([&] {
+          return mlxq_rms_norm(&xh, code_of(x.scalar_type()), T, D, res.defined() ? &rh : nullptr, sum.defined() ? &sh : nullptr, ptr(w),
+                               w_dt, eps, mx ? nullptr : &yh, mx ? &q.m : nullptr, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    if (mx) return sum.defined() ? tuple_of({q.codes, q.scales, sum}) : tuple_of({q.codes, q.scales});
+    return sum.defined() ? tuple_of({y, sum}) : THPVariable_Wrap(std::move(y));
+  });
+}
+
+// rms_norm_backward(dy, x, weight, dsum, eps) -> (dx, dweight)
+PyObject* rms_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    at::Tensor x, dy, ds, w, dw;
+    mlxq_heads xh, yh, sh, oh;
+    int64_t T;
+    float eps;
+    int w_dt;
+    if (n != 5 || a[0] == Py_None || !number(a[4], eps) || !get_rows(a[1], x, xh, T) || !get_rows_like(a[0], x, dy, yh) ||
+        !get_rows_like(a[3], x, ds, sh))
+      return nullptr;
+    const int64_t D = x.size(-1);
+    if (!get_float(a[2], {D}, x, w, w_dt)) return nullptr;
+    bool ok;
+    void* st = stream_of(x, ok);
+    if (!ok) return nullptr;
+    at::Tensor dx = new_rows(x, xh, oh);
+    size_t need = 0;
+    if (w.defined()) {
+      dw = at::empty(w.sizes(), w.options());
+      need = mlxq_rms_norm_backward_workspace_size(T, xh.heads, D, code_of(x.scalar_type()));
+    }
+    at::Tensor ws = workspace(x, need);
+    if (unlocked([&] {
+          return mlxq_rms_norm_backward(&yh, &xh, code_of(x.scalar_type()), T, D, ptr(w), w_dt, ds.defined() ? &sh : nullptr, eps, &oh,
+                                        ptr(dw), ptr(ws), need, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    if (dw.defined()) return tuple_of({dx, dw});
+    PyObject* first = THPVariable_Wrap(std::move(dx));
+    PyObject* out = first ? PyTuple_Pack(2, first, Py_None) : nullptr;
+    Py_XDECREF(first);
+    return out;
+  });
+}
+
+bool get_scoring(PyObject* o, int& v) {
+  if (!PyUnicode_CheckExact(o)) return false;
+  if (PyUnicode_CompareWithASCIIString(o, "softmax") == 0) v = MLXQ_ROUTE_SOFTMAX;
+  else if (PyUnicode_CompareWithASCIIString(o, "sigmoid") == 0) v = MLXQ_ROUTE_SIGMOID;
+  else return false;
+  return true;
+}
+
+bool get_logits(PyObject* o, at::Tensor& z) {
+  const at::Tensor* p = any_gpu(o);
+  if (!p || p->dim() != 2 || code_of(p->scalar_type()) < 0 || (p->stride(1) != 1 && p->size(1) > 1)) return false;
+  z = *p;
+  return true;
+}
+
+// route_experts(logits, top_k, scoring, bias, groups, kept_groups, group_best, normalize, scale, active)
+PyObject* route_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    at::Tensor z, bias, active;
+    mlxq_router r = {};
+    long k, g[3];
+    if (n != 10 || !get_logits(a[0], z) || !ints(a + 1, 1, &k) || !get_scoring(a[2], r.scoring) || !ints(a + 4, 3, g) ||
+        !truth(a[7], r.normalize) || !number(a[8], r.scale) || k < 1 || k > 64)
+      return nullptr;
+    const int64_t T = z.size(0), E = z.size(1);
+    if (a[3] != Py_None) {
+      const at::Tensor* t = get_exact(a[3], at::kFloat, {E}, z);
+      if (!t) return nullptr;
+      bias = *t;
+    }
+    if (a[9] != Py_None) {
+      const at::Tensor* t = plain(a[9], 1);
+      if (!t || t->scalar_type() != at::kBool || t->dim() != 1 || t->size(0) != T || t->device() != z.device()) return nullptr;
+      active = *t;
+    }
+    r.top_k = k;
+    r.bias = (const float*)ptr(bias);
+    r.groups = g[0];
+    r.kept_groups = g[1];
+    r.group_best = g[2];
+    bool ok;
+    void* st = stream_of(z, ok);
+    if (!ok) return nullptr;
+    at::Tensor ids = at::empty({T, k}, z.options().dtype(at::kInt)), w = at::empty({T, k}, z.options().dtype(at::kFloat)),
+               starts = at::empty({E + 1}, z.options().dtype(at::kInt)), rows = at::empty({T * k}, z.options().dtype(at::kInt));
+    const mlxq_routing out = {ids.data_ptr<int32_t>(), w.data_ptr<float>(), starts.data_ptr<int32_t>(), rows.data_ptr<int32_t>(), T, k, E};
+    const size_t need = mlxq_route_workspace_size(T * k, E);
+    at::Tensor ws = workspace(z, need);
+    if (unlocked([&] {
+          return mlxq_route_experts(z.data_ptr(), code_of(z.scalar_type()), z.stride(0), &r, (const uint8_t*)ptr(active), &out, ptr(ws),
+                                    need, st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return tuple_of({ids, w, starts, rows});
+  });
+}
+
+// route_experts_backward(dweights, logits, ids, scoring, normalize, scale)
+PyObject* route_experts_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    at::Tensor z;
+    mlxq_router r = {};
+    if (n != 6 || !get_logits(a[1], z) || !get_scoring(a[3], r.scoring) || !truth(a[4], r.normalize) || !number(a[5], r.scale)) return nullptr;
+    const at::Tensor* ip = plain(a[2], 4);
+    if (!ip || ip->scalar_type() != at::kInt || ip->dim() != 2 || ip->size(0) != z.size(0) || ip->device() != z.device()) return nullptr;
+    const at::Tensor ids = *ip;
+    const int64_t k = ids.size(1);
+    const at::Tensor* wp = get_exact(a[0], at::kFloat, {z.size(0), k}, z);
+    if (!wp || k < 1) return nullptr;
+    const at::Tensor dw = *wp;
+    bool ok;
+    void* st = stream_of(z, ok);
+    if (!ok) return nullptr;
+    r.top_k = k;
+    at::Tensor out = at::empty(z.sizes(), z.options());
+    const mlxq_routing routing = {ids.data_ptr<int32_t>(), nullptr, nullptr, nullptr, z.size(0), k, z.size(1)};
+    if (unlocked([&] {
+          return mlxq_route_experts_backward(dw.data_ptr<float>(), z.data_ptr(), code_of(z.scalar_type()), z.stride(0), &r, &routing,
+                                             out.data_ptr(), st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// mx_experts(x, w, routing, bias, combine, dtype code)
+PyObject* mx_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    MxOperand x, w;
+    int combine;
+    long dt;
+    if (n != 6 || !get_mx(a[0], x) || !get_mx(a[1], w) || !truth(a[4], combine) || !ints(a + 5, 1, &dt)) return nullptr;
+    if (w.codes.dim() != 3 || w.K != x.K || w.codes.device() != x.codes.device()) return nullptr;
+    const int64_t E = w.codes.size(0), N = w.codes.size(1);
+    if (!PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) != 4) return nullptr;
+    const at::Tensor* ip = plain(PyTuple_GET_ITEM(a[2], 0), 4);
+    if (!ip || ip->scalar_type() != at::kInt || ip->dim() != 2 || ip->device() != x.codes.device()) return nullptr;
+    const at::Tensor ids = *ip;
+    const int64_t T = ids.size(0), k = ids.size(1), xd = x.codes.dim();
+    const at::Tensor* wt = get_exact(PyTuple_GET_ITEM(a[2], 1), at::kFloat, {T, k}, ids);
+    const at::Tensor* sp = get_exact(PyTuple_GET_ITEM(a[2], 2), at::kInt, {E + 1}, ids);
+    const at::Tensor* rp = get_exact(PyTuple_GET_ITEM(a[2], 3), at::kInt, {T * k}, ids);
+    if (!wt || !sp || !rp || (xd != 2 && xd != 3) || x.codes.size(0) != T || (xd == 3 && x.codes.size(1) != k)) return nullptr;
+    const at::Tensor weights = *wt, starts = *sp, rows = *rp;
+    at::Tensor bias;
+    int bias_dt;
+    const int64_t bias_shape[2] = {E, N};
+    if (!get_float(a[3], at::IntArrayRef(bias_shape, 2), x.codes, bias, bias_dt)) return nullptr;
+    bool ok;
+    void* st = stream_of(x.codes, ok);
+    if (!ok) return nullptr;
+    const auto options = x.codes.options().dtype(float_type((int)dt));
+    at::Tensor out = combine ? at::empty({T, N}, options) : at::empty({T, k, N}, options);
+    const mlxq_routing routing = {ids.data_ptr<int32_t>(), weights.data_ptr<float>(), starts.data_ptr<int32_t>(), rows.data_ptr<int32_t>(),
+                                  T, k, E};
+    const size_t need = mlxq_mx_experts_workspace_size(T, k, E, x.K, N, x.m.format, combine, (int)dt);
+    at::Tensor ws = workspace(x.codes, need);
+    if (unlocked([&] {
+          return mlxq_mx_experts(&x.m, xd == 3, x.K, &w.m, N, ptr(bias), bias_dt, &routing, combine, out.data_ptr(), (int)dt, ptr(ws), need,
+                                 st);
+        }) != MLXQ_OK)
+      return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // set_error_type(MlxqError)
 PyObject* set_error_type(PyObject*, PyObject* type) {
   Py_INCREF(type);
@@ -644,6 +1052,14 @@ PyMethodDef kMethods[] = {
     {"cache_append", (PyCFunction)(void*)cache_append, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},
     {"copy_pages", (PyCFunction)(void*)copy_pages, METH_FASTCALL, nullptr},
+    {"mx_quantize", (PyCFunction)(void*)mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_dequantize", (PyCFunction)(void*)mx_dequantize, METH_FASTCALL, nullptr},
+    {"mx_matmul", (PyCFunction)(void*)mx_matmul, METH_FASTCALL, nullptr},
+    {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, nullptr},
+    {"rms_norm_backward", (PyCFunction)(void*)rms_norm_backward, METH_FASTCALL, nullptr},
+    {"route_experts", (PyCFunction)(void*)route_experts, METH_FASTCALL, nullptr},
+    {"route_experts_backward", (PyCFunction)(void*)route_experts_backward, METH_FASTCALL, nullptr},
+    {"mx_experts", (PyCFunction)(void*)mx_experts, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -32,6 +32,12 @@ MLXQ_ROPE_NTK = 2
 MLXQ_ROPE_YARN = 3
 MLXQ_ROPE_LLAMA3 = 4
 
+MLXQ_MX_E2M1 = 0
+MLXQ_MX_E4M3 = 1
+
+MLXQ_ROUTE_SOFTMAX = 0
+MLXQ_ROUTE_SIGMOID = 1
+
 # Size of the static per-device scratch array behind mlxq_linear_noalloc.
 MLXQ_NOALLOC_SCRATCH_BYTES = 8 << 20
 
@@ -66,6 +72,19 @@ EXPORTS = (
     "mlxq_paged_attention_workspace_size",
     "mlxq_paged_attention",
     "mlxq_cache_copy_pages",
+    "mlxq_mx_quantize",
+    "mlxq_mx_dequantize",
+    "mlxq_mx_matmul_workspace_size",
+    "mlxq_mx_matmul",
+    "mlxq_rms_norm",
+    "mlxq_rms_norm_backward_workspace_size",
+    "mlxq_rms_norm_backward",
+    "mlxq_route_workspace_size",
+    "mlxq_route_experts",
+    "mlxq_route_plan",
+    "mlxq_route_experts_backward",
+    "mlxq_mx_experts_workspace_size",
+    "mlxq_mx_experts",
 )
 
 
@@ -116,6 +135,22 @@ class Attention(ctypes.Structure):
     _fields_ = [("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_int64),
                 ("softcap", ctypes.c_float), ("prefix_lens", ctypes.c_void_p), ("alibi_slopes", ctypes.c_void_p),
                 ("sinks", ctypes.c_void_p)]
+
+
+class Mx(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("scale_stride", ctypes.c_int64),
+                ("format", ctypes.c_int)]
+
+
+class Router(ctypes.Structure):
+    _fields_ = [("scoring", ctypes.c_int), ("top_k", ctypes.c_int64), ("bias", ctypes.c_void_p), ("groups", ctypes.c_int64),
+                ("kept_groups", ctypes.c_int64), ("group_best", ctypes.c_int64), ("normalize", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
+class Routed(ctypes.Structure):
+    _fields_ = [("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("rows", ctypes.c_void_p),
+                ("tokens", ctypes.c_int64), ("top_k", ctypes.c_int64), ("experts", ctypes.c_int64)]
 
 
 _lib = None
@@ -180,6 +215,26 @@ def load():
     lib.mlxq_paged_attention_workspace_size.restype = ctypes.c_size_t
     lib.mlxq_paged_attention.argtypes = [_heads, _i64, _cache, _batch, _attn, _heads, _vp, ctypes.c_size_t, _vp]
     lib.mlxq_cache_copy_pages.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp]
+    _mx, _router, _routed = (ctypes.POINTER(t) for t in (Mx, Router, Routed))
+    _f32, _size = ctypes.c_float, ctypes.c_size_t
+    lib.mlxq_mx_quantize.argtypes = [_vp, _int, _i64, _i64, _i64, _mx, _vp]
+    lib.mlxq_mx_dequantize.argtypes = [_mx, _i64, _i64, _vp, _int, _vp]
+    lib.mlxq_mx_matmul_workspace_size.argtypes = [_i64, _i64, _i64, _int]
+    lib.mlxq_mx_matmul.argtypes = [_mx, _i64, _i64, _mx, _i64, _vp, _int, _vp, _int, _vp, _size, _vp]
+    lib.mlxq_rms_norm.argtypes = [_heads, _int, _i64, _i64, _heads, _heads, _vp, _int, _f32, _heads, _mx, _vp]
+    lib.mlxq_rms_norm_backward_workspace_size.argtypes = [_i64, _i64, _i64, _int]
+    lib.mlxq_rms_norm_backward.argtypes = [_heads, _heads, _int, _i64, _i64, _vp, _int, _heads, _f32, _heads, _vp, _vp, _size, _vp]
+    lib.mlxq_route_workspace_size.argtypes = [_i64, _i64]
+    lib.mlxq_route_experts.argtypes = [_vp, _int, _i64, _router, _vp, _routed, _vp, _size, _vp]
+    lib.mlxq_route_plan.argtypes = [_routed, _vp, _size, _vp]
+    lib.mlxq_route_experts_backward.argtypes = [_vp, _vp, _int, _i64, _router, _routed, _vp, _vp]
+    lib.mlxq_mx_experts_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _int, _int, _int]
+    lib.mlxq_mx_experts.argtypes = [_mx, _int, _i64, _mx, _i64, _vp, _int, _routed, _int, _vp, _int, _vp, _size, _vp]
+    for name in ("mlxq_mx_matmul", "mlxq_rms_norm_backward", "mlxq_route", "mlxq_mx_experts"):
+        getattr(lib, name + "_workspace_size").restype = _size
+    for name in ("mlxq_mx_quantize", "mlxq_mx_dequantize", "mlxq_mx_matmul", "mlxq_rms_norm", "mlxq_rms_norm_backward",
+                 "mlxq_route_experts", "mlxq_route_plan", "mlxq_route_experts_backward", "mlxq_mx_experts"):
+        getattr(lib, name).restype = _int
     for name in ("mlxq_rotary_frequencies", "mlxq_rotary_table", "mlxq_rotary", "mlxq_cache_append",
                  "mlxq_paged_attention", "mlxq_cache_copy_pages"):
         getattr(lib, name).restype = _int
