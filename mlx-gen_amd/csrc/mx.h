@@ -106,6 +106,7 @@ struct MxProduct {
   // routed: E experts' runs of `rows`; E = 0: dense
   int E;
   const int32_t *starts, *rows;
+  bool skip_none;        // rows of choices without an expert are not written
   Divisor by_choices;    // x row of a choice: choice / by_choices (1: a row for each choice)
 };
 int64_t mx_product_splits(int64_t M, int64_t K, int64_t N, int format, int64_t E);

@@ -375,6 +375,7 @@ int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx
   p.E = (int)E;
   p.starts = routing->starts;
   p.rows = routing->rows;
+  p.skip_none = combine != 0;  // the sum leaves them out
   p.by_choices = Divisor(x_per_choice ? 1 : k);
   if ((rc = run_mx_product(p, x->format, (hipStream_t)stream))) return rc;
   if (!combine) return MLXQ_OK;

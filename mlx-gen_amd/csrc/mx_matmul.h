@@ -82,23 +82,25 @@ struct MxTiles {
   }
 };
 
-// Four neighbouring features of a row, rounded to y's type (f32 partial sums where K is split).
-__device__ __forceinline__ float mx_bias(const MxProduct& p, int64_t at) {
-  return p.bias_dtype == MLXQ_BFLOAT16 ? Act<uint16_t>::ld((const uint16_t*)p.bias, at)
-         : p.bias_dtype == MLXQ_FLOAT16 ? Act<_Float16>::ld((const _Float16*)p.bias, at) : ((const float*)p.bias)[at];
+// The bias of four neighbouring features of expert e; 0 past the last.
+__device__ __forceinline__ f32x4 mx_bias(const MxProduct& p, int e, int n) {
+  f32x4 v = {0, 0, 0, 0};
+  if (!p.bias || e >= max(p.E, 1)) return v;
+  const int64_t at = (int64_t)e * p.N;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = at + min(n + i, (int)p.N - 1);
+    v[i] = p.bias_dtype == MLXQ_BFLOAT16 ? Act<uint16_t>::ld((const uint16_t*)p.bias, k)
+           : p.bias_dtype == MLXQ_FLOAT16 ? Act<_Float16>::ld((const _Float16*)p.bias, k) : ((const float*)p.bias)[k];
+  }
+  return v;
 }
-__device__ __forceinline__ void mx_store(const MxProduct& p, int e, int row, int n, f32x4 v) {
+// Four neighbouring features of a row, rounded to y's type.  Rows of any N start at any element.
+__device__ __forceinline__ void mx_store(const MxProduct& p, int row, int n, const f32x4& v) {
   const int N = (int)p.N;
   if (n >= N) return;
   const int64_t at = (int64_t)row * N + n;
   const bool four = n + 4 <= N;
-  if (p.bias && e < max(p.E, 1)) {
-    const int64_t b = (int64_t)e * N + n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < N) v[i] += mx_bias(p, b + i);
-  }
-  // Rows of any N start at any element.
   if (p.y_dtype == MLXQ_FLOAT32) {
     float* y = (float*)p.y + at;
     if (four) {
@@ -190,30 +192,39 @@ __device__ __forceinline__ void mx_dma4(const unsigned char* from, uint32_t lds)
 #undef MLXQ_DMA
 
 // A workgroup of WM x WN waves takes TM rows by TN features; steps of 128 values of K go through a ring of STAGES
-// buffers in LDS by DMA, one barrier a step.
+// buffers in LDS by DMA, one barrier a step.  The scales of four steps go together, 16 bytes of 16 rows a load: a row's
+// scales of one step are 4 bytes of a cache line of their own, and fetched step by step they were half of all requests.
 template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int n_tiles) {
   constexpr int NW = WM * WN, XB = XF == kE4M3 ? 128 : 64, XN = XF == kE4M3 ? 2 : 1;
   constexpr int FM = TM / WM / 16, FN = TN / WN / 16;
-  constexpr int XI = TM * XB / 1024 / NW, WI = TN * 64 / 1024 / NW, PER = XI + WI + 1;  // DMA loads of a wave a step
-  constexpr int W0 = TM * XB, S0 = W0 + TN * 64, STAGE = S0 + (TM + TN) * 4;
-  static_assert(XI >= 1 && WI >= 1 && STAGE * STAGES <= 163840 && (TM + TN) / 64 <= NW, "a step is whole loads of each wave");
-  __shared__ __align__(1024) unsigned char lds[STAGE * STAGES];
+  constexpr int XI = TM * XB / 1024 / NW, WI = TN * 64 / 1024 / NW, PER = XI + WI;  // DMA loads of a wave a step
+  constexpr int W0 = TM * XB, STAGE = W0 + TN * 64;
+  // A group of scales: loads of 16 rows each, in up to four parts of a load a wave.
+  constexpr int SP = (TM + TN) / 16, GROUP = (TM + TN) * 16, GROUPS = STAGES == 3 ? 2 : 3, S0 = STAGE * STAGES;
+  static_assert(XI >= 1 && WI >= 1 && S0 + GROUP * GROUPS <= 163840 && SP <= 4 * NW, "a step is whole loads of each wave");
+  __shared__ __align__(1024) unsigned char lds[S0 + GROUP * GROUPS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
 
-  // Neighbouring workgroups go to different dies: each die takes a run of tiles of its own, in blocks of 8 tiles of
-  // rows by all of the features, so that what its workgroups read at a time shares its cache.
+  // Neighbouring workgroups go to different dies: each die takes a run of tiles of its own, in bands of 4 tiles of
+  // rows by all of the features, so that what its workgroups read at a time shares its cache (8192 rows, 14336 features,
+  // K 4096: bands of 4, 8 and 16 tiles 416, 422 and 431 us).
+  constexpr int BAND = 4;
   MxTiles tiles{p, TM};
   const int m_tiles = tiles.total(), all = m_tiles * n_tiles, chunk = (all + 7) / 8;
   const int l = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= chunk || l >= all) return;
-  const int band = l / (8 * n_tiles), in = l - band * 8 * n_tiles, high = min(8, m_tiles - 8 * band);
-  const int nt = in / high, mt = 8 * band + in - nt * high;
+  const int band = l / (BAND * n_tiles), in = l - band * BAND * n_tiles, high = min(BAND, m_tiles - BAND * band);
+  const int nt = in / high, mt = BAND * band + in - nt * high;
   const MxTile tile = tiles.find(mt);
-  if (!tile.found) return;
+  if (!tile.found || (p.skip_none && tile.e == p.E)) return;
   const int n0 = nt * TN, N = (int)p.N, K = (int)p.K;
-  const int steps = (K + 127) / 128, s0 = 0, s1 = steps;
+  const int steps = (K + 127) / 128;
+  // Waves of one SIMD (w and w + 4) hold different rows: where a run's last tile has half its rows or fewer, a wave of
+  // each SIMD has none and leaves the matrix cores to the other.
+  const int wm = w / WN, wn = w % WN;
+  const bool idle = wm * (TM / WM) >= tile.count;
 
   f32x4 acc[FN][FM];
 #pragma unroll
@@ -222,16 +233,16 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
     for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
   if (tile.e < max(p.E, 1)) {
-    const unsigned char *xp[XI], *wp[WI], *sp;
+    const unsigned char *xp[XI], *wp[WI], *sp[4];
     int xk[XI], wk;  // the first value of K of a lane's piece
     const int64_t x_pitch = XF == kE4M3 ? K : K / 2, w_pitch = K / 2;
+    auto x_row = [&](int r) { return tiles.x_row(tiles.row(tile.first + min(r, tile.count - 1))); };
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
       const int j = w * XI + i, r = XF == kE4M3 ? 8 * j + (lane >> 3) : 16 * j + (lane >> 2);
       const int piece = XF == kE4M3 ? (lane & 7) ^ (r & 7) : (lane & 3) ^ (r >> 1 & 3);
-      const int64_t row = tiles.x_row(tiles.row(tile.first + min(r, tile.count - 1)));
       xk[i] = piece * (XF == kE4M3 ? 16 : 32);
-      xp[i] = p.x.codes + row * x_pitch + piece * 16;
+      xp[i] = p.x.codes + x_row(r) * x_pitch + piece * 16;
     }
     const int64_t w_row0 = (int64_t)tile.e * N;
 #pragma unroll
@@ -240,14 +251,35 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
       wk = piece * 32;
       wp[i] = p.w.codes + (w_row0 + min(n0 + r, N - 1)) * w_pitch + piece * 16;
     }
-    const int si = min(w, (TM + TN) / 64 - 1), sr = 64 * si + lane;
-    sp = sr < TM ? p.x.scales + tiles.x_row(tiles.row(tile.first + min(sr, tile.count - 1))) * p.x.scale_stride
-                 : p.w.scales + (w_row0 + min(n0 + sr - TM, N - 1)) * p.w.scale_stride;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * (i * NW + w) + (lane >> 2);
+      if (i * NW + w < SP)
+        sp[i] = r < TM ? p.x.scales + x_row(r) * p.x.scale_stride : p.w.scales + (w_row0 + min(n0 + r - TM, N - 1)) * p.w.scale_stride;
+    }
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
     const unsigned char* zeros = reinterpret_cast<const unsigned char*>(&mx_zeros);
     const bool ragged = K % 128 != 0;
+    const int last_dword = (K / 32 - 1) & ~3;  // of a row's scales
 
+    auto load_scales = [&](int group, int part) {
+      if (group * 4 >= steps || part * NW + w >= SP) return;
+      mx_dma4(sp[part] + min(group * 16 + 4 * (lane & 3), last_dword), base + S0 + (uint32_t)(group % GROUPS) * GROUP + (part * NW + w) * 256);
+    };
     auto load = [&](int s) {
+      // The parts of a group are spread over the steps before it so that two groups are held at a time (STAGES 3).  They
+      // come before the step's codes: a wait for these is one for all scales before them.
+      if (s == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_scales(0, i);
+      } else if ((s & 3) == 2) {
+        load_scales((s >> 2) + 1, 0);
+        load_scales((s >> 2) + 1, 1);
+      } else if ((s & 3) == 3) {
+        load_scales((s >> 2) + 1, 2);
+      } else if ((s & 3) == 0) {
+        load_scales(s >> 2, 3);
+      }
       const uint32_t to = base + (uint32_t)(s % STAGES) * STAGE;
       const int left = ragged && s == steps - 1 ? K - s * 128 : 128;
 #pragma unroll
@@ -255,142 +287,174 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
         mx_dma16(xk[i] < left ? xp[i] + (int64_t)s * XB : zeros, to + (w * XI + i) * 1024);
 #pragma unroll
       for (int i = 0; i < WI; ++i) mx_dma16(wk < left ? wp[i] + (int64_t)s * 64 : zeros, to + W0 + (w * WI + i) * 1024);
-      mx_dma4(sp + s * 4, to + S0 + si * 256);
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
-      if (s0 + i < s1) load(s0 + i);
+      if (i < steps) load(i);
 
-    const int wm = w % WM, wn = w / WM;
     const int xr = wm * (TM / WM) + c, wr = wn * (TN / WN) + c;  // this lane's rows of the first fragments
     // Of an e4m3 row a lane reads pieces g and g + 4 (EXACT: 2 g and 2 g + 1); piece i of row r lies at i ^ (r % 8).
     constexpr int SECOND = EXACT ? 16 : 64;
     const int x_at = XF == kE4M3 ? xr * 128 + (((EXACT ? 2 * g : g) ^ (c & 7)) * 16) : xr * 64 + ((g ^ (c >> 1 & 3)) * 16);
     const int w_at = W0 + wr * 64 + ((g ^ (c >> 1 & 3)) * 16);
-    const int xs_at = S0 + xr * 4 + g, ws_at = S0 + (TM + wr) * 4 + g;
+    const int xs_at = xr * 16 + g, ws_at = (TM + wr) * 16 + g;
 
-    for (int s = s0; s < s1; ++s) {
-      if (s + STAGES - 2 < s1) mlxq_vmcnt<(STAGES - 2) * PER>();
-      else mlxq_vmcnt<0>();
+    // One step.  Fragments are read a few at a time, those of a square that grows by one of x and Q of the weights, and
+    // multiplied as soon as a square is there: after a barrier all waves read at once, and the matrix cores would wait
+    // until the last had everything.
+    constexpr int Q = FN / FM;
+    static_assert(FN % FM == 0, "squares of fragments");
+    auto step = [&](int s, bool wait_all, bool ahead, auto LAST) {
+      if (wait_all) mlxq_vmcnt<0>();
+      else mlxq_vmcnt<(STAGES - 2) * PER>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s + STAGES - 1 < s1) load(s + STAGES - 1);
-      const unsigned char* b = lds + (s % STAGES) * STAGE;
-      const bool past = ragged && s == steps - 1 && g * 32 >= K - s * 128;  // this lane's block is past K
+      const unsigned char *b = lds + (s % STAGES) * STAGE, *sb = lds + S0 + ((s >> 2) % GROUPS) * GROUP + (s & 3) * 4;
+      const bool past = decltype(LAST)::value && g * 32 >= K - s * 128;  // this lane's block is past K
       MxFrag<XF, EXACT> x[FM];
-#pragma unroll
-      for (int j = 0; j < FM; ++j) {
+      MxFrag<kE2M1, EXACT> a[FN];
+      auto read = [&](int j) {
         u32x4 v[XN];
         v[0] = *reinterpret_cast<const u32x4*>(b + x_at + j * 16 * XB);
         if constexpr (XN == 2) v[1] = *reinterpret_cast<const u32x4*>(b + (x_at ^ SECOND) + j * 16 * XB);
-        x[j].set(v, past ? 0 : b[xs_at + j * 64]);
-      }
+        const int xs = sb[xs_at + j * 256];
+        x[j].set(v, past ? 0 : xs);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        MxFrag<kE2M1, EXACT> a;
-        const u32x4 v[1] = {*reinterpret_cast<const u32x4*>(b + w_at + i * 1024)};
-        a.set(v, past ? 0 : b[ws_at + i * 64]);
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = mx_mma<XF, EXACT>(a, x[j], acc[i][j]);
+        for (int i = j * Q; i < (j + 1) * Q; ++i) {
+          const u32x4 u[1] = {*reinterpret_cast<const u32x4*>(b + w_at + i * 1024)};
+          const int ws = sb[ws_at + i * 256];
+          a[i].set(u, past ? 0 : ws);
+        }
+      };
+      if (idle) {
+        if (ahead) load(s + STAGES - 1);
+        return;
       }
-    }
+      read(0);
+      if constexpr (FM > 1) read(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        if (j > 0 && j + 1 < FM) read(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (j == 0 && ahead) load(s + STAGES - 1);
+#pragma unroll
+        for (int i = 0; i < (j + 1) * Q; ++i)
+#pragma unroll
+          for (int k = 0; k <= j; ++k)
+            if (k == j || i >= j * Q) acc[i][k] = mx_mma<XF, EXACT>(a[i], x[k], acc[i][k]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int s = 0; s + 1 < steps; ++s)
+      step(s, s + STAGES - 2 >= steps, s + STAGES - 1 < steps, std::false_type{});
+    step(steps - 1, true, false, std::true_type{});
   }
-  const int wm = w % WM, wn = w / WM;
+  if (idle) return;
+  int row[FM];
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int r = wm * (TM / WM) + j * 16 + c;
-    if (r >= tile.count) continue;
-    const int row = tiles.row(tile.first + r);
-    if (row < 0) continue;
+    row[j] = r < tile.count ? tiles.row(tile.first + r) : -1;
+  }
 #pragma unroll
-    for (int i = 0; i < FN; ++i) mx_store(p, tile.e, row, n0 + wn * (TN / WN) + i * 16 + 4 * g, acc[i][j]);
+  for (int i = 0; i < FN; ++i) {
+    const int n = n0 + wn * (TN / WN) + i * 16 + 4 * g;
+    const f32x4 bias = mx_bias(p, tile.e, n);
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+      if (row[j] >= 0) mx_store(p, row[j], n, acc[i][j] + bias);
   }
 }
 
 // ---- few rows ------------------------------------------------------------------------------------
 
-// 16 FM rows by 16 features a workgroup; its NW waves take a run of K each, weights and x straight from memory to the
-// operands, and join their sums in LDS.
-template <int XF, bool EXACT, int FM, int NW>
-__global__ __launch_bounds__(64 * NW) void mx_stream_kernel(MxProduct p, int n_tiles) {
-  constexpr int XN = XF == kE4M3 ? 2 : 1, AHEAD = FM > 1 ? 2 : 4;
-  __shared__ f32x4 part[NW][FM][64];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+// 16 FM rows by 16 features a wave, weights and x straight from memory to the operands, four steps of K ahead in
+// registers.  KS waves of a workgroup share a tile, a run of K each, and join their sums in LDS.  Bound by the reading of the
+// weights; their loads go out before the rows of x are looked up in the plan.
+template <int XF, bool EXACT, int FM, int KS>
+__global__ __launch_bounds__(KS > 4 ? 64 * KS : 256) void mx_stream_kernel(MxProduct p, int n_tiles) {
+  constexpr int XN = XF == kE4M3 ? 2 : 1, AHEAD = FM > 1 ? 2 : 4, NW = KS > 4 ? KS : 4, NT = NW / KS;
+  __shared__ f32x4 part[KS > 1 ? NW : 1][FM][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   MxTiles tiles{p, 16 * FM};
-  const int mt = blockIdx.x / n_tiles, n0 = (blockIdx.x - mt * n_tiles) * 16;
+  const int mt = blockIdx.x / n_tiles, n0 = ((blockIdx.x - mt * n_tiles) * NT + w / KS) * 16;
   const MxTile tile = tiles.find(mt);
-  if (!tile.found) return;
+  if (!tile.found || (p.skip_none && tile.e == p.E)) return;
   const int N = (int)p.N, K = (int)p.K, steps = (K + 127) / 128;
   f32x4 acc[FM];
 #pragma unroll
   for (int j = 0; j < FM; ++j) acc[j] = f32x4{0, 0, 0, 0};
-  if (tile.e < max(p.E, 1)) {
+  if (tile.e < max(p.E, 1) && n0 < N) {
     const int64_t wrow = (int64_t)tile.e * N + min(n0 + c, N - 1);
-    const unsigned char *wp = p.w.codes + wrow * (K / 2) + g * 16, *ws = p.w.scales + wrow * p.w.scale_stride + g;
+    const unsigned char *wp = p.w.codes + wrow * (K / 2) + g * 16, *ws = p.w.scales + wrow * p.w.scale_stride;
     const unsigned char *xp[FM], *xs[FM];
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int64_t row = tiles.x_row(tiles.row(tile.first + min(j * 16 + c, tile.count - 1)));
-      xp[j] = p.x.codes + row * (XF == kE4M3 ? K : K / 2) + g * (EXACT && XF == kE4M3 ? 32 : 16);
-      xs[j] = p.x.scales + row * p.x.scale_stride + g;
-    }
-    const int per = (steps + NW - 1) / NW, s0 = min(steps, w * per), s1 = min(steps, s0 + per);
-    const int blocks = K / 32;
+    const int per = (steps + KS - 1) / KS, s0 = min(steps, w % KS * per), s1 = min(steps, s0 + per);
+    // Loads past a wave's run or the end of K are of zeros: a load that is made or not is a branch and a wait.
+    const unsigned char* zeros = reinterpret_cast<const unsigned char*>(&mx_zeros);
+    constexpr int SECOND = EXACT ? 16 : 64, XB = XF == kE4M3 ? 128 : 64;
     for (int s = s0; s < s1; s += AHEAD) {
       u32x4 a[AHEAD], x[AHEAD][FM][XN];
-      int as[AHEAD], bs[AHEAD][FM];
+      uint32_t as[AHEAD], bs[AHEAD][FM];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        // Past the end of K (or of the wave's run) codes and scales are 0.
-        const int t = s + k, block = 4 * t + g;
-        const bool in = t < s1 && block < blocks;
-        a[k] = u32x4{0, 0, 0, 0};
-        as[k] = 0;
-        if (in) {
-          a[k] = *reinterpret_cast<const u32x4*>(wp + (int64_t)t * 64);
-          as[k] = ws[4 * t];
-        }
+        const bool in = s + k < s1 && 128 * (s + k) + 32 * g < K;
+        a[k] = *reinterpret_cast<const u32x4*>(in ? wp + (int64_t)(s + k) * 64 : zeros);
+        as[k] = *reinterpret_cast<const uint32_t*>(in ? ws + 4 * (s + k) : zeros);
+      }
+      if (s == s0) {
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
-          bs[k][j] = in ? xs[j][4 * t] : 0;
-          if constexpr (XF == kE4M3) {
-            x[k][j][0] = x[k][j][1] = u32x4{0, 0, 0, 0};
-            constexpr int SECOND = EXACT ? 16 : 64;
-            const int first = 128 * t + (EXACT ? 32 : 16) * g;
-            if (t < s1 && first < K) x[k][j][0] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 128);
-            if (t < s1 && first + SECOND < K) x[k][j][1] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 128 + SECOND);
-          } else {
-            x[k][j][0] = u32x4{0, 0, 0, 0};
-            if (in) x[k][j][0] = *reinterpret_cast<const u32x4*>(xp[j] + (int64_t)t * 64);
-          }
+          const int64_t row = tiles.x_row(tiles.row(tile.first + min(j * 16 + c, tile.count - 1)));
+          xp[j] = p.x.codes + row * (XF == kE4M3 ? K : K / 2) + g * (EXACT && XF == kE4M3 ? 32 : 16);
+          xs[j] = p.x.scales + row * p.x.scale_stride;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const bool run = s + k < s1, in = run && 128 * (s + k) + 32 * g < K;
+        const int first = 128 * (s + k) + (XF == kE4M3 && !EXACT ? 16 : 32) * g;
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+#pragma unroll
+          for (int i = 0; i < XN; ++i)
+            x[k][j][i] = *reinterpret_cast<const u32x4*>(run && first + i * SECOND < K ? xp[j] + (int64_t)(s + k) * XB + i * SECOND : zeros);
+          bs[k][j] = *reinterpret_cast<const uint32_t*>(in ? xs[j] + 4 * (s + k) : zeros);
         }
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         MxFrag<kE2M1, EXACT> fa;
         const u32x4 v[1] = {a[k]};
-        fa.set(v, as[k]);
+        fa.set(v, as[k] >> 8 * g & 255);
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
           MxFrag<XF, EXACT> fx;
-          fx.set(x[k][j], bs[k][j]);
+          fx.set(x[k][j], bs[k][j] >> 8 * g & 255);
           acc[j] = mx_mma<XF, EXACT>(fa, fx, acc[j]);
         }
       }
     }
   }
+  if constexpr (KS > 1) {
 #pragma unroll
-  for (int j = 0; j < FM; ++j) part[w][j][lane] = acc[j];
-  __syncthreads();
-  for (int j = w; j < FM; j += NW) {
-    f32x4 v = part[0][j][lane];
+    for (int j = 0; j < FM; ++j) part[w][j][lane] = acc[j];
+    __syncthreads();
+  }
 #pragma unroll
-    for (int k = 1; k < NW; ++k) v += part[k][j][lane];
+  for (int j = 0; j < FM; ++j) {
+    if (KS > 1 && j % KS != w % KS) continue;
+    f32x4 v = acc[j];
+    if constexpr (KS > 1) {
+      v = part[w / KS * KS][j][lane];
+#pragma unroll
+      for (int k = 1; k < KS; ++k) v += part[w / KS * KS + k][j][lane];
+    }
     const int r = j * 16 + c;
-    if (r >= tile.count) continue;
+    if (r >= tile.count || n0 >= N) continue;
     const int row = tiles.row(tile.first + r);
-    if (row >= 0) mx_store(p, tile.e, row, n0 + 4 * g, v);
+    if (row >= 0) mx_store(p, row, n0 + 4 * g, v + mx_bias(p, tile.e, n0 + 4 * g));
   }
 }
 
@@ -410,19 +474,31 @@ int mx_launch_tile(const MxProduct& p, hipStream_t st) {
   return check_launch("mx product");
 }
 
-template <int XF, bool EXACT, int FM, int NW>
+template <int XF, bool EXACT, int FM, int KS>
 int mx_launch_stream(const MxProduct& p, hipStream_t st) {
-  const int64_t n_tiles = (p.N + 15) / 16, grid = mx_most_tiles(p, 16 * FM) * n_tiles;
+  constexpr int NW = KS > 4 ? KS : 4, NT = NW / KS;
+  const int64_t n_tiles = (p.N + 16 * NT - 1) / (16 * NT), grid = mx_most_tiles(p, 16 * FM) * n_tiles;
   if (grid > 0x7fffffff) return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles", (long long)grid);
-  mx_stream_kernel<XF, EXACT, FM, NW><<<(unsigned)grid, 64 * NW, 0, st>>>(p, (int)n_tiles);
+  mx_stream_kernel<XF, EXACT, FM, KS><<<(unsigned)grid, 64 * NW, 0, st>>>(p, (int)n_tiles);
   return check_launch("mx product");
+}
+
+// Waves that share a tile: as many as give the chip's SIMDs four waves each.
+template <int XF, bool EXACT, int FM>
+int mx_stream(const MxProduct& p, hipStream_t st) {
+  const int64_t tiles = mx_most_tiles(p, 16 * FM) * ((p.N + 15) / 16);
+  if (tiles >= 3072) return mx_launch_stream<XF, EXACT, FM, 1>(p, st);
+  if (tiles >= 1536) return mx_launch_stream<XF, EXACT, FM, 2>(p, st);
+  if (tiles >= 768) return mx_launch_stream<XF, EXACT, FM, 4>(p, st);
+  return mx_launch_stream<XF, EXACT, FM, 8>(p, st);
 }
 
 template <int XF, bool EXACT>
 int mx_product(const MxProduct& p, hipStream_t st) {
   const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;  // of an expert, about
-  if (rows <= 16) return mx_launch_stream<XF, EXACT, 1, 8>(p, st);
-  if (rows <= 64) return mx_launch_stream<XF, EXACT, 4, 8>(p, st);
+  if (rows <= 16) return mx_stream<XF, EXACT, 1>(p, st);
+  if (rows <= 32) return mx_stream<XF, EXACT, 2>(p, st);
+  if (rows <= 64) return mx_stream<XF, EXACT, 4>(p, st);
   const int64_t big = mx_most_tiles(p, 256) * ((p.N + 255) / 256), mid = mx_most_tiles(p, 128) * ((p.N + 127) / 128);
   if (big >= 512) return mx_launch_tile<XF, EXACT, 256, 256, 4, 2, 3>(p, st);
   if (mid >= 256) return mx_launch_tile<XF, EXACT, 128, 128, 2, 2, 3>(p, st);

@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restr
   });
 }
 
-constexpr int kOneGroup = 16384;  // choices that one workgroup sorts by itself
+constexpr int kOneGroup = 2048;  // choices that one workgroup sorts by itself
 int64_t segment_of(int64_t n) { return std::max<int64_t>(1024, ((n + 255) / 256 + 63) / 64 * 64); }
 
 template <typename F>
