@@ -33,6 +33,44 @@ __device__ __forceinline__ float mx_scale(uint32_t b) {
   return b == 255 ? __uint_as_float(0x7fc00000u) : b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
 }
 
+// v of another lane by a data-parallel move within the vector unit (a shuffle goes through LDS and takes ten times as long).
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_move(V v) {
+  if constexpr (sizeof(V) == 4) {
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, CTRL, 15, 15, false));
+  } else {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const int a = (int)w[0], b = (int)w[1];
+    return __builtin_bit_cast(V, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(a, a, CTRL, 15, 15, false),
+                                       (uint32_t)__builtin_amdgcn_update_dpp(b, b, CTRL, 15, 15, false)});
+  }
+}
+template <typename V>
+__device__ __forceinline__ V lane_value(V v, int lane) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(V, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)w[0], lane),
+                                       (uint32_t)__builtin_amdgcn_readlane((int)w[1], lane)});
+  }
+}
+// v of all lanes of a group of LANES (2 to 64, aligned) combined by f, in each of them.
+template <int LANES = 64, typename V, typename F>
+__device__ __forceinline__ V lanes_reduce(V v, F&& f) {
+  v = f(v, dpp_move<0xb1>(v));                            // quad_perm 1, 0, 3, 2
+  if constexpr (LANES > 2) v = f(v, dpp_move<0x4e>(v));   // quad_perm 2, 3, 0, 1
+  if constexpr (LANES > 4) v = f(v, dpp_move<0x141>(v));  // row_half_mirror
+  if constexpr (LANES > 8) v = f(v, dpp_move<0x140>(v));  // row_mirror
+  if constexpr (LANES == 32) {
+    const V a = lane_value(v, 0), b = lane_value(v, 16), c = lane_value(v, 32), d = lane_value(v, 48);
+    return (threadIdx.x & 32) ? f(c, d) : f(a, b);
+  }
+  if constexpr (LANES == 64) return f(f(lane_value(v, 0), lane_value(v, 16)), f(lane_value(v, 32), lane_value(v, 48)));
+  return v;
+}
+
 // A microscaled matrix as kernels see it.
 struct MxView {
   unsigned char* codes;

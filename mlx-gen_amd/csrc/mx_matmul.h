@@ -326,10 +326,6 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
           a[i].set(u, past ? 0 : ws);
         }
       };
-      if (idle) {
-        if (ahead) load(s + STAGES - 1);
-        return;
-      }
       read(0);
       if constexpr (FM > 1) read(1);
       __builtin_amdgcn_sched_barrier(0);
@@ -346,24 +342,30 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
         __builtin_amdgcn_sched_barrier(0);
       }
     };
+    if (idle) {
+      for (int s = 0; s < steps; ++s) {
+        if (s + STAGES - 2 >= steps || s + 1 == steps) mlxq_vmcnt<0>();
+        else mlxq_vmcnt<(STAGES - 2) * PER>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + STAGES - 1 < steps) load(s + STAGES - 1);
+      }
+      return;
+    }
     for (int s = 0; s + 1 < steps; ++s)
       step(s, s + STAGES - 2 >= steps, s + STAGES - 1 < steps, std::false_type{});
     step(steps - 1, true, false, std::true_type{});
   }
   if (idle) return;
-  int row[FM];
+  f32x4 bias[FN];
+#pragma unroll
+  for (int i = 0; i < FN; ++i) bias[i] = mx_bias(p, tile.e, n0 + wn * (TN / WN) + i * 16 + 4 * g);
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
-    const int r = wm * (TM / WM) + j * 16 + c;
-    row[j] = r < tile.count ? tiles.row(tile.first + r) : -1;
-  }
+    const int r = wm * (TM / WM) + j * 16 + c, row = r < tile.count ? tiles.row(tile.first + r) : -1;
+    if (row < 0) continue;
 #pragma unroll
-  for (int i = 0; i < FN; ++i) {
-    const int n = n0 + wn * (TN / WN) + i * 16 + 4 * g;
-    const f32x4 bias = mx_bias(p, tile.e, n);
-#pragma unroll
-    for (int j = 0; j < FM; ++j)
-      if (row[j] >= 0) mx_store(p, row[j], n, acc[i][j] + bias);
+    for (int i = 0; i < FN; ++i) mx_store(p, row, n0 + wn * (TN / WN) + i * 16 + 4 * g, acc[i][j] + bias[i]);
   }
 }
 

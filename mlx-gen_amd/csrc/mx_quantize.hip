@@ -42,8 +42,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
     uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(in[k].get(e)) & 0x7fffffffu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    top = lanes_reduce<4>(top, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
     const bool bad = top >= 0x7f800000u;
     const int ex = mx_exponent<FMT>(top);
     float f[8];

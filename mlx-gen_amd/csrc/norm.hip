@@ -22,21 +22,29 @@ namespace {
 template <typename T>
 constexpr int kC = Elem<T>::C;
 
-// 16 bytes at any element of a row; the part past its end is zero.
-template <typename T>
-__device__ __forceinline__ u32x4 load_piece(const T* row, int e, int D) {
-  u32x4 v = {0, 0, 0, 0};
-  if (e + kC<T> <= D) {
-    __builtin_memcpy(&v, row + e, 16);
-  } else if (e < D) {
+// A row's pieces of 16 bytes, the i-th of a lane at element (i LANES + lane) C.  Every load is made, so that all of them are
+// in flight together: a piece that reaches past the row's end is read from further to the left, and set_right once it is
+// used; one that begins past it holds anything.  Rows shorter than a piece go element by element.
+template <typename T, int LANES, int CH>
+__device__ __forceinline__ void load_row(u32x4 (&v)[CH], const T* row, int lane, int D) {
+  if (D >= kC<T>) {
 #pragma unroll
-    for (int i = 0; i < kC<T>; ++i)
-      if (e + i < D) {
-        if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(row[e + i]);
-        else v[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[e + i]) << 16 * (i % 2);
-      }
+    for (int i = 0; i < CH; ++i) __builtin_memcpy(&v[i], row + min((i * LANES + lane) * kC<T>, D - kC<T>), 16);
+  } else {
+    v[0] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < D; ++i) {
+      if constexpr (sizeof(T) == 4) v[0][i] = __float_as_uint(row[i]);
+      else v[0][i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[i]) << 16 * (i % 2);
+    }
   }
-  return v;
+}
+template <typename T>
+__device__ __forceinline__ void set_right(u32x4& v, int e, int D) {
+  if (D >= kC<T> && e + kC<T> > D)
+    for (int k = e + kC<T> - D; k > 0; --k) {
+      if constexpr (sizeof(T) == 4) v = u32x4{v[1], v[2], v[3], 0};
+      else v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    }
 }
 template <typename T>
 __device__ __forceinline__ void store_piece(T* row, int e, int D, const u32x4& v) {
@@ -54,11 +62,23 @@ __device__ __forceinline__ void store_piece(T* row, int e, int D, const u32x4& v
 
 template <typename W, int C>
 __device__ __forceinline__ void load_weights_of(const W* w, int e, int D, float (&f)[C]) {
+  if (D >= C) {
+    const int at = min(e, D - C);
+    constexpr int N = C > kC<W> ? C / kC<W> : 1, B = C < kC<W> ? C * (int)sizeof(W) : 16;
+    u32x4 v[N];
 #pragma unroll
-  for (int k = 0; k < C; k += kC<W>) {
-    const u32x4 v = load_piece(w, e + k, D);
+    for (int k = 0; k < N; ++k) __builtin_memcpy(&v[k], w + at + k * kC<W>, B);
 #pragma unroll
-    for (int i = 0; i < kC<W> && i < C; ++i) f[k + i] = Elem<W>::get(v, i);
+    for (int i = 0; i < C; ++i) f[i] = Elem<W>::get(v[i / kC<W>], i % kC<W>);
+    if (e < D)
+      for (int k = e - at; k > 0; --k) {
+#pragma unroll
+        for (int i = 0; i + 1 < C; ++i) f[i] = f[i + 1];
+        f[C - 1] = 0.0f;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) f[i] = e + i < D ? Act<W>::ld(w, e + i) : 0.0f;
   }
 }
 // C weights from feature e on; ones without a weight.
@@ -81,20 +101,20 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, int e, in
 template <int LANES, int N, typename V>
 __device__ __forceinline__ void row_sum(V (&v)[N], V* slot) {
 #pragma unroll
-  for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d);
+  for (int i = 0; i < N; ++i) v[i] = lanes_reduce<(LANES < 64 ? LANES : 64)>(v[i], [](V a, V b) { return a + b; });
   if constexpr (LANES > 64) {
-    constexpr int W = LANES / 64;
     const int w = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) slot[w * N + i] = v[i];
-    __syncthreads();
+    // Of LDS alone: a barrier for all memory would wait for the next row's loads.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = slot[i];
 #pragma unroll
-    for (int k = 1; k < W; ++k)
+    for (int k = 1; k < LANES / 64; ++k)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += slot[k * N + i];
   }
@@ -129,22 +149,25 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
   const int t = a.by_heads.div(row), h = row - t * a.heads;
   const T* x = row_of<const T>(a.x, t, h);
   u32x4 v[CH];
-#pragma unroll
-  for (int i = 0; i < CH; ++i) v[i] = load_piece(x, (i * LANES + lane) * C, D);
+  load_row<T, LANES>(v, x, lane, D);
   if (a.res.p) {
-    const T* res = row_of<const T>(a.res, t, h);
     u32x4 r[CH];
-#pragma unroll
-    for (int i = 0; i < CH; ++i) r[i] = load_piece(res, (i * LANES + lane) * C, D);
+    load_row<T, LANES>(r, row_of<const T>(a.res, t, h), lane, D);
     T* sum = row_of<T>(a.sum, t, h);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
+      const int e0 = (i * LANES + lane) * C;
+      if (e0 >= D) continue;
       float f[C];
 #pragma unroll
       for (int e = 0; e < C; ++e) f[e] = Elem<T>::get(v[i], e) + Elem<T>::get(r[i], e);
       v[i] = pack_chunk<T>(f);
-      if (live) store_piece(sum, (i * LANES + lane) * C, D, v[i]);
+      set_right<T>(v[i], e0, D);
+      if (live) store_piece(sum, e0, D, v[i]);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) set_right<T>(v[i], (i * LANES + lane) * C, D);
   }
   // The weights of short rows are under way while the sum is taken.
   constexpr bool EARLY = CH <= 2;
@@ -155,11 +178,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
   Sum s[1] = {0};
 #pragma unroll
   for (int i = 0; i < CH; ++i)
+    if ((i * LANES + lane) * C < D)
 #pragma unroll
-    for (int e = 0; e < C; ++e) {
-      const Sum f = Elem<T>::get(v[i], e);
-      s[0] += f * f;
-    }
+      for (int e = 0; e < C; ++e) {
+        const Sum f = Elem<T>::get(v[i], e);
+        s[0] += f * f;
+      }
   row_sum<LANES>(s, slot);
   if constexpr (!MX) {
     const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps);
@@ -168,6 +192,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e0 = (i * LANES + lane) * C;
+      if (e0 >= D) break;
       if constexpr (!EARLY) load_weights(a.w, a.w_dtype, e0, D, w[0]);
       float f[C];
 #pragma unroll
@@ -193,8 +218,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
         y[e] = (double)Elem<T>::get(v[i], e) * r * (double)w[EARLY ? i : 0][e];
         top = max(top, (unsigned long long)__double_as_longlong(y[e]) & 0x7fffffffffffffffull);
       }
-#pragma unroll
-      for (int d = 1; d < 32 / C; d <<= 1) top = max(top, (unsigned long long)__shfl_xor((long long)top, d));
+      top = lanes_reduce<32 / C>(top, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
       // 448 = 1.75 * 2^8; magnitudes past f32 are as infinite as f32's infinity
       int ex = max((int)(top >> 52) - 1023 - 8 + ((top & 0xfffffffffffffull) > 0xc000000000000ull), -127);
       const bool bad = top >= 0x47f0000000000000ull;
@@ -232,16 +256,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
   u32x4 x[CH], dy[CH], ds[LEAN ? 1 : CH];
   auto load = [&](int64_t at) {
     const int row = (int)min(at, a.rows - 1), t = a.by_heads.div(row), h = row - t * a.heads;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int e = (i * LANES + lane) * C;
-      x[i] = load_piece(row_of<const T>(a.x, t, h), e, D);
-      dy[i] = load_piece(row_of<const T>(a.dy, t, h), e, D);
-    }
+    load_row<T, LANES>(x, row_of<const T>(a.x, t, h), lane, D);
+    load_row<T, LANES>(dy, row_of<const T>(a.dy, t, h), lane, D);
     if constexpr (!LEAN)
-      if (a.dsum.p)
-#pragma unroll
-        for (int i = 0; i < CH; ++i) ds[i] = load_piece(row_of<const T>(a.dsum, t, h), (i * LANES + lane) * C, D);
+      if (a.dsum.p) load_row<T, LANES>(ds, row_of<const T>(a.dsum, t, h), lane, D);
   };
   const int64_t step = (int64_t)gridDim.x * R;
   int64_t first = (int64_t)blockIdx.x * R;
@@ -253,7 +271,11 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if constexpr (LEAN) load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[0]);
+      const int e0 = (i * LANES + lane) * C;
+      if (e0 >= D) continue;
+      if constexpr (LEAN) load_weights(a.w, a.w_dtype, e0, D, w[0]);
+      set_right<T>(x[i], e0, D);
+      set_right<T>(dy[i], e0, D);
 #pragma unroll
       for (int e = 0; e < C; ++e) {
         const float xv = Elem<T>::get(x[i], e);
@@ -277,9 +299,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e0 = (i * LANES + lane) * C;
+      if (e0 >= D) continue;
       if constexpr (LEAN) {
         load_weights(a.w, a.w_dtype, e0, D, w[0]);
-        if (a.dsum.p) ds0[0] = load_piece(row_of<const T>(a.dsum, t, h), e0, D);
+        if (a.dsum.p) {
+          u32x4 one[1];
+          load_row<T, LANES>(one, row_of<const T>(a.dsum, t, h), i * LANES + lane, D);
+          ds0[0] = one[0];
+        }
       }
       float f[C];
 #pragma unroll
@@ -288,9 +315,11 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
         f[e] = r * (g * w[LEAN ? 0 : i][e]) - c * xv;
         dw[i][e] = fmaf(g, xv * r, dw[i][e]);
       }
-      if (a.dsum.p)
+      if (a.dsum.p) {
+        set_right<T>(ds0[LEAN ? 0 : i], e0, D);
 #pragma unroll
         for (int e = 0; e < C; ++e) f[e] += Elem<T>::get(ds0[LEAN ? 0 : i], e);
+      }
       store_piece(dx, e0, D, pack_chunk<T>(f));
     }
     if (LEAN && first + step < a.rows) load(at + step);
@@ -390,13 +419,13 @@ int run_rms_norm(const NormArgs& a, int dtype, hipStream_t st) {
   return norm<float>(a, st);
 }
 
-// Workgroups of the gradient: two to a CU of the MI355X's 256 (four of short rows), fewer where there are no rows for
+// Workgroups of the gradient: three to a CU of the MI355X's 256 (four of short rows), fewer where there are no rows for
 // them.  By sizes alone, so that sums are the same everywhere.
 int64_t norm_grad_parts(int64_t rows, int64_t D, int dtype) {
   const int64_t C = dtype == MLXQ_FLOAT32 ? 4 : 8, pieces = (D + C - 1) / C;
   const int64_t lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : pieces <= 128 ? 64 : 256;
   const int64_t groups = (rows + 256 / lanes - 1) / (256 / lanes);
-  return std::min<int64_t>(groups, pieces <= 128 ? 1024 : 512);
+  return std::min<int64_t>(groups, pieces <= 128 ? 1024 : 768);
 }
 
 int run_rms_norm_backward(const NormGradArgs& a, int dtype, hipStream_t st) {

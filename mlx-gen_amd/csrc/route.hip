@@ -28,26 +28,13 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
   return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-  return v;
-}
-__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = max(v, (unsigned long long)__shfl_xor((long long)v, d));
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+template <typename V>
+__device__ __forceinline__ V wave_max(V v) {
+  return lanes_reduce(v, [](V a, V b) { return a > b ? a : b; });  // of floats: a NaN is passed over, or stays
 }
 template <typename V>
 __device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return v;
+  return lanes_reduce(v, [](V a, V b) { return a + b; });
 }
 
 // WIDE: the choice is by s + bias, or a group's score is a sum: scores in 64 bits.
@@ -180,87 +167,78 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   }
 }
 
-// dz from dw.  p: the scores; up: what arrives at a chosen one's.
+// exp of x <= 0, correct to f32: the rounding of the product with log2 e is added back.
+__device__ __forceinline__ float exp_of(float x) {
+  const float t = x * 1.44269504088896341f, lost = fmaf(x, 1.44269504088896341f, -t) + x * 1.925963033500e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return e > 0.0f ? fmaf(e, lost * 0.693147180559945f, e) : e;  // -infinity: 0, and lost is no number
+}
+
+// dz from dw, with p the scores of a token and w = scale p / (their sum over the chosen, or 1):
+//   softmax: dz = p (up - sum up p),  sigmoid: dz = up p (1 - p),  up_j = scale (dw_j - sum dw w / scale) / sum,
+// up being 0 for experts that were not chosen.  Lane j < k works out its choice's up; scores and ups change lanes in LDS.
 template <typename T, int NE>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const float* __restrict__ dweights, T* __restrict__ dz) {
+  __shared__ float swap[4][NE * 64];
   const int lane = threadIdx.x & 63, E = a.E;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= a.T) return;
-  float p[NE], up[NE];
+  if (t >= a.T) return;  // whole waves; no barrier below
+  float* mine = swap[threadIdx.x >> 6];
+  float p[NE], q[NE];  // q: 1 - p of a sigmoid
   const T* row = (const T*)a.logits + t * a.row_stride;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    p[i] = i * 64 + lane < E ? Act<T>::ld(row, i * 64 + lane) : -INFINITY;
-    up[i] = 0.0f;
-  }
-  int id = -1;
-  float dw = 0.0f;
-  if (lane < a.k) {
-    id = a.ids[(int64_t)t * a.k + lane];
-    dw = dweights[(int64_t)t * a.k + lane] * a.scale;
-  }
+  for (int i = 0; i < NE; ++i) p[i] = Act<T>::ld(row, min(i * 64 + lane, E - 1));
+  const int64_t at = (int64_t)t * a.k + min(lane, a.k - 1);
+  int id = a.ids[at];
+  float up = dweights[at] * a.scale;
+  const bool chosen = lane < a.k && (unsigned)id < (unsigned)E;
   const bool soft = a.scoring == MLXQ_ROUTE_SOFTMAX;
-  float q[NE];  // sigmoid: 1 - p
   if (soft) {
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) top = fmaxf(top, p[i]);
-    top = wave_max(top);
+    for (int i = 0; i < NE; ++i) top = fmaxf(top, p[i]);  // the last logit again past the end
+    top = lanes_reduce(top, [](float u, float v) { return fmaxf(u, v); });
     if (top == -INFINITY) top = 0.0f;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      p[i] = expf(p[i] - top);
+      p[i] = i * 64 + lane < E ? exp_of(p[i] - top) : 0.0f;
       sum += p[i];
     }
     sum = wave_sum(sum);
-    const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < NE; ++i) p[i] *= inv;
   } else {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const float e = expf(-fabsf(p[i])), big = 1.0f / (1.0f + e), small = e * big;
+      const float e = exp_of(-fabsf(p[i])), big = 1.0f / (1.0f + e), small = e * big;
       q[i] = p[i] >= 0.0f ? small : big;
-      p[i] = p[i] >= 0.0f ? big : p[i] != p[i] ? p[i] : small;
+      p[i] = p[i] >= 0.0f ? big : small;
     }
   }
-  // The choices go to their experts' lanes; what they share is summed on the way.
-  float sum = 0.0f, dot = 0.0f;
-  bool chosen[NE];
 #pragma unroll
-  for (int i = 0; i < NE; ++i) chosen[i] = false;
-  for (int j = 0; j < a.k; ++j) {
-    const int e = __builtin_amdgcn_readlane(id, j);
-    if ((unsigned)e >= (unsigned)E) continue;
-    const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dw), j));
-#pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (i * 64 + lane == e) {
-        up[i] = g;
-        chosen[i] = true;
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < NE; ++i)
-    if (chosen[i]) {
-      sum += p[i];
-      dot += up[i] * p[i];
-    }
-  sum = wave_sum(sum);
-  dot = wave_sum(dot);
+  for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = p[i];
+  __builtin_amdgcn_wave_barrier();
+  const float pj = chosen ? mine[id] : 0.0f;
+  if (!chosen) up = 0.0f;
+  float dot = wave_sum(up * pj);
   if (a.normalize) {
-    // w = p / sum: what arrives at p is (dw - dot / sum) / sum, and its mean under p is 0
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    const float mean = dot * inv;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) up[i] = chosen[i] ? (up[i] - mean) * inv : 0.0f;
-    dot = 0.0f;
+    const float sum = wave_sum(pj), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    up = (up - dot * inv) * inv;
+    dot = 0.0f;  // the mean of these ups under p
   }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = 0.0f;
+  __builtin_amdgcn_wave_barrier();
+  if (chosen) mine[id] = up;
+  __builtin_amdgcn_wave_barrier();
   T* out = dz + (int64_t)t * E;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = i * 64 + lane;
-    if (e < E) Act<T>::st(out, e, soft ? p[i] * (up[i] - dot) : up[i] * p[i] * q[i]);
+    const float u = mine[e];
+    if (e < E) Act<T>::st(out, e, soft ? p[i] * (u - dot) : u * p[i] * q[i]);
   }
 }
 
@@ -276,16 +254,22 @@ __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
   return m;
 }
 
-// A segment of choices, by one wave, in steps of 64: f(choice, expert (E: none), lanes with the same one).
+// A run of choices, by one wave, 64 at a time and the loads of four times as many together: f(choice, whether there is
+// one, its expert (E: none), lanes with the same one).
 template <typename F>
 __device__ __forceinline__ void walk(const int32_t* ids, int first, int last, int E, int bits, F&& f) {
   const int lane = threadIdx.x & 63;
-  for (int c0 = first; c0 < last; c0 += 64) {
-    const int c = c0 + lane;
-    int e = c < last ? ids[c] : -1;
-    e = (unsigned)e < (unsigned)E ? e : E;
-    const unsigned long long in = __ballot(c < last);
-    f(c, c < last, e, same_expert(e, bits) & in);
+  for (int c0 = first; c0 < last; c0 += 256) {
+    int e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = ids[min(c0 + 64 * i + lane, last - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + 64 * i + lane;
+      if (c0 + 64 * i >= last) break;
+      const int x = (unsigned)e[i] < (unsigned)E ? e[i] : E;
+      f(c, c < last, x, same_expert(x, bits) & __ballot(c < last));
+    }
   }
 }
 
@@ -362,21 +346,30 @@ __global__ __launch_bounds__(1024) void route_small_plan_kernel(const int32_t* _
   });
 }
 
-// Segment blockIdx.x's choices to their places: the totals of all segments, then those of the earlier ones.
+// Segment blockIdx.x's choices to their places: the totals of all segments, then those of the earlier ones.  Each of the
+// four waves adds up every fourth segment.
 __global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
                                                           const int32_t* __restrict__ counts, int segments,
                                                           int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
-  __shared__ int sums[1025], next[1025];
-  const int tid = threadIdx.x, lane = tid & 63, mine = blockIdx.x;
-  for (int e = tid; e <= E; e += 256) {
+  __shared__ int sums[1025], next[1025], some[4][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, mine = blockIdx.x;
+  for (int e0 = 0; e0 <= E; e0 += 64) {
+    const int e = min(e0 + lane, E);
     int all = 0, before = 0;
-    for (int s = 0; s < segments; ++s) {
+#pragma unroll 8
+    for (int s = w; s < segments; s += 4) {
       const int c = counts[(int64_t)s * (E + 1) + e];
       all += c;
       before += s < mine ? c : 0;
     }
-    sums[e] = all;
-    next[e] = before;
+    some[w][0][lane] = all;
+    some[w][1][lane] = before;
+    __syncthreads();
+    if (w == 0 && e0 + lane <= E) {
+      sums[e] = some[0][0][lane] + some[1][0][lane] + some[2][0][lane] + some[3][0][lane];
+      next[e] = some[0][1][lane] + some[1][1][lane] + some[2][1][lane] + some[3][1][lane];
+    }
+    __syncthreads();
   }
   __syncthreads();
   if (tid >= 64) return;
@@ -409,7 +402,7 @@ __global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restr
 }
 
 constexpr int kOneGroup = 2048;  // choices that one workgroup sorts by itself
-int64_t segment_of(int64_t n) { return std::max<int64_t>(1024, ((n + 255) / 256 + 63) / 64 * 64); }
+int64_t segment_of(int64_t n) { return ((n + 255) / 256 + 255) / 256 * 256; }  // at most 256 segments
 
 template <typename F>
 int by_experts(int E, F&& f) {
