@@ -305,6 +305,80 @@ struct PagedAttention {
 void copy_pages(const Array& cache, int dim, const Array& src, const Array& dst, const Array* block_tables = nullptr,
                 hipStream_t s = nullptr);
 
+// ---- a decoder block in microscaled types (no counterpart in the reference) -------------------------------------
+// K values a row in blocks of 32: codes (uint8) [..., K / 2] for MLXQ_MX_E2M1, two to a byte, or [..., K] for MLXQ_MX_E4M3,
+// and scales (uint8) [..., 4 * ceil(K / 128)], of which the first K / 32 of a row count.
+struct Mx {
+  Array codes, scales;
+  int format = 0;  // mlxq_mx_format
+  int64_t K() const { return codes.dim(-1) * (format == 0 ? 2 : 1); }
+};
+Mx mx_quantize(const Array& x, int format, hipStream_t s = nullptr);
+Array mx_dequantize(const Mx& x, Dtype dt = Dtype::Bfloat16, hipStream_t s = nullptr);
+
+// x [..., K] . w^T + bias for e2m1 weights [N, K].  Workspaces as PagedAttention's: the object's own, one stream at a time.
+struct MxLinear {
+  Mx w;
+  std::optional<Array> bias;  // [N]
+  Dtype out = Dtype::Bfloat16;
+
+  Array forward(const Mx& x, hipStream_t s = nullptr) const;
+  void forward_into(const Mx& x, const Array& y, hipStream_t s = nullptr) const;
+
+  mutable Workspace workspace_;
+};
+
+// The norm of x (or of x + residual, the sum) over its last dimension, in x's dtype or as e4m3 (mx).
+struct Normed {
+  Array y, sum;
+  Mx mx;
+};
+Normed rms_norm(const Array& x, const Array* weight = nullptr, const Array* residual = nullptr, float eps = 1e-6f,
+                bool mx = false, hipStream_t s = nullptr);
+struct RmsNormGradient {
+  float eps = 1e-6f;
+  // (dx, dweight): x is what was normed, dsum the gradient that arrives at it from elsewhere; dweight is empty without a weight.
+  std::pair<Array, Array> backward(const Array& dy, const Array& x, const Array* weight = nullptr, const Array* dsum = nullptr,
+                                   hipStream_t s = nullptr) const;
+
+  mutable Workspace workspace_;
+};
+
+// Where tokens go (mlxq_routing): ids and weights [T, top_k], starts [experts + 1], rows [T * top_k].
+struct Routing {
+  Array ids, weights, starts, rows;
+};
+struct Router {
+  int64_t top_k = 1;
+  int scoring = 0;            // mlxq_route_scoring
+  std::optional<Array> bias;  // [experts] f32, for the choice only
+  int64_t groups = 1, kept_groups = 1, group_best = 1;
+  bool normalize = true;
+  float scale = 1.0f;
+
+  // active (Bool [T]): tokens that are 0 go nowhere.
+  Routing forward(const Array& logits, const Array* active = nullptr, hipStream_t s = nullptr) const;
+  // starts and rows for ids of one's own (weights [T, top_k] are passed on).
+  Routing plan(const Array& ids, const Array& weights, int64_t experts, hipStream_t s = nullptr) const;
+  // The gradient of the logits from that of the weights, for the choice ids.
+  Array backward(const Array& dweights, const Array& logits, const Array& ids, hipStream_t s = nullptr) const;
+
+  mutable Workspace workspace_;
+};
+
+// The products of the experts that tokens were routed to: w [experts, N, K] e2m1, bias [experts, N].
+struct MxExperts {
+  Mx w;
+  std::optional<Array> bias;
+  Dtype out = Dtype::Bfloat16;
+
+  // x [T, K], or [T, top_k, K] with a row for each choice -> [T, top_k, N], or with combine [T, N], summed with the weights.
+  Array forward(const Mx& x, const Routing& r, bool combine = false, hipStream_t s = nullptr) const;
+  void forward_into(const Mx& x, const Routing& r, bool combine, const Array& y, hipStream_t s = nullptr) const;
+
+  mutable Workspace workspace_;
+};
+
 // ---- quant.rs --------------------------------------------------------------------------------
 using Weights = std::map<std::string, Array>;
 const Array& require(const Weights& w, const std::string& key);  // throws on a missing key
