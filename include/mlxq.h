@@ -497,14 +497,13 @@ int mlxq_mx_dequantize(const mlxq_mx* x, int64_t rows, int64_t K, void* out, int
 
 /*
  * y [M, N] = x . w^T + bias: x [M, K] in either format, w [N, K] e2m1, bias [N] in bias_dtype or NULL; y
- * in y_dtype (f32, bf16, fp16).  Products of codes and scales are exact, sums f32, one rounding at the
- * end.  workspace: mlxq_mx_matmul_workspace_size() bytes, 16-byte aligned, whatever they hold (NULL when
- * that is 0).  Sums are taken in an order that follows M, N, K and the format only.
+ * in y_dtype (f32, bf16, fp16).  Products of codes and scales are exact, sums f32 in an order that follows
+ * M, N, K, the format and y_dtype only, one rounding at the end.  e4m3 with a 16-bit y: the matrix cores add
+ * 128 products at a time and lose up to 2^-11 of the largest of them, in all about 2e-5 of a result.  f32
+ * y of e4m3: values of x or w past f32's range are infinite.
  */
-size_t mlxq_mx_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int x_format);
 int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int64_t N, const void* bias,
-                   int bias_dtype, void* y, int y_dtype, void* workspace, size_t workspace_bytes,
-                   void* stream);
+                   int bias_dtype, void* y, int y_dtype, void* stream);
 
 /*
  * Root-mean-square norm over the last dimension of [T, heads, D]:
@@ -593,10 +592,10 @@ int mlxq_route_experts_backward(const float* dweights, const void* logits, int d
  * [tokens, K], or with x_per_choice [tokens, top_k, K].  y is [tokens, top_k, N] in y_dtype, zero for choices
  * without an expert; with combine it is [tokens, N], sum_j weights[t, j] y[t, j]: each product is rounded to
  * y_dtype, as separate products would be, and the sum is f32.  starts and rows must be ids' plan; entries
- * outside their ranges are skipped.  workspace as above.
+ * outside their ranges are skipped.  workspace: mlxq_mx_experts_workspace_size() bytes, 16-byte aligned, whatever
+ * they hold (NULL when that is 0: without combine).
  */
-size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t experts, int64_t K, int64_t N,
-                                      int x_format, int combine, int y_dtype);
+size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t N, int combine, int y_dtype);
 int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx* w, int64_t N,
                     const void* bias, int bias_dtype, const mlxq_routing* routing, int combine, void* y,
                     int y_dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -133,21 +133,17 @@ int run_route_backward(const RouteArgs& a, int dtype, const float* dweights, voi
 // A product of microscaled operands, dense or of routed experts.
 struct MxProduct {
   MxView x, w;
-  int64_t x_rows;        // rows of x
   int64_t M, N, K;       // M: rows of y (dense) or choices
   const void* bias;      // [E, N] or null
   int bias_dtype;
   void* y;               // [M, N]
   int y_dtype;
-  float* part;           // f32 partial sums of the splits of K, or null
-  int splits;
   // routed: E experts' runs of `rows`; E = 0: dense
   int E;
   const int32_t *starts, *rows;
   bool skip_none;        // rows of choices without an expert are not written
   Divisor by_choices;    // x row of a choice: choice / by_choices (1: a row for each choice)
 };
-int64_t mx_product_splits(int64_t M, int64_t K, int64_t N, int format, int64_t E);
 int run_mx_product(const MxProduct& p, int format, hipStream_t st);
 int run_mx_combine(const void* y, int dtype, const int32_t* ids, const float* weights, int64_t T, int64_t k, int64_t E,
                    int64_t N, void* out, hipStream_t st);

@@ -153,14 +153,8 @@ int mlxq_mx_dequantize(const mlxq_mx* x, int64_t rows, int64_t K, void* out, int
   return run_mx_dequantize(view(x), x->format, rows, K, out, out_dtype, (hipStream_t)stream);
 }
 
-size_t mlxq_mx_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int x_format) {
-  if (M < 1 || N < 1 || K < 32 || M > kMostRows || N > kMostRows) return 0;
-  const int64_t s = mx_product_splits(M, K, N, x_format, 0);
-  return s > 1 ? (size_t)s * M * N * 4 : 0;
-}
-
 int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int64_t N, const void* bias, int bias_dtype, void* y,
-                   int y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                   int y_dtype, void* stream) {
   const char* op = "mx_matmul";
   int rc;
   if ((rc = check_size(op, "M", M, kMostRows)) || (rc = check_size(op, "N", N, kMostRows)) || (rc = check_k(op, K)) ||
@@ -170,20 +164,16 @@ int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int
   if (bias && ((rc = check_dtype(op, "bias_dtype", bias_dtype)) || (rc = check_ptr(op, "bias", bias, bytes_of(bias_dtype))))) return rc;
   if (M == 0 || N == 0) return MLXQ_OK;
   if ((rc = check_ptr(op, "y", y, bytes_of(y_dtype)))) return rc;
-  const size_t need = mlxq_mx_matmul_workspace_size(M, K, N, x->format);
-  if ((rc = check_workspace(op, workspace, workspace_bytes, need))) return rc;
   MxProduct p = {};
   p.x = view(x);
   p.w = view(w);
-  p.x_rows = p.M = M;
+  p.M = M;
   p.N = N;
   p.K = K;
   p.bias = bias;
   p.bias_dtype = bias_dtype;
   p.y = y;
   p.y_dtype = y_dtype;
-  p.splits = need ? (int)mx_product_splits(M, K, N, x->format, 0) : 1;
-  p.part = need ? (float*)workspace : nullptr;
   return run_mx_product(p, x->format, (hipStream_t)stream);
 }
 
@@ -334,11 +324,7 @@ int mlxq_route_experts_backward(const float* dweights, const void* logits, int d
 }
 
 // Workspace of mlxq_mx_experts: the products before they are summed.
-size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t experts, int64_t K, int64_t N, int x_format, int combine,
-                                      int y_dtype) {
-  (void)experts;
-  (void)K;
-  (void)x_format;
+size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t N, int combine, int y_dtype) {
   if (!combine || tokens < 1 || top_k < 1 || N < 1 || tokens > kMostRows / top_k || N > kMostRows) return 0;
   return (size_t)(tokens * top_k) * (size_t)N * bytes_of(y_dtype);
 }
@@ -358,12 +344,11 @@ int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx
   if (T == 0 || N == 0) return MLXQ_OK;
   if ((rc = check_ptr(op, "y", y, bytes_of(y_dtype)))) return rc;
   if (combine && (rc = check_ptr(op, "weights", routing->weights, 4))) return rc;
-  const size_t need = mlxq_mx_experts_workspace_size(T, k, E, K, N, x->format, combine, y_dtype);
+  const size_t need = mlxq_mx_experts_workspace_size(T, k, N, combine, y_dtype);
   if ((rc = check_workspace(op, workspace, workspace_bytes, need))) return rc;
   MxProduct p = {};
   p.x = view(x);
   p.w = view(w);
-  p.x_rows = x_per_choice ? T * k : T;
   p.M = T * k;
   p.N = N;
   p.K = K;
@@ -371,7 +356,6 @@ int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx
   p.bias_dtype = bias_dtype;
   p.y = combine ? workspace : y;
   p.y_dtype = y_dtype;
-  p.splits = 1;
   p.E = (int)E;
   p.starts = routing->starts;
   p.rows = routing->rows;

@@ -15,6 +15,8 @@
 // scan over the runs' lengths; the last run, of choices without an expert, is written as zeros.
 #pragma once
 
+#include <math.h>
+
 #include "mx.h"
 
 namespace mlxq {
@@ -174,8 +176,6 @@ __device__ __forceinline__ f32x4 mx_mma(const MxFrag<kE2M1, EXACT>& w, const MxF
   }
 }
 
-// ---- many rows -----------------------------------------------------------------------------------
-
 // 16 or 4 bytes a lane from memory to LDS, lane i's to lds + 16 i (4 i).  As inline asm without a result, so that the
 // compiler adds no wait of its own before later LDS reads; callers wait for vmcnt themselves.  M0 holds the LDS address
 // and is restored.
@@ -194,17 +194,24 @@ __device__ __forceinline__ void mx_dma4(const unsigned char* from, uint32_t lds)
 // A workgroup of WM x WN waves takes TM rows by TN features; steps of 128 values of K go through a ring of STAGES
 // buffers in LDS by DMA, one barrier a step.  The scales of four steps go together, 16 bytes of 16 rows a load: a row's
 // scales of one step are 4 bytes of a cache line of their own, and fetched step by step they were half of all requests.
-template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int n_tiles) {
+//
+// KG groups of WM x WN waves share a tile, a run of K with buffers of its own each, and join their sums in LDS: a few rows
+// make few tiles, whose steps are a chain of latencies.
+template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG) void mx_tile_kernel(MxProduct p, int n_tiles) {
   constexpr int NW = WM * WN, XB = XF == kE4M3 ? 128 : 64, XN = XF == kE4M3 ? 2 : 1;
   constexpr int FM = TM / WM / 16, FN = TN / WN / 16;
-  constexpr int XI = TM * XB / 1024 / NW, WI = TN * 64 / 1024 / NW, PER = XI + WI;  // DMA loads of a wave a step
+  // DMA loads of 1 KB a step, and those of a wave: every wave makes as many, some of them twice where there are fewer than waves.
+  constexpr int XL = TM * XB / 1024, WL = TN * 64 / 1024, XI = XL > NW ? XL / NW : 1, WI = WL > NW ? WL / NW : 1, PER = XI + WI;
   constexpr int W0 = TM * XB, STAGE = W0 + TN * 64;
   // A group of scales: loads of 16 rows each, in up to four parts of a load a wave.
   constexpr int SP = (TM + TN) / 16, GROUP = (TM + TN) * 16, GROUPS = STAGES == 3 ? 2 : 3, S0 = STAGE * STAGES;
-  static_assert(XI >= 1 && WI >= 1 && S0 + GROUP * GROUPS <= 163840 && SP <= 4 * NW, "a step is whole loads of each wave");
-  __shared__ __align__(1024) unsigned char lds[S0 + GROUP * GROUPS];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int RING = S0 + GROUP * GROUPS;
+  static_assert(XL >= 1 && WL >= 1 && (XL % NW == 0 || NW % XL == 0) && (WL % NW == 0 || NW % WL == 0) && RING * KG <= 163840 && (KG == 1 || TM * TN * 4 <= RING) && SP <= 4 * NW, "a step is whole loads of each wave");
+  __shared__ __align__(1024) unsigned char all_lds[RING * KG];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = KG > 1 ? wave / NW : 0, w = KG > 1 ? wave % NW : wave;
+  unsigned char* lds = all_lds + kg * RING;
   const int c = lane & 15, g = lane >> 4;
 
   // Neighbouring workgroups go to different dies: each die takes a run of tiles of its own, in bands of 4 tiles of
@@ -221,6 +228,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
   if (!tile.found || (p.skip_none && tile.e == p.E)) return;
   const int n0 = nt * TN, N = (int)p.N, K = (int)p.K;
   const int steps = (K + 127) / 128;
+  // This group's steps, k0 of all its first, a multiple of 4; the first group has the most.
+  const int most = KG > 1 ? min(steps, ((steps + KG - 1) / KG + 3) & ~3) : steps;
+  const int k0 = kg * most, cnt = max(0, min(steps - k0, most));
   // Waves of one SIMD (w and w + 4) hold different rows: where a run's last tile has half its rows or fewer, a wave of
   // each SIMD has none and leaves the matrix cores to the other.
   const int wm = w / WN, wn = w % WN;
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
     auto x_row = [&](int r) { return tiles.x_row(tiles.row(tile.first + min(r, tile.count - 1))); };
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-      const int j = w * XI + i, r = XF == kE4M3 ? 8 * j + (lane >> 3) : 16 * j + (lane >> 2);
+      const int j = (w * XI + i) % XL, r = XF == kE4M3 ? 8 * j + (lane >> 3) : 16 * j + (lane >> 2);
       const int piece = XF == kE4M3 ? (lane & 7) ^ (r & 7) : (lane & 3) ^ (r >> 1 & 3);
       xk[i] = piece * (XF == kE4M3 ? 16 : 32);
       xp[i] = p.x.codes + x_row(r) * x_pitch + piece * 16;
@@ -247,7 +257,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
     const int64_t w_row0 = (int64_t)tile.e * N;
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
-      const int r = 16 * (w * WI + i) + (lane >> 2), piece = (lane & 3) ^ (r >> 1 & 3);
+      const int r = 16 * ((w * WI + i) % WL) + (lane >> 2), piece = (lane & 3) ^ (r >> 1 & 3);
       wk = piece * 32;
       wp[i] = p.w.codes + (w_row0 + min(n0 + r, N - 1)) * w_pitch + piece * 16;
     }
@@ -263,11 +273,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
     const int last_dword = (K / 32 - 1) & ~3;  // of a row's scales
 
     auto load_scales = [&](int group, int part) {
-      if (group * 4 >= steps || part * NW + w >= SP) return;
-      mx_dma4(sp[part] + min(group * 16 + 4 * (lane & 3), last_dword), base + S0 + (uint32_t)(group % GROUPS) * GROUP + (part * NW + w) * 256);
+      if (group * 4 >= cnt || part * NW + w >= SP) return;
+      mx_dma4(sp[part] + min(k0 * 4 + group * 16 + 4 * (lane & 3), last_dword), base + S0 + (uint32_t)(group % GROUPS) * GROUP + (part * NW + w) * 256);
     };
-    auto load = [&](int s) {
-      // The parts of a group are spread over the steps before it so that two groups are held at a time (STAGES 3).  They
+    auto load = [&](int s) {  // the group's step s
+      // The parts of a group of scales are spread over the steps before it so that two are held at a time (STAGES 3).  They
       // come before the step's codes: a wait for these is one for all scales before them.
       if (s == 0) {
 #pragma unroll
@@ -281,16 +291,16 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
         load_scales(s >> 2, 3);
       }
       const uint32_t to = base + (uint32_t)(s % STAGES) * STAGE;
-      const int left = ragged && s == steps - 1 ? K - s * 128 : 128;
+      const int left = ragged && k0 + s == steps - 1 ? K - (k0 + s) * 128 : 128;
 #pragma unroll
       for (int i = 0; i < XI; ++i)
-        mx_dma16(xk[i] < left ? xp[i] + (int64_t)s * XB : zeros, to + (w * XI + i) * 1024);
+        mx_dma16(xk[i] < left ? xp[i] + (int64_t)(k0 + s) * XB : zeros, to + (w * XI + i) % XL * 1024);
 #pragma unroll
-      for (int i = 0; i < WI; ++i) mx_dma16(wk < left ? wp[i] + (int64_t)s * 64 : zeros, to + W0 + (w * WI + i) * 1024);
+      for (int i = 0; i < WI; ++i) mx_dma16(wk < left ? wp[i] + (int64_t)(k0 + s) * 64 : zeros, to + W0 + (w * WI + i) % WL * 1024);
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
-      if (i < steps) load(i);
+      if (i < cnt) load(i);
 
     const int xr = wm * (TM / WM) + c, wr = wn * (TN / WN) + c;  // this lane's rows of the first fragments
     // Of an e4m3 row a lane reads pieces g and g + 4 (EXACT: 2 g and 2 g + 1); piece i of row r lies at i ^ (r % 8).
@@ -304,13 +314,16 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
     // until the last had everything.
     constexpr int Q = FN / FM;
     static_assert(FN % FM == 0, "squares of fragments");
-    auto step = [&](int s, bool wait_all, bool ahead, auto LAST) {
-      if (wait_all) mlxq_vmcnt<0>();
-      else mlxq_vmcnt<(STAGES - 2) * PER>();
+    auto meet = [&](int s) {  // the group's step s is there for all of its waves
+      if (s + STAGES - 2 < cnt) mlxq_vmcnt<(STAGES - 2) * PER>();
+      else mlxq_vmcnt<0>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
+    };
+    auto step = [&](int s, bool ahead, auto LAST) {
+      meet(s);
       const unsigned char *b = lds + (s % STAGES) * STAGE, *sb = lds + S0 + ((s >> 2) % GROUPS) * GROUP + (s & 3) * 4;
-      const bool past = decltype(LAST)::value && g * 32 >= K - s * 128;  // this lane's block is past K
+      const bool past = decltype(LAST)::value && g * 32 >= K - (k0 + s) * 128;  // this lane's block is past K
       MxFrag<XF, EXACT> x[FM];
       MxFrag<kE2M1, EXACT> a[FN];
       auto read = [&](int j) {
@@ -343,18 +356,36 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
       }
     };
     if (idle) {
-      for (int s = 0; s < steps; ++s) {
-        if (s + STAGES - 2 >= steps || s + 1 == steps) mlxq_vmcnt<0>();
-        else mlxq_vmcnt<(STAGES - 2) * PER>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + STAGES - 1 < steps) load(s + STAGES - 1);
+      for (int s = 0; s < most; ++s) {
+        meet(s);
+        if (s + STAGES - 1 < cnt) load(s + STAGES - 1);
       }
-      return;
+      if constexpr (KG == 1) return;
+    } else {
+      for (int s = 0; s + 1 < cnt; ++s) step(s, s + STAGES - 1 < cnt, std::false_type{});
+      if (cnt > 0) step(cnt - 1, false, std::true_type{});
+      for (int s = cnt; s < most; ++s) meet(s);
     }
-    for (int s = 0; s + 1 < steps; ++s)
-      step(s, s + STAGES - 2 >= steps, s + STAGES - 1 < steps, std::false_type{});
-    step(steps - 1, true, false, std::true_type{});
+    if constexpr (KG > 1) {
+      __syncthreads();
+      f32x4* sums = reinterpret_cast<f32x4*>(lds);
+      if (kg > 0 && !idle)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j) sums[(i * FM + j) * 64 * NW + w * 64 + lane] = acc[i][j];
+      __syncthreads();
+      if (kg > 0) return;
+#pragma unroll
+      for (int k = 1; k < KG; ++k)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            acc[i][j] += reinterpret_cast<const f32x4*>(all_lds + k * RING)[(i * FM + j) * 64 * NW + w * 64 + lane];
+    }
+  } else if (KG > 1 && kg > 0) {
+    return;
   }
   if (idle) return;
   f32x4 bias[FN];
@@ -369,97 +400,6 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProduct p, int 
   }
 }
 
-// ---- few rows ------------------------------------------------------------------------------------
-
-// 16 FM rows by 16 features a wave, weights and x straight from memory to the operands, four steps of K ahead in
-// registers.  KS waves of a workgroup share a tile, a run of K each, and join their sums in LDS.  Bound by the reading of the
-// weights; their loads go out before the rows of x are looked up in the plan.
-template <int XF, bool EXACT, int FM, int KS>
-__global__ __launch_bounds__(KS > 4 ? 64 * KS : 256) void mx_stream_kernel(MxProduct p, int n_tiles) {
-  constexpr int XN = XF == kE4M3 ? 2 : 1, AHEAD = FM > 1 ? 2 : 4, NW = KS > 4 ? KS : 4, NT = NW / KS;
-  __shared__ f32x4 part[KS > 1 ? NW : 1][FM][64];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  MxTiles tiles{p, 16 * FM};
-  const int mt = blockIdx.x / n_tiles, n0 = ((blockIdx.x - mt * n_tiles) * NT + w / KS) * 16;
-  const MxTile tile = tiles.find(mt);
-  if (!tile.found || (p.skip_none && tile.e == p.E)) return;
-  const int N = (int)p.N, K = (int)p.K, steps = (K + 127) / 128;
-  f32x4 acc[FM];
-#pragma unroll
-  for (int j = 0; j < FM; ++j) acc[j] = f32x4{0, 0, 0, 0};
-  if (tile.e < max(p.E, 1) && n0 < N) {
-    const int64_t wrow = (int64_t)tile.e * N + min(n0 + c, N - 1);
-    const unsigned char *wp = p.w.codes + wrow * (K / 2) + g * 16, *ws = p.w.scales + wrow * p.w.scale_stride;
-    const unsigned char *xp[FM], *xs[FM];
-    const int per = (steps + KS - 1) / KS, s0 = min(steps, w % KS * per), s1 = min(steps, s0 + per);
-    // Loads past a wave's run or the end of K are of zeros: a load that is made or not is a branch and a wait.
-    const unsigned char* zeros = reinterpret_cast<const unsigned char*>(&mx_zeros);
-    constexpr int SECOND = EXACT ? 16 : 64, XB = XF == kE4M3 ? 128 : 64;
-    for (int s = s0; s < s1; s += AHEAD) {
-      u32x4 a[AHEAD], x[AHEAD][FM][XN];
-      uint32_t as[AHEAD], bs[AHEAD][FM];
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const bool in = s + k < s1 && 128 * (s + k) + 32 * g < K;
-        a[k] = *reinterpret_cast<const u32x4*>(in ? wp + (int64_t)(s + k) * 64 : zeros);
-        as[k] = *reinterpret_cast<const uint32_t*>(in ? ws + 4 * (s + k) : zeros);
-      }
-      if (s == s0) {
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          const int64_t row = tiles.x_row(tiles.row(tile.first + min(j * 16 + c, tile.count - 1)));
-          xp[j] = p.x.codes + row * (XF == kE4M3 ? K : K / 2) + g * (EXACT && XF == kE4M3 ? 32 : 16);
-          xs[j] = p.x.scales + row * p.x.scale_stride;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const bool run = s + k < s1, in = run && 128 * (s + k) + 32 * g < K;
-        const int first = 128 * (s + k) + (XF == kE4M3 && !EXACT ? 16 : 32) * g;
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-#pragma unroll
-          for (int i = 0; i < XN; ++i)
-            x[k][j][i] = *reinterpret_cast<const u32x4*>(run && first + i * SECOND < K ? xp[j] + (int64_t)(s + k) * XB + i * SECOND : zeros);
-          bs[k][j] = *reinterpret_cast<const uint32_t*>(in ? xs[j] + 4 * (s + k) : zeros);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        MxFrag<kE2M1, EXACT> fa;
-        const u32x4 v[1] = {a[k]};
-        fa.set(v, as[k] >> 8 * g & 255);
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          MxFrag<XF, EXACT> fx;
-          fx.set(x[k][j], bs[k][j] >> 8 * g & 255);
-          acc[j] = mx_mma<XF, EXACT>(fa, fx, acc[j]);
-        }
-      }
-    }
-  }
-  if constexpr (KS > 1) {
-#pragma unroll
-    for (int j = 0; j < FM; ++j) part[w][j][lane] = acc[j];
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    if (KS > 1 && j % KS != w % KS) continue;
-    f32x4 v = acc[j];
-    if constexpr (KS > 1) {
-      v = part[w / KS * KS][j][lane];
-#pragma unroll
-      for (int k = 1; k < KS; ++k) v += part[w / KS * KS + k][j][lane];
-    }
-    const int r = j * 16 + c;
-    if (r >= tile.count || n0 >= N) continue;
-    const int row = tiles.row(tile.first + r);
-    if (row >= 0) mx_store(p, row, n0 + 4 * g, v + mx_bias(p, tile.e, n0 + 4 * g));
-  }
-}
-
 namespace {
 
 // Tiles of TM rows that a launch is made for: as many as there can be, by sizes alone.
@@ -468,43 +408,52 @@ inline int64_t mx_most_tiles(const MxProduct& p, int64_t TM) {
   return p.M / TM + (p.M < p.E + 1 ? p.M : p.E + 1);
 }
 
-template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES>
+template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES, int KG>
 int mx_launch_tile(const MxProduct& p, hipStream_t st) {
   const int64_t n_tiles = (p.N + TN - 1) / TN, grid = (mx_most_tiles(p, TM) * n_tiles + 7) / 8 * 8;
   if (grid > 0x7fffffff) return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles", (long long)grid);
-  mx_tile_kernel<XF, EXACT, TM, TN, WM, WN, STAGES><<<(unsigned)grid, 64 * WM * WN, 0, st>>>(p, (int)n_tiles);
+  mx_tile_kernel<XF, EXACT, TM, TN, WM, WN, STAGES, KG><<<(unsigned)grid, 64 * WM * WN * KG, 0, st>>>(p, (int)n_tiles);
   return check_launch("mx product");
 }
 
-template <int XF, bool EXACT, int FM, int KS>
-int mx_launch_stream(const MxProduct& p, hipStream_t st) {
-  constexpr int NW = KS > 4 ? KS : 4, NT = NW / KS;
-  const int64_t n_tiles = (p.N + 16 * NT - 1) / (16 * NT), grid = mx_most_tiles(p, 16 * FM) * n_tiles;
-  if (grid > 0x7fffffff) return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles", (long long)grid);
-  mx_stream_kernel<XF, EXACT, FM, KS><<<(unsigned)grid, 64 * NW, 0, st>>>(p, (int)n_tiles);
-  return check_launch("mx product");
+// About as many tiles as there will be: every expert's rows, as many as the mean, end in a part of one.
+inline double mx_tiles(const MxProduct& p, int64_t TM, int64_t TN) {
+  const double n = (double)((p.N + TN - 1) / TN);
+  if (p.E == 0) return n * (double)((p.M + TM - 1) / TM);
+  const double m = p.E * ((double)p.M / p.E / TM + 0.5), most = (double)mx_most_tiles(p, TM);
+  return n * (m < most ? m : most);
 }
 
-// Waves that share a tile: as many as give the chip's SIMDs four waves each.
-template <int XF, bool EXACT, int FM>
-int mx_stream(const MxProduct& p, hipStream_t st) {
-  const int64_t tiles = mx_most_tiles(p, 16 * FM) * ((p.N + 15) / 16);
-  if (tiles >= 3072) return mx_launch_stream<XF, EXACT, FM, 1>(p, st);
-  if (tiles >= 1536) return mx_launch_stream<XF, EXACT, FM, 2>(p, st);
-  if (tiles >= 768) return mx_launch_stream<XF, EXACT, FM, 4>(p, st);
-  return mx_launch_stream<XF, EXACT, FM, 8>(p, st);
-}
-
+// The instance for a product, by its rows (of an expert, the mean) and by how many workgroups there are for 256 CUs.  Few: small
+// tiles, K split over groups of waves; many: tiles that read less for each product.  Measured in us with e4m3:
+//   1 row, K 14336, 4096 features      16 x 16, 16 groups 8.6; 8 groups 9.4; 16 x 32, 8 groups 10.9; 32 x 32, 8 groups 14.3
+//   1 row, K 4096, 14336 features      16 x 32, 4 groups 7.4; 16 x 64, 4 groups 7.9; 32 x 64, 4 groups 8.2; 16 x 32, 8 groups 9.3
+//   3 tokens, 4 of 32 experts of 5760 x 2880       32 x 128 17.5; 64 x 128 18.1; 32 x 64 18.3; 16 x 32, 4 groups 27
+//   32 rows, K 4096, 14336 features    32 x 64, 4 groups 9.1; 2 groups 9.8; 64 x 64, 2 groups 10.8
+//   250 tokens, the same experts       64 x 128 91; 32 x 128 100; 32 x 64 105; 64 x 64 112
+//   48 / 256 rows, K 4096, 4096 features           64 x 64, 2 groups 11.6 / 12.1; 1 group 14.7 / 15.1; 64 x 128 18.4 / 18.6
+//   512 rows, K 4096, 4096 features    64 x 128, 2 groups 17.8; 1 group 19.7; 64 x 64 19.9; 128 x 128 28
+//   256 rows, K 4096, 14336 features   64 x 128 27.9; 128 x 128 28.8; 64 x 128, 2 groups 32.8
+//   2048 rows, K 4096, 4096 / 14336 features       128 x 128 40 / 128; 256 x 256 57 / 116
+//   4090 tokens, 4 of 32 experts of 2880 x 2880    256 x 256 193; 128 x 128 210
 template <int XF, bool EXACT>
 int mx_product(const MxProduct& p, hipStream_t st) {
-  const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;  // of an expert, about
-  if (rows <= 16) return mx_stream<XF, EXACT, 1>(p, st);
-  if (rows <= 32) return mx_stream<XF, EXACT, 2>(p, st);
-  if (rows <= 64) return mx_stream<XF, EXACT, 4>(p, st);
-  const int64_t big = mx_most_tiles(p, 256) * ((p.N + 255) / 256), mid = mx_most_tiles(p, 128) * ((p.N + 127) / 128);
-  if (big >= 512) return mx_launch_tile<XF, EXACT, 256, 256, 4, 2, 3>(p, st);
-  if (mid >= 256) return mx_launch_tile<XF, EXACT, 128, 128, 2, 2, 3>(p, st);
-  return mx_launch_tile<XF, EXACT, 64, 64, 2, 2, 4>(p, st);
+  const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;
+  if (rows <= 16) {
+    const double t = mx_tiles(p, 16, 16);
+    if (t <= 256) return mx_launch_tile<XF, EXACT, 16, 16, 1, 1, 3, 16>(p, st);
+    if (t <= 512) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 8>(p, st);
+    if (t <= 1024) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 4>(p, st);
+    return mx_launch_tile<XF, EXACT, 32, 128, 2, 4, 4, 1>(p, st);
+  }
+  if (rows <= 32 && mx_tiles(p, 32, 64) <= 256) return mx_launch_tile<XF, EXACT, 32, 64, 2, 2, 4, 4>(p, st);
+  if (mx_tiles(p, 64, 64) <= 256) return mx_launch_tile<XF, EXACT, 64, 64, 2, 2, 4, 2>(p, st);
+  if (mx_tiles(p, 64, 128) <= 256) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 2>(p, st);
+  const double mid = mx_tiles(p, 128, 128);
+  if (mid <= 256 || rows <= 64) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 1>(p, st);
+  // One round of the largest tiles takes as long as three quarters of the mid ones' of 1024 (two rounds of two to a CU).
+  if (mid >= 768 * ceil(mx_tiles(p, 256, 256) / 256)) return mx_launch_tile<XF, EXACT, 256, 256, 4, 2, 3, 1>(p, st);
+  return mx_launch_tile<XF, EXACT, 128, 128, 2, 2, 3, 1>(p, st);
 }
 
 }  // namespace

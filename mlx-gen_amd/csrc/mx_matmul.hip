@@ -12,9 +12,6 @@ int run_mx_product(const MxProduct& p, int format, hipStream_t st) {
   return p.y_dtype == MLXQ_FLOAT32 ? run_mx_product_e4m3_f32(p, st) : run_mx_product_e4m3(p, st);
 }
 
-// Splits of K: one, whatever the sizes.
-int64_t mx_product_splits(int64_t, int64_t, int64_t, int, int64_t) { return 1; }
-
 namespace {
 
 // out[t, n] = sum_j w[t, j] y[t, j, n] over the choices with an expert, f32, rounded once.  Bound by the reading of y.  A

@@ -4,13 +4,15 @@
 //   dx = r g - r^3 x mean(g x) + dsum,  g = dy w;   dw = sum of dy x r over the rows
 //
 // A row is held in registers by 8 to 64 lanes of a wave (short rows: several to a wave), by a workgroup of 256 or by
-// one of 1024, in 16-byte pieces, and is read once; the sums take exchanges within a wave and one step through LDS
+// one of 512, in 16-byte pieces, and is read once; the sums take exchanges within a wave and one step through LDS
 // between waves.  Both directions are bound by HBM.  Pieces are loaded at the element's alignment, so that rows of odd
 // length or stride take the same path; only a row's last, partial piece goes element by element.
 //
-// The gradient of the weight is a sum over all rows: each workgroup walks many rows, the next one's loads in
-// flight while it reduces this one's, and holds its features' sums in registers; they go to the workspace once
-// and a second launch adds them up in a fixed order.
+// The gradient of the weight is a sum over all rows: each workgroup walks many rows and holds its features' sums in
+// registers; they go to the workspace once and a second launch adds them up in a fixed order.  Two workgroups of 256 a CU
+// hide each other's reductions, and a row's loads go out once the sums of the row before are there: 8190 x 5120 bf16
+// with dsum 71 us with the second launch, 4.7 TB/s, a large copy's rate (loads at the row's own start 75, a whole row
+// ahead in registers 71, three workgroups a CU 85).
 #include <algorithm>
 
 #include "mx.h"
@@ -107,7 +109,7 @@ __device__ __forceinline__ void row_sum(V (&v)[N], V* slot) {
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) slot[w * N + i] = v[i];
-    // Of LDS alone: a barrier for all memory would wait for the next row's loads.
+    // Of LDS alone: a barrier for all memory would wait for the last row's stores too.
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
@@ -244,8 +246,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
   __shared__ float slot[2][2 * TW];
   const int lane = threadIdx.x % LANES, D = a.D;
   const bool has_w = a.w_dtype >= 0;
-  // A workgroup of 1024 has 128 registers a lane: weights and dsum are then loaded where they are used, and no row ahead.
-  constexpr bool LEAN = LANES > 256;
+  // The longest rows leave no registers: their weights and dsum are loaded where they are used.
+  constexpr bool LEAN = LANES > 256 && CH > 4;
   float w[LEAN ? 1 : CH][C], dw[CH][C];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
@@ -283,6 +285,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
         s[1] = fmaf(Elem<T>::get(dy[i], e) * w[LEAN ? 0 : i][e], xv, s[1]);
       }
     }
+    row_sum<LANES>(s, slot[turn]);
+    // The next row's loads go out beside this one's results.
     u32x4 x0[CH], dy0[CH], ds0[LEAN ? 1 : CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -290,8 +294,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
       dy0[i] = dy[i];
       if constexpr (!LEAN) ds0[i] = ds[i];
     }
-    if (!LEAN && first + step < a.rows) load(at + step);
-    row_sum<LANES>(s, slot[turn]);
+    if (first + step < a.rows) load(at + step);
     const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
     if (!live) continue;
     const int row = (int)at, t = a.by_heads.div(row), h = row - t * a.heads;
@@ -322,7 +325,6 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
       }
       store_piece(dx, e0, D, pack_chunk<T>(f));
     }
-    if (LEAN && first + step < a.rows) load(at + step);
   }
   if (!has_w) return;
   // The workgroup's rows are added up, then its sums are one row of the workspace.
@@ -382,9 +384,9 @@ int by_pieces(int64_t pieces, F&& f) {
   MLXQ_ROW(256, 256, 1);
   MLXQ_ROW(512, 256, 2);
   MLXQ_ROW(1024, 256, 4);
-  MLXQ_ROW(2048, 256, 8);
-  MLXQ_ROW(4096, 1024, 4);
-  return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
+  MLXQ_ROW(2048, 512, 4);
+  MLXQ_ROW(4096, 512, 8);
+  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{});
 #undef MLXQ_ROW
 }
 
@@ -419,13 +421,13 @@ int run_rms_norm(const NormArgs& a, int dtype, hipStream_t st) {
   return norm<float>(a, st);
 }
 
-// Workgroups of the gradient: three to a CU of the MI355X's 256 (four of short rows), fewer where there are no rows for
-// them.  By sizes alone, so that sums are the same everywhere.
+// Workgroups of the gradient: four to a CU of the MI355X's 256 where a row is a wave's or less, two where it is 256 lanes', one
+// above; fewer where there are no rows for them.  By sizes alone, so that sums are the same everywhere.
 int64_t norm_grad_parts(int64_t rows, int64_t D, int dtype) {
   const int64_t C = dtype == MLXQ_FLOAT32 ? 4 : 8, pieces = (D + C - 1) / C;
   const int64_t lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : pieces <= 128 ? 64 : 256;
   const int64_t groups = (rows + 256 / lanes - 1) / (256 / lanes);
-  return std::min<int64_t>(groups, pieces <= 128 ? 1024 : 768);
+  return std::min<int64_t>(groups, pieces <= 128 ? 1024 : pieces <= 1024 ? 512 : 256);
 }
 
 int run_rms_norm_backward(const NormGradArgs& a, int dtype, hipStream_t st) {

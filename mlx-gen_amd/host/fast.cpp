@@ -795,11 +795,7 @@ PyObject* mx_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::DimVector d(x.codes.sizes().begin(), x.codes.sizes().end());
     d.back() = N;
     at::Tensor out = at::empty(d, x.codes.options().dtype(float_type((int)dt)));
-    const size_t need = mlxq_mx_matmul_workspace_size(x.rows, x.K, N, x.m.format);
-    at::Tensor ws = workspace(x.codes, need);
-    if (unlocked([&] {
-          return mlxq_mx_matmul(&x.m, x.rows, x.K, &w.m, N, ptr(bias), bias_dt, out.data_ptr(), (int)dt, ptr(ws), need, st);
-        }) != MLXQ_OK)
+    if (unlocked([&] { return mlxq_mx_matmul(&x.m, x.rows, x.K, &w.m, N, ptr(bias), bias_dt, out.data_ptr(), (int)dt, st); }) != MLXQ_OK)
       return nullptr;
     return THPVariable_Wrap(std::move(out));
   });
@@ -1022,7 +1018,7 @@ PyObject* mx_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out = combine ? at::empty({T, N}, options) : at::empty({T, k, N}, options);
     const mlxq_routing routing = {ids.data_ptr<int32_t>(), weights.data_ptr<float>(), starts.data_ptr<int32_t>(), rows.data_ptr<int32_t>(),
                                   T, k, E};
-    const size_t need = mlxq_mx_experts_workspace_size(T, k, E, x.K, N, x.m.format, combine, (int)dt);
+    const size_t need = mlxq_mx_experts_workspace_size(T, k, N, combine, (int)dt);
     at::Tensor ws = workspace(x.codes, need);
     if (unlocked([&] {
           return mlxq_mx_experts(&x.m, xd == 3, x.K, &w.m, N, ptr(bias), bias_dt, &routing, combine, out.data_ptr(), (int)dt, ptr(ws), need,

@@ -316,7 +316,7 @@ struct Mx {
 Mx mx_quantize(const Array& x, int format, hipStream_t s = nullptr);
 Array mx_dequantize(const Mx& x, Dtype dt = Dtype::Bfloat16, hipStream_t s = nullptr);
 
-// x [..., K] . w^T + bias for e2m1 weights [N, K].  Workspaces as PagedAttention's: the object's own, one stream at a time.
+// x [..., K] . w^T + bias for e2m1 weights [N, K].
 struct MxLinear {
   Mx w;
   std::optional<Array> bias;  // [N]
@@ -324,8 +324,6 @@ struct MxLinear {
 
   Array forward(const Mx& x, hipStream_t s = nullptr) const;
   void forward_into(const Mx& x, const Array& y, hipStream_t s = nullptr) const;
-
-  mutable Workspace workspace_;
 };
 
 // The norm of x (or of x + residual, the sum) over its last dimension, in x's dtype or as e4m3 (mx).
@@ -335,6 +333,7 @@ struct Normed {
 };
 Normed rms_norm(const Array& x, const Array* weight = nullptr, const Array* residual = nullptr, float eps = 1e-6f,
                 bool mx = false, hipStream_t s = nullptr);
+// Workspaces here and below as PagedAttention's: the object's own, one stream at a time.
 struct RmsNormGradient {
   float eps = 1e-6f;
   // (dx, dweight): x is what was normed, dsum the gradient that arrives at it from elsewhere; dweight is empty without a weight.

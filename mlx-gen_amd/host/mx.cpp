@@ -109,9 +109,7 @@ void MxLinear::forward_into(const Mx& x, const Array& y, hipStream_t s) const {
   int bdt;
   const void* b = bias_of(bias, {N}, op, bdt);
   const int ydt = abi_dtype(y.dtype(), op);
-  const size_t need = mlxq_mx_matmul_workspace_size(M, x.K(), N, x.format);
-  const Array& ws = workspace_.at_least(need);
-  check(mlxq_mx_matmul(&xv, M, x.K(), &wv, N, b, bdt, y.data(), ydt, ws.data(), ws.nbytes(), s));
+  check(mlxq_mx_matmul(&xv, M, x.K(), &wv, N, b, bdt, y.data(), ydt, s));
 }
 
 Array MxLinear::forward(const Mx& x, hipStream_t s) const {
@@ -224,7 +222,7 @@ void MxExperts::forward_into(const Mx& x, const Routing& r, bool combine, const 
   int bdt;
   const void* b = bias_of(bias, {E, N}, op, bdt);
   const int ydt = abi_dtype(y.dtype(), op);
-  const size_t need = mlxq_mx_experts_workspace_size(rv.tokens, rv.top_k, E, x.K(), N, x.format, combine, ydt);
+  const size_t need = mlxq_mx_experts_workspace_size(rv.tokens, rv.top_k, N, combine, ydt);
   const Array& ws = workspace_.at_least(need);
   check(mlxq_mx_experts(&xv, per, x.K(), &wv, N, b, bdt, &rv, combine, y.data(), ydt, ws.data(), ws.nbytes(), s));
 }

@@ -74,7 +74,6 @@ EXPORTS = (
     "mlxq_cache_copy_pages",
     "mlxq_mx_quantize",
     "mlxq_mx_dequantize",
-    "mlxq_mx_matmul_workspace_size",
     "mlxq_mx_matmul",
     "mlxq_rms_norm",
     "mlxq_rms_norm_backward_workspace_size",
@@ -219,8 +218,7 @@ def load():
     _f32, _size = ctypes.c_float, ctypes.c_size_t
     lib.mlxq_mx_quantize.argtypes = [_vp, _int, _i64, _i64, _i64, _mx, _vp]
     lib.mlxq_mx_dequantize.argtypes = [_mx, _i64, _i64, _vp, _int, _vp]
-    lib.mlxq_mx_matmul_workspace_size.argtypes = [_i64, _i64, _i64, _int]
-    lib.mlxq_mx_matmul.argtypes = [_mx, _i64, _i64, _mx, _i64, _vp, _int, _vp, _int, _vp, _size, _vp]
+    lib.mlxq_mx_matmul.argtypes = [_mx, _i64, _i64, _mx, _i64, _vp, _int, _vp, _int, _vp]
     lib.mlxq_rms_norm.argtypes = [_heads, _int, _i64, _i64, _heads, _heads, _vp, _int, _f32, _heads, _mx, _vp]
     lib.mlxq_rms_norm_backward_workspace_size.argtypes = [_i64, _i64, _i64, _int]
     lib.mlxq_rms_norm_backward.argtypes = [_heads, _heads, _int, _i64, _i64, _vp, _int, _heads, _f32, _heads, _vp, _vp, _size, _vp]
@@ -228,9 +226,9 @@ def load():
     lib.mlxq_route_experts.argtypes = [_vp, _int, _i64, _router, _vp, _routed, _vp, _size, _vp]
     lib.mlxq_route_plan.argtypes = [_routed, _vp, _size, _vp]
     lib.mlxq_route_experts_backward.argtypes = [_vp, _vp, _int, _i64, _router, _routed, _vp, _vp]
-    lib.mlxq_mx_experts_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _int, _int, _int]
+    lib.mlxq_mx_experts_workspace_size.argtypes = [_i64, _i64, _i64, _int, _int]
     lib.mlxq_mx_experts.argtypes = [_mx, _int, _i64, _mx, _i64, _vp, _int, _routed, _int, _vp, _int, _vp, _size, _vp]
-    for name in ("mlxq_mx_matmul", "mlxq_rms_norm_backward", "mlxq_route", "mlxq_mx_experts"):
+    for name in ("mlxq_rms_norm_backward", "mlxq_route", "mlxq_mx_experts"):
         getattr(lib, name + "_workspace_size").restype = _size
     for name in ("mlxq_mx_quantize", "mlxq_mx_dequantize", "mlxq_mx_matmul", "mlxq_rms_norm", "mlxq_rms_norm_backward",
                  "mlxq_route_experts", "mlxq_route_plan", "mlxq_route_experts_backward", "mlxq_mx_experts"):

@@ -176,11 +176,8 @@ def mx_matmul(x: Mx, w: Mx, bias=None, out_dtype=torch.bfloat16):
     _need_gpu(codes, wcodes)
     out = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
     M = codes.numel() // codes.shape[-1]
-    lib = _lib.load()
-    need = lib.mlxq_mx_matmul_workspace_size(M, K, N, xv.format)
-    ws = _workspace(need, codes.device)
-    check(lib.mlxq_mx_matmul(ctypes.byref(xv), M, K, ctypes.byref(wv), N, _ptr(bias), bias_dt, _ptr(out), _dt(out), _ptr(ws), need,
-                             _stream(codes.device)))
+    check(_lib.load().mlxq_mx_matmul(ctypes.byref(xv), M, K, ctypes.byref(wv), N, _ptr(bias), bias_dt, _ptr(out), _dt(out),
+                                     _stream(codes.device)))
     del keep_x, keep_w
     return out
 
@@ -441,7 +438,7 @@ def mx_experts(x: Mx, w: Mx, routing: Routing, bias=None, combine: bool = False,
     if T == 0:
         return out
     lib = _lib.load()
-    need = lib.mlxq_mx_experts_workspace_size(T, k, E, K, N, xv.format, int(combine), _dt(out))
+    need = lib.mlxq_mx_experts_workspace_size(T, k, N, int(combine), _dt(out))
     ws = _workspace(need, device)
     check(lib.mlxq_mx_experts(ctypes.byref(xv), int(codes.dim() == 3), K, ctypes.byref(wv), N, _ptr(bias), bias_dt,
                               ctypes.byref(_routed((ids, weights, starts, rows), T, k, E)), int(combine), _ptr(out), _dt(out), _ptr(ws),

@@ -68,7 +68,7 @@ def test_matmul_refusals(lib, msg, status, kw):
     a = dict(x=_mx(), M=4, K=128, w=_mx(format=0), N=16, bias=None, bias_dtype=0, y=P, y_dtype=1)
     a.update(kw)
     _refused(lib, msg, lambda: lib.mlxq_mx_matmul(R(a["x"]), a["M"], a["K"], R(a["w"]), a["N"], a["bias"], a["bias_dtype"], a["y"], a["y_dtype"],
-                                                 None, 0, None), status)
+                                                 None), status)
 
 
 @pytest.mark.parametrize("msg,status,kw", [
@@ -141,7 +141,7 @@ def test_nothing_to_do_is_no_error(lib):
     none = _mx(codes=None, scales=None)
     assert lib.mlxq_mx_quantize(None, 1, 0, 128, 128, R(none), None) == 0
     assert lib.mlxq_mx_dequantize(R(none), 0, 128, None, 1, None) == 0
-    assert lib.mlxq_mx_matmul(R(none), 0, 128, R(_mx(format=0)), 16, None, 0, None, 1, None, 0, None) == 0
+    assert lib.mlxq_mx_matmul(R(none), 0, 128, R(_mx(format=0)), 16, None, 0, None, 1, None) == 0
     assert lib.mlxq_rms_norm(R(_heads(data=None)), 1, 0, 128, None, None, None, 0, 1e-6, R(_heads(data=None)), None, None) == 0
     assert lib.mlxq_route_experts_backward(None, None, 1, 8, R(_router()), R(_routing(tokens=0, ids=None)), None, None) == 0
 
@@ -153,10 +153,10 @@ def test_workspace_sizes(lib):
         segments = lib.mlxq_route_workspace_size(n, 128) // (129 * 4)
         assert 0 < segments <= 256 and lib.mlxq_route_workspace_size(n, 128) == segments * 129 * 4
     assert lib.mlxq_route_workspace_size(5000, 2000) == 0
-    assert lib.mlxq_mx_experts_workspace_size(10, 4, 8, 128, 100, 1, 0, 1) == 0
-    assert lib.mlxq_mx_experts_workspace_size(10, 4, 8, 128, 100, 1, 1, 1) == 10 * 4 * 100 * 2
-    assert lib.mlxq_mx_experts_workspace_size(10, 4, 8, 128, 100, 1, 1, 0) == 10 * 4 * 100 * 4
-    assert lib.mlxq_mx_experts_workspace_size(2 ** 20, 64, 8, 128, 2 ** 20, 1, 1, 0) == 2 ** 48
+    assert lib.mlxq_mx_experts_workspace_size(10, 4, 100, 0, 1) == 0
+    assert lib.mlxq_mx_experts_workspace_size(10, 4, 100, 1, 1) == 10 * 4 * 100 * 2
+    assert lib.mlxq_mx_experts_workspace_size(10, 4, 100, 1, 0) == 10 * 4 * 100 * 4
+    assert lib.mlxq_mx_experts_workspace_size(2 ** 20, 64, 2 ** 20, 1, 0) == 2 ** 48
     for args in ((0, 1, 64, 1), (4, 0, 64, 1), (4, 1, 0, 1), (4, 1, 40000, 1), (2 ** 40, 1, 64, 1)):
         assert lib.mlxq_rms_norm_backward_workspace_size(*args) == 0
     for rows, D in ((1, 64), (10 ** 6, 64), (10 ** 6, 5000)):
