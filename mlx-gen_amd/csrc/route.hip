@@ -37,6 +37,22 @@ __device__ __forceinline__ V wave_sum(V v) {
   return lanes_reduce(v, [](V a, V b) { return a + b; });
 }
 
+// The largest of the wave's keys, and the lanes that hold it.  64-bit keys mostly differ in their upper halves.
+__device__ __forceinline__ uint32_t wave_top(uint32_t k, unsigned long long& lanes) {
+  const uint32_t m = wave_max(k);
+  lanes = __ballot(k == m);
+  return m;
+}
+__device__ __forceinline__ unsigned long long wave_top(unsigned long long k, unsigned long long& lanes) {
+  const uint32_t hi = wave_max((uint32_t)(k >> 32));
+  lanes = __ballot((uint32_t)(k >> 32) == hi);
+  if ((lanes & (lanes - 1)) == 0) return (unsigned long long)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, __builtin_ctzll(lanes));
+  const uint32_t lo = wave_max((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  const unsigned long long m = (unsigned long long)hi << 32 | lo;
+  lanes = __ballot(k == m);
+  return m;
+}
+
 // WIDE: the choice is by s + bias, or a group's score is a sum: scores in 64 bits.
 template <typename T, int NE, bool WIDE>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
@@ -84,12 +100,13 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   };
   Val val[NE];
   Key key[NE];
+  double own[WIDE ? NE : 1];  // scores
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = i * 64 + lane;
     if constexpr (WIDE) {
       // A group's score without a bias is of scores; the choice then goes by the logits, whose order is theirs.
-      val[i] = e < E ? score(z[i]) : 0.0;
+      val[i] = own[i] = e < E ? score(z[i]) : 0.0;
       if (a.bias) val[i] += e < E ? (double)a.bias[e] : 0.0;
       key[i] = e < E ? a.bias ? key_of(val[i]) : (Key)key_of(z[i]) : 0;
     } else {
@@ -106,20 +123,24 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     __builtin_amdgcn_wave_barrier();
     Val best = -INFINITY, next = -INFINITY;
     if (lane < a.groups)
-      for (int e = 0; e < size; ++e) {
-        const Val v = mine[lane * size + e];
-        if (v > best) {
-          next = best;
-          best = v;
-        } else if (v > next) {
-          next = v;
+      for (int e0 = 0; e0 < size; e0 += 8) {
+        Val v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mine[lane * size + min(e0 + e, size - 1)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Val x = e0 + e < size ? v[e] : -INFINITY;
+          const Val low = x > best ? best : x;  // of a NaN both comparisons fail
+          if (x > best) best = x;
+          if (low > next) next = low;
         }
       }
     Key gk = lane < a.groups ? key_of(a.best > 1 && size > 1 ? best + next : best) : 0;
     unsigned long long kept = 0;
     for (int j = 0; j < a.kept; ++j) {
-      const Key m = wave_max(gk);
-      const int g = __builtin_ctzll(__ballot(gk == m));
+      unsigned long long lanes;
+      wave_top(gk, lanes);
+      const int g = __builtin_ctzll(lanes);
       kept |= 1ull << g;
       if (lane == g) gk = 0;
     }
@@ -129,33 +150,40 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
       if (e < E && !(kept >> (e / size) & 1)) key[i] = 0;
     }
   }
-  int id = 0;  // lane j < k: the j-th choice
+  int id = 0;  // lane j < k: the j-th choice, and its logit or score
   float zj = 0.0f;
+  double wj = 0.0;
   for (int j = 0; j < a.k; ++j) {
     Key m = key[0];
 #pragma unroll
     for (int i = 1; i < NE; ++i) m = max(m, key[i]);
-    m = wave_max(m);
-    int e = 0;
-    float v = 0.0f;
+    unsigned long long lanes;
+    m = wave_top(m, lanes);
+    // Expert i * 64 + lane: the lowest has the lowest i, then the lowest lane.
     bool found = false;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const unsigned long long has = __ballot(key[i] == m);
+      const unsigned long long has = NE == 1 ? lanes : __ballot(key[i] == m);
       if (!found && has) {
         const int l = __builtin_ctzll(has);
         found = true;
-        e = i * 64 + l;
-        v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(z[i]), l));
         if (lane == l) key[i] = 0;
+        if constexpr (WIDE) {
+          const double v = lane_value(own[i], l);
+          if (lane == j) wj = v;
+        } else {
+          const float v = lane_value(z[i], l);
+          if (lane == j) zj = v;
+        }
+        if (lane == j) id = i * 64 + l;
       }
     }
-    if (lane == j) {
-      id = e;
-      zj = v;
-    }
   }
-  double w = lane < a.k ? score(zj) : 0.0;
+  double w = 0.0;
+  if (lane < a.k) {
+    if constexpr (WIDE) w = wj;
+    else w = score(zj);
+  }
   if (a.normalize) {
     const double sum = wave_sum(w);
     w = sum == 0.0 ? 0.0 : w / sum;

@@ -80,7 +80,10 @@ def product_bound(x, w, dtype, format):
     b = (K / 32 + 16) * 2.0 ** -23 * mag
     if format == "e4m3" and dtype != torch.float32:
         for k in range(0, K, 128):
-            b += 2.0 ** -11 * (x[:, None, k:k + 128].abs() * w[None, :, k:k + 128].abs()).amax(-1)
+            xk, wk = x[:, k:k + 128].abs(), w[:, k:k + 128].abs()
+            # of many results the largest factors stand for the largest product
+            big = xk.shape[0] * wk.shape[0] > 10 ** 6
+            b += 2.0 ** -11 * (xk.amax(-1)[:, None] * wk.amax(-1)[None] if big else (xk[:, None] * wk[None]).amax(-1))
     return b + UNIT[dtype] * (y + b) + TINY[dtype]
 
 
