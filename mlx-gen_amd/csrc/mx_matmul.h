@@ -97,6 +97,11 @@ __device__ __forceinline__ f32x4 mx_bias(const MxProduct& p, int e, int n) {
   }
   return v;
 }
+// Four neighbouring features in a type of 16 bits.
+__device__ __forceinline__ u32x2 mx_round(const MxProduct& p, const f32x4& v) {
+  return p.y_dtype == MLXQ_BFLOAT16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
+                                    : u32x2{Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
+}
 // Four neighbouring features of a row, rounded to y's type.  Rows of any N start at any element.
 __device__ __forceinline__ void mx_store(const MxProduct& p, int row, int n, const f32x4& v) {
   const int N = (int)p.N;
@@ -113,14 +118,34 @@ __device__ __forceinline__ void mx_store(const MxProduct& p, int row, int n, con
     }
     return;
   }
-  const u32x2 h = p.y_dtype == MLXQ_BFLOAT16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
-                                             : u32x2{Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
+  const u32x2 h = mx_round(p, v);
   uint16_t* y = (uint16_t*)p.y + at;
   if (four) {
     __builtin_memcpy(y, &h, 8);
   } else {
     for (int i = 0; i < 4; ++i)
       if (n + i < N) y[i] = (uint16_t)(h[i / 2] >> 16 * (i % 2));
+  }
+}
+
+// Eight neighbouring features of a row, past the caches or not.
+__device__ __forceinline__ void mx_store8(const MxProduct& p, int row, int n, const u32x4& v, bool past) {
+  typedef u32x4 __attribute__((aligned(2))) any_u32x4;
+  const int N = (int)p.N;
+  uint16_t* y = (uint16_t*)p.y + (int64_t)row * N + n;
+  if (n + 8 <= N) {
+    if (past) {
+      // between two statements that keep the compiler from making one ordinary store of both
+      asm volatile("");
+      __builtin_nontemporal_store(v, reinterpret_cast<any_u32x4*>(y));
+      asm volatile("");
+    } else {
+      *reinterpret_cast<any_u32x4*>(y) = v;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < N) y[i] = (uint16_t)(v[i / 2] >> 16 * (i % 2));
   }
 }
 
@@ -388,15 +413,49 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_tile_kernel(MxProduct p,
     return;
   }
   if (idle) return;
+  constexpr int WT = TN / WN;  // a wave's features
+  const int n_wave = n0 + wn * WT;
   f32x4 bias[FN];
 #pragma unroll
-  for (int i = 0; i < FN; ++i) bias[i] = mx_bias(p, tile.e, n0 + wn * (TN / WN) + i * 16 + 4 * g);
+  for (int i = 0; i < FN; ++i) bias[i] = mx_bias(p, tile.e, n_wave + i * 16 + 4 * g);
+  // A lane's four features are 8 bytes of a row, and stores of such pieces touch 16 rows each.  The large tiles' results of 16
+  // bits are turned around in LDS, 16 rows of the wave at a time, and written as whole lines (8192 rows, 14336 features, K 4096:
+  // 415 -> 393 us).  The buffer of the step that is not there any more is free: its last readers have passed the last step's
+  // barrier.  Piece i of row r lies at i ^ r.  A result of more than half of the 256 MB that all dies share goes past the
+  // caches, where it would take the operands' place (235 MB: 394 -> 379 us); a smaller one is left there for its reader (94 MB of
+  // experts' products, then their sum: 215 + 24 us; past the caches 207 + 32).
+  if constexpr (KG == 1 && WT >= 64) {
+    if (p.y_dtype != MLXQ_FLOAT32) {
+      constexpr int PIECES = WT / 8;
+      static_assert(NW * 16 * WT * 2 <= STAGE && 16 * PIECES % 64 == 0);
+      const bool past = p.M * p.N > (int64_t)64 << 20;
+      unsigned char* own = lds + cnt % STAGES * STAGE + w * (16 * WT * 2);
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+          *reinterpret_cast<u32x2*>(own + c * WT * 2 + ((2 * i + (g >> 1)) ^ (c % PIECES)) * 16 + (g & 1) * 8) =
+              mx_round(p, acc[i][j] + bias[i]);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < 16 * PIECES / 64; ++t) {
+          const int r = t * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(own + r * WT * 2 + (piece ^ (r % PIECES)) * 16);
+          const int at = wm * (TM / WM) + j * 16 + r, row = at < tile.count ? tiles.row(tile.first + at) : -1;
+          const int n = n_wave + piece * 8;
+          if (row >= 0 && n < N) mx_store8(p, row, n, v, past);
+        }
+        asm volatile("" ::: "memory");
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int r = wm * (TM / WM) + j * 16 + c, row = r < tile.count ? tiles.row(tile.first + r) : -1;
     if (row < 0) continue;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) mx_store(p, row, n0 + wn * (TN / WN) + i * 16 + 4 * g, acc[i][j] + bias[i]);
+    for (int i = 0; i < FN; ++i) mx_store(p, row, n_wave + i * 16 + 4 * g, acc[i][j] + bias[i]);
   }
 }
 
@@ -434,8 +493,8 @@ inline double mx_tiles(const MxProduct& p, int64_t TM, int64_t TN) {
 //   48 / 256 rows, K 4096, 4096 features           64 x 64, 2 groups 11.6 / 12.1; 1 group 14.7 / 15.1; 64 x 128 18.4 / 18.6
 //   512 rows, K 4096, 4096 features    64 x 128, 2 groups 17.8; 1 group 19.7; 64 x 64 19.9; 128 x 128 28
 //   256 rows, K 4096, 14336 features   64 x 128 27.9; 128 x 128 28.8; 64 x 128, 2 groups 32.8
-//   2048 rows, K 4096, 4096 / 14336 features       128 x 128 40 / 128; 256 x 256 57 / 116
-//   4090 tokens, 4 of 32 experts of 2880 x 2880    256 x 256 193; 128 x 128 210
+//   2048 rows, K 4096, 4096 / 14336 features       128 x 128 37 / 118; 256 x 256 52 / 105
+//   4090 tokens, 4 of 32 experts of 2880 x 2880    256 x 256 173; 128 x 128 183
 template <int XF, bool EXACT>
 int mx_product(const MxProduct& p, hipStream_t st) {
   const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;

@@ -120,6 +120,19 @@ UNIT_SUM = 2.0 ** -23  # the addition of the bias in f32
 
 
 @pytest.mark.parametrize("format", ["e2m1", "e4m3"])
+def test_matmul_large_result(mlxq, format):
+    """A result past 2^31 values, whose rows end inside a piece of eight: rows at the start, at the border and at the end."""
+    M, K, N = 66001, 64, 32771
+    x, w = ref.random_mx(1, (M,), K, format), ref.random_mx(2, (N,), K, "e2m1")
+    banner("mx_matmul", format, M, K, N)
+    y = mlxq.mx_matmul(mlxq.Mx(x[0].cuda(), x[1].cuda()), mlxq.Mx(w[0].cuda(), w[1].cuda()), out_dtype=BF16)
+    border = 2 ** 31 // N
+    for rows in (slice(0, 20), slice(border - 10, border + 10), slice(M - 20, M)):
+        xv, wv = ref.values((x[0][rows], x[1][rows])), ref.values(w)
+        assert ((y[rows].cpu().double() - xv @ wv.t()).abs() <= ref.product_bound(xv, wv, BF16, format)).all()
+
+
+@pytest.mark.parametrize("format", ["e2m1", "e4m3"])
 @pytest.mark.parametrize("M", [3, 40, 200])
 def test_matmul_special_scales(mlxq, format, M):
     """NaN blocks make their rows and columns NaN and nothing else; the smallest and large scales are as exact as others."""
