@@ -42,7 +42,7 @@ __device__ __forceinline__ void load_row(u32x4 (&v)[CH], const T* row, int lane,
 }
 template <typename T>
 __device__ __forceinline__ void set_right(u32x4& v, int e, int D) {
-  if (D >= kC<T> && e + kC<T> > D)
+  if (D >= kC<T> && e < D && e + kC<T> > D)
     for (int k = e + kC<T> - D; k > 0; --k) {
       if constexpr (sizeof(T) == 4) v = u32x4{v[1], v[2], v[3], 0};
       else v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
@@ -246,22 +246,19 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
   __shared__ float slot[2][2 * TW];
   const int lane = threadIdx.x % LANES, D = a.D;
   const bool has_w = a.w_dtype >= 0;
-  // The longest rows leave no registers: their weights and dsum are loaded where they are used.
-  constexpr bool LEAN = LANES > 256 && CH > 4;
-  float w[LEAN ? 1 : CH][C], dw[CH][C];
+  float w[CH][C], dw[CH][C];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    if constexpr (!LEAN) load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[i]);
+    load_weights(a.w, a.w_dtype, (i * LANES + lane) * C, D, w[i]);
 #pragma unroll
     for (int e = 0; e < C; ++e) dw[i][e] = 0.0f;
   }
-  u32x4 x[CH], dy[CH], ds[LEAN ? 1 : CH];
+  u32x4 x[CH], dy[CH], ds[CH];
   auto load = [&](int64_t at) {
     const int row = (int)min(at, a.rows - 1), t = a.by_heads.div(row), h = row - t * a.heads;
     load_row<T, LANES>(x, row_of<const T>(a.x, t, h), lane, D);
     load_row<T, LANES>(dy, row_of<const T>(a.dy, t, h), lane, D);
-    if constexpr (!LEAN)
-      if (a.dsum.p) load_row<T, LANES>(ds, row_of<const T>(a.dsum, t, h), lane, D);
+    if (a.dsum.p) load_row<T, LANES>(ds, row_of<const T>(a.dsum, t, h), lane, D);
   };
   const int64_t step = (int64_t)gridDim.x * R;
   int64_t first = (int64_t)blockIdx.x * R;
@@ -275,24 +272,23 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
     for (int i = 0; i < CH; ++i) {
       const int e0 = (i * LANES + lane) * C;
       if (e0 >= D) continue;
-      if constexpr (LEAN) load_weights(a.w, a.w_dtype, e0, D, w[0]);
       set_right<T>(x[i], e0, D);
       set_right<T>(dy[i], e0, D);
 #pragma unroll
       for (int e = 0; e < C; ++e) {
         const float xv = Elem<T>::get(x[i], e);
         s[0] = fmaf(xv, xv, s[0]);
-        s[1] = fmaf(Elem<T>::get(dy[i], e) * w[LEAN ? 0 : i][e], xv, s[1]);
+        s[1] = fmaf(Elem<T>::get(dy[i], e) * w[i][e], xv, s[1]);
       }
     }
     row_sum<LANES>(s, slot[turn]);
     // The next row's loads go out beside this one's results.
-    u32x4 x0[CH], dy0[CH], ds0[LEAN ? 1 : CH];
+    u32x4 x0[CH], dy0[CH], ds0[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       x0[i] = x[i];
       dy0[i] = dy[i];
-      if constexpr (!LEAN) ds0[i] = ds[i];
+      ds0[i] = ds[i];
     }
     if (first + step < a.rows) load(at + step);
     const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
@@ -303,25 +299,17 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
     for (int i = 0; i < CH; ++i) {
       const int e0 = (i * LANES + lane) * C;
       if (e0 >= D) continue;
-      if constexpr (LEAN) {
-        load_weights(a.w, a.w_dtype, e0, D, w[0]);
-        if (a.dsum.p) {
-          u32x4 one[1];
-          load_row<T, LANES>(one, row_of<const T>(a.dsum, t, h), i * LANES + lane, D);
-          ds0[0] = one[0];
-        }
-      }
       float f[C];
 #pragma unroll
       for (int e = 0; e < C; ++e) {
         const float xv = Elem<T>::get(x0[i], e), g = Elem<T>::get(dy0[i], e);
-        f[e] = r * (g * w[LEAN ? 0 : i][e]) - c * xv;
+        f[e] = r * (g * w[i][e]) - c * xv;
         dw[i][e] = fmaf(g, xv * r, dw[i][e]);
       }
       if (a.dsum.p) {
-        set_right<T>(ds0[LEAN ? 0 : i], e0, D);
+        set_right<T>(ds0[i], e0, D);
 #pragma unroll
-        for (int e = 0; e < C; ++e) f[e] += Elem<T>::get(ds0[LEAN ? 0 : i], e);
+        for (int e = 0; e < C; ++e) f[e] += Elem<T>::get(ds0[i], e);
       }
       store_piece(dx, e0, D, pack_chunk<T>(f));
     }
@@ -350,6 +338,71 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
         if (at < D) part[at] = dw[i][e];
       }
   }
+}
+
+// Rows of more than 2048 pieces leave no registers for themselves: a workgroup of sixteen waves reads them twice, the second time
+// from the cache, and the weight's sums are in LDS, each lane's its own.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a) {
+  constexpr int C = kC<T>, LANES = 1024;
+  __shared__ float slot[2][2 * LANES / 64];
+  __shared__ __align__(16) float dw[32768];
+  const int D = a.D, e_first = threadIdx.x * C;
+  for (int e0 = e_first; e0 < D; e0 += LANES * C)
+#pragma unroll
+    for (int e = 0; e < C; ++e) dw[e0 + e] = 0.0f;
+  int turn = 0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const int t = a.by_heads.div(row), h = row - t * a.heads;
+    const T *x = row_of<const T>(a.x, t, h), *dy = row_of<const T>(a.dy, t, h);
+    const T* ds = a.dsum.p ? row_of<const T>(a.dsum, t, h) : nullptr;
+    T* dx = row_of<T>(a.dx, t, h);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll 2
+    for (int e0 = e_first; e0 < D; e0 += LANES * C) {
+      u32x4 xv[1], g[1];
+      float w[C];
+      load_row<T, 1>(xv, x, e0 / C, D);
+      load_row<T, 1>(g, dy, e0 / C, D);
+      load_weights(a.w, a.w_dtype, e0, D, w);
+      set_right<T>(xv[0], e0, D);
+      set_right<T>(g[0], e0, D);
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const float v = Elem<T>::get(xv[0], e);
+        s[0] = fmaf(v, v, s[0]);
+        s[1] = fmaf(Elem<T>::get(g[0], e) * w[e], v, s[1]);
+      }
+    }
+    row_sum<LANES>(s, slot[turn]);
+    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
+#pragma unroll 2
+    for (int e0 = e_first; e0 < D; e0 += LANES * C) {
+      u32x4 xv[1], g[1], d[1] = {u32x4{0, 0, 0, 0}};
+      float w[C], f[C];
+      load_row<T, 1>(xv, x, e0 / C, D);
+      load_row<T, 1>(g, dy, e0 / C, D);
+      if (ds) load_row<T, 1>(d, ds, e0 / C, D);
+      load_weights(a.w, a.w_dtype, e0, D, w);
+      set_right<T>(xv[0], e0, D);
+      set_right<T>(g[0], e0, D);
+      if (ds) set_right<T>(d[0], e0, D);
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const float v = Elem<T>::get(xv[0], e), gv = Elem<T>::get(g[0], e);
+        f[e] = r * (gv * w[e]) - c * v;
+        dw[e0 + e] = fmaf(gv, v * r, dw[e0 + e]);
+        if (ds) f[e] += Elem<T>::get(d[0], e);
+      }
+      store_piece(dx, e0, D, pack_chunk<T>(f));
+    }
+  }
+  if (a.w_dtype < 0) return;
+  float* part = a.part + (int64_t)blockIdx.x * D;
+  for (int e0 = e_first; e0 < D; e0 += LANES * C)
+#pragma unroll
+    for (int e = 0; e < C; ++e)
+      if (e0 + e < D) part[e0 + e] = dw[e0 + e];
 }
 
 // 64 features a workgroup, its sixteen waves a sixteenth of the parts each.
@@ -405,9 +458,14 @@ int norm(const NormArgs& a, hipStream_t st) {
 
 template <typename T>
 int norm_grad(const NormGradArgs& a, hipStream_t st) {
-  return by_pieces((a.D + kC<T> - 1) / kC<T>, [&](auto lanes, auto ch) {
+  const int64_t pieces = (a.D + kC<T> - 1) / kC<T>;
+  if (pieces > 2048) {
+    rms_norm_grad_long_kernel<T><<<(unsigned)a.parts, 1024, 0, st>>>(a);
+    return check_launch("rms_norm_backward");
+  }
+  return by_pieces(pieces, [&](auto lanes, auto ch) {
     constexpr int LANES = decltype(lanes)::value, CH = decltype(ch)::value;
-    if constexpr (LANES * CH * kC<T> <= 32768)
+    if constexpr (LANES * CH <= 2048)
       rms_norm_grad_kernel<T, LANES, CH><<<(unsigned)a.parts, LANES > 256 ? LANES : 256, 0, st>>>(a);
     return check_launch("rms_norm_backward");
   });

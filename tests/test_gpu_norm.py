@@ -1,4 +1,6 @@
 """rms_norm and rms_norm_backward against their definitions (mx_ref), on the GPU."""
+import ctypes
+
 import pytest
 import torch
 
@@ -103,7 +105,6 @@ def test_norm_strides(mlxq):
 
 def test_norm_writes_its_rows_only(mlxq):
     """In place through the C interface, with rows apart: what lies between them stays."""
-    import ctypes
     from mlxq import _lib
     for D in (5, 64, 77, 2048):
         buf = torch.full((6, D + 9), 5.0, device="cuda", dtype=BF16)
@@ -167,6 +168,25 @@ def test_gradient_is_that_of_differences(mlxq):
         up[e] += h
         dn[e] -= h
         assert abs(float(dw[e] - (f(x, up) - f(x, dn)) / (2 * h))) <= float(mag_w[e]) * 200 * 2.0 ** -24 + 2.0 ** -50 * 100 / h
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 515), (F32, 1026), (BF16, 5121), (F16, 16399), (BF16, 24580), (F32, 8195), (F32, 20001)])
+def test_gradient_in_place(mlxq, dtype, D):
+    """dx over dy, and over dsum, with rows that end inside a piece and a buffer that goes on behind them: the same bits."""
+    x, dy, ds = (_x(D + i, (300, D), dtype).cuda() for i in range(3))
+    w = (1 + 0.3 * _x(7, (D,), F32)).to(dtype).cuda()
+    want, want_w = mlxq.rms_norm_backward(dy, x, w, ds, 1e-5)
+    lib, code = mlxq._lib.load(), mlxq.mx._dt(x)
+    need = lib.mlxq_rms_norm_backward_workspace_size(300, 1, D, code)
+    ws, dw = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda"), torch.empty_like(w)
+    view = lambda t: ctypes.byref(mlxq._lib.Heads(t.data_ptr(), 1, t.stride(0), 0))  # noqa: E731
+    for over in (0, 1):
+        bufs = [torch.full((300, D + 7), 5.0, dtype=dtype, device="cuda") for _ in range(2)]
+        bufs[0][:, :D], bufs[1][:, :D] = dy, ds
+        mlxq._lib.check(lib.mlxq_rms_norm_backward(view(bufs[0]), view(x), code, 300, D, w.data_ptr(), code, view(bufs[1]), 1e-5,
+                                                   view(bufs[over]), dw.data_ptr(), ws.data_ptr(), need,
+                                                   torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(bufs[over][:, :D], want) and torch.equal(dw, want_w) and (bufs[over][:, D:] == 5).all()
 
 
 def test_gradient_bits_repeat(mlxq):
