@@ -202,9 +202,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
       store_piece(y, e0, D, pack_chunk<T>(f));
     }
   } else {
-    // In 64 bits up to the rounding to 8: which code a value next to a border gets, and a block its scale, is then
-    // not a matter of the order of the sum.
+    // As in 64 bits up to the rounding to 8: which code a value next to a border gets, and a block its scale, is then
+    // not a matter of the order of the sum.  In 32 bits a value is off by less than 2^-22 of it (its two products, r's rounding),
+    // so where codes and scale are the same 2^-21 to either side they are right; one piece of a wave in a hundred has
+    // another, and takes the 64 bits (8190 x 5120 bf16: all pieces in 64 bits 43 us).
     const double r = 1.0 / sqrt(s[0] / (double)D + (double)a.eps);
+    const float r32 = (float)r;
     if (!live) return;
     unsigned char* codes = a.mx.codes + (int64_t)row * D;
     unsigned char* scales = a.mx.scales + row * a.mx.scale_stride;
@@ -213,24 +216,55 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
       const int e0 = (i * LANES + lane) * C;
       if (e0 >= D) break;  // D is a multiple of 32: whole blocks of lanes
       if constexpr (!EARLY) load_weights(a.w, a.w_dtype, e0, D, w[0]);
-      double y[C];
-      unsigned long long top = 0;
+      uint32_t code[C / 4];
+      int ex;
+      bool bad = false, sure = r32 >= 0x1p-60f && r32 <= 0x1p60f;
+      {
+        float y[C];
+        uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < C; ++e) {
-        y[e] = (double)Elem<T>::get(v[i], e) * r * (double)w[EARLY ? i : 0][e];
-        top = max(top, (unsigned long long)__double_as_longlong(y[e]) & 0x7fffffffffffffffull);
+        for (int e = 0; e < C; ++e) {
+          const float x = Elem<T>::get(v[i], e), n = x * r32, weight = w[EARLY ? i : 0][e];
+          y[e] = n * weight;
+          // a product next to f32's smallest numbers is off by more; NaN is never sure
+          sure &= (fabsf(n) >= 0x1p-100f && fabsf(y[e]) >= 0x1p-100f) || (x == 0.0f && fabsf(weight) < INFINITY);
+          top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+        }
+        top = lanes_reduce<32 / C>(top, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        ex = mx_exponent<kE4M3>(top + 16);
+        sure &= top + 16 < 0x7f800000u && ex == mx_exponent<kE4M3>(max(top, 16u) - 16);
+        float lo[C], hi[C];
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          const float f = __builtin_amdgcn_ldexpf(y[e], -ex);
+          lo[e] = f * (1.0f - 0x1p-21f);
+          hi[e] = f * (1.0f + 0x1p-21f);
+        }
+#pragma unroll
+        for (int k = 0; k < C; k += 4) {
+          code[k / 4] = mx_pack_e4m3(lo[k], lo[k + 1], lo[k + 2], lo[k + 3]);
+          sure &= code[k / 4] == mx_pack_e4m3(hi[k], hi[k + 1], hi[k + 2], hi[k + 3]);
+        }
       }
-      top = lanes_reduce<32 / C>(top, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-      // 448 = 1.75 * 2^8; magnitudes past f32 are as infinite as f32's infinity
-      int ex = max((int)(top >> 52) - 1023 - 8 + ((top & 0xfffffffffffffull) > 0xc000000000000ull), -127);
-      const bool bad = top >= 0x47f0000000000000ull;
-      float f[C];
+      if (__any(!sure)) {
+        double y[C];
+        unsigned long long top = 0;
 #pragma unroll
-      for (int e = 0; e < C; ++e) f[e] = bad ? 0.0f : round_to_odd(ldexp_f64(y[e], -ex));
-      if constexpr (C == 8)
-        *reinterpret_cast<u32x2*>(codes + e0) = u32x2{mx_pack_e4m3(f[0], f[1], f[2], f[3]), mx_pack_e4m3(f[4], f[5], f[6], f[7])};
-      else
-        *reinterpret_cast<uint32_t*>(codes + e0) = mx_pack_e4m3(f[0], f[1], f[2], f[3]);
+        for (int e = 0; e < C; ++e) {
+          y[e] = (double)Elem<T>::get(v[i], e) * r * (double)w[EARLY ? i : 0][e];
+          top = max(top, (unsigned long long)__double_as_longlong(y[e]) & 0x7fffffffffffffffull);
+        }
+        top = lanes_reduce<32 / C>(top, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
+        // 448 = 1.75 * 2^8; magnitudes past f32 are as infinite as f32's infinity
+        ex = max((int)(top >> 52) - 1023 - 8 + ((top & 0xfffffffffffffull) > 0xc000000000000ull), -127);
+        bad = top >= 0x47f0000000000000ull;
+        float f[C];
+#pragma unroll
+        for (int e = 0; e < C; ++e) f[e] = bad ? 0.0f : round_to_odd(ldexp_f64(y[e], -ex));
+#pragma unroll
+        for (int k = 0; k < C; k += 4) code[k / 4] = mx_pack_e4m3(f[k], f[k + 1], f[k + 2], f[k + 3]);
+      }
+      __builtin_memcpy(codes + e0, code, C);
       if (e0 % 32 == 0) {
         scales[e0 / 32] = bad ? 255 : (unsigned char)(ex + 127);
         if (e0 + 32 == D)
