@@ -342,7 +342,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_tile_kernel(MxProduct p,
     auto meet = [&](int s) {  // the group's step s is there for all of its waves
       if (s + STAGES - 2 < cnt) mlxq_vmcnt<(STAGES - 2) * PER>();
       else mlxq_vmcnt<0>();
-      __builtin_amdgcn_s_barrier();
+      if constexpr (NW > 1) __builtin_amdgcn_s_barrier();  // a group of one wave has its buffers to itself
       asm volatile("" ::: "memory");
     };
     auto step = [&](int s, bool ahead, auto LAST) {
@@ -389,7 +389,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_tile_kernel(MxProduct p,
     } else {
       for (int s = 0; s + 1 < cnt; ++s) step(s, s + STAGES - 1 < cnt, std::false_type{});
       if (cnt > 0) step(cnt - 1, false, std::true_type{});
-      for (int s = cnt; s < most; ++s) meet(s);
+      if constexpr (NW > 1)
+        for (int s = cnt; s < most; ++s) meet(s);
     }
     if constexpr (KG > 1) {
       __syncthreads();
