@@ -511,7 +511,7 @@ int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int
  *   y = h * (mean(h^2) + eps)^(-1/2) * weight            (weight [D] in weight_dtype, NULL: ones)
  * x, residual, sum and y have one dtype and any strides that are whole elements.  Sums are f32, and y is
  * rounded once.  Exactly one of y and y_mx is given: y_mx (e4m3, rows T * heads of D, D a multiple of 32)
- * is what mlxq_mx_quantize would make of the exact norm, which is taken in 64 bits there, so that
+ * is what mlxq_mx_quantize would make of the exact norm, which is taken in 64 bits wherever it matters, so that
  * no code depends on the order of a sum.  sum may be x or residual (same strides), y may be x; otherwise
  * nothing may overlap.  D up to 32768.
  */

