@@ -30,8 +30,10 @@ struct MxTile {
   bool found;
 };
 
-// Tile `at` of `tiles`, cut TM rows at a time; `total` gives all tiles of all runs.
+// Tile `at` of `tiles`, cut TM rows at a time; `total` gives all tiles of all runs.  Starts that are no plan's may make runs that
+// overlap, and more tiles than there are integers: sums stop at kMost, which no plan reaches.
 struct MxTiles {
+  static constexpr int kMost = (1 << 30) - 1;
   const MxProduct& p;
   int TM;
   __device__ __forceinline__ int bound(int i) const {  // the start of run i; the last ends with the choices
@@ -46,14 +48,14 @@ struct MxTiles {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(s, d);
-      if (lane >= d) s += o;
+      if (lane >= d) s = min(s + o, kMost);
     }
     return s;
   }
   __device__ __forceinline__ int total() const {
     if (p.E == 0) return ((int)p.M + TM - 1) / TM;
     int n = 0, own;
-    for (int i0 = 0; i0 <= p.E; i0 += 64) n += __builtin_amdgcn_readlane(scan(i0 + (threadIdx.x & 63), own), 63);
+    for (int i0 = 0; i0 <= p.E; i0 += 64) n = min(n + __builtin_amdgcn_readlane(scan(i0 + (threadIdx.x & 63), own), 63), kMost);
     return n;
   }
   __device__ __forceinline__ MxTile find(int at) const {
@@ -65,6 +67,7 @@ struct MxTiles {
       if (at < all) {
         const int l = __builtin_ctzll(__ballot(s > at)), i = i0 + l;
         const int k = at - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(own, l));
+        if (k >= __builtin_amdgcn_readlane(own, l)) return {0, 0, 0, false};
         const int first = bound(i) + k * TM;
         return {first, min(TM, bound(i + 1) - first), i, true};
       }
@@ -250,7 +253,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_tile_kernel(MxProduct p,
   // K 4096: bands of 4, 8 and 16 tiles 416, 422 and 431 us).
   constexpr int BAND = 4;
   MxTiles tiles{p, TM};
-  const int m_tiles = tiles.total(), all = m_tiles * n_tiles, chunk = (all + 7) / 8;
+  // A launch has workgroups for every tile of a plan.
+  const int m_tiles = min(tiles.total(), (int)(gridDim.x / (unsigned)n_tiles)), all = m_tiles * n_tiles, chunk = (all + 7) / 8;
   const int l = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= chunk || l >= all) return;
   const int band = l / (BAND * n_tiles), in = l - band * BAND * n_tiles, high = min(BAND, m_tiles - BAND * band);

@@ -260,6 +260,22 @@ def test_a_broken_plan_stays_in_bounds(mlxq):
     assert torch.equal(mlxq.mx_experts(x, w, good), mlxq.mx_experts(x, w, mlxq.route_plan(good.ids, good.weights, E)))
 
 
+def test_overlapping_runs_of_many_choices(mlxq):
+    """Starts of 512 runs that each hold all of 2^25 choices: more tiles than 2^31.  Results mean nothing; memory is left alone."""
+    T, k, E = 2 ** 19, 64, 1024
+    x = mlxq.Mx(torch.zeros(T, 16, dtype=torch.uint8, device="cuda"), torch.full((T, 4), 127, dtype=torch.uint8, device="cuda")[:, :1])
+    w = mlxq.Mx(torch.zeros(E, 1, 16, dtype=torch.uint8, device="cuda"), torch.full((E, 1, 4), 127, dtype=torch.uint8, device="cuda")[..., :1])
+    starts = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    starts[1::2] = T * k
+    routing = mlxq.Routing(torch.zeros(T, k, dtype=torch.int32, device="cuda"), torch.zeros(T, k, device="cuda"), starts,
+                           torch.arange(T * k, dtype=torch.int32, device="cuda"))
+    y = mlxq.mx_experts(x, w, routing)
+    assert not y[:1000].any()
+    # and a plan after it is as good as ever
+    good = mlxq.route_plan(routing.ids[:100], routing.weights[:100], E)
+    assert torch.equal(good.rows.cpu(), torch.arange(6400, dtype=torch.int32))
+
+
 def test_repeated_calls_and_streams(mlxq):
     """The same bits on any stream and from call to call, with other calls between."""
     x = mlxq.mx_quantize(torch.randn(500, 1056, device="cuda"), "e4m3")
