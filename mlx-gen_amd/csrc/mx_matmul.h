@@ -223,7 +223,8 @@ __device__ __forceinline__ void mx_dma4(const unsigned char* from, uint32_t lds)
 // them: 8190 rows, K 4096, 14336 features of e4m3 380 us, 2.53 PFLOP/s (e2m1 277 us, 3.5; a large library product of 8-bit operands 2.8
 // to 3.2).  The large tile without its matrix instructions takes 265 us, without its loads 346, with both 415 before its results were
 // written as whole lines: neither side hides the other in full, at two waves a SIMD.  Matrix cores 52 % busy, L2 hits 90 %.  Loads
-// spread between the matrix instructions took 5 % more, deeper rings do not fit LDS, smaller tiles read more.
+// spread between the matrix instructions took 5 % more, leaving out the loads of rows that a short tile lacks 4 % (the waits then
+// branch); deeper rings do not fit LDS, smaller tiles read more.
 //
 // A workgroup of WM x WN waves takes TM rows by TN features; steps of 128 values of K go through a ring of STAGES
 // buffers in LDS by DMA, one barrier a step.  The scales of four steps go together, 16 bytes of 16 rows a load: a row's
@@ -500,7 +501,7 @@ inline double mx_tiles(const MxProduct& p, int64_t TM, int64_t TN) {
 //   1 row, K 4096, 14336 features      16 x 32, 4 groups 7.4; 16 x 64, 4 groups 7.9; 32 x 64, 4 groups 8.2; 16 x 32, 8 groups 9.3
 //   3 tokens, 4 of 32 experts of 5760 x 2880       32 x 128 17.5; 64 x 128 18.1; 32 x 64 18.3; 16 x 32, 4 groups 27
 //   32 rows, K 4096, 14336 features    32 x 64, 4 groups 9.1; 2 groups 9.8; 64 x 64, 2 groups 10.8
-//   250 tokens, the same experts       64 x 128 91; 32 x 128 100; 32 x 64 105; 64 x 64 112
+//   120 / 500 tokens, 4 of 32 experts of 2880 x 2880   64 x 128 44 / 73 (three stages 46 / 74); 128 x 128 53 / 71; 32 x 128 50 / 80; 64 x 64 67 / 112
 //   48 / 256 rows, K 4096, 4096 features           64 x 64, 2 groups 11.6 / 12.1; 1 group 14.7 / 15.1; 64 x 128 18.4 / 18.6
 //   512 rows, K 4096, 4096 features    64 x 128, 2 groups 17.8; 1 group 19.7; 64 x 64 19.9; 128 x 128 28
 //   256 rows, K 4096, 14336 features   64 x 128 27.9; 128 x 128 28.8; 64 x 128, 2 groups 32.8
@@ -520,7 +521,7 @@ int mx_product(const MxProduct& p, hipStream_t st) {
   if (mx_tiles(p, 64, 64) <= 256) return mx_launch_tile<XF, EXACT, 64, 64, 2, 2, 4, 2>(p, st);
   if (mx_tiles(p, 64, 128) <= 256) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 2>(p, st);
   const double mid = mx_tiles(p, 128, 128);
-  if (mid <= 256 || rows <= 64) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 1>(p, st);
+  if (mid <= 256 || rows <= 64) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 4, 1>(p, st);
   // One round of the largest tiles takes as long as three quarters of the mid ones' of 1024 (two rounds of two to a CU).  Their
   // operands as bf16 do not fit the registers (8190 rows, K 4096, 14336 features in f32: 3.5 ms; the mid ones 0.94).
   if (!EXACT && mid >= 768 * ceil(mx_tiles(p, 256, 256) / 256)) return mx_launch_tile<XF, false, 256, 256, 4, 2, 3, 1>(p, st);
