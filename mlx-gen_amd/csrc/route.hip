@@ -4,12 +4,12 @@
 // the numbers: the logits' own bits where there is no bias (f32: exact, and as the scores' order), else s + bias in 64
 // bits.  top_k rounds of a maximum over the wave; ballots then find the lowest expert that has it.  A few loads and a few
 // hundred instructions a token: a short call is a launch's latency, a long one bound by the vector units (17 tokens, 8 of 128
-// experts in groups, f32 logits with a bias 6.5 us; 16381 tokens, 8 of 256 experts 43 us with the plan).  A second kernel makes
+// experts in groups, f32 logits with a bias 6.5 us; 16381 tokens, 8 of 256 experts 26.5 us with the plan).  A second kernel makes
 // the plan: with a wave a token and the plan in one workgroup, a launch less, 8 tokens took 9.3 us for 10.5, but 17 12.3 for 10.6.
 //
 // The plan is a stable counting sort of the choices by expert: segments count their experts, and each choice's place is
-// its expert's start, plus that expert's choices in earlier segments, plus its rank in its own; the rank among 64 is
-// found by ballots, so that no result depends on the order of an atomic.
+// its expert's start, plus that expert's choices in earlier segments and in earlier waves of its own, plus its rank in its
+// wave; the rank among 64 is found by ballots, so that no result depends on the order of an atomic.
 #include <algorithm>
 
 #include "mx.h"
@@ -303,22 +303,19 @@ __device__ __forceinline__ void walk(const int32_t* ids, int first, int last, in
   }
 }
 
-// Counts of each segment's experts, [segments][E + 1].
-__global__ __launch_bounds__(64) void route_count_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
-                                                         int32_t* __restrict__ counts) {
+// Counts of each segment's experts, [segments][E + 1].  Sums of integers: the order of the additions does not matter.
+__global__ __launch_bounds__(1024) void route_count_kernel(const int32_t* __restrict__ ids, int n, int E, int segment,
+                                                           int32_t* __restrict__ counts) {
   __shared__ int count[1025];
-  const int lane = threadIdx.x, first = blockIdx.x * segment;
-  for (int e = lane; e <= E; e += 64) count[e] = 0;
+  const int first = blockIdx.x * segment, last = min(n, first + segment);
+  for (int e = threadIdx.x; e <= E; e += 1024) count[e] = 0;
   __syncthreads();
-  walk(ids, first, min(n, first + segment), E, bits, [&](int, bool live, int e, unsigned long long same) {
-    if (live && lane == __builtin_ctzll(same)) count[e] += __popcll(same);
-    __builtin_amdgcn_wave_barrier();
-  });
+  for (int c = first + threadIdx.x; c < last; c += 1024) atomicAdd(&count[(unsigned)ids[c] < (unsigned)E ? ids[c] : E], 1);
   __syncthreads();
-  for (int e = lane; e <= E; e += 64) counts[(int64_t)blockIdx.x * (E + 1) + e] = count[e];
+  for (int e = threadIdx.x; e <= E; e += 1024) counts[(int64_t)blockIdx.x * (E + 1) + e] = count[e];
 }
 
-// A segment a workgroup of W waves... with one segment there are no counts yet.
+// The plan of a few choices, by one workgroup: a part of them a wave.
 __global__ __launch_bounds__(1024) void route_small_plan_kernel(const int32_t* __restrict__ ids, int n, int E, int bits,
                                                                 int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
   __shared__ int next[16][1025];  // a wave's counts, then where its next choice of an expert goes
@@ -376,18 +373,21 @@ __global__ __launch_bounds__(1024) void route_small_plan_kernel(const int32_t* _
   });
 }
 
-// Segment blockIdx.x's choices to their places: the totals of all segments, then those of the earlier ones.  Each of the
-// four waves adds up every fourth segment.
-__global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
-                                                          const int32_t* __restrict__ counts, int segments,
-                                                          int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
-  __shared__ int sums[1025], next[1025], some[4][2][64];
+// Segment blockIdx.x's choices to their places: its experts' starts are the totals of all segments and the counts of earlier
+// ones, of which each of sixteen waves adds up every sixteenth; within the segment each wave has a part, as in a small plan.
+// 131048 choices of 256 experts: 22 us with four waves and a segment of 512 walked by one, 9 so.
+constexpr int kPlaceWaves = 16;
+__global__ __launch_bounds__(64 * kPlaceWaves) void route_place_kernel(const int32_t* __restrict__ ids, int n, int E, int bits, int segment,
+                                                                       const int32_t* __restrict__ counts, int segments,
+                                                                       int32_t* __restrict__ starts, int32_t* __restrict__ rows) {
+  __shared__ int next[kPlaceWaves][1025];  // a wave's counts, then where its next choice of an expert goes
+  __shared__ int sums[1025], base[1025], some[kPlaceWaves][2][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, mine = blockIdx.x;
   for (int e0 = 0; e0 <= E; e0 += 64) {
     const int e = min(e0 + lane, E);
     int all = 0, before = 0;
 #pragma unroll 8
-    for (int s = w; s < segments; s += 4) {
+    for (int s = w; s < segments; s += kPlaceWaves) {
       const int c = counts[(int64_t)s * (E + 1) + e];
       all += c;
       before += s < mine ? c : 0;
@@ -395,44 +395,62 @@ __global__ __launch_bounds__(256) void route_place_kernel(const int32_t* __restr
     some[w][0][lane] = all;
     some[w][1][lane] = before;
     __syncthreads();
-    if (w == 0 && e0 + lane <= E) {
-      sums[e] = some[0][0][lane] + some[1][0][lane] + some[2][0][lane] + some[3][0][lane];
-      next[e] = some[0][1][lane] + some[1][1][lane] + some[2][1][lane] + some[3][1][lane];
+    if (w < 2 && e0 + lane <= E) {
+      int s = 0;
+#pragma unroll
+      for (int k = 0; k < kPlaceWaves; ++k) s += some[k][w][lane];
+      (w == 0 ? sums : base)[e] = s;
     }
     __syncthreads();
   }
-  __syncthreads();
-  if (tid >= 64) return;
-  int before = 0;
-  for (int e0 = 0; e0 <= E; e0 += 64) {
-    const int e = e0 + lane, own = e <= E ? sums[e] : 0;
-    int s = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(s, d);
-      if (lane >= d) s += o;
-    }
-    if (e <= E) {
-      next[e] += before + s - own;
-      if (mine == 0) starts[e] = before + s - own;
-    }
-    before += __builtin_amdgcn_readlane(s, 63);
-  }
+  const int end = min(n, (mine + 1) * segment), per = ((end - mine * segment + kPlaceWaves - 1) / kPlaceWaves + 63) & ~63;
+  const int first = min(end, mine * segment + w * per), last = min(end, first + per);
+  for (int e = lane; e <= E; e += 64) next[w][e] = 0;
   __builtin_amdgcn_wave_barrier();
-  const int first = mine * segment;
-  walk(ids, first, min(n, first + segment), E, bits, [&](int c, bool live, int e, unsigned long long same) {
-    const int at = live ? next[e] : 0, rank = __popcll(same & ((1ull << lane) - 1));
+  walk(ids, first, last, E, bits, [&](int, bool live, int e, unsigned long long same) {
+    if (live && lane == __builtin_ctzll(same)) next[w][e] += __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  });
+  if (w == 0) {
+    int before = 0;
+    for (int e0 = 0; e0 <= E; e0 += 64) {
+      const int e = e0 + lane, own = e <= E ? sums[e] : 0;
+      int s = own;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+      }
+      if (e <= E) {
+        base[e] += before + s - own;
+        if (mine == 0) starts[e] = before + s - own;
+      }
+      before += __builtin_amdgcn_readlane(s, 63);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e <= E; e += 64 * kPlaceWaves) {
+    int s = base[e];
+    for (int k = 0; k < kPlaceWaves; ++k) {
+      const int c = next[k][e];
+      next[k][e] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+  walk(ids, first, last, E, bits, [&](int c, bool live, int e, unsigned long long same) {
+    const int at = live ? next[w][e] : 0, rank = __popcll(same & ((1ull << lane) - 1));
     __builtin_amdgcn_wave_barrier();
     if (live) {
       rows[at + rank] = c;
-      if (rank == 0) next[e] = at + __popcll(same);
+      if (rank == 0) next[w][e] = at + __popcll(same);
     }
     __builtin_amdgcn_wave_barrier();
   });
 }
 
 constexpr int kOneGroup = 2048;  // choices that one workgroup sorts by itself
-int64_t segment_of(int64_t n) { return ((n + 255) / 256 + 255) / 256 * 256; }  // at most 256 segments
+int64_t segment_of(int64_t n) { return ((n + 255) / 256 + 1023) / 1024 * 1024; }  // at most 256 segments
 
 template <typename F>
 int by_experts(int E, F&& f) {
@@ -491,9 +509,9 @@ int run_route_plan(const int32_t* ids, int64_t choices, int64_t E, int32_t* star
     return check_launch("route_plan");
   }
   const int64_t seg = segment_of(choices), n = (choices + seg - 1) / seg;
-  route_count_kernel<<<(unsigned)n, 64, 0, st>>>(ids, (int)choices, (int)E, bits, (int)seg, (int32_t*)ws);
+  route_count_kernel<<<(unsigned)n, 1024, 0, st>>>(ids, (int)choices, (int)E, (int)seg, (int32_t*)ws);
   if (int rc = check_launch("route_plan")) return rc;
-  route_place_kernel<<<(unsigned)n, 256, 0, st>>>(ids, (int)choices, (int)E, bits, (int)seg, (const int32_t*)ws, (int)n, starts, rows);
+  route_place_kernel<<<(unsigned)n, 64 * kPlaceWaves, 0, st>>>(ids, (int)choices, (int)E, bits, (int)seg, (const int32_t*)ws, (int)n, starts, rows);
   return check_launch("route_plan");
 }
 

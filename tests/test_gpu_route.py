@@ -110,7 +110,8 @@ def test_strides_and_paths(mlxq, monkeypatch):
 
 
 @pytest.mark.parametrize("n,k,E", [(1, 1, 1), (5, 3, 7), (63, 1, 64), (64, 1, 2), (65, 2, 9), (1023, 2, 33), (1024, 2, 3), (700, 3, 1024), (4099, 8, 60),
-                                   (9000, 8, 128), (70001, 2, 256), (40000, 8, 5)])
+                                   (9000, 8, 128), (70001, 2, 256), (40000, 8, 5), (30001, 5, 1024),
+                                   (300007, 1, 100)])
 @pytest.mark.parametrize("lost", [0.0, 0.25, 1.0])
 def test_plan(mlxq, n, k, E, lost):
     banner("route_plan", n, k, E, lost)
