@@ -502,7 +502,9 @@ inline double mx_tiles(const MxProduct& p, int64_t TM, int64_t TN) {
 //   3 tokens, 4 of 32 experts of 5760 x 2880       32 x 128 17.5; 64 x 128 18.1; 32 x 64 18.3; 16 x 32, 4 groups 27
 //   32 rows, K 4096, 14336 features    32 x 64, 4 groups 9.1; 2 groups 9.8; 64 x 64, 2 groups 10.8
 //   120 / 500 tokens, 4 of 32 experts of 2880 x 2880   64 x 128 44 / 73 (three stages 46 / 74); 128 x 128 53 / 71; 32 x 128 50 / 80; 64 x 64 67 / 112
-//   48 / 256 rows, K 4096, 4096 features           64 x 64, 2 groups 11.6 / 12.1; 1 group 14.7 / 15.1; 64 x 128 18.4 / 18.6
+//   64 / 128 rows, K 4096, 2000 features           16 x 32, 8 groups 6.5 / 9.2; 4 groups 6.8 / 7.5; 32 x 64 8.9 / 9.0; 64 x 64 11.4 / 11.5
+//   256 / 512 rows, K 4096, 1000 features          16 x 32, 4 groups 7.5 / 12.1; 32 x 64 9.0 / 9.2; 64 x 64 11.4 / 11.5
+//   256 rows, K 4096, 4096 features    64 x 64, 2 groups 11.8; 1 group 15.1; 64 x 128, 2 groups 16.1; 32 x 64 16.7
 //   512 rows, K 4096, 4096 features    64 x 128, 2 groups 17.8; 1 group 19.7; 64 x 64 19.9; 128 x 128 28
 //   256 rows, K 4096, 14336 features   64 x 128 27.9; 128 x 128 28.8; 64 x 128, 2 groups 32.8
 //   2048 rows, K 4096, 4096 / 14336 features       128 x 128 37 / 118; 256 x 256 52 / 105
@@ -510,14 +512,12 @@ inline double mx_tiles(const MxProduct& p, int64_t TM, int64_t TN) {
 template <int XF, bool EXACT>
 int mx_product(const MxProduct& p, hipStream_t st) {
   const int64_t rows = p.E ? (p.M + p.E - 1) / p.E : p.M;
-  if (rows <= 16) {
-    const double t = mx_tiles(p, 16, 16);
-    if (t <= 256) return mx_launch_tile<XF, EXACT, 16, 16, 1, 1, 3, 16>(p, st);
-    if (t <= 512) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 8>(p, st);
-    if (t <= 1024) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 4>(p, st);
-    return mx_launch_tile<XF, EXACT, 32, 128, 2, 4, 4, 1>(p, st);
-  }
-  if (rows <= 32 && mx_tiles(p, 32, 64) <= 256) return mx_launch_tile<XF, EXACT, 32, 64, 2, 2, 4, 4>(p, st);
+  const double t = mx_tiles(p, 16, 16);
+  if (t <= 256) return mx_launch_tile<XF, EXACT, 16, 16, 1, 1, 3, 16>(p, st);
+  if (t <= 512) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 8>(p, st);
+  if (t <= 1024) return mx_launch_tile<XF, EXACT, 16, 32, 1, 1, 4, 4>(p, st);
+  if (rows <= 16) return mx_launch_tile<XF, EXACT, 32, 128, 2, 4, 4, 1>(p, st);
+  if (mx_tiles(p, 32, 64) <= 256) return mx_launch_tile<XF, EXACT, 32, 64, 2, 2, 4, 4>(p, st);
   if (mx_tiles(p, 64, 64) <= 256) return mx_launch_tile<XF, EXACT, 64, 64, 2, 2, 4, 2>(p, st);
   if (mx_tiles(p, 64, 128) <= 256) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 2>(p, st);
   const double mid = mx_tiles(p, 128, 128);

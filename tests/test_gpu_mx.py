@@ -92,7 +92,9 @@ SHAPES = [(1, 32, 1), (1, 4096, 16), (2, 96, 17), (7, 160, 33), (15, 2912, 70), 
           (63, 288, 100), (64, 544, 260), (65, 96, 65), (100, 1312, 300), (129, 128, 520), (257, 672, 130), (300, 224, 3000), (1030, 160, 2100),
           # more features than 256 workgroups of the smallest tiles have: every other tile
           (5, 160, 6001), (16, 96, 12010), (11, 288, 20003), (20, 160, 5000), (32, 96, 20010), (100, 160, 12001), (150, 288, 14002), (200, 160, 20001),
-          (3001, 160, 9003), (2100, 800, 12301)]
+          (3001, 160, 9003), (2100, 800, 12301),
+          # groups of waves that split K, with runs of several steps and some without
+          (60, 2912, 1900), (250, 1312, 1000), (100, 2912, 4000), (250, 2912, 3900), (500, 1312, 4000)]
 
 
 @pytest.mark.parametrize("format", ["e2m1", "e4m3"])
