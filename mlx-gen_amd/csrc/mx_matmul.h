@@ -522,9 +522,11 @@ int mx_product(const MxProduct& p, hipStream_t st) {
   if (mx_tiles(p, 64, 128) <= 256) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 3, 2>(p, st);
   const double mid = mx_tiles(p, 128, 128);
   if (mid <= 256 || rows <= 64) return mx_launch_tile<XF, EXACT, 64, 128, 2, 4, 4, 1>(p, st);
-  // One round of the largest tiles takes as long as three quarters of the mid ones' of 1024 (two rounds of two to a CU).  Their
-  // operands as bf16 do not fit the registers (8190 rows, K 4096, 14336 features in f32: 3.5 ms; the mid ones 0.94).
-  if (!EXACT && mid >= 768 * ceil(mx_tiles(p, 256, 256) / 256)) return mx_launch_tile<XF, false, 256, 256, 4, 2, 3, 1>(p, st);
+  // One round of the largest tiles takes a little less than the mid ones' second of 512 (2048 rows, 6000 features: 54 for 56 us);
+  // several take as long as three quarters of 1024 of them each (4096 rows, 6000 features: 105 for 99).  Their operands as bf16 do
+  // not fit the registers (8190 rows, K 4096, 14336 features in f32: 3.5 ms; the mid ones 0.91).
+  const double rounds = ceil(mx_tiles(p, 256, 256) / 256);
+  if (!EXACT && mid >= (rounds > 1 ? 768 * rounds : 513)) return mx_launch_tile<XF, false, 256, 256, 4, 2, 3, 1>(p, st);
   return mx_launch_tile<XF, EXACT, 128, 128, 2, 2, 3, 1>(p, st);
 }
 
