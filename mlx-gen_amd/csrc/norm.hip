@@ -1,7 +1,10 @@
 // norm.hip — root-mean-square norms with the residual's addition, their 8-bit results, and their gradient.
 //
 //   y = h (mean(h^2) + eps)^(-1/2) w,  h = x + residual
-//   dx = r g - r^3 x mean(g x) + dsum,  g = dy w;   dw = sum of dy x r over the rows
+//   dx = r (g - n mean(g n)) + dsum,  n = x r,  g = dy w;   dw = sum of dy n over the rows
+//
+// The gradient is multiplied in this order, mean(g n) being mean(g x) r: r^3 is subnormal from rows of 5e12 on, and infinite below
+// 1e-13 with eps 0, where r, the sums and the result are ordinary numbers.
 //
 // A row is held in registers by 8 to 64 lanes of a wave (short rows: several to a wave), by a workgroup of 256 or by
 // one of 512, in 16-byte pieces, and is read once; the sums take exchanges within a wave and one step through LDS
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
       ds0[i] = ds[i];
     }
     if (first + step < a.rows) load(at + step);
-    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
+    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), mean = s[1] / (float)D * r;
     if (!live) continue;
     const int row = (int)at, t = a.by_heads.div(row), h = row - t * a.heads;
     T* dx = row_of<T>(a.dx, t, h);
@@ -337,9 +340,9 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_grad_kerne
       float f[C];
 #pragma unroll
       for (int e = 0; e < C; ++e) {
-        const float xv = Elem<T>::get(x0[i], e), g = Elem<T>::get(dy0[i], e);
-        f[e] = r * (g * w[i][e]) - c * xv;
-        dw[i][e] = fmaf(g, xv * r, dw[i][e]);
+        const float n = Elem<T>::get(x0[i], e) * r, g = Elem<T>::get(dy0[i], e);
+        f[e] = r * fmaf(-n, mean, g * w[i][e]);
+        dw[i][e] = fmaf(g, n, dw[i][e]);
       }
       if (a.dsum.p) {
         set_right<T>(ds0[i], e0, D);
@@ -410,7 +413,7 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a
       }
     }
     row_sum<LANES>(s, slot[turn]);
-    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), c = r * r * r * (s[1] / (float)D);
+    const float r = 1.0f / sqrtf(s[0] / (float)D + a.eps), mean = s[1] / (float)D * r;
 #pragma unroll 2
     for (int e0 = e_first; e0 < D; e0 += LANES * C) {
       u32x4 xv[1], g[1], d[1] = {u32x4{0, 0, 0, 0}};
@@ -424,9 +427,9 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a
       if (ds) set_right<T>(d[0], e0, D);
 #pragma unroll
       for (int e = 0; e < C; ++e) {
-        const float v = Elem<T>::get(xv[0], e), gv = Elem<T>::get(g[0], e);
-        f[e] = r * (gv * w[e]) - c * v;
-        dw[e0 + e] = fmaf(gv, v * r, dw[e0 + e]);
+        const float n = Elem<T>::get(xv[0], e) * r, gv = Elem<T>::get(g[0], e);
+        f[e] = r * fmaf(-n, mean, gv * w[e]);
+        dw[e0 + e] = fmaf(gv, n, dw[e0 + e]);
         if (ds) f[e] += Elem<T>::get(d[0], e);
       }
       store_piece(dx, e0, D, pack_chunk<T>(f));
