@@ -204,9 +204,14 @@ __device__ __forceinline__ float exp_of(float x) {
   return e > 0.0f ? fmaf(e, lost * 0.693147180559945f, e) : e;  // -infinity: 0, and lost is no number
 }
 
-// dz from dw, with p the scores of a token and w = scale p / (their sum over the chosen, or 1):
-//   softmax: dz = p (up - sum up p),  sigmoid: dz = up p (1 - p),  up_j = scale (dw_j - sum dw w / scale) / sum,
-// up being 0 for experts that were not chosen.  Lane j < k works out its choice's up; scores and ups change lanes in LDS.
+// dz from dw, with s the scores of a token and w = scale s / (their sum over the chosen, or 1), d = scale dw:
+//   not normalized: softmax dz = s (d - sum d s), d being 0 for experts that were not chosen; sigmoid dz = d s (1 - s)
+//   normalized: the chosen experts alone, with their shares v = s / (sum of s): dz = v (d - sum d v), times 1 - s of a sigmoid
+// Lane j < k works out its choice; logits and results change lanes in LDS.
+//
+// Shares are ordinary numbers where scores leave f32's range (experts chosen by a bias, some 87 below the row's largest logit or
+// below 0), so the exponentials are taken relative to the largest chosen logit: a sigmoid of z < 0 is exp(z) (1 - s).  Where the
+// weights' scores are all 0 in the router's 64 bits, so are weights and gradient.
 template <typename T, int NE>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const float* __restrict__ dweights, T* __restrict__ dz) {
   __shared__ float swap[4][NE * 64];
@@ -214,61 +219,77 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const floa
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;  // whole waves; no barrier below
   float* mine = swap[threadIdx.x >> 6];
-  float p[NE], q[NE];  // q: 1 - p of a sigmoid
+  float z[NE];  // of a softmax without normalization later the scores
   const T* row = (const T*)a.logits + t * a.row_stride;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) p[i] = Act<T>::ld(row, min(i * 64 + lane, E - 1));
+  for (int i = 0; i < NE; ++i) z[i] = Act<T>::ld(row, min(i * 64 + lane, E - 1));
   const int64_t at = (int64_t)t * a.k + min(lane, a.k - 1);
-  int id = a.ids[at];
+  const int id = a.ids[at];
   float up = dweights[at] * a.scale;
   const bool chosen = lane < a.k && (unsigned)id < (unsigned)E;
-  const bool soft = a.scoring == MLXQ_ROUTE_SOFTMAX;
-  if (soft) {
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) top = fmaxf(top, p[i]);  // the last logit again past the end
-    top = lanes_reduce(top, [](float u, float v) { return fmaxf(u, v); });
-    if (top == -INFINITY) top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      p[i] = i * 64 + lane < E ? exp_of(p[i] - top) : 0.0f;
-      sum += p[i];
-    }
-    sum = wave_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) p[i] *= inv;
-  } else {
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const float e = exp_of(-fabsf(p[i])), big = 1.0f / (1.0f + e), small = e * big;
-      q[i] = p[i] >= 0.0f ? small : big;
-      p[i] = p[i] >= 0.0f ? big : small;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = p[i];
-  __builtin_amdgcn_wave_barrier();
-  const float pj = chosen ? mine[id] : 0.0f;
   if (!chosen) up = 0.0f;
-  float dot = wave_sum(up * pj);
-  if (a.normalize) {
-    const float sum = wave_sum(pj), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    up = (up - dot * inv) * inv;
-    dot = 0.0f;  // the mean of these ups under p
-  }
+  const bool soft = a.scoring == MLXQ_ROUTE_SOFTMAX;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = z[i];
+  __builtin_amdgcn_wave_barrier();
+  const float zj = chosen ? mine[id] : -INFINITY;
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int i = 0; i < NE; ++i) mine[i * 64 + lane] = 0.0f;
   __builtin_amdgcn_wave_barrier();
-  if (chosen) mine[id] = up;
+  const auto larger = [](float u, float v) { return fmaxf(u, v); };  // of a number and NaN the number
+  float top = -INFINITY;
+  bool undefined = false;  // softmax of a row with NaN or +infinity
+  if (soft) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      top = fmaxf(top, z[i]);  // the last logit again past the end
+      undefined |= !(z[i] < INFINITY);
+    }
+    top = lanes_reduce(top, larger);
+    if (top == -INFINITY) top = 0.0f;
+    undefined = __any(undefined);
+  }
+  float dot = 0.0f, dj;  // dj: dz of a chosen expert, or of a softmax without normalization d
+  if (a.normalize) {
+    const float most = lanes_reduce(zj, larger);
+    float v, q = 1.0f;
+    if (soft) {
+      v = exp_of(zj - (top - most <= 745.13f ? most : top));
+    } else {
+      const float e = exp_of(-fabsf(zj)), big = 1.0f / (1.0f + e), small = e * big;
+      q = zj >= 0.0f ? small : big;
+      v = most < 0.0f && most >= -709.78f ? exp_of(zj - most) * q : zj >= 0.0f ? big : small;
+    }
+    if (!chosen) v = 0.0f;
+    const float sum = wave_sum(v);
+    v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    dj = v * (up - wave_sum(up * v)) * q;
+  } else if (soft) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      z[i] = i * 64 + lane < E ? exp_of(z[i] - top) : 0.0f;
+      sum += z[i];
+    }
+    sum = wave_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) z[i] *= inv;
+    dot = wave_sum(chosen ? up * (exp_of(zj - top) * inv) : 0.0f);
+    dj = up;
+  } else {
+    const float e = exp_of(-fabsf(zj)), big = 1.0f / (1.0f + e);
+    dj = up * big * (e * big);
+  }
+  if (chosen) mine[id] = dj;
   __builtin_amdgcn_wave_barrier();
   T* out = dz + (int64_t)t * E;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = i * 64 + lane;
-    const float u = mine[e];
-    if (e < E) Act<T>::st(out, e, soft ? p[i] * (u - dot) : u * p[i] * q[i]);
+    const float v = mine[e];
+    if (e < E) Act<T>::st(out, e, undefined ? NAN : soft && !a.normalize ? z[i] * (v - dot) : v);
   }
 }
 
