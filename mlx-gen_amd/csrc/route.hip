@@ -240,6 +240,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const floa
   const auto larger = [](float u, float v) { return fmaxf(u, v); };  // of a number and NaN the number
   float top = -INFINITY;
   bool undefined = false;  // softmax of a row with NaN or +infinity
+  // A token without an expert, as of a padded batch, passes nothing on, whatever its logits hold.
+  const bool none = !__any(chosen);
   if (soft) {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a, const floa
   for (int i = 0; i < NE; ++i) {
     const int e = i * 64 + lane;
     const float v = mine[e];
-    if (e < E) Act<T>::st(out, e, undefined ? NAN : soft && !a.normalize ? z[i] * (v - dot) : v);
+    if (e < E) Act<T>::st(out, e, none ? 0.0f : undefined ? NAN : soft && !a.normalize ? z[i] * (v - dot) : v);
   }
 }
 

@@ -113,3 +113,26 @@ def test_no_weight_has_no_gradient(mlxq):
         r = mlxq.route_experts(z.cuda(), 4, scoring, bias=bias.cuda())
         assert (r.ids.sort(-1).values.cpu() == ids).all() and not r.weights.any()
         assert not mlxq.route_experts_backward(torch.randn(4, 4).cuda(), z.cuda(), ids.cuda(), scoring).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_tokens_without_an_expert_pass_nothing_on(mlxq, dtype, scoring, normalize):
+    """Rows of a padded batch may hold anything; so may the logits of experts that a sigmoid's token did not choose."""
+    z = _randn(1, 8, 96).to(dtype)
+    z[1], z[2, 5], z[3], z[4, 70] = float("nan"), float("nan"), float("inf"), float("inf")
+    active = torch.tensor([True, False, False, False, False, True, True, True])
+    r = mlxq.route_experts(z.cuda(), 4, scoring, normalize=normalize, active=active.cuda())
+    dw = _randn(2, 8, 4)
+    dw[1] = float("nan")
+    got = mlxq.route_experts_backward(dw.cuda(), z.cuda(), r.ids, scoring, normalize).cpu()
+    assert not got[~active].any() and got.isfinite().all() and got[active].any(-1).all()
+    alone = mlxq.route_experts_backward(dw[active].cuda(), z[active].cuda(), r.ids[active.cuda()], scoring, normalize).cpu()
+    assert torch.equal(got[active], alone)
+    if scoring == "sigmoid":
+        ids = torch.tensor([[3, 9, 40, 95]], dtype=torch.int32)
+        y = z[5:6].clone()
+        y[0, 7], y[0, 50] = float("nan"), float("inf")
+        clean = mlxq.route_experts_backward(dw[5:6].cuda(), z[5:6].cuda(), ids.cuda(), scoring, normalize)
+        assert torch.equal(mlxq.route_experts_backward(dw[5:6].cuda(), y.cuda(), ids.cuda(), scoring, normalize), clean)
