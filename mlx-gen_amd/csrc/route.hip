@@ -100,6 +100,9 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     const double e = exp((double)v - top64);
     return WIDE || !a.normalize ? (total > 0.0 ? e / total : 0.0) : e;
   };
+  // A softmax's row with NaN or +infinity has no scores: the choice goes by its logits alone, without the bias and a group by its
+  // best, so that NaN still comes last.
+  const bool alone = soft && undefined;
   Val val[NE];
   Key key[NE];
   double own[WIDE ? NE : 1];  // scores
@@ -110,6 +113,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
       // A group's score without a bias is of scores; the choice then goes by the logits, whose order is theirs.
       val[i] = own[i] = e < E ? score(z[i]) : 0.0;
       if (a.bias) val[i] += e < E ? (double)a.bias[e] : 0.0;
+      if (alone) val[i] = z[i];
       key[i] = e < E ? a.bias ? key_of(val[i]) : (Key)key_of(z[i]) : 0;
     } else {
       val[i] = z[i];
@@ -137,7 +141,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
           if (low > next) next = low;
         }
       }
-    Key gk = lane < a.groups ? key_of(a.best > 1 && size > 1 ? best + next : best) : 0;
+    Key gk = lane < a.groups ? key_of(a.best > 1 && size > 1 && !alone ? best + next : best) : 0;
     unsigned long long kept = 0;
     for (int j = 0; j < a.kept; ++j) {
       unsigned long long lanes;

@@ -136,3 +136,48 @@ def test_tokens_without_an_expert_pass_nothing_on(mlxq, dtype, scoring, normaliz
         y[0, 7], y[0, 50] = float("nan"), float("inf")
         clean = mlxq.route_experts_backward(dw[5:6].cuda(), z[5:6].cuda(), ids.cuda(), scoring, normalize)
         assert torch.equal(mlxq.route_experts_backward(dw[5:6].cuda(), y.cuda(), ids.cuda(), scoring, normalize), clean)
+
+
+def _undefined_choice(zt, k, groups, kept):
+    """The choice of a softmax's row that holds a NaN or +infinity: by its logits alone, NaN last, a group by its best."""
+    E = len(zt)
+    size = E // groups
+    low = [v if v == v else float("-inf") for v in zt]
+    best = [max(low[g * size:(g + 1) * size]) for g in range(groups)]
+    keep = sorted(range(groups), key=lambda g: (-best[g], g))[:kept] if kept < groups else range(groups)
+    allowed = [e for e in range(E) if e // size in keep]
+    return sorted(allowed, key=lambda e: (zt[e] != zt[e], -low[e], e))[:k]
+
+
+@pytest.mark.parametrize("best", [1, 2])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_choice_of_undefined_rows(mlxq, scoring, biased, best):
+    """NaN logits come after all others, with a bias and in groups too; other rows are as ever."""
+    E = 48
+    z = _randn(4, 14, E)
+    z[1, 7] = float("nan")
+    z[2, 9] = float("inf")
+    z[3, 4:] = float("nan")
+    z[4] = float("nan")
+    z[5, ::2] = float("nan")
+    z[6, 3], z[6, 30] = float("inf"), float("nan")
+    z[7, 40:] = float("inf")
+    z[8, :30], z[8, 40] = float("-inf"), float("nan")
+    bias = 2 * _randn(5, E) if biased else None
+    if biased:
+        bias[7], bias[9] = 50.0, -50.0
+    for groups, kept in ((1, 1), (4, 2), (8, 3)):
+        for k in (1, 5, 12):
+            got = mlxq.route_experts(z.cuda(), k, scoring, bias=None if bias is None else bias.cuda(), groups=groups, kept_groups=kept, group_best=best)
+            ids, w = ref.route(z, k, scoring, bias=bias, groups=groups, kept=kept, best=best)
+            if scoring == "softmax":
+                for t in range(14):
+                    if not bool((z[t] < float("inf")).all()):
+                        ids[t] = torch.tensor(_undefined_choice(z[t].tolist(), k, groups, kept), dtype=torch.int32)
+            banner("route_experts", scoring, biased, best, groups, kept, k)
+            assert torch.equal(got.ids.cpu(), ids)
+            g = got.weights.cpu().double()
+            assert torch.equal(g.isnan(), w.isnan()) and ((g - w).abs() <= (2.0 ** -24 + 2.0 ** -40) * w.abs() + 2.0 ** -149)[~w.isnan()].all()
+            starts, rows = ref.plan(ids, E)
+            assert torch.equal(got.starts.cpu(), starts) and torch.equal(got.rows.cpu(), rows)
