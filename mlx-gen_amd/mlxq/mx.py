@@ -191,13 +191,15 @@ def _rows(op, what, t, like=None):
         _bad(op, f"{what} must have a last dimension")
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
         _bad(op, f"{what} must be {like.dtype} of {tuple(like.shape)} on {like.device}, got {t.dtype} of {tuple(t.shape)} on {t.device}")
+    if t.numel() == 0:  # nothing is read, whichever dimension is empty
+        return t, (0, t.shape[-2] if t.dim() > 2 else 1, 0, 0)
     for turn in range(2):
-        if t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1:
+        if t.shape[-1] == 1 or t.stride(-1) == 1:
             if t.dim() <= 2:
                 return t, (t.shape[0] if t.dim() == 2 else 1, 1, t.stride(0) if t.dim() == 2 else t.shape[-1], 0)
             stride = _row_stride(t[..., 0, :])
             if stride is not None:
-                tokens = t.numel() // max(t.shape[-1] * t.shape[-2], 1)
+                tokens = t.numel() // (t.shape[-1] * t.shape[-2])
                 return t, (tokens, t.shape[-2], stride if t.dim() > 2 else 0, t.stride(-2))
         t = t.contiguous()
     raise AssertionError(f"{op}: no strides for {what}")
