@@ -9,7 +9,7 @@ int run_mx_product_e2m1(const MxProduct& p, hipStream_t st);
 
 int run_mx_product(const MxProduct& p, int format, hipStream_t st) {
   if (format == kE2M1) return run_mx_product_e2m1(p, st);
-  return p.y_dtype == MLXQ_FLOAT32 ? run_mx_product_e4m3_f32(p, st) : run_mx_product_e4m3(p, st);
+  return p.y_dtype == MLXQ_BFLOAT16 ? run_mx_product_e4m3(p, st) : run_mx_product_e4m3_f32(p, st);
 }
 
 namespace {

@@ -1,4 +1,4 @@
-// mx_matmul_e4m3.hip — products with 8-bit activations, 16-bit results (mx_matmul.h).
+// mx_matmul_e4m3.hip — products with 8-bit activations, bf16 results (mx_matmul.h).
 #include "mx_matmul.h"
 
 namespace mlxq {

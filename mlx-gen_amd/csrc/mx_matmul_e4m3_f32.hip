@@ -1,4 +1,4 @@
-// mx_matmul_e4m3_f32.hip — products with 8-bit activations, f32 results (mx_matmul.h).
+// mx_matmul_e4m3_f32.hip — products with 8-bit activations, f32 and fp16 results (mx_matmul.h).
 #include "mx_matmul.h"
 
 namespace mlxq {
