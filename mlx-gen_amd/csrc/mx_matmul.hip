@@ -20,8 +20,8 @@ namespace {
 template <typename T>
 __global__ __launch_bounds__(256) void mx_combine_kernel(const T* __restrict__ y, const int32_t* __restrict__ ids,
                                                          const float* __restrict__ weights, int k, int E, int N, int units,
-                                                         int64_t total, T* __restrict__ out) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                         int64_t first, int64_t total, T* __restrict__ out) {
+  const int64_t u = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= total) return;
   const int64_t t = u / units;
   const int n = (int)(u - t * units) * 4, count = min(4, N - n);
@@ -51,9 +51,9 @@ template <typename T>
 int combine(const void* y, const int32_t* ids, const float* weights, int64_t T_, int64_t k, int64_t E, int64_t N, void* out,
             hipStream_t st) {
   const int64_t units = (N + 3) / 4, total = T_ * units;
-  mx_combine_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, st>>>((const T*)y, ids, weights, (int)k, (int)E, (int)N, (int)units,
-                                                                      total, (T*)out);
-  return check_launch("mx_experts");
+  return in_launches("mx_experts", (total + 255) / 256, 256, [&](int64_t group, unsigned grid) {
+    mx_combine_kernel<T><<<grid, 256, 0, st>>>((const T*)y, ids, weights, (int)k, (int)E, (int)N, (int)units, group * 256, total, (T*)out);
+  });
 }
 
 }  // namespace

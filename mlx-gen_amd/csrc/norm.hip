@@ -149,7 +149,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_kernel(Nor
   using Sum = typename std::conditional<MX, double, float>::type;
   __shared__ Sum slot[TW];
   const int lane = threadIdx.x % LANES, D = a.D;
-  const int64_t at = (int64_t)blockIdx.x * R + threadIdx.x / LANES;
+  const int64_t at = a.first + (int64_t)blockIdx.x * R + threadIdx.x / LANES;
   const bool live = at < a.rows;
   const int row = (int)(live ? at : a.rows - 1);
   const int t = a.by_heads.div(row), h = row - t * a.heads;
@@ -485,12 +485,17 @@ template <typename T>
 int norm(const NormArgs& a, hipStream_t st) {
   return by_pieces((a.D + kC<T> - 1) / kC<T>, [&](auto lanes, auto ch) {
     constexpr int LANES = decltype(lanes)::value, CH = decltype(ch)::value, R = LANES > 256 ? 1 : 256 / LANES;
+    int rc = MLXQ_OK;
     if constexpr (LANES * CH * kC<T> <= 32768) {
-      const unsigned grid = (unsigned)((a.rows + R - 1) / R), threads = LANES > 256 ? LANES : 256;
-      if (a.mx.codes) rms_norm_kernel<T, LANES, CH, true><<<grid, threads, 0, st>>>(a);
-      else rms_norm_kernel<T, LANES, CH, false><<<grid, threads, 0, st>>>(a);
+      constexpr int threads = LANES > 256 ? LANES : 256;
+      NormArgs part = a;
+      rc = in_launches("rms_norm", (a.rows + R - 1) / R, threads, [&](int64_t group, unsigned grid) {
+        part.first = group * R;
+        if (a.mx.codes) rms_norm_kernel<T, LANES, CH, true><<<grid, threads, 0, st>>>(part);
+        else rms_norm_kernel<T, LANES, CH, false><<<grid, threads, 0, st>>>(part);
+      });
     }
-    return check_launch("rms_norm");
+    return rc;
   });
 }
 

@@ -488,22 +488,39 @@ int by_experts(int E, F&& f) {
   return f(std::integral_constant<int, 16>{});
 }
 
+// Four tokens a workgroup; those from the launch's first on.
+template <typename T, typename F>
+int by_tokens(const char* what, const RouteArgs& a, F&& launch) {
+  return in_launches(what, ((int64_t)a.T + 3) / 4, 256, [&](int64_t group, unsigned grid) {
+    const int64_t t = group * 4;
+    RouteArgs part = a;
+    part.logits = (const T*)a.logits + t * a.row_stride;
+    part.T = (int)(a.T - t);
+    part.ids += t * a.k;
+    if (a.weights) part.weights += t * a.k;
+    if (a.active) part.active += t;
+    launch(part, t, grid);
+  });
+}
+
 template <typename T>
 int route(const RouteArgs& a, hipStream_t st) {
   return by_experts(a.E, [&](auto n) {
     constexpr int NE = decltype(n)::value;
-    const unsigned grid = (unsigned)((a.T + 3) / 4);
-    if (a.bias || (a.kept < a.groups && a.best > 1)) route_kernel<T, NE, true><<<grid, 256, 0, st>>>(a);
-    else route_kernel<T, NE, false><<<grid, 256, 0, st>>>(a);
-    return check_launch("route_experts");
+    const bool wide = a.bias || (a.kept < a.groups && a.best > 1);
+    return by_tokens<T>("route_experts", a, [&](const RouteArgs& part, int64_t, unsigned grid) {
+      if (wide) route_kernel<T, NE, true><<<grid, 256, 0, st>>>(part);
+      else route_kernel<T, NE, false><<<grid, 256, 0, st>>>(part);
+    });
   });
 }
 
 template <typename T>
 int route_backward(const RouteArgs& a, const float* dweights, void* dz, hipStream_t st) {
   return by_experts(a.E, [&](auto n) {
-    route_grad_kernel<T, decltype(n)::value><<<(unsigned)((a.T + 3) / 4), 256, 0, st>>>(a, dweights, (T*)dz);
-    return check_launch("route_experts_backward");
+    return by_tokens<T>("route_experts_backward", a, [&](const RouteArgs& part, int64_t t, unsigned grid) {
+      route_grad_kernel<T, decltype(n)::value><<<grid, 256, 0, st>>>(part, dweights + t * a.k, (T*)dz + t * a.E);
+    });
   });
 }
 

@@ -32,3 +32,69 @@ def test_no_heads(mlxq, shape):
     assert mlxq.mx_dequantize(mlxq.mx_quantize(x)).shape == shape
     few = mlxq.mx_quantize(torch.randn(5, shape[-1], device="cuda"))
     assert mlxq.mx_matmul(mlxq.mx_quantize(x, "e4m3"), few).shape == (*shape[:-1], 5)
+
+
+def test_norm_of_more_rows_than_a_launch_has_threads_for(mlxq):
+    """2^29 rows of 8 lanes are 2^32 threads: rows at both ends and around the border."""
+    rows = 2 ** 29 + 1000
+    x = torch.randn(rows, 1, device="cuda", generator=torch.Generator("cuda").manual_seed(1), dtype=BF16)
+    banner("rms_norm", rows)
+    y = torch.empty_like(x)
+    for part in range(2):  # y holds what no norm gives, so that rows left out show
+        y.fill_(7.0)
+        del y
+        y = mlxq.rms_norm(x)
+    border = 16777215 * 32
+    for a, b in ((0, 1000), (border - 1000, border + 1000), (2 ** 29 - 1000, 2 ** 29), (rows - 1000, rows)):
+        want = ref.rms_norm(x[a:b].cpu(), None, 1e-6)
+        assert ((y[a:b].cpu().double() - want).abs() <= (96 * 2.0 ** -24 + 2.0 ** -8) * want.abs() + 2.0 ** -134).all()
+    # every row: signs survive, and no magnitude passes 1
+    assert bool((torch.sign(y) == torch.sign(x)).all()) and bool((y.abs() <= 1).all())
+
+
+def test_routing_of_more_tokens_than_a_launch_has_threads_for(mlxq):
+    """2^26 tokens, a wave each."""
+    T, E = 2 ** 26 + 9, 4
+    z = torch.randn(T, E, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    active = torch.ones(T, dtype=torch.bool, device="cuda")
+    active[-3], active[5] = False, False
+    banner("route_experts", T, E)
+    r = mlxq.route_experts(z, 1, normalize=False, active=active)
+    none = r.ids[:, 0] < 0
+    assert torch.equal(none, ~active)
+    top = z.amax(-1)
+    at = torch.where(none, 0, r.ids[:, 0]).long()
+    assert bool(((z.gather(1, at[:, None])[:, 0] == top) | none).all())
+    counts = torch.stack([(r.ids == e).sum() for e in range(E)])
+    assert torch.equal(r.starts.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+    key = torch.where(none, E, r.ids[:, 0])[r.rows.long()]
+    assert bool((key[1:] >= key[:-1]).all()) and bool(((r.rows[1:] > r.rows[:-1]) | (key[1:] > key[:-1])).all())
+    del key, at, top
+    dw = torch.randn(T, 1, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    dz = mlxq.route_experts_backward(dw, z, r.ids, normalize=False)
+    border = 16777215 * 4
+    for a, b in ((0, 100), (border - 100, border + 100), (T - 200, T)):
+        zc, ids = z[a:b].cpu(), r.ids[a:b].cpu()
+        want, w = ref.route(zc, 1, normalize=False, active=active[a:b].cpu())
+        assert torch.equal(ids, want) and ((r.weights[a:b].cpu().double() - w).abs() <= 2.0 ** -23 * w).all()
+        want, mag = ref.route_gradient(dw[a:b].cpu(), zc, ids, "softmax", False, 1.0)
+        assert ((dz[a:b].cpu().double() - want).abs() <= 64 * 2.0 ** -24 * mag + 2.0 ** -24 * want.abs() + 2.0 ** -150).all()
+
+
+def test_experts_sums_of_more_features_than_a_launch_has_threads_for(mlxq):
+    """2^34 results, four a thread."""
+    T, K, N = 1048400, 32, 16388
+    x, w = ref.random_mx(1, (T,), K, "e2m1", device="cuda"), ref.random_mx(2, (1, N), K, "e2m1", device="cuda")
+    weights = torch.rand(T, 1, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    routing = mlxq.route_plan(torch.zeros(T, 1, dtype=torch.int32, device="cuda"), weights, 1)
+    banner("mx_experts", T, K, N)
+    y = mlxq.mx_experts(mlxq.Mx(*x), mlxq.Mx(*w), routing, combine=True)
+    wv = ref.values(w)[0]
+    border = 16777215 * 256 // 4097
+    for rows in (slice(0, 20), slice(border - 10, border + 10), slice(T - 20, T)):
+        xv, s = ref.values((x[0][rows], x[1][rows])), weights[rows].cpu().double()
+        want = xv @ wv.t()
+        tol = ref.product_bound(xv, wv, BF16, "e2m1")
+        assert ((y[rows].cpu().double() - want * s).abs() <= tol * s + 2.0 ** -8 * (want.abs() + tol) * s * (1 + 2.0 ** -20) + 2.0 ** -133).all()
+    del y
+    torch.cuda.empty_cache()
