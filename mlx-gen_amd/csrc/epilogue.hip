@@ -322,7 +322,7 @@ static int lora_prep_f32(const void* x, int64_t M, int64_t K, const void* A, con
                          int R, void* xa, void* lbt, hipStream_t st) {
   const auto aligned = [](const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; };
   const int64_t xa_blocks = (M + 15) / 16, bt_blocks = (N * (R / 8) + kXaWaves * 64 - 1) / (kXaWaves * 64);
-  if (K % 16 == 0 && aligned(x, 4 * sizeof(XT)) && K < (1LL << 31) && xa_blocks + bt_blocks < (1LL << 31)) {
+  if (K % 16 == 0 && aligned(x, 4 * sizeof(XT)) && K < (1LL << 31) && xa_blocks + bt_blocks <= most_groups(kXaWaves * 64)) {
 #define MLXQ_XA(C)                                                                                               \
   hipLaunchKernelGGL((lora_xa_f32_kernel<XT, FT, C>), dim3((unsigned)(xa_blocks + bt_blocks), (unsigned)((R + 16 * C - 1) / (16 * C))), \
                      dim3(kXaWaves * 64), 0, st, (const XT*)x, M, K, (const FT*)A, (const FT*)B, N, rank, R,     \
@@ -334,7 +334,7 @@ static int lora_prep_f32(const void* x, int64_t M, int64_t K, const void* A, con
     return check_launch("lora_prep");
   }
   const int64_t blocks = (M * R + N * R + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "lora: problem too large");
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "lora: problem too large");
   hipLaunchKernelGGL((lora_prep_f32_kernel<XT, FT>), dim3((unsigned)blocks), dim3(256), 0, st, (const XT*)x, M, K,
                      (const FT*)A, (const FT*)B, N, rank, R, (float*)xa, (float*)lbt);
   return check_launch("lora_prep");
@@ -345,7 +345,7 @@ int run_lora_prep(const void* x, int x_dtype, int64_t M, int64_t K, const void* 
   const int64_t total = M * R + N * R;
   if (total == 0) return MLXQ_OK;
   const int64_t blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "lora: problem too large");
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "lora: problem too large");
   if (x_dtype != MLXQ_BFLOAT16 || lora_dtype != MLXQ_BFLOAT16) {
     const bool fb = lora_dtype == MLXQ_BFLOAT16;
     if (x_dtype == MLXQ_FLOAT16)
@@ -356,7 +356,7 @@ int run_lora_prep(const void* x, int x_dtype, int64_t M, int64_t K, const void* 
               : lora_prep_f32<float, float>(x, M, K, A, B, N, rank, R, xa, lbt, st);
   }
   const int64_t bt_blocks = (N * R + kXaWaves * 64 - 1) / (kXaWaves * 64);
-  if (K % 32 == 0 && M < (1LL << 31) / 16 && K < (1LL << 31) && bt_blocks < (1LL << 30)) {
+  if (K % 32 == 0 && K < (1LL << 31) && (M + 15) / 16 + bt_blocks <= most_groups(kXaWaves * 64)) {
     // x.A workgroups (`rows` rows x 16 columns each), then the B^T workgroups.
     const int rows = M > 16 * 256 && M <= 32 * 256 ? (int)((M + 255) / 256) : 16;
     const int xa_blocks = (int)((M + rows - 1) / rows);
@@ -413,8 +413,8 @@ __device__ __forceinline__ float epilogue_finish(const LinearEpilogueArgs& a, fl
 
 // Without LoRA (R == 0): one thread per output.
 template <typename YI, typename YO>
-__global__ void linear_epilogue_kernel(LinearEpilogueArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+__global__ void linear_epilogue_kernel(LinearEpilogueArgs a, int64_t first) {
+  const int64_t t = first + (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= a.M * a.N) return;
   const float o = Act<YI>::ld(static_cast<const YI*>(a.y_in), t);
   Act<YO>::st(static_cast<YO*>(a.y_out), t, epilogue_finish(a, o, t % a.N, a.res != nullptr, a.res ? a.res[t] : 0.0f));
@@ -524,8 +524,6 @@ static int lora_epilogue_split(int64_t tiles) { return tiles <= 64 ? 16 : tiles 
 int run_linear_epilogue(const LinearEpilogueArgs& a, hipStream_t st) {
   const int64_t total = a.M * a.N;
   if (total == 0) return MLXQ_OK;
-  const int64_t blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "linear epilogue: problem too large");
   const bool table_act = a.act == MLXQ_ACT_GELU_TANH || a.act == MLXQ_ACT_GELU_EXACT;
   if (table_act && a.d2_bf16 && a.act_table == nullptr)
     return set_error(MLXQ_EINVAL, "linear epilogue: activation table missing");
@@ -533,6 +531,7 @@ int run_linear_epilogue(const LinearEpilogueArgs& a, hipStream_t st) {
   if (a.R > 0) {
     const int64_t tiles_n = (a.N + 63) / 64, tiles = (a.M + 31) / 32 * tiles_n;
     const int split = lora_epilogue_split(tiles);
+    if ((tiles * split + 3) / 4 > most_groups(256)) return set_error(MLXQ_EINVAL, "linear epilogue: problem too large");
     const dim3 g((unsigned)((tiles * split + 3) / 4));
 #define MLXQ_LES(YI, YO, S)                                                                             \
   do {                                                                                                  \
@@ -553,12 +552,14 @@ int run_linear_epilogue(const LinearEpilogueArgs& a, hipStream_t st) {
 #undef MLXQ_LES
     return check_launch("linear_epilogue");
   }
-  const dim3 g((unsigned)blocks);
-  if (a.y_in_bf16 && a.y_out_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<uint16_t, uint16_t>), g, b, 0, st, a);
-  else if (a.y_in_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<uint16_t, float>), g, b, 0, st, a);
-  else if (a.y_out_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<float, uint16_t>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((linear_epilogue_kernel<float, float>), g, b, 0, st, a);
-  return check_launch("linear_epilogue");
+  return in_launches("linear_epilogue", (total + 255) / 256, 256, [&](int64_t group, unsigned blocks) {
+    const dim3 g(blocks);
+    const int64_t first = group * 256;
+    if (a.y_in_bf16 && a.y_out_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<uint16_t, uint16_t>), g, b, 0, st, a, first);
+    else if (a.y_in_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<uint16_t, float>), g, b, 0, st, a, first);
+    else if (a.y_out_bf16) hipLaunchKernelGGL((linear_epilogue_kernel<float, uint16_t>), g, b, 0, st, a, first);
+    else hipLaunchKernelGGL((linear_epilogue_kernel<float, float>), g, b, 0, st, a, first);
+  });
 }
 
 // dst[i] = src[i] converted between f32 and bf16 (round to nearest even) or copied.
@@ -570,18 +571,20 @@ __global__ void cast_kernel(const ST* __restrict__ src, DT* __restrict__ dst, in
 
 int run_cast(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n, hipStream_t st) {
   if (n == 0) return MLXQ_OK;
-  const int64_t blocks = (n + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "cast: %lld elements is too many", (long long)n);
-  const dim3 g((unsigned)blocks), b(256);
-  if (src_dtype == MLXQ_BFLOAT16 && dst_dtype == MLXQ_BFLOAT16)
-    hipLaunchKernelGGL((cast_kernel<uint16_t, uint16_t>), g, b, 0, st, (const uint16_t*)src, (uint16_t*)dst, n);
-  else if (src_dtype == MLXQ_BFLOAT16)
-    hipLaunchKernelGGL((cast_kernel<uint16_t, float>), g, b, 0, st, (const uint16_t*)src, (float*)dst, n);
-  else if (dst_dtype == MLXQ_BFLOAT16)
-    hipLaunchKernelGGL((cast_kernel<float, uint16_t>), g, b, 0, st, (const float*)src, (uint16_t*)dst, n);
-  else
-    hipLaunchKernelGGL((cast_kernel<float, float>), g, b, 0, st, (const float*)src, (float*)dst, n);
-  return check_launch("cast");
+  return in_launches("cast", (n + 255) / 256, 256, [&](int64_t group, unsigned blocks) {
+    const dim3 g(blocks), b(256);
+    const int64_t first = group * 256, left = n - first;
+    const char* from = (const char*)src + first * (src_dtype == MLXQ_BFLOAT16 ? 2 : 4);
+    char* to = (char*)dst + first * (dst_dtype == MLXQ_BFLOAT16 ? 2 : 4);
+    if (src_dtype == MLXQ_BFLOAT16 && dst_dtype == MLXQ_BFLOAT16)
+      hipLaunchKernelGGL((cast_kernel<uint16_t, uint16_t>), g, b, 0, st, (const uint16_t*)from, (uint16_t*)to, left);
+    else if (src_dtype == MLXQ_BFLOAT16)
+      hipLaunchKernelGGL((cast_kernel<uint16_t, float>), g, b, 0, st, (const uint16_t*)from, (float*)to, left);
+    else if (dst_dtype == MLXQ_BFLOAT16)
+      hipLaunchKernelGGL((cast_kernel<float, uint16_t>), g, b, 0, st, (const float*)from, (uint16_t*)to, left);
+    else
+      hipLaunchKernelGGL((cast_kernel<float, float>), g, b, 0, st, (const float*)from, (float*)to, left);
+  });
 }
 
 }  // namespace mlxq

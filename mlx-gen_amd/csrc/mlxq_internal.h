@@ -60,6 +60,20 @@ struct QmmBatch {
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+// Workgroups of a launch, along x: it counts its threads in 32 bits, and of more of them it runs a part without an error.
+constexpr int64_t most_groups(int threads) { return 0xffffffffll / threads; }
+
+// Calls launch(first workgroup, workgroups) until all `groups` of `threads` each are under way.
+template <typename F>
+int in_launches(const char* what, int64_t groups, int threads, F&& launch) {
+  const int64_t most = most_groups(threads);
+  for (int64_t g = 0; g < groups; g += most) {
+    launch(g, (unsigned)(groups - g < most ? groups - g : most));
+    if (int rc = check_launch(what)) return rc;
+  }
+  return MLXQ_OK;
+}
+
 int run_quantize(const void* w, int dtype, int64_t N, int64_t K, int gs, int bits, uint32_t* wq,
                  void* s, void* b, hipStream_t st);
 int run_quantize_batched(const void* const* w, int count, int dtype, int64_t N, int64_t K, int gs, int bits,

@@ -71,18 +71,6 @@ __device__ __forceinline__ V lanes_reduce(V v, F&& f) {
   return v;
 }
 
-// Calls launch(first workgroup, workgroups) until all `groups` of `threads` each are under way: a launch counts its threads in 32
-// bits, and of more of them it runs a part without an error.
-template <typename F>
-int in_launches(const char* what, int64_t groups, int threads, F&& launch) {
-  const int64_t most = 0xffffffffll / threads;
-  for (int64_t g = 0; g < groups; g += most) {
-    launch(g, (unsigned)(groups - g < most ? groups - g : most));
-    if (int rc = check_launch(what)) return rc;
-  }
-  return MLXQ_OK;
-}
-
 // A microscaled matrix as kernels see it.
 struct MxView {
   unsigned char* codes;

@@ -487,7 +487,7 @@ template <int XF, bool EXACT, int TM, int TN, int WM, int WN, int STAGES, int KG
 int mx_launch_tile(const MxProduct& p, hipStream_t st) {
   const int64_t n_tiles = (p.N + TN - 1) / TN, grid = (mx_most_tiles(p, TM) * n_tiles + 7) / 8 * 8;
   constexpr int threads = 64 * WM * WN * KG;
-  if (grid > 0xffffffffll / threads)
+  if (grid > most_groups(threads))
     return set_error(MLXQ_EUNSUPPORTED, "mx product: %lld tiles of %d threads are too many for one launch", (long long)grid, threads);
   mx_tile_kernel<XF, EXACT, TM, TN, WM, WN, STAGES, KG><<<(unsigned)grid, threads, 0, st>>>(p, (int)n_tiles);
   return check_launch("mx product");
