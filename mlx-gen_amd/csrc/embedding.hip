@@ -63,7 +63,7 @@ static int launch_embedding(const int32_t* ids, int64_t T, const uint32_t* wq, c
   const int64_t n = T * (hidden / 8);
   if (n == 0) return MLXQ_OK;
   const int64_t blocks = (n + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "embedding: problem too large");
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "embedding: problem too large");
   hipLaunchKernelGGL((embedding_kernel<SB, OT, BITS, GS>), dim3((unsigned)blocks), dim3(256), 0, st,
                      ids, T, wq, (const SB*)s, (const SB*)b, vocab, hidden, (OT*)out);
   return check_launch("embedding");

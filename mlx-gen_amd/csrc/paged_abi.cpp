@@ -131,14 +131,14 @@ int check_attention(const char* op, int64_t T, int64_t q_heads, const mlxq_paged
   return MLXQ_OK;
 }
 
-// The plan of a checked call, unless its workgroups pass 31 bits.
+// The plan of a checked call, unless its workgroups pass what a launch has.
 int plan_of(const char* op, int64_t T, int64_t q_heads, const mlxq_paged_cache* c, const mlxq_paged_batch* b,
             const mlxq_attention* o, AttnPlan& plan) {
   const int64_t capacity = b->table_width * c->page_size;
   const int64_t max_q = std::min<int64_t>(std::max<int64_t>(b->max_q, 1), 0x3fffffff);
   plan = plan_attention(T, q_heads, c->heads, c->head_dim, c->dtype, b->sequences, max_q,
                         std::min(std::max<int64_t>(b->max_kv, 1), std::max<int64_t>(capacity, 1)), window_of(o), o->causal != 0);
-  if (plan.blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
+  if (plan.blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   return MLXQ_OK;
 }
 
@@ -274,7 +274,7 @@ int mlxq_cache_append(const mlxq_heads* k, const mlxq_heads* v, int64_t T, const
   // A token each: a sequence is a unit.  Else a sequence of n tokens lies in at most n / 16 + 2 blocks.
   a.direct = batch->max_q <= 1;
   const int64_t units = a.direct ? batch->sequences : T / 16 + 2 * std::min(batch->sequences, T);
-  if (units * cache->heads > 0x7fffffff) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
+  if (units * cache->heads > most_groups(256)) return set_error(MLXQ_EINVAL, "%s: problem too large", op);
   return run_cache_append(a, cache->dtype, units, (hipStream_t)stream);
 }
 

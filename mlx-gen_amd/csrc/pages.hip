@@ -75,7 +75,7 @@ int run_copy_pages(void* cache, int64_t planes, int64_t plane_stride, int64_t pa
                    int64_t rows, int64_t width, int64_t table_stride, hipStream_t st) {
   const int64_t pieces = (page_bytes + kPiece - 1) / kPiece, copies = planes * count * pieces;
   const int64_t entries = tables ? rows * width : 0, blocks = copies + (entries + 1023) / 1024;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "copy_pages: problem too large");
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "copy_pages: problem too large");
   if (blocks == 0) return MLXQ_OK;
   hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)blocks), dim3(256), 0, st, (unsigned char*)cache, plane_stride,
                      page_stride, page_bytes, (int)pages, src, dst, count, (int)pieces, copies, tables, entries, width,

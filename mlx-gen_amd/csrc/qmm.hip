@@ -250,7 +250,7 @@ static int launch_qmm(const void* x, int64_t M, int64_t K, const uint32_t* wq, c
                       const void* b, int64_t N, void* y, const QmmEpilogue& epi, hipStream_t st) {
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles == 0) return MLXQ_OK;
-  if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm: problem too large");
+  if (tiles > most_groups(256)) return set_error(MLXQ_EINVAL, "qmm: problem too large");
   if (epi.rank16 != 0 && epi.rank16 != 16)
     return set_error(MLXQ_EINVAL, "qmm: the fused epilogue takes LoRA rank <= 16");
   const bool fused = epi.bias || epi.rank16 || epi.act != kFusedActNone;

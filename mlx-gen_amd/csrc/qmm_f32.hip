@@ -445,7 +445,7 @@ static int launch_qmm_f32(const void* x, int64_t M, int64_t K, const uint32_t* w
   constexpr int WAVES = 8, BN = 256, BK = 32;
   const int64_t tiles = ((M + kF32BM - 1) / kF32BM) * ((N + BN - 1) / BN);
   if (tiles == 0) return MLXQ_OK;
-  if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm_f32: problem too large");
+  if (tiles > most_groups(WAVES * 64)) return set_error(MLXQ_EINVAL, "qmm_f32: problem too large");
   const int gs_log2 = gs == 32 ? 5 : gs == 64 ? 6 : 7;
   if (epi.bias || epi.act != MLXQ_ACT_NONE)
     hipLaunchKernelGGL((qmm_f32_kernel<XT, SB, BITS, WAVES, BN, BK, true>), dim3((unsigned)tiles),
@@ -499,7 +499,7 @@ int run_dense_f32(const void* x, int x_dtype, int64_t M, int64_t K, const void* 
   if (K % BK != 0) return set_error(MLXQ_EINVAL, "dense product: K=%lld is not a multiple of 32", (long long)K);
   const int64_t tiles = ((M + kF32BM - 1) / kF32BM) * ((N + BN - 1) / BN);
   if (tiles == 0) return MLXQ_OK;
-  if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "dense product: problem too large");
+  if (tiles > most_groups(WAVES * 64)) return set_error(MLXQ_EINVAL, "dense product: problem too large");
   const F32Epilogue none{};
 #define MLXQ_D(XT, WT)                                                                                    \
   hipLaunchKernelGGL((qmm_f32_kernel<XT, float, 4, WAVES, BN, BK, false, WT>), dim3((unsigned)tiles), \

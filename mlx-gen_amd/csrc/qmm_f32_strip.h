@@ -652,7 +652,7 @@ static int launch_strip(const void* x, int64_t M, int64_t K, const uint32_t* wq,
                         int64_t N, void* y, const F32Epilogue& epi, hipStream_t st) {
   constexpr int BN = 256 / KS * TN;
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm_f32: problem too large");
+  if (tiles > most_groups(512)) return set_error(MLXQ_EINVAL, "qmm_f32: problem too large");
   hipLaunchKernelGGL((qmm_f32_strip_kernel<XT, SB, BITS, GS, BM, KS, TN>), dim3((unsigned)tiles), dim3(512), 0, st,
                      (const XT*)x, M, K, wq, (const SB*)s, (const SB*)b, N, (float*)y, epi);
   return check_launch("qmm_f32");

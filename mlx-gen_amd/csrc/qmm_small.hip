@@ -382,7 +382,7 @@ static int launch_small(const void* x, int64_t M, int64_t K, const uint32_t* wq,
 bool qmm_small_fits(int64_t M, int64_t K, int64_t N, int gs, int bits, int sb_bytes) {
   const int64_t lim = (int64_t)1 << 32;
   return K % 64 == 0 && M * K * 2 < lim && N * (K * bits / 32) * 4 < lim &&
-         N * (K / gs) * sb_bytes < lim && (M + kTile - 1) / kTile * ((N + kTile - 1) / kTile) < 0x7fffffff;
+         N * (K / gs) * sb_bytes < lim && (M + kTile - 1) / kTile * ((N + kTile - 1) / kTile) <= most_groups(512);
 }
 
 int run_qmm_small(const void* x, int64_t M, int64_t K, const uint32_t* wq, const void* s,

@@ -840,7 +840,7 @@ static int launch_wide(const void* x, int64_t M, int64_t K, const uint32_t* wq, 
   const bool mid = narrow && ((M + kBM - 1) / kBM) * ((N + 127) / 128) * bat.count < 128;
   if (mid) {
     const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm: problem too large");
+    if (tiles > most_groups(256)) return set_error(MLXQ_EINVAL, "qmm: problem too large");
     if constexpr (kBf16) {
       if (szl) return launch_wide_w<SB, BITS, GS, 4, 128, true, 128>(x, M, K, wq, s, b, N, y, epi, st, tiles, bat);
     }
@@ -848,7 +848,7 @@ static int launch_wide(const void* x, int64_t M, int64_t K, const uint32_t* wq, 
   }
   if (narrow) {
     const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + 127) / 128);
-    if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm: problem too large");
+    if (tiles > most_groups(256)) return set_error(MLXQ_EINVAL, "qmm: problem too large");
     if constexpr (kBf16) {
       if (szl) return launch_wide_w<SB, BITS, GS, 4, kBM, true, 128>(x, M, K, wq, s, b, N, y, epi, st, tiles, bat);
     }
@@ -856,7 +856,7 @@ static int launch_wide(const void* x, int64_t M, int64_t K, const uint32_t* wq, 
   }
   const int bm = szl ? qmm_wide_tile_rows(M, N, bat.count) : kBM;
   const int64_t tiles = ((M + bm - 1) / bm) * ((N + kBN - 1) / kBN);
-  if (tiles > 0x7fffffff) return set_error(MLXQ_EINVAL, "qmm: problem too large");
+  if (tiles > most_groups(512)) return set_error(MLXQ_EINVAL, "qmm: problem too large");
   if constexpr (kBf16) {
     if (szl && bm == 224) return launch_wide_w<SB, BITS, GS, 8, 224, true, kBN>(x, M, K, wq, s, b, N, y, epi, st, tiles, bat);
     if (szl) return launch_wide_w<SB, BITS, GS, 8, kBM, true, kBN>(x, M, K, wq, s, b, N, y, epi, st, tiles, bat);

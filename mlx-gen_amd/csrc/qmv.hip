@@ -168,6 +168,7 @@ static int launch_qmv(const void* x, int64_t M, int64_t K, const uint32_t* wq, c
   const int64_t gx = (N + rows_per_block - 1) / rows_per_block;
   const int64_t gy = (M + MR - 1) / MR;
   if (gx == 0 || gy == 0) return MLXQ_OK;
+  if (gx > most_groups(256)) return set_error(MLXQ_EINVAL, "qmv: N=%lld too large for the f32 kernel", (long long)N);
   if (gy > 65535) return set_error(MLXQ_EINVAL, "qmv: M=%lld too large for the f32 kernel", (long long)M);
   hipLaunchKernelGGL((qmv_kernel<XT, SB, BITS, GS, MR, ROWS>), dim3((unsigned)gx, (unsigned)gy),
                      dim3(256), 0, st, (const XT*)x, (int)M, K, wq, (const SB*)s, (const SB*)b, N,

@@ -206,6 +206,7 @@ static int launch_quantize(const void* w, int64_t N, int64_t K, uint32_t* wq, vo
   const int64_t n_chunks = N * K / 32;  // K % GS == 0 and GS >= 32, so K % 32 == 0
   if (n_chunks == 0) return MLXQ_OK;
   const int64_t blocks = (n_chunks + 255) / 256;
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "quantize: problem too large");
   hipLaunchKernelGGL((quantize_kernel<T, BITS, GS>), dim3((unsigned)blocks), dim3(256), 0, st,
                      (const T*)w, n_chunks, wq, (T*)s, (T*)b);
   return check_launch("quantize");
@@ -218,6 +219,7 @@ static int launch_quantize_batched(const void* const* w, int count, int64_t N, i
   const int64_t n_chunks = N * K / 32;
   if (n_chunks == 0) return MLXQ_OK;
   const int64_t blocks = (n_chunks + 255) / 256;
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "quantize_batched: problem too large");
   for (int e0 = 0; e0 < count; e0 += kQuantizeBatch) {
     const int n = count - e0 < kQuantizeBatch ? count - e0 : kQuantizeBatch;
     QuantizeBatch<T> batch = {};
@@ -241,6 +243,7 @@ static int launch_dequantize(const uint32_t* wq, const void* s, const void* b, i
   const int64_t n_chunks = N * K / 8;
   if (n_chunks == 0) return MLXQ_OK;
   const int64_t blocks = (n_chunks + 255) / 256;
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "dequantize: problem too large");
   hipLaunchKernelGGL((dequantize_kernel<T, BITS, GS>), dim3((unsigned)blocks), dim3(256), 0, st, wq,
                      (const T*)s, (const T*)b, n_chunks, (T*)out);
   return check_launch("dequantize");

@@ -137,7 +137,7 @@ static int launch_rotary(const Heads& x, int64_t T_, int64_t H, int64_t D, const
   const int hpt = (int)std::min<int64_t>(std::max<int64_t>(one / (device_cu_count() * 512), 1), 8);
   const int groups = (int)((H + hpt - 1) / hpt);
   const int64_t total = T_ * units * groups, blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "rotary: problem too large");
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "rotary: problem too large");
   hipLaunchKernelGGL((rotary_kernel<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, st, x, y, r, total, units, groups, hpt,
                      (int)H);
   return check_launch("rotary");
@@ -181,7 +181,7 @@ int run_rotary_table(const double* inv_freq, int64_t half, double magnitude, int
   Frequencies fr = {};
   for (int64_t i = 0; i < half; ++i) fr.f[i] = inv_freq[i];
   const int64_t total = positions * half, blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(MLXQ_EINVAL, "rotary_table: %lld positions are too many", (long long)positions);
+  if (blocks > most_groups(256)) return set_error(MLXQ_EINVAL, "rotary_table: %lld positions are too many", (long long)positions);
   hipLaunchKernelGGL(rotary_table_kernel, dim3((unsigned)blocks), dim3(256), 0, st, fr, (int)half, magnitude, total,
                      (f32x2*)table);
   return check_launch("rotary_table");
