@@ -98,3 +98,56 @@ def test_experts_sums_of_more_features_than_a_launch_has_threads_for(mlxq):
         assert ((y[rows].cpu().double() - want * s).abs() <= tol * s + 2.0 ** -8 * (want.abs() + tol) * s * (1 + 2.0 ** -20) + 2.0 ** -133).all()
     del y
     torch.cuda.empty_cache()
+
+
+class _Walled:
+    """Memory for a result between two walls of 1 MB of a pattern, which must be there afterwards."""
+    WALL = 1 << 20
+
+    def __init__(self, nbytes):
+        self.n = nbytes
+        self.buf = torch.full((2 * self.WALL + -(-nbytes // 256) * 256,), 0xa5, dtype=torch.uint8, device="cuda")
+
+    def ptr(self):
+        return self.buf.data_ptr() + self.WALL
+
+    def inside(self, dtype):
+        return self.buf[self.WALL:self.WALL + self.n].view(dtype)
+
+    def whole(self):
+        return bool((self.buf[:self.WALL] == 0xa5).all()) and bool((self.buf[self.WALL + self.n:] == 0xa5).all())
+
+
+# tiles of 16 and 32 rows, of 64, of 128 and of 256, whose results go by different ways
+@pytest.mark.parametrize("T,k,E,K,N", [(40, 2, 4, 64, 33), (9, 3, 5, 416, 1100), (300, 2, 4, 160, 2050), (2100, 4, 3, 96, 1030), (6000, 2, 2, 64, 5001)])
+@pytest.mark.parametrize("format", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_no_plan_writes_beside_the_results(mlxq, T, k, E, K, N, format, dtype):
+    """starts and rows that are no plan's: results that mean nothing, and not a byte beside them or the workspace."""
+    from mlxq import _lib
+    lib, g = _lib.load(), torch.Generator().manual_seed(T)
+    x = mlxq.mx_quantize(torch.randn(T, K, generator=g).cuda(), format)
+    w = mlxq.mx_quantize(torch.randn(E, N, K, generator=g).cuda())
+    ids = torch.randint(-1, E + 1, (T, k), generator=g, dtype=torch.int32).cuda()
+    good = mlxq.route_plan(ids, torch.rand(T, k, generator=g).cuda(), E)
+    M = T * k
+    junk = torch.randint(-2 ** 31, 2 ** 31 - 1, (M,), generator=g, dtype=torch.int64).int().cuda()
+    near = torch.randint(-3, M + 3, (M,), generator=g).int().cuda()
+    st = lambda *v: torch.tensor([v[i % len(v)] for i in range(E + 1)], dtype=torch.int64).int().cuda()  # noqa: E731
+    bad = [(st(-5, 10 ** 9, 3, -1, 2 ** 30), good.rows), (good.starts, torch.full_like(good.rows, 2 ** 30)), (good.starts, junk), (good.starts, near),
+           (st(0, M, 0, M), near), (st(M - 1, 0), junk), (st(2 ** 31 - 1, -2 ** 31), near), (torch.zeros_like(good.starts), good.rows)]
+    xv, _, keep_x = mlxq.mx._view("test", "x", x)
+    wv, _, keep_w = mlxq.mx._view("test", "w", w)
+    code = mlxq.mx._dt_of(dtype)
+    for combine in (0, 1):
+        need = lib.mlxq_mx_experts_workspace_size(T, k, N, combine, code)
+        want = mlxq.mx_experts(x, w, good, combine=bool(combine), out_dtype=dtype)
+        for i, (starts, rows) in enumerate(bad + [(good.starts, good.rows)]):
+            banner("mx_experts", T, k, E, K, N, format, dtype, combine, i)
+            y, ws = _Walled(want.numel() * want.element_size()), _Walled(need)
+            routed = mlxq.mx._routed((ids, good.weights, starts, rows), T, k, E)
+            _lib.check(lib.mlxq_mx_experts(ctypes.byref(xv), 0, K, ctypes.byref(wv), N, None, 0, ctypes.byref(routed), combine, y.ptr(), code,
+                                           ws.ptr() if need else None, need, torch.cuda.current_stream().cuda_stream))
+            assert y.whole() and ws.whole()
+        assert torch.equal(y.inside(dtype).view(want.shape), want)  # the last one is a plan
+    del keep_x, keep_w
