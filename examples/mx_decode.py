@@ -4,7 +4,8 @@
 
 Random weights.  A block is rms_norm of the residual's sum to 8 bits, a 4-bit packed qkv projection, cache_append and
 paged_attention, the packed output projection, rms_norm again, a router, the chosen experts' packed SwiGLU MLPs and
-their weighted sum; `train` fits a router and a norm through their gradients, the experts' packed weights held.  The run
+their weighted sum; `train` fits a router and the norm before it through their gradients, the experts' packed weights and inputs
+held (products of microscaled operands have no gradient).  The run
 prefills prompts of different lengths, captures a decode step in a HIP graph and replays it for every token.
 """
 import argparse

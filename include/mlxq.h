@@ -486,21 +486,27 @@ typedef struct {
  * microscaled codes.  A block's scale is the smallest power of two from 2^-127 on by which its largest
  * magnitude divided is at most 6 (e2m1) or 448 (e4m3), so that nothing saturates; values are rounded to
  * nearest, ties to even.  A block with an infinity or a NaN has scale 255 and codes 0.  Every step
- * but the rounding is exact.
+ * but the rounding is exact.  The types are the Open Compute Project's; the choice of a scale is not its
+ * conversion's, which takes the power of two of the largest magnitude and saturates: codes differ from such a
+ * quantiser's wherever that magnitude's significand is above 1.5 (e2m1) or 1.75 (e4m3).
  */
 int mlxq_mx_quantize(const void* x, int dtype, int64_t rows, int64_t K, int64_t row_stride,
                      const mlxq_mx* out, void* stream);
 
-/* out [rows, K] in out_dtype: code times scale, rounded once (bf16 and f32 hold all of them but bf16 those
- * below 2^-133; fp16 overflows past 65504). */
+/* out [rows, K] in out_dtype: code times scale, rounded once.  f32 holds all of them and bf16 those from 2^-126 on,
+ * but for the largest codes under the largest scales, which are infinite from 2^128 on (a block of the largest f32
+ * has one: it is quantised to 2^128); fp16 overflows past 65504. */
 int mlxq_mx_dequantize(const mlxq_mx* x, int64_t rows, int64_t K, void* out, int out_dtype, void* stream);
 
 /*
  * y [M, N] = x . w^T + bias: x [M, K] in either format, w [N, K] e2m1, bias [N] in bias_dtype or NULL; y
  * in y_dtype (f32, bf16, fp16).  Products of codes and scales are exact, sums f32 in an order that follows
- * M, N, K, the format and y_dtype only, one rounding at the end.  e4m3 with a 16-bit y: the matrix cores add
- * 128 products at a time and lose up to 2^-11 of the largest of them, in all about 2e-5 of a result.  f32
- * y of e4m3: values of x or w past f32's range are infinite.
+ * M, N, K, the format and y_dtype only, one rounding at the end.  But for e4m3 with a bf16 y: the matrix cores
+ * then add eight neighbouring products at a time and cut each below 2^-13 of the largest, so that up to 7 2^-13 of
+ * the largest of every eight is lost, less than 2^-10 of sum |x w| and than half a rounding to bf16 of a result
+ * that does not cancel; y_dtype f32 asks for f32 sums.  f32 and fp16 y of e4m3: values of x or w from 2^128 on are
+ * infinite, and those below 2^-126 have the bits of bf16's subnormals.  Sizes that take more tiles than a launch
+ * has (2^30 features, or results of some 100 GB) are MLXQ_EUNSUPPORTED.
  */
 int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int64_t N, const void* bias,
                    int bias_dtype, void* y, int y_dtype, void* stream);
@@ -509,11 +515,12 @@ int mlxq_mx_matmul(const mlxq_mx* x, int64_t M, int64_t K, const mlxq_mx* w, int
  * Root-mean-square norm over the last dimension of [T, heads, D]:
  *   h = x + residual (rounded to dtype and written to sum; without residual h = x and sum is NULL)
  *   y = h * (mean(h^2) + eps)^(-1/2) * weight            (weight [D] in weight_dtype, NULL: ones)
- * x, residual, sum and y have one dtype and any strides that are whole elements.  Sums are f32, and y is
- * rounded once.  Exactly one of y and y_mx is given: y_mx (e4m3, rows T * heads of D, D a multiple of 32)
- * is what mlxq_mx_quantize would make of the exact norm, which is taken in 64 bits wherever it matters, so that
- * no code depends on the order of a sum.  sum may be x or residual (same strides), y may be x; otherwise
- * nothing may overlap.  D up to 32768.
+ * x, residual, sum and y have one dtype and any strides that are whole elements. Sums are f32, and y is
+ * rounded once: a row whose squares add up past f32's range counts as infinite, and with eps 0 squares
+ * below 2^-126 lose bits (rows from 1e-18 to 1e16 are in range at any D). Exactly one of y and y_mx is
+ * given: y_mx (e4m3, rows T * heads of D, D a multiple of 32) is what mlxq_mx_quantize would make of the
+ * exact norm, which is taken in 64 bits wherever it matters, so that no code depends on the order of a
+ * sum. sum may be x or residual (same strides), y may be x; otherwise nothing may overlap. D up to 32768.
  */
 int mlxq_rms_norm(const mlxq_heads* x, int dtype, int64_t T, int64_t D, const mlxq_heads* residual,
                   const mlxq_heads* sum, const void* weight, int weight_dtype, float eps,
@@ -523,8 +530,9 @@ int mlxq_rms_norm(const mlxq_heads* x, int dtype, int64_t T, int64_t D, const ml
  * Its gradient.  With r = (mean(x^2) + eps)^(-1/2), n = x r and g = dy * weight:
  *   dx = r (g - n mean(g n)) + dsum,     dweight = sum over tokens and heads of dy n
  * x is what was normed (the sum, if there was a residual: dx is then the gradient of both), dsum (NULL =
- * none) the gradient that arrives at the sum from elsewhere.  dweight [D] in weight_dtype, NULL when
- * weight is.  f32 sums in a fixed order, each result rounded once.  dx may be dy or dsum (same strides).
+ * none) the gradient that arrives at the sum from elsewhere. dweight [D] in weight_dtype, NULL when weight
+ * is. f32 sums in a fixed order, each result rounded once, over the norm's range (and the sum of g x
+ * within f32's). dx may be dy or dsum (same strides).
  * workspace: mlxq_rms_norm_backward_workspace_size() bytes, 16-byte aligned, whatever they hold.
  */
 size_t mlxq_rms_norm_backward_workspace_size(int64_t T, int64_t heads, int64_t D, int dtype);
@@ -564,9 +572,10 @@ typedef struct {
  * experts with the largest s + bias (without a bias: the largest logits) among the kept groups, best first,
  * the lowest expert first among equal ones; weights are s of the chosen, normalized and scaled.  The choice
  * is made in 64 bits.  active (NULL = all): tokens whose byte is 0 get ids -1 and weights 0.
- * NaN logits come after all others of the kept groups; a row with a NaN or +infinity has NaN weights under
- * softmax, and where the chosen scores sum to 0 (all -infinity) the weights are 0.  top_k is at most
- * kept_groups * (experts / groups).  experts up to 1024, tokens * top_k below 2^31 - 2^20.
+ * NaN logits come after all others of the kept groups.  Under softmax a row with a NaN or +infinity has no
+ * scores: its logits alone choose (no bias, a group by its best) and its weights are NaN.  Where the chosen
+ * scores sum to 0 in 64 bits (all -infinity, or some 709 below 0 or 745 below the row's largest) the weights are 0.
+ * top_k is at most kept_groups * (experts / groups).  experts up to 1024, tokens * top_k below 2^31 - 2^20.
  * workspace: mlxq_route_workspace_size() bytes, 16-byte aligned, whatever they hold.
  */
 size_t mlxq_route_workspace_size(int64_t choices, int64_t experts);
@@ -580,20 +589,24 @@ int mlxq_route_plan(const mlxq_routing* out, void* workspace, size_t workspace_b
 /*
  * The gradient of the logits from that of the weights, dweights [tokens, top_k] f32, for the choice that
  * ids holds (ids outside [0, experts) pass nothing on; no expert twice in a row): dlogits [tokens, experts]
- * contiguous, in dtype.  f32 arithmetic.  Of router, scoring, normalize and scale are read.
+ * contiguous, in dtype.  f32 arithmetic; normalized weights by their shares, so that scores may be of any size, and
+ * where the weights are 0 the gradient is.  A token without an expert has a gradient of 0 whatever its logits
+ * hold; under softmax another row with a NaN or +infinity has NaN.  Of router, scoring, normalize and scale are read.
  */
 int mlxq_route_experts_backward(const float* dweights, const void* logits, int dtype, int64_t row_stride,
                                 const mlxq_router* router, const mlxq_routing* routing, void* dlogits,
                                 void* stream);
 
 /*
- * The products of the experts that tokens were routed to: y[t, j] = x[t] . w[ids[t, j]]^T + bias[ids[t, j]]
- * with w [experts, N, K] e2m1 (one stack of experts * N rows), bias [experts, N] in bias_dtype or NULL, x
- * [tokens, K], or with x_per_choice [tokens, top_k, K].  y is [tokens, top_k, N] in y_dtype, zero for choices
- * without an expert; with combine it is [tokens, N], sum_j weights[t, j] y[t, j]: each product is rounded to
- * y_dtype, as separate products would be, and the sum is f32.  starts and rows must be ids' plan; entries
- * outside their ranges are skipped.  workspace: mlxq_mx_experts_workspace_size() bytes, 16-byte aligned, whatever
- * they hold (NULL when that is 0: without combine).
+ * The products of the experts that tokens were routed to: y[t, j] = x[t] . w[ids[t, j]]^T + bias[ids[t,
+ * j]] with w [experts, N, K] e2m1 (one stack of experts * N rows), bias [experts, N] in bias_dtype or
+ * NULL, x [tokens, K], or with x_per_choice [tokens, top_k, K]. y is [tokens, top_k, N] in y_dtype, zero
+ * for choices without an expert; with combine it is [tokens, N], sum_j weights[t, j] y[t, j]: each product
+ * is rounded to y_dtype first, as separate products would be (fp16: past 65504 infinite), and the sum is
+ * f32 and rounded again; y_dtype f32 keeps the products in f32. Sums and sizes otherwise as
+ * mlxq_mx_matmul's. starts and rows must be ids' plan; entries outside their ranges are skipped.
+ * workspace: mlxq_mx_experts_workspace_size() bytes, 16-byte aligned, whatever they hold (NULL when that
+ * is 0: without combine).
  */
 size_t mlxq_mx_experts_workspace_size(int64_t tokens, int64_t top_k, int64_t N, int combine, int y_dtype);
 int mlxq_mx_experts(const mlxq_mx* x, int x_per_choice, int64_t K, const mlxq_mx* w, int64_t N,

@@ -26,8 +26,9 @@ _SCORING = {"softmax": MLXQ_ROUTE_SOFTMAX, "sigmoid": MLXQ_ROUTE_SIGMOID}
 class Mx(NamedTuple):
     """A microscaled tensor [..., K]: codes, e2m1 as uint8 [..., K/2] (two to a byte, the first in the low half) or
     float8_e4m3fn [..., K], and scales, uint8 [..., K/32] (2^(b - 127); 255: NaN), one for 32 values.  Scales
-    whose rows do not start at multiples of 4 bytes are copied by each call that reads them; mx_quantize's and
-    rms_norm's do."""
+    whose rows do not start at multiples of 4 bytes (a checkpoint's, where K / 32 is no multiple of 4) are copied by each
+    call that reads them; mx_quantize's and rms_norm's do.  A program that keeps such scales pads them once:
+    Mx(codes, F.pad(scales, (0, -n % 4))[..., :n]) for scales [..., n]."""
     codes: torch.Tensor
     scales: torch.Tensor
 
@@ -160,7 +161,9 @@ def mx_dequantize(x: Mx, dtype=torch.bfloat16):
 
 def mx_matmul(x: Mx, w: Mx, bias=None, out_dtype=torch.bfloat16):
     """x [..., K] . w^T + bias for w [N, K] e2m1: [..., N] in out_dtype.  x in either format; bias [N] in any of the
-    three dtypes.  Sums are f32, rounded once."""
+    three dtypes.  Sums are f32, rounded once, but for e4m3 rows with a bf16 result: the matrix cores then lose up to
+    7 2^-13 of the largest of every eight neighbouring products (less than half a rounding to bf16 of a result that does
+    not cancel).  out_dtype float32 or float16 asks for f32 sums."""
     op = "mx_matmul"
     _float(op, "out_dtype", out_dtype)
     y = _lib.fast().mx_matmul(x, w, bias, _dt_of(out_dtype))
@@ -325,7 +328,8 @@ def route_experts(logits, top_k: int, scoring: str = "softmax", bias=None, group
     Scores are softmax(logits) or sigmoid(logits); the experts with the largest score + bias [experts] (f32, for the
     choice only) are taken, best first, the lowest first among equal ones.  With groups (equal runs of experts) only
     those of the kept_groups best are, by the sum of a group's group_best (1 or 2) best.  Weights are the chosen scores,
-    divided by their sum when normalize, times scale.  Tokens whose active [T] (bool) is False get ids -1 and weights 0."""
+    divided by their sum when normalize, times scale.  Tokens whose active [T] (bool) is False get ids -1 and weights 0.
+    NaN logits come last; a softmax's row with NaN or +infinity is chosen by its logits alone and has NaN weights."""
     op = "route_experts"
     y = _lib.fast().route_experts(logits, top_k, scoring, bias, groups, kept_groups, group_best, normalize, scale, active)
     if y is not None:
@@ -385,7 +389,8 @@ def route_plan(ids, weights, experts: int) -> Routing:
 
 
 def route_experts_backward(dweights, logits, ids, scoring: str = "softmax", normalize: bool = True, scale: float = 1.0):
-    """The gradient of the logits, in their dtype, from that of route_experts' weights [T, top_k] (f32), for the choice ids."""
+    """The gradient of the logits, in their dtype, from that of route_experts' weights [T, top_k] (f32), for the choice ids
+    (no expert twice in a row; an id outside the experts passes nothing on, and a token without any has a gradient of 0)."""
     op = "route_experts_backward"
     y = _lib.fast().route_experts_backward(dweights, logits, ids, scoring, normalize, scale)
     if y is not None:
@@ -409,7 +414,8 @@ def route_experts_backward(dweights, logits, ids, scoring: str = "softmax", norm
 
 def mx_experts(x: Mx, w: Mx, routing: Routing, bias=None, combine: bool = False, out_dtype=torch.bfloat16):
     """The products of the experts that tokens were routed to: x[t] . w[ids[t, j]]^T + bias[ids[t, j]], [T, top_k, N] in
-    out_dtype, zero where ids names no expert; with combine their sum over j with the routing's weights, [T, N].
+    out_dtype, zero where ids names no expert; with combine their sum over j with the routing's weights, [T, N], of
+    products that are rounded to out_dtype first, as separate products would be (float32 keeps them in f32).
 
     x [T, K], or [T, top_k, K] with a row for each choice, in either format; w [experts, N, K] e2m1; bias [experts, N]."""
     op = "mx_experts"

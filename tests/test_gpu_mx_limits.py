@@ -151,3 +151,20 @@ def test_no_plan_writes_beside_the_results(mlxq, T, k, E, K, N, format, dtype):
             assert y.whole() and ws.whole()
         assert torch.equal(y.inside(dtype).view(want.shape), want)  # the last one is a plan
     del keep_x, keep_w
+
+
+def test_scales_padded_once(mlxq):
+    """90 scales a row as a checkpoint stores them, and the same laid out once as Mx says: the one is copied by each call, the other
+    goes to the library as it is."""
+    import torch.nn.functional as F
+    x = ref.random_mx(1, (3,), 2880, "e4m3", device="cuda")
+    codes, scales = ref.random_mx(2, (4, 70), 2880, "e2m1", device="cuda")
+    n = scales.shape[-1]
+    assert n == 90
+    held, rows = mlxq.Mx(codes, F.pad(scales, (0, -n % 4))[..., :n]), mlxq.Mx(x[0], F.pad(x[1], (0, -n % 4))[..., :n])
+    routing = mlxq.route_plan(torch.tensor([[0, 3], [1, 2], [3, 0]], dtype=torch.int32, device="cuda"), torch.rand(3, 2, device="cuda"), 4)
+    native = mlxq._lib.fast()
+    code = mlxq.mx._dt_of(BF16)
+    assert native.mx_experts(rows, mlxq.Mx(codes, scales), routing, None, False, code) is None
+    y = native.mx_experts(rows, held, routing, None, False, code)
+    assert y is not None and torch.equal(y, mlxq.mx_experts(mlxq.Mx(*x), mlxq.Mx(codes, scales), routing))
